@@ -431,6 +431,109 @@ int sf_spike_attention(const void* q, const void* k, const void* v,
                        float threshold, void* y, const int64_t* y_strides,
                        int32_t out_dtype, void* stream);
 
+/* ---- state space operators -------------------------------------------------- */
+
+/* Sequences.  Dense: `batch` sequences of `tokens` tokens each.  Packed
+ * (offsets != NULL): sequence b is rows offsets[b] .. offsets[b + 1] - 1 of
+ * `tokens` rows in all (offsets: int32 [batch + 1] on the device, not
+ * decreasing; bounds outside 0 .. tokens are clamped); max_len, the longest
+ * sequence, only sizes the launch.  A sequence may be empty.
+ *
+ * States.  Row slots[b] (slots NULL: row b) of a pool of `states` rows belongs
+ * to sequence b; no two sequences of a call share a row.  A row outside the
+ * pool: the sequence starts from a zero state and its state is not kept, and a
+ * step leaves the pool as it is and writes zeros to y.  initial_state NULL: a
+ * zero state.  final_state NULL: the state is not kept.  Both may be the same
+ * pool. */
+
+#define SF_ACT_NONE 0
+#define SF_ACT_SILU 1
+#define SF_ACT_SIGMOID 2
+
+/* Causal depthwise convolution of each channel over its last `kernel` tokens:
+ *   y[t, c] = act(bias[c] + sum_k weight[c, k] * u[t - kernel + 1 + k, c])
+ * where u before the sequence's start is the state [kernel - 1, channels]
+ * (oldest row first) and the final state is the last kernel - 1 rows of u.
+ * x, y and states have `dtype`; element (b, t, c) of x sits at b * strides[0] +
+ * t * strides[1] + c (packed: strides[0] unused); weight f32
+ * [channels, kernel], bias f32 (or NULL); 1 <= kernel <= 8; f32 sums. */
+typedef struct sf_conv1d_desc {
+  int64_t batch, tokens, max_len, states;
+  int64_t x_strides[2], y_strides[2];
+  int32_t channels, kernel, dtype, activation;
+} sf_conv1d_desc;
+
+int sf_causal_conv1d(const sf_conv1d_desc* desc, const void* x,
+                     const float* weight, const float* bias,
+                     const int32_t* offsets, const int32_t* slots,
+                     const void* initial_state, void* y, void* final_state,
+                     void* stream);
+/* One token of each sequence (tokens, max_len, strides[1] unused); the state
+ * rows are updated in place. */
+int sf_causal_conv1d_step(const sf_conv1d_desc* desc, void* state,
+                          const void* x, const float* weight,
+                          const float* bias, const int32_t* slots, void* y,
+                          void* stream);
+
+/* Selective state space scan.  Per sequence and head, from the state h
+ * [head_dim, state_dim]:
+ *   d_t = dt_t + dt_bias (dt_softplus: log(1 + exp(.)) of it)
+ *   h_t = exp(A d_t) h_{t-1} + d_t x_t (outer) B_t
+ *   y_t = h_t C_t + D x_t
+ * Heads share the B and C of their group (heads / groups in a row).  x, dt, B, C
+ * and y have `dtype`; element (b, t, i, j) sits at b * strides[0] +
+ * t * strides[1] + i * strides[2] + j, i the head (of B and C the group) and j
+ * the last axis (dt has none); A f32 [heads]; D, dt_bias f32 [heads] or NULL;
+ * states f32 [states, heads, head_dim, state_dim].  state_dim <= 256.  States
+ * and sums are f32. */
+typedef struct sf_scan_desc {
+  int64_t batch, tokens, max_len, states;
+  int64_t x_strides[3], dt_strides[3], b_strides[3], c_strides[3], y_strides[3];
+  int32_t heads, head_dim, groups, state_dim, dtype, dt_softplus;
+} sf_scan_desc;
+
+size_t sf_selective_scan_workspace_size(const sf_scan_desc* desc);
+int sf_selective_scan(const sf_scan_desc* desc, const void* x, const void* dt,
+                      const float* A, const void* B, const void* C,
+                      const float* D, const float* dt_bias,
+                      const int32_t* offsets, const int32_t* slots,
+                      const float* initial_state, void* y, float* final_state,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* One token of each sequence (tokens, max_len, strides[1] unused); the state
+ * rows are updated in place. */
+int sf_selective_scan_step(const sf_scan_desc* desc, float* state,
+                           const void* x, const void* dt, const float* A,
+                           const void* B, const void* C, const float* D,
+                           const float* dt_bias, const int32_t* slots, void* y,
+                           void* stream);
+
+/* The norms around a block with its gate and residual scale, one pass over
+ * [outer, inner, dim] rows:
+ *   t = x;  gate_first: t *= act(gate)
+ *   post_weight: t *= post_weight / sqrt(mean(t^2) + eps), the mean over each
+ *                group_size columns
+ *   gate after:  t *= act(gate)
+ *   r = residual + scale * scale_weight * t
+ *   pre_weight:  h = r * pre_weight / sqrt(mean(r^2) + eps), the mean over dim
+ * gate, post_weight, residual, scale_weight [dim] and pre_weight [dim] may be
+ * NULL (weights are f32).  x, gate and h have `dtype`, residual and r
+ * `residual_dtype` (`dtype` or f32); h is taken from the f32 value of r.  r_out
+ * may be NULL where pre_weight is given, h_out where it is not; r_out may be the
+ * residual and h_out may be x.  Element (o, i, c) of a tensor sits at
+ * o * strides[0] + i * strides[1] + c (a stride of inputs may be 0).
+ * dim <= 16384, group_size divides dim; f32 sums. */
+typedef struct sf_norm_desc {
+  int64_t outer, inner;
+  int64_t x_strides[2], gate_strides[2], residual_strides[2], r_strides[2], h_strides[2];
+  int32_t dim, group_size, dtype, residual_dtype, activation, gate_first;
+  float eps, scale;
+} sf_norm_desc;
+
+int sf_block_norm(const sf_norm_desc* desc, const void* x, const void* gate,
+                  const float* post_weight, const void* residual,
+                  const float* scale_weight, const float* pre_weight,
+                  void* r_out, void* h_out, void* stream);
+
 /* ---- launch plans (host only) --------------------------------------------- */
 
 /* How sf_conv2d_sparse (fused_lif = 0) or sf_conv_lif_forward (1) launches the
@@ -451,7 +554,7 @@ int sf_conv2d_launch_plan(const sf_conv_desc* desc, int32_t fused_lif,
  * "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3", "lif_multistep",
  * "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
  * "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused",
- * "conv_dense_mfma").
+ * "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm").
  * Returns the
  * number of launches recorded for that kernel. */
 int sf_timing_enable(int32_t enable);

@@ -1,0 +1,73 @@
+"""What the state space entry points share: their checks of arguments, and
+sequences and state pools on host tensors.
+
+A prompt comes dense, [batch, tokens, ...], or packed, [total, ...] with
+`offsets` (int32 [sequences + 1]): sequence b is rows offsets[b] to
+offsets[b + 1] - 1.  The state of sequence b is row slots[b] of a pool (without
+slots: row b)."""
+
+from __future__ import annotations
+
+from typing import List, Optional, Tuple
+
+import torch
+
+FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def check_input(t: torch.Tensor, name: str) -> None:
+    if t.dtype not in FLOATS:
+        from .. import _lib
+
+        raise _lib.UnsupportedError(f"{name} is {t.dtype}: float32, float16 or bfloat16 is wanted")
+
+
+def check_like(t: torch.Tensor, x: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
+    if tuple(t.shape) != shape or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {shape} {x.dtype} on {x.device} is wanted")
+
+
+def check_param(t: Optional[torch.Tensor], x: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
+    if t is None:
+        return
+    if tuple(t.shape) != shape or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: a contiguous {shape} float32 on "
+                         f"{x.device} is wanted")
+
+
+def check_index(t: Optional[torch.Tensor], x: torch.Tensor, name: str, size: int) -> None:
+    if t is None:
+        return
+    if t.dim() != 1 or t.numel() != size or t.dtype != torch.int32 or t.device != x.device or not t.is_contiguous():
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: a contiguous ({size},) int32 on "
+                         f"{x.device} is wanted")
+
+
+def check_pool(t: Optional[torch.Tensor], x: torch.Tensor, name: str, row: Tuple[int, ...], dtype: torch.dtype,
+               batch: int, slots: Optional[torch.Tensor]) -> None:
+    if t is None:
+        return
+    if t.dim() != len(row) + 1 or tuple(t.shape[1:]) != row or t.dtype != dtype or t.device != x.device \
+            or not t.is_contiguous() or (slots is None and t.shape[0] != batch):
+        rows = f"{batch}" if slots is None else "rows"
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: a contiguous "
+                         f"({rows}, {', '.join(map(str, row))}) {dtype} on {x.device} is wanted")
+
+
+def last_contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def host_spans(x: torch.Tensor, offsets: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """Host: every sequence's [tokens, ...] view of x."""
+    if offsets is None:
+        return list(x.unbind(0))
+    total = x.shape[0]
+    at = [min(max(int(v), 0), total) for v in offsets]
+    return [x[a:max(a, b)] for a, b in zip(at, at[1:])]
+
+
+def host_slots(batch: int, rows: int, slots: Optional[torch.Tensor]) -> List[int]:
+    """Host: every sequence's row of the pool, -1 where it has none."""
+    pick = range(batch) if slots is None else [int(v) for v in slots]
+    return [s if 0 <= s < rows else -1 for s in pick]

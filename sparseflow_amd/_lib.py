@@ -88,6 +88,12 @@ EXPORTS = {
     "sf_spike_attention_supported": (c_int, [c_int32, c_int32]),
     "sf_spike_attention": (c_int, [_P, _P, _P, c_int32, c_int64, c_int32, c_int32, c_int32, _P, c_float, c_float, _P,
                                    _P, c_int32, _P]),
+    "sf_causal_conv1d": (c_int, [_P] * 10),
+    "sf_causal_conv1d_step": (c_int, [_P] * 8),
+    "sf_selective_scan_workspace_size": (c_size_t, [_P]),
+    "sf_selective_scan": (c_int, [_P] * 13 + [_P, c_size_t, _P]),
+    "sf_selective_scan_step": (c_int, [_P] * 12),
+    "sf_block_norm": (c_int, [_P] * 10),
     "sf_timing_enable": (c_int, [c_int32]),
     "sf_timing_collect": (c_int, []),
     "sf_timing_query": (c_int64, [ctypes.c_char_p, ctypes.POINTER(c_double)]),
@@ -117,6 +123,35 @@ class LifParams(ctypes.Structure):
     _fields_ = [
         ("tau", c_float), ("v_threshold", c_float), ("v_reset", c_float),
         ("hard_reset", c_int32), ("decay_input", c_int32),
+    ]
+
+
+class Conv1dDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int64), ("tokens", c_int64), ("max_len", c_int64), ("states", c_int64),
+        ("x_strides", c_int64 * 2), ("y_strides", c_int64 * 2),
+        ("channels", c_int32), ("kernel", c_int32), ("dtype", c_int32), ("activation", c_int32),
+    ]
+
+
+class ScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int64), ("tokens", c_int64), ("max_len", c_int64), ("states", c_int64),
+        ("x_strides", c_int64 * 3), ("dt_strides", c_int64 * 3), ("b_strides", c_int64 * 3),
+        ("c_strides", c_int64 * 3), ("y_strides", c_int64 * 3),
+        ("heads", c_int32), ("head_dim", c_int32), ("groups", c_int32), ("state_dim", c_int32),
+        ("dtype", c_int32), ("dt_softplus", c_int32),
+    ]
+
+
+class NormDesc(ctypes.Structure):
+    _fields_ = [
+        ("outer", c_int64), ("inner", c_int64),
+        ("x_strides", c_int64 * 2), ("gate_strides", c_int64 * 2), ("residual_strides", c_int64 * 2),
+        ("r_strides", c_int64 * 2), ("h_strides", c_int64 * 2),
+        ("dim", c_int32), ("group_size", c_int32), ("dtype", c_int32), ("residual_dtype", c_int32),
+        ("activation", c_int32), ("gate_first", c_int32),
+        ("eps", c_float), ("scale", c_float),
     ]
 
 
@@ -569,12 +604,99 @@ def spike_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
 
 
 # ---------------------------------------------------------------------------
+# State space operators
+# ---------------------------------------------------------------------------
+
+SF_ACT = {None: 0, "silu": 1, "sigmoid": 2}
+
+
+# Descriptors hold sizes and strides only; a call repeats its predecessor's far
+# more often than not, and filling a ctypes struct costs more than a launch.
+@functools.lru_cache(maxsize=1024)
+def conv1d_desc(batch: int, tokens: int, max_len: int, states: int, x_strides: tuple, y_strides: tuple, channels: int,
+                kernel: int, dtype: torch.dtype, activation: Optional[str]):
+    """(the descriptor, its address)."""
+    d = Conv1dDesc(batch, tokens, max_len, states, x_strides, y_strides, channels, kernel, dtype_code(dtype),
+                   SF_ACT[activation])
+    return d, ctypes.addressof(d)
+
+
+def _raw(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def causal_conv1d(desc, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                  offsets: Optional[torch.Tensor], slots: Optional[torch.Tensor], initial: Optional[torch.Tensor],
+                  y: torch.Tensor, final: Optional[torch.Tensor]) -> None:
+    rc = lib().sf_causal_conv1d(desc[1], x.data_ptr(), weight.data_ptr(), _raw(bias), _raw(offsets), _raw(slots),
+                                _raw(initial), y.data_ptr(), _raw(final), raw_stream(x.device.index))
+    _check(rc, "sf_causal_conv1d")
+
+
+def causal_conv1d_step(desc, state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                       bias: Optional[torch.Tensor], slots: Optional[torch.Tensor], y: torch.Tensor) -> None:
+    rc = lib().sf_causal_conv1d_step(desc[1], state.data_ptr(), x.data_ptr(), weight.data_ptr(), _raw(bias),
+                                     _raw(slots), y.data_ptr(), raw_stream(x.device.index))
+    _check(rc, "sf_causal_conv1d_step")
+
+
+@functools.lru_cache(maxsize=1024)
+def scan_desc(batch: int, tokens: int, max_len: int, states: int, x_strides: tuple, dt_strides: tuple,
+              b_strides: tuple, c_strides: tuple, y_strides: tuple, heads: int, head_dim: int, groups: int,
+              state_dim: int, dtype: torch.dtype, dt_softplus: bool):
+    """(the descriptor, its address, the bytes of workspace of a scan with it)."""
+    d = ScanDesc(batch, tokens, max_len, states, x_strides, dt_strides, b_strides, c_strides, y_strides, heads,
+                 head_dim, groups, state_dim, dtype_code(dtype), int(dt_softplus))
+    at = ctypes.addressof(d)
+    return d, at, int(lib().sf_selective_scan_workspace_size(at))
+
+
+def selective_scan(desc, x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                   D: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], offsets: Optional[torch.Tensor],
+                   slots: Optional[torch.Tensor], initial: Optional[torch.Tensor], y: torch.Tensor,
+                   final: Optional[torch.Tensor], workspace: Optional[torch.Tensor]) -> None:
+    rc = lib().sf_selective_scan(desc[1], x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
+                                 _raw(D), _raw(dt_bias), _raw(offsets), _raw(slots), _raw(initial), y.data_ptr(),
+                                 _raw(final), _raw(workspace),
+                                 0 if workspace is None else workspace.numel() * workspace.element_size(),
+                                 raw_stream(x.device.index))
+    _check(rc, "sf_selective_scan")
+
+
+def selective_scan_step(desc, state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor,
+                        B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor],
+                        dt_bias: Optional[torch.Tensor], slots: Optional[torch.Tensor], y: torch.Tensor) -> None:
+    rc = lib().sf_selective_scan_step(desc[1], state.data_ptr(), x.data_ptr(), dt.data_ptr(), A.data_ptr(),
+                                      B.data_ptr(), C.data_ptr(), _raw(D), _raw(dt_bias), _raw(slots), y.data_ptr(),
+                                      raw_stream(x.device.index))
+    _check(rc, "sf_selective_scan_step")
+
+
+@functools.lru_cache(maxsize=1024)
+def norm_desc(outer: int, inner: int, x_strides: tuple, gate_strides: tuple, residual_strides: tuple,
+              r_strides: tuple, h_strides: tuple, dim: int, group_size: int, dtype: torch.dtype,
+              residual_dtype: torch.dtype, activation: Optional[str], gate_first: bool, eps: float, scale: float):
+    d = NormDesc(outer, inner, x_strides, gate_strides, residual_strides, r_strides, h_strides, dim, group_size,
+                 dtype_code(dtype), dtype_code(residual_dtype), SF_ACT[activation], int(gate_first), eps, scale)
+    return d, ctypes.addressof(d)
+
+
+def block_norm(desc, x: torch.Tensor, gate: Optional[torch.Tensor], post_weight: Optional[torch.Tensor],
+               residual: Optional[torch.Tensor], scale_weight: Optional[torch.Tensor],
+               pre_weight: Optional[torch.Tensor], r: Optional[torch.Tensor], h: Optional[torch.Tensor]) -> None:
+    rc = lib().sf_block_norm(desc[1], x.data_ptr(), _raw(gate), _raw(post_weight), _raw(residual),
+                             _raw(scale_weight), _raw(pre_weight), _raw(r), _raw(h), raw_stream(x.device.index))
+    _check(rc, "sf_block_norm")
+
+
+# ---------------------------------------------------------------------------
 # Per-kernel timing (bench instrumentation)
 # ---------------------------------------------------------------------------
 
 KERNEL_NAMES = ("prescan_pack", "prescan_tiles", "conv_gather", "conv_lif", "conv_rows", "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3",
                 "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
-                "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused", "conv_dense_mfma")
+                "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused", "conv_dense_mfma",
+                "causal_conv1d", "scan_seq", "block_norm")
 
 
 def timing_enable(on: bool) -> None:

@@ -256,7 +256,7 @@ const char* g_names[sf::K_COUNT] = {"prescan_pack", "prescan_tiles", "conv_gathe
                                      "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3",
                                      "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse",
                                      "spike_attention", "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma",
-                                     "conv_rows_fused", "conv_dense_mfma"};
+                                     "conv_rows_fused", "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm"};
 
 }  // namespace
 
@@ -721,6 +721,212 @@ int sf_spike_attention(const void* q, const void* k, const void* v, int32_t in_d
   a.cutoff = sf_activity_cutoff(threshold);
   const int rc = sf::launch_spike_attn(a, in_dtype, out_dtype, static_cast<hipStream_t>(stream));
   if (rc != hipSuccess) return hip_fail(rc, "spike_attention launch");
+  return SF_OK;
+}
+
+// ---- state space operators ---------------------------------------------------
+
+static int check_seq(int64_t batch, int64_t tokens, int64_t states, bool has_state) {
+  if (batch < 0 || tokens < 0) return fail(SF_ERR_INVALID, "batch < 0 or tokens < 0");
+  if (batch > (1ll << 31) - 1 || tokens > (1ll << 31) - 1) return fail(SF_ERR_UNSUPPORTED, "batch or tokens over 2^31 - 1");
+  if (has_state && states < 0) return fail(SF_ERR_INVALID, "states < 0");
+  return SF_OK;
+}
+
+static int check_conv1d(const sf_conv1d_desc* d, bool has_state) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  if (d->channels < 1 || d->kernel < 1) return fail(SF_ERR_INVALID, "non-positive channels or kernel");
+  if (!dtype_ok(d->dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (d->activation != SF_ACT_NONE && d->activation != SF_ACT_SILU)
+    return fail(SF_ERR_UNSUPPORTED, "activation must be none or silu");
+  if (d->kernel > 8) return fail(SF_ERR_UNSUPPORTED, "kernel > 8");
+  return check_seq(d->batch, d->tokens, d->states, has_state);
+}
+
+static sf::Conv1dArgs conv1d_args(const sf_conv1d_desc* d, const void* x, const float* weight, const float* bias,
+                                  const int32_t* offsets, const int32_t* slots, const void* before, void* y,
+                                  void* after, bool step) {
+  sf::Conv1dArgs a{};
+  a.seq = {offsets, slots, d->batch, step ? 1 : d->tokens, d->states};
+  a.x = x;
+  a.weight = weight;
+  a.bias = bias;
+  a.before = before;
+  a.after = after;
+  a.y = y;
+  a.max_len = step ? 1 : offsets == nullptr ? d->tokens : d->max_len;
+  a.x_b = offsets == nullptr ? d->x_strides[0] : 0;
+  a.x_t = step ? 0 : d->x_strides[1];
+  a.y_b = offsets == nullptr ? d->y_strides[0] : 0;
+  a.y_t = step ? 0 : d->y_strides[1];
+  a.channels = d->channels;
+  a.kernel = d->kernel;
+  a.act = d->activation;
+  a.step = step ? 1 : 0;
+  return a;
+}
+
+int sf_causal_conv1d(const sf_conv1d_desc* d, const void* x, const float* weight, const float* bias,
+                     const int32_t* offsets, const int32_t* slots, const void* initial_state, void* y,
+                     void* final_state, void* stream) {
+  const int rc = check_conv1d(d, initial_state != nullptr || final_state != nullptr);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0) return SF_OK;
+  if (weight == nullptr || (d->tokens > 0 && (x == nullptr || y == nullptr))) return fail(SF_ERR_INVALID, "NULL pointer");
+  const sf::Conv1dArgs a = conv1d_args(d, x, weight, bias, offsets, slots, initial_state, y, final_state, false);
+  const int e = sf::launch_conv1d(a, d->dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "causal_conv1d launch");
+  return SF_OK;
+}
+
+int sf_causal_conv1d_step(const sf_conv1d_desc* d, void* state, const void* x, const float* weight, const float* bias,
+                          const int32_t* slots, void* y, void* stream) {
+  const int rc = check_conv1d(d, true);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0) return SF_OK;
+  if (x == nullptr || y == nullptr || weight == nullptr || (state == nullptr && d->kernel > 1 && d->states > 0))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  const sf::Conv1dArgs a = conv1d_args(d, x, weight, bias, nullptr, slots, state, y, state, true);
+  const int e = sf::launch_conv1d(a, d->dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "causal_conv1d launch");
+  return SF_OK;
+}
+
+static int check_scan(const sf_scan_desc* d, bool has_state) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  if (d->heads < 1 || d->head_dim < 1 || d->groups < 1 || d->state_dim < 1)
+    return fail(SF_ERR_INVALID, "non-positive dimension");
+  if (d->heads % d->groups != 0) return fail(SF_ERR_INVALID, "groups does not divide heads");
+  if (!dtype_ok(d->dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (d->state_dim > sf::kScanMaxState) return fail(SF_ERR_UNSUPPORTED, "state_dim > 256");
+  return check_seq(d->batch, d->tokens, d->states, has_state);
+}
+
+static sf::ScanArgs scan_args(const sf_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
+                              const void* C, const float* D, const float* dt_bias, const int32_t* offsets,
+                              const int32_t* slots, const float* h0, void* y, float* h1, bool step) {
+  sf::ScanArgs a{};
+  a.seq = {offsets, slots, d->batch, step ? 1 : d->tokens, d->states};
+  a.x = x;
+  a.dt = dt;
+  a.b = B;
+  a.c = C;
+  a.A = A;
+  a.D = D;
+  a.dt_bias = dt_bias;
+  a.h0 = h0;
+  a.h1 = h1;
+  a.y = y;
+  a.max_len = step ? 1 : offsets == nullptr ? d->tokens : d->max_len;
+  const int64_t dense = offsets == nullptr ? 1 : 0, walk = step ? 0 : 1;
+  a.x_b = d->x_strides[0] * dense;
+  a.x_t = d->x_strides[1] * walk;
+  a.x_h = d->x_strides[2];
+  a.dt_b = d->dt_strides[0] * dense;
+  a.dt_t = d->dt_strides[1] * walk;
+  a.dt_h = d->dt_strides[2];
+  a.b_b = d->b_strides[0] * dense;
+  a.b_t = d->b_strides[1] * walk;
+  a.b_g = d->b_strides[2];
+  a.c_b = d->c_strides[0] * dense;
+  a.c_t = d->c_strides[1] * walk;
+  a.c_g = d->c_strides[2];
+  a.y_b = d->y_strides[0] * dense;
+  a.y_t = d->y_strides[1] * walk;
+  a.y_h = d->y_strides[2];
+  a.heads = d->heads;
+  a.head_dim = d->head_dim;
+  a.groups = d->groups;
+  a.state_dim = d->state_dim;
+  a.softplus = d->dt_softplus != 0;
+  a.step = step ? 1 : 0;
+  return a;
+}
+
+size_t sf_selective_scan_workspace_size(const sf_scan_desc* d) {
+  (void)d;
+  return 0;
+}
+
+int sf_selective_scan(const sf_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
+                      const void* C, const float* D, const float* dt_bias, const int32_t* offsets,
+                      const int32_t* slots, const float* initial_state, void* y, float* final_state, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const int rc = check_scan(d, initial_state != nullptr || final_state != nullptr);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0) return SF_OK;
+  if (A == nullptr || (d->tokens > 0 && (x == nullptr || dt == nullptr || B == nullptr || C == nullptr || y == nullptr)))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  const size_t need = sf_selective_scan_workspace_size(d);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return fail(SF_ERR_WORKSPACE, "workspace too small");
+  const sf::ScanArgs a =
+      scan_args(d, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, y, final_state, false);
+  const int e = sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "selective_scan launch");
+  return SF_OK;
+}
+
+int sf_selective_scan_step(const sf_scan_desc* d, float* state, const void* x, const void* dt, const float* A,
+                           const void* B, const void* C, const float* D, const float* dt_bias, const int32_t* slots,
+                           void* y, void* stream) {
+  const int rc = check_scan(d, true);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0) return SF_OK;
+  if (A == nullptr || x == nullptr || dt == nullptr || B == nullptr || C == nullptr || y == nullptr ||
+      (state == nullptr && d->states > 0))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  const sf::ScanArgs a = scan_args(d, x, dt, A, B, C, D, dt_bias, nullptr, slots, state, y, state, true);
+  const int e = sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "selective_scan launch");
+  return SF_OK;
+}
+
+int sf_block_norm(const sf_norm_desc* d, const void* x, const void* gate, const float* post_weight,
+                  const void* residual, const float* scale_weight, const float* pre_weight, void* r_out, void* h_out,
+                  void* stream) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  if (d->outer < 0 || d->inner < 0) return fail(SF_ERR_INVALID, "negative rows");
+  if (d->dim < 1 || d->group_size < 1 || d->dim % d->group_size != 0)
+    return fail(SF_ERR_INVALID, "group_size does not divide dim");
+  if (!dtype_ok(d->dtype) || !dtype_ok(d->residual_dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (d->residual_dtype != d->dtype && d->residual_dtype != SF_F32)
+    return fail(SF_ERR_UNSUPPORTED, "residual_dtype must equal dtype or be f32");
+  if (d->activation < SF_ACT_NONE || d->activation > SF_ACT_SIGMOID)
+    return fail(SF_ERR_UNSUPPORTED, "unknown activation");
+  if (d->dim > sf::kNormMaxDim) return fail(SF_ERR_UNSUPPORTED, "dim > 16384");
+  if (d->inner > 0 && d->outer > ((1ll << 62) / d->inner) / d->dim) return fail(SF_ERR_UNSUPPORTED, "too many rows");
+  if (d->outer == 0 || d->inner == 0) return SF_OK;
+  if (x == nullptr || (r_out == nullptr && pre_weight == nullptr) || (h_out == nullptr) != (pre_weight == nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  sf::NormArgs a{};
+  a.x = x;
+  a.gate = gate;
+  a.post_w = post_weight;
+  a.res = residual;
+  a.scale_w = scale_weight;
+  a.pre_w = pre_weight;
+  a.r = r_out;
+  a.h = h_out;
+  a.outer = d->outer;
+  a.inner = d->inner;
+  a.x_o = d->x_strides[0];
+  a.x_i = d->x_strides[1];
+  a.g_o = d->gate_strides[0];
+  a.g_i = d->gate_strides[1];
+  a.res_o = d->residual_strides[0];
+  a.res_i = d->residual_strides[1];
+  a.r_o = d->r_strides[0];
+  a.r_i = d->r_strides[1];
+  a.h_o = d->h_strides[0];
+  a.h_i = d->h_strides[1];
+  a.dim = d->dim;
+  a.group = post_weight == nullptr ? d->dim : d->group_size;
+  a.act = d->activation;
+  a.gate_first = d->gate_first != 0;
+  a.eps = d->eps;
+  a.scale = d->scale;
+  const int rc = sf::launch_block_norm(a, d->dtype, d->residual_dtype, static_cast<hipStream_t>(stream));
+  if (rc != hipSuccess) return hip_fail(rc, "block_norm launch");
   return SF_OK;
 }
 

@@ -266,6 +266,70 @@ struct AttnArgs {
 int attn_max_tokens(int d);  // of a supported head_dim d, otherwise 0
 int launch_spike_attn(const AttnArgs& a, int in_dtype, int out_dtype, hipStream_t stream);
 
+// State space operators (see sparseflow.h for the mathematics).  Sequence b of
+// a call: rows [first, first + n) of the token axis and its row of the pool.
+struct SeqAxis {
+  const int32_t* offsets;  // packed: [batch + 1], otherwise NULL
+  const int32_t* slots;    // NULL: row b
+  int64_t batch, tokens, states;
+};
+
+struct Conv1dArgs {
+  SeqAxis seq;
+  const void* x;
+  const float* weight;
+  const float* bias;
+  const void* before;  // initial state
+  void* after;         // final state
+  void* y;
+  int64_t max_len;
+  int64_t x_b, x_t, y_b, y_t;  // strides (elements); packed: x_b, y_b = 0
+  int64_t block0;              // first workgroup of the launch
+  int channels, kernel, act;
+  int step;                    // one token of each sequence; sequences without a row give zeros
+};
+int launch_conv1d(const Conv1dArgs& a, int dtype, hipStream_t stream);
+
+struct ScanArgs {
+  SeqAxis seq;
+  const void* x;
+  const void* dt;
+  const void* b;
+  const void* c;
+  const float* A;
+  const float* D;
+  const float* dt_bias;
+  const float* h0;
+  float* h1;
+  void* y;
+  int64_t max_len;
+  // Strides (elements) of sequence, token and head / group; packed: *_b = 0.
+  int64_t x_b, x_t, x_h, dt_b, dt_t, dt_h, b_b, b_t, b_g, c_b, c_t, c_g, y_b, y_t, y_h;
+  int64_t block0;
+  int heads, head_dim, groups, state_dim, softplus;
+  int step;
+};
+constexpr int kScanMaxState = 256;
+int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);
+
+struct NormArgs {
+  const void* x;
+  const void* gate;
+  const float* post_w;
+  const void* res;
+  const float* scale_w;
+  const float* pre_w;
+  void* r;
+  void* h;
+  int64_t outer, inner;
+  int64_t x_o, x_i, g_o, g_i, res_o, res_i, r_o, r_i, h_o, h_i;
+  int64_t item0;
+  int dim, group, act, gate_first;
+  float eps, scale;
+};
+constexpr int kNormMaxDim = 16384;
+int launch_block_norm(const NormArgs& a, int dtype, int res_dtype, hipStream_t stream);
+
 // Raise kernel K's dynamic-LDS ceiling to `bytes` (the default limit is
 // 64 KB) once per device and process.  Thread-safe: two first calls racing
 // set the same attribute twice, which is harmless; a failure is returned and
@@ -289,7 +353,7 @@ void conv_geometry(ConvArgs& a, bool lif);
 // Per-kernel event timing hooks used by the launchers.
 void timing_begin(int kernel_id, hipStream_t stream);
 void timing_end(int kernel_id, hipStream_t stream);
-enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_COUNT = 20 };
+enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_CONV1D = 20, K_SCAN_SEQ = 21, K_NORM = 22, K_COUNT = 23 };
 
 // ---------------------------------------------------------------------------
 // Device helpers.

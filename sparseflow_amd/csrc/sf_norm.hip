@@ -1,0 +1,211 @@
+// The norms around a block with its gate and residual scale, in one pass over
+// each row:
+//   t = act(gate) x (gate first), t *= w / rms(t) over each group, t *= act(gate),
+//   r = residual + scale t, h = r w' / rms(r)
+// A row is held in registers by LT threads, E elements in each as vectors of V:
+// read once, two sums over it, written once.  Bound by HBM.
+//
+// Groups are rows of their own where no norm of the whole row follows; otherwise
+// a workgroup holds the row and the groups' sums meet in LDS.
+#include "sf_seq.h"
+
+namespace sf {
+
+namespace {
+
+constexpr int kBlock = 256;
+
+__device__ __forceinline__ float act_of(int act, float v) {
+  return act == SF_ACT_SILU ? silu(v) : act == SF_ACT_SIGMOID ? sigmoid(v) : v;
+}
+
+// The sum of v over the LT threads of a row (in an order of its own for every
+// thread of a wavefront, the same bits in all: xor butterflies).
+template <int LT>
+__device__ __forceinline__ float row_sum(float v, float* s_part) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if constexpr (LT > kWave) {
+    __syncthreads();  // an earlier sum's readers
+    if (lane_id() == 0) s_part[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LT / kWave; ++w) v += s_part[w];
+  }
+  return v;
+}
+
+// sub: groups that are rows of their own (1: the whole row).  GROUPED: groups
+// inside the row (LT = the workgroup, group % V == 0).
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED>
+__global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormArgs a, int sub) {
+  constexpr int kRowsPerBlock = (LT > kBlock ? LT : kBlock) / LT;
+  __shared__ float s_part[LT / kWave];
+  const int lt = threadIdx.x % LT;
+  const int width = a.dim / sub;
+  const int64_t item = (a.item0 + blockIdx.x) * kRowsPerBlock + threadIdx.x / LT;
+  if (item >= a.outer * a.inner * sub) return;  // (LT > 64 has one row to a workgroup)
+  const int64_t row = item / sub;
+  const int c0 = (int)(item - row * sub) * width;
+  const int64_t o = row / a.inner, i = row - o * a.inner;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + o * a.x_o + i * a.x_i + c0;
+  float t[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * LT + lt) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[k][e] = 0.f;
+    if (c < width) load_f32<T, V>(x + c, t[k]);
+  }
+  auto gate = [&]() {
+    const T* __restrict__ g = static_cast<const T*>(a.gate) + o * a.g_o + i * a.g_i + c0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LT + lt) * V;
+      if (c >= width) continue;
+      float v[V];
+      load_f32<T, V>(g + c, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[k][e] *= act_of(a.act, v[e]);
+    }
+  };
+  auto squares = [&]() {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s = fmaf(t[k][e], t[k][e], s);
+    return s;
+  };
+  if (a.gate != nullptr && a.gate_first) gate();
+  if (a.post_w != nullptr) {
+    if constexpr (GROUPED) {
+      extern __shared__ float s_group[];  // a sum of squares per vector, then 1 / rms per group
+      const int vecs = a.dim / V, per = a.group / V, groups = a.dim / a.group;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) s = fmaf(t[k][e], t[k][e], s);
+        if (k * LT + lt < vecs) s_group[k * LT + lt] = s;
+      }
+      __syncthreads();
+      for (int g = threadIdx.x / kWave; g < groups; g += LT / kWave) {
+        float s = 0.f;
+        for (int v = lane_id(); v < per; v += kWave) s += s_group[g * per + v];
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+        if (lane_id() == 0) s_group[vecs + g] = 1.f / sqrtf(s / (float)a.group + a.eps);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * LT + lt) * V;
+        if (c >= width) continue;
+        const float f = s_group[vecs + c / a.group];
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[k][e] *= f;
+      }
+    } else {
+      const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[k][e] *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LT + lt) * V;
+      if (c >= width) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[k][e] *= a.post_w[c0 + c + e];
+    }
+  }
+  if (a.gate != nullptr && !a.gate_first) gate();
+  const TR* __restrict__ res = a.res == nullptr ? nullptr : static_cast<const TR*>(a.res) + o * a.res_o + i * a.res_i + c0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * LT + lt) * V;
+    if (c >= width) continue;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.f;
+    if (res != nullptr) load_f32<TR, V>(res + c, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float f = a.scale_w != nullptr ? a.scale * a.scale_w[c0 + c + e] : a.scale;
+      t[k][e] = res != nullptr ? fmaf(f, t[k][e], v[e]) : f * t[k][e];
+    }
+    if (a.r != nullptr) store_f32<TR, V>(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0 + c, t[k]);
+  }
+  if (a.pre_w == nullptr) return;
+  const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
+  T* __restrict__ h = static_cast<T*>(a.h) + o * a.h_o + i * a.h_i;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * LT + lt) * V;
+    if (c >= width) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[k][e] *= f * a.pre_w[c0 + c + e];
+    store_f32<T, V>(h + c0 + c, t[k]);
+  }
+}
+
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED>
+int launch_norm_k(const NormArgs& a, int sub, hipStream_t stream) {
+  constexpr int threads = LT > kBlock ? LT : kBlock, rows = threads / LT;
+  const int64_t items = a.outer * a.inner * sub;
+  const size_t lds = GROUPED ? (size_t)(a.dim / V + a.dim / a.group) * sizeof(float) : 0;
+  if (lds > 48 * 1024) {
+    const int rc = set_lds_limit_once<k_block_norm<T, TR, LT, V, NV, GROUPED>>(kMaxLdsBytes - 1024);
+    if (rc != (int)hipSuccess) return rc;
+  }
+  return launch_blocks(a, &NormArgs::item0, (items + rows - 1) / rows, [&](const NormArgs& la, unsigned n) {
+    hipLaunchKernelGGL((k_block_norm<T, TR, LT, V, NV, GROUPED>), dim3(n), dim3(threads), lds, stream, la, sub);
+  });
+}
+
+template <typename T, typename TR, int V, int M>
+int launch_norm_v(const NormArgs& a, hipStream_t stream) {
+  const bool grouped = a.post_w != nullptr && a.group != a.dim;
+  if (grouped && a.pre_w != nullptr) {
+    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true>(a, 1, stream);
+    return launch_norm_k<T, TR, 1024, V, M, true>(a, 1, stream);
+  }
+  const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
+  if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false>(a, sub, stream);
+  if (width <= 64 * V * M) return launch_norm_k<T, TR, 64, V, M, false>(a, sub, stream);
+  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false>(a, sub, stream);
+  return launch_norm_k<T, TR, 1024, V, M, false>(a, sub, stream);
+}
+
+template <typename T, typename TR>
+int launch_norm_t(const NormArgs& a, hipStream_t stream) {
+  constexpr int V = 4;
+  const int64_t strides = a.x_o | a.x_i | a.r_o | a.r_i | a.h_o | a.h_i |
+                          (a.gate != nullptr ? a.g_o | a.g_i : 0) | (a.res != nullptr ? a.res_o | a.res_i : 0);
+  const bool vec = a.dim % V == 0 && a.group % V == 0 && strides % V == 0 && aligned_to(a.x, V * sizeof(T)) &&
+                   aligned_to(a.gate, V * sizeof(T)) && aligned_to(a.h, V * sizeof(T)) &&
+                   aligned_to(a.res, V * sizeof(TR)) && aligned_to(a.r, V * sizeof(TR));
+  return vec ? launch_norm_v<T, TR, V, 4>(a, stream) : launch_norm_v<T, TR, 1, 16>(a, stream);
+}
+
+template <typename T>
+int launch_norm_r(const NormArgs& a, int res_dtype, hipStream_t stream) {
+  if (res_dtype == SF_F32) return launch_norm_t<T, float>(a, stream);
+  return launch_norm_t<T, T>(a, stream);
+}
+
+}  // namespace
+
+int launch_block_norm(const NormArgs& a, int dtype, int res_dtype, hipStream_t stream) {
+  timing_begin(K_NORM, stream);
+  const int rc = dtype == SF_F16    ? launch_norm_r<__half>(a, res_dtype, stream)
+                 : dtype == SF_BF16 ? launch_norm_r<__hip_bfloat16>(a, res_dtype, stream)
+                                    : launch_norm_r<float>(a, res_dtype, stream);
+  timing_end(K_NORM, stream);
+  return rc;
+}
+
+}  // namespace sf
