@@ -492,6 +492,7 @@ typedef struct sf_scan_desc {
   int32_t heads, head_dim, groups, state_dim, dtype, dt_softplus;
 } sf_scan_desc;
 
+/* Dense sequences: max_len = tokens.  The workspace is 16-byte aligned. */
 size_t sf_selective_scan_workspace_size(const sf_scan_desc* desc);
 int sf_selective_scan(const sf_scan_desc* desc, const void* x, const void* dt,
                       const float* A, const void* B, const void* C,
@@ -554,7 +555,8 @@ int sf_conv2d_launch_plan(const sf_conv_desc* desc, int32_t fused_lif,
  * "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3", "lif_multistep",
  * "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
  * "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused",
- * "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm").
+ * "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm",
+ * "scan_chunk", "scan_parts").
  * Returns the
  * number of launches recorded for that kernel. */
 int sf_timing_enable(int32_t enable);

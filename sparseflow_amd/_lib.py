@@ -696,7 +696,7 @@ def block_norm(desc, x: torch.Tensor, gate: Optional[torch.Tensor], post_weight:
 KERNEL_NAMES = ("prescan_pack", "prescan_tiles", "conv_gather", "conv_lif", "conv_rows", "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3",
                 "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
                 "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused", "conv_dense_mfma",
-                "causal_conv1d", "scan_seq", "block_norm")
+                "causal_conv1d", "scan_seq", "block_norm", "scan_chunk", "scan_parts")
 
 
 def timing_enable(on: bool) -> None:

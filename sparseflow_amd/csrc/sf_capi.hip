@@ -256,7 +256,8 @@ const char* g_names[sf::K_COUNT] = {"prescan_pack", "prescan_tiles", "conv_gathe
                                      "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3",
                                      "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse",
                                      "spike_attention", "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma",
-                                     "conv_rows_fused", "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm"};
+                                     "conv_rows_fused", "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm",
+                                     "scan_chunk", "scan_parts"};
 
 }  // namespace
 
@@ -843,9 +844,13 @@ static sf::ScanArgs scan_args(const sf_scan_desc* d, const void* x, const void* 
   return a;
 }
 
+static sf::ScanPlan plan_of(const sf_scan_desc* d) {
+  return sf::scan_plan(d->batch, d->max_len < d->tokens ? d->max_len : d->tokens, d->heads, d->head_dim, d->groups,
+                       d->state_dim, d->dtype);
+}
+
 size_t sf_selective_scan_workspace_size(const sf_scan_desc* d) {
-  (void)d;
-  return 0;
+  return check_scan(d, false) == SF_OK ? plan_of(d).bytes : 0;
 }
 
 int sf_selective_scan(const sf_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
@@ -857,11 +862,13 @@ int sf_selective_scan(const sf_scan_desc* d, const void* x, const void* dt, cons
   if (d->batch == 0) return SF_OK;
   if (A == nullptr || (d->tokens > 0 && (x == nullptr || dt == nullptr || B == nullptr || C == nullptr || y == nullptr)))
     return fail(SF_ERR_INVALID, "NULL pointer");
-  const size_t need = sf_selective_scan_workspace_size(d);
-  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return fail(SF_ERR_WORKSPACE, "workspace too small");
+  const sf::ScanPlan plan = plan_of(d);
+  if (workspace_bytes < plan.bytes || (plan.bytes > 0 && workspace == nullptr))
+    return fail(SF_ERR_WORKSPACE, "workspace too small");
   const sf::ScanArgs a =
       scan_args(d, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, y, final_state, false);
-  const int e = sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
+  const int e = plan.chunked ? sf::launch_scan_chunk(a, plan, workspace, d->dtype, static_cast<hipStream_t>(stream))
+                             : sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "selective_scan launch");
   return SF_OK;
 }

@@ -312,6 +312,25 @@ struct ScanArgs {
 constexpr int kScanMaxState = 256;
 int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);
 
+// Prompts chunk by chunk: how the work is cut.
+constexpr int kScanChunkFrom = 24;  // longest sequence from which chunks are used
+struct ScanSplit {
+  float* parts;  // [batch, segments, heads, head_dim, state_dim]
+  float* sums;   // [batch, segments, heads] exponents
+  int segments;  // of the token axis
+  int chunks;    // of a segment
+  int blocks;    // workgroups per (sequence, segment, group)
+};
+struct ScanPlan {
+  ScanSplit split;
+  bool chunked;
+  int waves;       // per workgroup
+  size_t sums_at;  // bytes into the workspace
+  size_t bytes;    // of workspace
+};
+ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype);
+int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int dtype, hipStream_t stream);
+
 struct NormArgs {
   const void* x;
   const void* gate;
@@ -353,7 +372,7 @@ void conv_geometry(ConvArgs& a, bool lif);
 // Per-kernel event timing hooks used by the launchers.
 void timing_begin(int kernel_id, hipStream_t stream);
 void timing_end(int kernel_id, hipStream_t stream);
-enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_CONV1D = 20, K_SCAN_SEQ = 21, K_NORM = 22, K_COUNT = 23 };
+enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_CONV1D = 20, K_SCAN_SEQ = 21, K_NORM = 22, K_SCAN_CHUNK = 23, K_SCAN_PARTS = 24, K_COUNT = 25 };
 
 // ---------------------------------------------------------------------------
 // Device helpers.
