@@ -867,8 +867,9 @@ int sf_selective_scan(const sf_scan_desc* d, const void* x, const void* dt, cons
     return fail(SF_ERR_WORKSPACE, "workspace too small");
   const sf::ScanArgs a =
       scan_args(d, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, y, final_state, false);
-  const int e = plan.chunked ? sf::launch_scan_chunk(a, plan, workspace, d->dtype, static_cast<hipStream_t>(stream))
-                             : sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
+  const int e = plan.chunked && sf::scan_chunk_takes(a)
+                    ? sf::launch_scan_chunk(a, plan, workspace, d->dtype, static_cast<hipStream_t>(stream))
+                    : sf::launch_scan_seq(a, d->dtype, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "selective_scan launch");
   return SF_OK;
 }

@@ -324,11 +324,11 @@ struct ScanSplit {
 struct ScanPlan {
   ScanSplit split;
   bool chunked;
-  int waves;       // per workgroup
   size_t sums_at;  // bytes into the workspace
   size_t bytes;    // of workspace
 };
 ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype);
+bool scan_chunk_takes(const ScanArgs& a);  // its token strides are within the kernel's range
 int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int dtype, hipStream_t stream);
 
 struct NormArgs {

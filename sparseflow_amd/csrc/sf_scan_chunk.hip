@@ -29,45 +29,63 @@
 #include "sf_seq.h"
 #include "sf_tile.h"
 
+#include <type_traits>
+
 namespace sf {
 
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSlice = 32;   // columns of x of a wavefront
-constexpr int kMaxWaves = 4;
+constexpr int kSlice = 32;  // columns of x of a wavefront
+constexpr int kWaves = 4;   // of a workgroup
+constexpr int kThreads = kWaves * kWave;
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 // ---- the two kinds of products ------------------------------------------------
 // A fragment is a lane's 8 values of a 16-deep slice of an operand: depths
 // 4 half + {0, 1, 2, 3} and 8 + 4 half + {0, 1, 2, 3}, half = lane / 32.
 
 struct MathBf16 {
-  typedef uint16_t E;      // as in LDS
-  typedef bf16x8 Frag;
+  typedef uint16_t E;  // as in LDS
+  typedef u32x4 Frag;  // pairs of bf16
   static constexpr int Q = 64;
   static constexpr int kUnit = 8;  // elements of 16 bytes
-  static constexpr int kXStride = 40;
   static constexpr int kPlanes = 3;
   static constexpr bool kPair = false;  // L as one float in the chunk
 
-  // Row of the 16-byte unit u of token j's row: spread so that neither a read
-  // of one unit of 16 rows nor a transposed one of two units of 4 rows meets a
-  // bank twice.
+  // Place of 16-byte unit u in token j's row: spread so that neither a read of
+  // one unit of 16 rows nor a transposed one of two units of 4 rows meets a bank
+  // twice.
   template <int NP>
   static __device__ __forceinline__ int unit(int j, int u) {
     if constexpr (NP >= 128) return u ^ ((2 * (j & 7)) | ((j >> 3) & 1));
     else if constexpr (NP == 64) return u ^ ((2 * ((j >> 1) & 3)) | ((j >> 3) & 1));
     else return u ^ ((2 * ((j >> 2) & 1)) | ((j >> 3) & 1));
   }
-  // Tokens as lanes: row j of tile m [.][NP], depths from n0 = 16 k.
+  static __device__ __forceinline__ Frag join(bf16x4 lo, bf16x4 hi) {
+    return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // Tokens as lanes: token j's row of tile m [.][NP], depths from 16 k (place:
+  // where its first ones are; the others differ in single bits of it).
   template <int NP>
-  static __device__ __forceinline__ Frag row(const E* m, int j, int k, int half) {
-    const bf16x4 lo = *reinterpret_cast<const bf16x4*>(m + j * NP + unit<NP>(j, 2 * k) * 8 + 4 * half);
-    const bf16x4 hi = *reinterpret_cast<const bf16x4*>(m + j * NP + unit<NP>(j, 2 * k + 1) * 8 + 4 * half);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  static __device__ __forceinline__ int row_place(int j, int half) {
+    return j * NP + unit<NP>(j, 0) * 8 + 4 * half;
+  }
+  static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
+    return join(*reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k))),
+                *reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k + 8))));
   }
   // Tokens as depth: columns n0 + lane % 32 of tile m, tokens from 16 k.  Four
   // lanes point at a token's 16 columns, and lane l of each 16 gets column l of
@@ -77,57 +95,63 @@ struct MathBf16 {
     return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<E*>(p)));
   }
   template <int NP>
-  static __device__ __forceinline__ Frag col(const E* m, int n0, int k, int lane) {
-    const int half = lane >> 5, s = lane & 15, n = n0 + (lane & 16) + 4 * (s & 3);
-    const int j = 16 * k + 4 * half + (s >> 2);
-    const bf16x4 lo = transposed(m + j * NP + unit<NP>(j, n >> 3) * 8 + (n & 7));
-    const bf16x4 hi = transposed(m + (j + 8) * NP + unit<NP>(j + 8, n >> 3) * 8 + (n & 7));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  static __device__ __forceinline__ int col_place(int lane) {
+    const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3), j = 4 * half + (s >> 2);
+    return j * NP + unit<NP>(j, n >> 3) * 8 + (n & 7);
+  }
+  template <int NP>
+  static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
+    return join(transposed(m + (place ^ (32 * nt)) + 16 * k * NP), transposed(m + (place ^ (32 * nt + 8)) + (16 * k + 8) * NP));
+  }
+  // The same of a slice of x, rows of 64 bytes: 4 rows are read at once transposed,
+  // 16 as rows.
+  static __device__ __forceinline__ int xat(int j, int c) {
+    return j * kSlice + ((c >> 3) ^ ((j >> 2) & 3)) * 8 + (c & 7);
   }
   static __device__ __forceinline__ Frag xcol(const E* x, int k, int lane) {
     const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3);
     const int j = 16 * k + 4 * half + (s >> 2);
-    const bf16x4 lo = transposed(x + j * kXStride + n);
-    const bf16x4 hi = transposed(x + (j + 8) * kXStride + n);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return join(transposed(x + xat(j, n)), transposed(x + xat(j + 8, n)));
   }
   static __device__ __forceinline__ Frag of(const float (&v)[8]) {
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (__bf16)v[e];
+    for (int i = 0; i < 4; ++i) f[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
     return f;
   }
-  static __device__ __forceinline__ float get(const Frag& f, int e) { return (float)f[e]; }
+  static __device__ __forceinline__ float get(const Frag& f, int e) {
+    return e % 2 == 0 ? low_bf16(f[e / 2]) : high_bf16(f[e / 2]);
+  }
   static __device__ __forceinline__ bool finite(const Frag (&x)[Q / 16]) {
-    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-    u16x8 most = {};
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
 #pragma unroll
     for (int k = 0; k < Q / 16; ++k)
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8, x[k]) & (uint16_t)0x7fff);
-    bool ok = true;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ok = ok && most[e] < 0x7f80;
-    return ok;
+      for (int i = 0; i < 4; ++i)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu));
+    return most[0] < 0x7f80 && most[1] < 0x7f80;
   }
   static __device__ __forceinline__ void four(const E* p, float (&v)[4]) {
-    const bf16x4 q = *reinterpret_cast<const bf16x4*>(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)q[e];
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = low_bf16(q.x), v[1] = high_bf16(q.x), v[2] = low_bf16(q.y), v[3] = high_bf16(q.y);
   }
   // v as a sum of kPlanes fragments.
   static __device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[kPlanes]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float r = v[e];
+    for (int i = 0; i < 4; ++i) {
+      float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
       for (int p = 0; p < kPlanes; ++p) {
-        f[p][e] = (__bf16)r;
-        r -= (float)f[p][e];
+        const uint32_t w = pack_bf16(a, b);
+        f[p][i] = w;
+        a -= low_bf16(w);
+        b -= high_bf16(w);
       }
     }
   }
   static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ E pack(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 };
@@ -139,7 +163,6 @@ struct MathF32 {
   };
   static constexpr int Q = 32;
   static constexpr int kUnit = 4;
-  static constexpr int kXStride = 36;
   static constexpr int kPlanes = 1;
   static constexpr bool kPair = true;
 
@@ -148,30 +171,37 @@ struct MathF32 {
     return u ^ (j & 7);
   }
   template <int NP>
-  static __device__ __forceinline__ Frag row(const E* m, int j, int k, int half) {
+  static __device__ __forceinline__ int row_place(int j, int half) {
+    return j * NP + unit<NP>(j, half) * 4;
+  }
+  static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
     Frag f;
-    const float4 lo = *reinterpret_cast<const float4*>(m + j * NP + unit<NP>(j, 4 * k + half) * 4);
-    const float4 hi = *reinterpret_cast<const float4*>(m + j * NP + unit<NP>(j, 4 * k + 2 + half) * 4);
+    const float4 lo = *reinterpret_cast<const float4*>(m + (place ^ (16 * k)));
+    const float4 hi = *reinterpret_cast<const float4*>(m + (place ^ (16 * k + 8)));
     f.e[0] = lo.x, f.e[1] = lo.y, f.e[2] = lo.z, f.e[3] = lo.w;
     f.e[4] = hi.x, f.e[5] = hi.y, f.e[6] = hi.z, f.e[7] = hi.w;
     return f;
   }
   template <int NP>
-  static __device__ __forceinline__ Frag col(const E* m, int n0, int k, int lane) {
-    const int half = lane >> 5, n = n0 + (lane & 31);
+  static __device__ __forceinline__ int col_place(int lane) {
+    const int half = lane >> 5, n = lane & 31;
+    return 4 * half * NP + (n ^ (16 * half));
+  }
+  template <int NP>
+  static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = 16 * k + 8 * (e >> 2) + 4 * half + (e & 3);
-      f.e[e] = m[j * NP + unit<NP>(j, n >> 2) * 4 + (n & 3)];
-    }
+    for (int e = 0; e < 8; ++e) f.e[e] = m[(place ^ (32 * nt + 4 * (e & 3))) + (16 * k + 8 * (e >> 2) + (e & 3)) * NP];
     return f;
+  }
+  static __device__ __forceinline__ int xat(int j, int c) {
+    return j * kSlice + ((c >> 2) ^ ((j >> 1) & 7)) * 4 + (c & 3);
   }
   static __device__ __forceinline__ Frag xcol(const E* x, int k, int lane) {
     const int half = lane >> 5;
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = x[(16 * k + 8 * (e >> 2) + 4 * half + (e & 3)) * kXStride + (lane & 31)];
+    for (int e = 0; e < 8; ++e) f.e[e] = x[xat(16 * k + 8 * (e >> 2) + 4 * half + (e & 3), lane & 31)];
     return f;
   }
   static __device__ __forceinline__ Frag of(const float (&v)[8]) {
@@ -199,63 +229,117 @@ struct MathF32 {
   static __device__ __forceinline__ E pack(float v) { return v; }
 };
 
-// Per token of a chunk, for one head.
+// Per token of a chunk, for one head (exponents of 2).  M is the L in the middle
+// of the token's 32.
+//            factors apart         a factor per element
+//   w        2^(L_end - L) d       the same
+//   p        2^(L - M)             L
+//   q        2^(M - L) d           d
+//   r        before 32: 2^(L_31 - L) d, from 32 on: 2^(L - L_31); what L loses as one float
 template <int Q>
 struct alignas(16) ChunkScalars {
-  float l[Q];   // L
-  float ll[Q];  // what L loses as one float
-  float d[Q];
-  float w[Q];   // 2^(L_end - L) d
-  float ab[Q];  // tokens before 32: 2^(L_31 - L) d, from 32 on: 2^(L - L_31)
+  float w[Q], p[Q], q[Q], r[Q];
 };
+
+// The sum of v over lanes 0 .. this one.
+__device__ __forceinline__ double wave_sum_up_to(double v) {
+  auto step = [&](auto ctrl, auto rows) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+  };
+  typedef std::integral_constant<int, 0xf> All;
+  step(std::integral_constant<int, 0x111>(), All());  // within rows of 16: from 1, 2, 4 and 8 lanes below
+  step(std::integral_constant<int, 0x112>(), All());
+  step(std::integral_constant<int, 0x114>(), All());
+  step(std::integral_constant<int, 0x118>(), All());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // lane 15 to row 1, 47 to row 3
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // lane 31 to rows 2 and 3
+  return v;
+}
+
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 
 template <typename M, int NP>
 struct ChunkLds {
   static constexpr int tile = M::Q * NP * (int)sizeof(typename M::E);
   static constexpr int tiles = M::Q == 64 ? 3 : 1;  // 32 x 32 tiles of G on and below the diagonal
-  static constexpr int x = M::Q * M::kXStride * (int)sizeof(typename M::E);
+  static constexpr int x = M::Q * kSlice * (int)sizeof(typename M::E);
   static constexpr int wave = x + (int)sizeof(ChunkScalars<M::Q>);
-  static constexpr int bytes(int waves, bool states) {
-    return (states ? tile : 2 * tile + tiles * 4096) + waves * wave;
-  }
+  // B twice (the next chunk's arrives while this one's is read), x and the
+  // scalars of each wavefront, C, G.
+  static constexpr int c = 2 * tile + kWaves * wave, g = c + tile;
+  static constexpr int bytes(bool states) { return states ? c : g + tiles * 4096; }
 };
 
-// kUnit elements of a row into LDS; what lies outside becomes 0.
+// 64 lanes' 16 bytes from base + off (bytes) to LDS at dst and on, lane by lane
+// (lanes that are off leave theirs as it was).  In asm because the compiler would
+// wait for the builtin's loads before the next LDS read of any kind: the caller
+// waits (lds_dma_wait) before the barrier that hands the data over.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 in the clobber list
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, const void* dst) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr_t)dst);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(l) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+
+// kUnit elements of a row into LDS by way of registers; what lies outside becomes 0.
 template <typename T, typename M>
 __device__ __forceinline__ void stage_unit(typename M::E* to, const T* __restrict__ from, int left, bool vec) {
-  float v[M::kUnit];
-  if (vec && left >= M::kUnit) {
-    if constexpr (sizeof(T) == 2 && sizeof(typename M::E) == 2) {
-      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-      return;
+  constexpr int U = M::kUnit;
+  if constexpr (sizeof(T) == 2 && sizeof(typename M::E) == 2) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (vec) {
+      if (left > 0) v = *reinterpret_cast<const uint4*>(from);
     } else {
-      load_f32<T, M::kUnit>(from, v);
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(from);
+      uint32_t e[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) e[i] = i < left ? p[i] : 0u;
+      v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
+    *reinterpret_cast<uint4*>(to) = v;
   } else {
+    float v[U];
 #pragma unroll
-    for (int e = 0; e < M::kUnit; ++e) v[e] = e < left ? to_f32<T>(from[e]) : 0.f;
+    for (int i = 0; i < U; ++i) v[i] = 0.f;
+    if (vec) {
+      if (left > 0) load_f32<T, U>(from, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (i < left) v[i] = to_f32<T>(from[i]);
+    }
+    store_f32<float, U>(reinterpret_cast<float*>(to), v);
   }
-#pragma unroll
-  for (int e = 0; e < M::kUnit; ++e) to[e] = M::pack(v[e]);
 }
 
 // STATES: a segment's own part of the state, from a zero state, to `parts`, with
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
+// vec: rows are whole units, 16 bytes (or what makes 16 bytes in LDS) aligned.
 template <typename T, typename M, int NP, bool STATES>
-__global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chunk(ScanArgs a, ScanSplit sp, bool vec) {
+__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(ScanArgs a, ScanSplit sp, bool vec) {
   typedef typename M::E E;
   typedef typename M::Frag Frag;
   constexpr int Q = M::Q, KB = Q / 16, IT = Q / 32, NT = NP / 32;
   constexpr int U = M::kUnit;
+  constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits, kRounds = Q / kRows;  // of B and C
+  constexpr int kXUnits = kSlice / U, kXRows = kWave / kXUnits, kXRounds = Q / kXRows;
+  constexpr bool kDma = sizeof(T) == sizeof(E);
   typedef ChunkLds<M, NP> Lds;
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int threads = blockDim.x;
   E* s_b = reinterpret_cast<E*>(lds);
-  E* s_c = reinterpret_cast<E*>(lds + Lds::tile);
-  float* s_g = reinterpret_cast<float*>(lds + 2 * Lds::tile);
-  char* s_wave = lds + (STATES ? Lds::tile : 2 * Lds::tile + Lds::tiles * 4096) + wave * Lds::wave;
+  E* s_c = reinterpret_cast<E*>(lds + Lds::c);
+  float* s_g = reinterpret_cast<float*>(lds + Lds::g);
+  char* s_wave = lds + 2 * Lds::tile + wave * Lds::wave;
   E* s_x = reinterpret_cast<E*>(s_wave);
   ChunkScalars<Q>& sc = *reinterpret_cast<ChunkScalars<Q>*>(s_wave + Lds::x);
 
@@ -268,7 +352,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
   const int seg = (int)(item % (STATES ? sp.segments - 1 : sp.segments));
   const int64_t b = item / (STATES ? sp.segments - 1 : sp.segments);
   const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
-  const int unit = ub * (threads / 64) + wave;
+  const int unit = ub * kWaves + wave;
   const bool on = unit < per_group * slices;
   const int hd = g * per_group + (on ? unit / slices : 0);
   const int p0 = on ? unit % slices * kSlice : 0;
@@ -278,11 +362,13 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
   const int64_t per_seg = (int64_t)sp.chunks * Q;
   int64_t t0 = seg * per_seg, t1 = t0 + per_seg;
   if (t1 > n || (!STATES && seg == sp.segments - 1)) t1 = n;
-  const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + first * a.x_t + hd * a.x_h + p0;
-  const T* __restrict__ dt = static_cast<const T*>(a.dt) + b * a.dt_b + first * a.dt_t + hd * a.dt_h;
-  const T* __restrict__ B = static_cast<const T*>(a.b) + b * a.b_b + first * a.b_t + g * a.b_g;
-  const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + first * a.c_t + g * a.c_g;
-  T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + first * a.y_t + hd * a.y_h + p0;
+  // (The launcher takes token strides below 2^24 only.)
+  const int x_t = (int)a.x_t, dt_t = (int)a.dt_t, b_t = (int)a.b_t, c_t = (int)a.c_t, y_t = (int)a.y_t;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + (first + t0) * a.x_t + hd * a.x_h + p0;
+  const T* __restrict__ dt = static_cast<const T*>(a.dt) + b * a.dt_b + (first + t0) * a.dt_t + hd * a.dt_h;
+  const T* __restrict__ B = static_cast<const T*>(a.b) + b * a.b_b + (first + t0) * a.b_t + g * a.b_g;
+  const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + (first + t0) * a.c_t + g * a.c_g;
+  T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + (first + t0) * a.y_t + hd * a.y_h + p0;
   const int64_t slot = seq_slot(a.seq, b);
   const float D = a.D != nullptr ? a.D[hd] : 0.f, bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.f;
   const double A2 = (double)a.A[hd] * 1.4426950408889634;  // exponents of 2
@@ -327,76 +413,128 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
   }
   double l_seg = 0.0;
 
-  for (int64_t t = t0; t < t1; t += Q) {
-    const int len = (int)(t1 - t < Q ? t1 - t : Q);
-    // ---- B, C (all wavefronts) and x, L (this one) into LDS ----
-    for (int i = threadIdx.x; i < Q * (NP / U); i += threads) {
-      const int j = i / (NP / U), u = i % (NP / U);
-      const int left = j < len ? N - u * U : 0;
-      stage_unit<T, M>(s_b + j * NP + M::template unit<NP>(j, u) * U, B + (t + j) * a.b_t + u * U, left, vec);
-      if constexpr (!STATES)
-        stage_unit<T, M>(s_c + j * NP + M::template unit<NP>(j, u) * U, C + (t + j) * a.c_t + u * U, left, vec);
+  // A whole chunk of aligned rows goes from memory to LDS while the chunk before
+  // it is worked on: B to its other buffer, C and x once their readers are done.
+  // Other chunks are staged by way of registers when their turn comes.
+  const int bj = threadIdx.x / kRowUnits, bv = threadIdx.x % kRowUnits;
+  const int xj = lane / kXUnits, xv = lane % kXUnits;
+  auto ahead = [&](int64_t rest) { return kDma && vec && rest >= Q; };
+  auto load_rows = [&](const T* base, int stride, E* to) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int u = M::template unit<NP>(r * kRows + bj, bv);
+      if (u * U < N)
+        load_to_lds(base + (int64_t)(r * kRows) * stride, (uint32_t)(bj * stride + u * U) * (uint32_t)sizeof(T),
+                    to + (r * kThreads + wave * kWave) * U);
     }
-    for (int i = lane; i < Q * (kSlice / U); i += kWave) {
-      const int j = i / (kSlice / U), u = i % (kSlice / U);
-      stage_unit<T, M>(s_x + j * M::kXStride + u * U, x + (t + j) * a.x_t + u * U, j < len && on ? P - p0 - u * U : 0, vec);
+  };
+  auto load_x = [&]() {
+    if (!on) return;
+#pragma unroll
+    for (int r = 0; r < kXRounds; ++r) {
+      const int u = M::xat(r * kXRows + xj, xv * U) % kSlice / U;
+      if (p0 + u * U < P)
+        load_to_lds(x + (int64_t)(r * kXRows) * x_t, (uint32_t)(xj * x_t + u * U) * (uint32_t)sizeof(T),
+                    s_x + r * kWave * U);
     }
-    float decay;  // 2^L_end
-    float my_l[IT], my_ll[IT], my_e[IT], my_alpha = 0.f;  // of the tokens col, 32 + col
+  };
+  auto stage_rows = [&](const T* base, int stride, E* to, int len) {
+    for (int r = 0; r < kRounds; ++r) {
+      const int j = r * kRows + bj;
+      stage_unit<T, M>(to + j * NP + M::template unit<NP>(j, bv) * U, base + ((int64_t)j * stride + bv * U),
+                       j < len ? N - bv * U : 0, vec);
+    }
+  };
+  int64_t left = t1 - t0;  // tokens from this chunk on
+  for (int i = threadIdx.x * 4; i < Lds::bytes(STATES) / 4; i += kThreads * 4)
+    store_f32<float, 4>(reinterpret_cast<float*>(lds) + i, {0.f, 0.f, 0.f, 0.f});
+  __syncthreads();
+  T ndt = from_f32<T>(0.f);
+  if (lane < left && lane < Q) ndt = dt[lane * dt_t];
+  if (ahead(left)) {
+    load_rows(B, b_t, s_b);
+    if constexpr (!STATES) load_rows(C, c_t, s_c);
+    load_x();
+  }
+
+  for (; left > 0; left -= Q) {
+    const int len = (int)(left < Q ? left : Q);
+    if (!ahead(left)) {
+      stage_rows(B, b_t, s_b, len);
+      if constexpr (!STATES) stage_rows(C, c_t, s_c, len);
+      for (int r = 0; r < kXRounds; ++r) {
+        const int j = r * kXRows + xj;
+        stage_unit<T, M>(s_x + M::xat(j, xv * U), x + ((int64_t)j * x_t + xv * U),
+                         on && j < len ? P - p0 - xv * U : 0, vec);
+      }
+    }
+    float decay;        // 2^L_end
+    float e_mid[2] = {0.f, 0.f};  // 2^M
+    bool wide = M::kPair;  // a factor per element: L moves far within 32 tokens, or as precise as float32 is
     {
       float d = 0.f;
       if (lane < len) {
-        d = to_f32<T>(dt[(t + lane) * a.dt_t]) + bias;
+        d = to_f32<T>(ndt) + bias;
         if (a.softplus) d = softplus(d);
       }
-      double l = lane < len ? A2 * (double)d : 0.0;
-#pragma unroll
-      for (int off = 1; off < Q; off <<= 1) {
-        const double v = __shfl_up(l, off, kWave);
-        if (lane >= off) l += v;
-      }
-      const double end = __shfl(l, Q - 1, kWave);
-      decay = exp2f((float)end);
+      const double l = wave_sum_up_to(lane < len ? A2 * (double)d : 0.0);
+      const double end = lane_of(l, Q - 1);
+      decay = exp2_hw((float)end);
       l_seg += end;
-      const float lf = (float)l, lr = (float)(l - (double)lf);
+      const float w = exp2_hw((float)(end - l)) * d;
+      float p = (float)l, q = d, r = (float)(l - (double)p);
+      if constexpr (!STATES && !M::kPair) {
+        const double mid = lane_of(l, 31), m0 = lane_of(l, 15), m1 = lane_of(l, 47);
+        const float off = (float)(l - (lane < 32 ? m0 : m1));
+        wide = __ballot(!(fabsf(off) < 100.f)) != 0ull;
+        if (!wide) {
+          p = exp2_hw(off);
+          q = exp2_hw(-off) * d;
+          r = lane < 32 ? exp2_hw((float)(mid - l)) * d : exp2_hw((float)(l - mid));
+          e_mid[0] = exp2_hw((float)m0);
+          e_mid[1] = exp2_hw((float)m1);
+        }
+      }
       if (lane < Q) {
-        sc.l[lane] = lf;
-        if constexpr (M::kPair) sc.ll[lane] = lr;
-        sc.d[lane] = d;
-        sc.w[lane] = exp2f((float)(end - l)) * d;
-      }
-      if constexpr (IT == 2 && !STATES) {
-        const double mid = __shfl(l, 31, kWave);
-        sc.ab[lane] = lane < 32 ? exp2f((float)(mid - l)) * d : exp2f((float)(l - mid));
-      }
-      if constexpr (!STATES) {
-#pragma unroll
-        for (int it = 0; it < IT; ++it) {
-          my_l[it] = __shfl(lf, 32 * it + col, kWave);
-          my_ll[it] = __shfl(lr, 32 * it + col, kWave);
-          my_e[it] = exp2f(my_l[it]);
+        sc.w[lane] = w;
+        if constexpr (!STATES) {
+          sc.p[lane] = p;
+          sc.q[lane] = q;
+          sc.r[lane] = r;
         }
       }
     }
+    // The steps to the next chunk.
+    B += (int64_t)Q * b_t;
+    C += (int64_t)Q * c_t;
+    x += (int64_t)Q * x_t;
+    dt += (int64_t)Q * dt_t;
+    lds_dma_wait();
     __syncthreads();
-    if constexpr (IT == 2 && !STATES) my_alpha = sc.ab[32 + col];
+    E* s_next = reinterpret_cast<E*>(lds + Lds::tile - (reinterpret_cast<char*>(s_b) - lds));
+    if (lane < left - Q && lane < Q) ndt = dt[lane * dt_t];
+    if (ahead(left - Q)) load_rows(B, b_t, s_next);
     Frag xf[KB];
 #pragma unroll
     for (int k = 0; k < KB; ++k) xf[k] = M::xcol(s_x, k, lane);
+    // (Opaque: the places of single reads are made from these when they are read,
+    // not kept in registers from chunk to chunk.)
+    int row_at = M::template row_place<NP>(col, half), col_at = M::template col_place<NP>(lane);
+    asm volatile("" : "+v"(row_at), "+v"(col_at));
 
     if constexpr (!STATES) {
       // ---- G = B C^T: lane = token i of C, registers = tokens j of B ----
-      for (int tile = wave; tile < Lds::tiles; tile += threads / 64) {
-        const int it = tile == 0 ? 0 : 1, jt = tile == 2 ? 1 : 0;  // (0, 0), (1, 0), (1, 1)
+      if (wave < Lds::tiles) {
+        const int it = wave == 0 ? 0 : 1, jt = wave == 2 ? 1 : 0;  // (0, 0), (1, 0), (1, 1)
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
         for (int k = 0; k < NP / 16; ++k)
-          acc = M::mma(M::template row<NP>(s_b, 32 * jt + col, k, half), M::template row<NP>(s_c, 32 * it + col, k, half), acc);
+          acc = M::mma(M::row(s_b + 32 * jt * NP, row_at, k), M::row(s_c + 32 * it * NP, row_at, k), acc);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(s_g + ((tile * 4 + q) * 64 + lane) * 4) =
+          *reinterpret_cast<float4*>(s_g + ((wave * 4 + q) * 64 + lane) * 4) =
               make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
       }
       // ---- 2^L_i h C_i^T + D x: lane = token i, registers = columns p ----
@@ -412,52 +550,67 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
         for (int e = 0; e < 8; ++e) hv[e] = h[k / 2][8 * (k % 2) + e];
         const Frag hf = M::of(hv);
 #pragma unroll
-        for (int it = 0; it < IT; ++it) acc[it] = M::mma(hf, M::template row<NP>(s_c, 32 * it + col, k, half), acc[it]);
+        for (int it = 0; it < IT; ++it) acc[it] = M::mma(hf, M::row(s_c + 32 * it * NP, row_at, k), acc[it]);
       }
+      float my_p[IT], my_r[IT];
 #pragma unroll
-      for (int it = 0; it < IT; ++it)
+      for (int it = 0; it < IT; ++it) {
+        my_p[it] = sc.p[32 * it + col];
+        my_r[it] = sc.r[32 * it + col];
+        const float my_e = wide ? exp2_hw(my_p[it]) : my_p[it] * e_mid[it];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float xv[4];
-          M::four(s_x + (32 * it + col) * M::kXStride + 8 * q + 4 * half, xv);
+          float xq[4];
+          M::four(s_x + M::xat(32 * it + col, 8 * q + 4 * half), xq);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[it][4 * q + e] = fmaf(acc[it][4 * q + e], my_e[it], D * xv[e]);
+          for (int e = 0; e < 4; ++e) acc[it][4 * q + e] = fmaf(acc[it][4 * q + e], my_e, D * xq[e]);
         }
+      }
       __syncthreads();
+      if (ahead(left - Q)) load_rows(C, c_t, s_c);
 
       // ---- x^T S: S[i][j] = G[i][j] 2^(L_i - L_j) d_j for j <= i ----
-      if (__ballot(!M::finite(xf)) == 0ull) {
+      // The factor for token j (its p, q and r); below: j's 32 tokens are earlier ones.
+      auto factor = [&](auto apart, int it, bool below, float pj, float qj, float rj) {
+        if constexpr (decltype(apart)::value) return below ? my_r[it] * rj : my_p[it] * qj;
+        float delta = my_p[it] - pj;
+        if constexpr (M::kPair) delta += my_r[it] - rj;
+        return exp2_hw(delta) * qj;
+      };
+      int reach = col - 4 * half;  // j <= i as a number of the fragment's place; opaque, so that the
+      asm volatile("" : "+v"(reach));  // comparisons are made here and not kept in registers
+      auto sum_near = [&](auto apart) {
+        constexpr bool kApart = decltype(apart)::value;
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
 #pragma unroll
           for (int k = 0; k < 2 * (it + 1); ++k) {
+            const bool below = k / 2 < it;
             float s[8];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               const int j0 = 16 * k + 8 * q + 4 * half;
-              float gv[4];
+              float gv[4], pv[4] = {0.f, 0.f, 0.f, 0.f}, qv[4] = {0.f, 0.f, 0.f, 0.f}, rv[4] = {0.f, 0.f, 0.f, 0.f};
               load_f32<float, 4>(s_g + (((it + k / 2) * 4 + 2 * (k % 2) + q) * 64 + lane) * 4, gv);
-              if (k / 2 < it) {
-                float bv[4];
-                load_f32<float, 4>(sc.ab + j0, bv);
+              if (!kApart) load_f32<float, 4>(sc.p + j0, pv);
+              if (!kApart || !below) load_f32<float, 4>(sc.q + j0, qv);
+              if (kApart ? below : M::kPair) load_f32<float, 4>(sc.r + j0, rv);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * q + e] = gv[e] * (my_alpha * bv[e]);
-              } else {
-                float lv[4], dv[4], rv[4] = {0.f, 0.f, 0.f, 0.f};
-                load_f32<float, 4>(sc.l + j0, lv);
-                load_f32<float, 4>(sc.d + j0, dv);
-                if constexpr (M::kPair) load_f32<float, 4>(sc.ll + j0, rv);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float delta = my_l[it] - lv[e];
-                  if constexpr (M::kPair) delta += my_ll[it] - rv[e];
-                  const float v = gv[e] * (exp2f(delta) * dv[e]);
-                  s[4 * q + e] = j0 + e <= 32 * it + col ? v : 0.f;
-                }
+              for (int e = 0; e < 4; ++e) {
+                const float v = gv[e] * factor(apart, it, below, pv[e], qv[e], rv[e]);
+                s[4 * q + e] = below || 16 * (k % 2) + 8 * q + e <= reach ? v : 0.f;
               }
             }
             acc[it] = M::mma(xf[k], M::of(s), acc[it]);
           }
+        }
+      };
+      if (__ballot(!M::finite(xf)) == 0ull) {
+        if constexpr (M::kPair) {
+          sum_near(std::false_type());
+        } else {
+          if (wide) sum_near(std::false_type());
+          else sum_near(std::true_type());
         }
       } else {
         // An x that is not finite must not meet the zeros of S: its terms one by one.
@@ -466,16 +619,15 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
           for (int j = 0; j < 32 * (it + 1); ++j) {
             const int tile = it + j / 32, jj = j % 32;
             const float gv = s_g[((tile * 4 + jj / 8) * 64 + col + 32 * ((jj / 4) % 2)) * 4 + jj % 4];
-            float delta = my_l[it] - sc.l[j];
-            if constexpr (M::kPair) delta += my_ll[it] - sc.ll[j];
-            const float s = gv * (exp2f(delta) * sc.d[j]);
+            const float s = gv * (wide ? factor(std::false_type(), it, j / 32 < it, sc.p[j], sc.q[j], sc.r[j])
+                                       : factor(std::true_type(), it, j / 32 < it, sc.p[j], sc.q[j], sc.r[j]));
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              float xv[4];
-              M::four(s_x + j * M::kXStride + 8 * q + 4 * half, xv);
+              float xq[4];
+              M::four(s_x + M::xat(j, 8 * q + 4 * half), xq);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                acc[it][4 * q + e] = j <= 32 * it + col ? fmaf(s, xv[e], acc[it][4 * q + e]) : acc[it][4 * q + e];
+                acc[it][4 * q + e] = j <= 32 * it + col ? fmaf(s, xq[e], acc[it][4 * q + e]) : acc[it][4 * q + e];
             }
           }
         }
@@ -483,21 +635,23 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
         if (!on || 32 * it + col >= len) continue;
-        T* row = y + (t + 32 * it + col) * a.y_t;
+        T* row = y + (int64_t)(32 * it) * y_t + (col * y_t + 4 * half);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int c = 8 * q + 4 * half;
+          const int c = p0 + 8 * q + 4 * half;
           const float v[4] = {acc[it][4 * q], acc[it][4 * q + 1], acc[it][4 * q + 2], acc[it][4 * q + 3]};
-          if (vec && p0 + c + 4 <= P) {
-            store_f32<T, 4>(row + c, v);
+          if (vec) {
+            if (c < P) store_f32<T, 4>(row + 8 * q, v);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (p0 + c + e < P) row[c + e] = from_f32<T>(v[e]);
+              if (c + e < P) row[8 * q + e] = from_f32<T>(v[e]);
           }
         }
       }
+      y += (int64_t)Q * y_t;
     }
+    if (ahead(left - Q)) load_x();
 
     // ---- h <- 2^L_end h + B^T v ----
 #pragma unroll
@@ -509,8 +663,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
       float v[8];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const float4 wq = *reinterpret_cast<const float4*>(sc.w + 16 * k + 8 * q + 4 * half);
-        const float wv[4] = {wq.x, wq.y, wq.z, wq.w};
+        float wv[4];
+        load_f32<float, 4>(sc.w + 16 * k + 8 * q + 4 * half, wv);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * q + e] = M::get(xf[k], 4 * q + e) * wv[e];
       }
@@ -518,12 +672,12 @@ __global__ __launch_bounds__(64 * kMaxWaves, NP == 256 ? 1 : 2) void k_scan_chun
       M::split(v, vf);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const Frag bt = M::template col<NP>(s_b, 32 * nt, k, lane);
+        const Frag bt = M::template col<NP>(s_b, col_at, nt, k);
 #pragma unroll
         for (int pl = 0; pl < M::kPlanes; ++pl) h[nt] = M::mma(bt, vf[pl], h[nt]);
       }
     }
-    __syncthreads();
+    s_b = s_next;
   }
 
   if (to != nullptr && mine) {
@@ -569,27 +723,25 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
 }
 
 template <typename T, typename M, int NP, bool STATES>
-int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, int waves, hipStream_t stream) {
+int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   typedef ChunkLds<M, NP> Lds;
   const int rc = set_lds_limit_once<k_scan_chunk<T, M, NP, STATES>>(kMaxLdsBytes);
   if (rc != (int)hipSuccess) return rc;
   constexpr int U = M::kUnit;
-  // kUnit elements of a row at a time (y: four).
   const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g | a.y_b | a.y_t | a.y_h;
-  const bool vec = strides % U == 0 && aligned_to(a.x, U * sizeof(T)) && aligned_to(a.b, U * sizeof(T)) &&
-                   aligned_to(a.c, U * sizeof(T)) && aligned_to(a.y, 4 * sizeof(T));
+  const bool vec = strides % U == 0 && a.head_dim % U == 0 && a.state_dim % U == 0 && aligned_to(a.x, U * sizeof(T)) &&
+                   aligned_to(a.b, U * sizeof(T)) && aligned_to(a.c, U * sizeof(T)) && aligned_to(a.y, U * sizeof(T));
   const int64_t blocks = a.seq.batch * (STATES ? sp.segments - 1 : sp.segments) * a.groups * sp.blocks;
   return launch_blocks(a, &ScanArgs::block0, blocks, [&](const ScanArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_scan_chunk<T, M, NP, STATES>), dim3(n), dim3(64 * waves), Lds::bytes(waves, STATES), stream, la,
-                       sp, vec);
+    hipLaunchKernelGGL((k_scan_chunk<T, M, NP, STATES>), dim3(n), dim3(kThreads), Lds::bytes(STATES), stream, la, sp, vec);
   });
 }
 
 template <typename T, typename M, int NP>
-int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, int waves, hipStream_t stream) {
+int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   if (sp.segments > 1) {
     timing_begin(K_SCAN_PARTS, stream);
-    int rc = launch_chunk_k<T, M, NP, true>(a, sp, waves, stream);
+    int rc = launch_chunk_k<T, M, NP, true>(a, sp, stream);
     if (rc == (int)hipSuccess) {
       const int64_t plane = (int64_t)a.head_dim * a.state_dim;
       const int64_t blocks = (plane + kChainThreads - 1) / kChainThreads;
@@ -601,17 +753,17 @@ int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, int waves, hipStream_
     if (rc != (int)hipSuccess) return rc;
   }
   timing_begin(K_SCAN_CHUNK, stream);
-  const int rc = launch_chunk_k<T, M, NP, false>(a, sp, waves, stream);
+  const int rc = launch_chunk_k<T, M, NP, false>(a, sp, stream);
   timing_end(K_SCAN_CHUNK, stream);
   return rc;
 }
 
 template <typename T, typename M>
-int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, int waves, hipStream_t stream) {
-  if (a.state_dim <= 32) return launch_chunk_n<T, M, 32>(a, sp, waves, stream);
-  if (a.state_dim <= 64) return launch_chunk_n<T, M, 64>(a, sp, waves, stream);
-  if (a.state_dim <= 128) return launch_chunk_n<T, M, 128>(a, sp, waves, stream);
-  return launch_chunk_n<T, M, 256>(a, sp, waves, stream);
+int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
+  if (a.state_dim <= 32) return launch_chunk_n<T, M, 32>(a, sp, stream);
+  if (a.state_dim <= 64) return launch_chunk_n<T, M, 64>(a, sp, stream);
+  if (a.state_dim <= 128) return launch_chunk_n<T, M, 128>(a, sp, stream);
+  return launch_chunk_n<T, M, 256>(a, sp, stream);
 }
 
 size_t align16(size_t v) { return (v + 15) / 16 * 16; }
@@ -625,8 +777,7 @@ ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int 
   if (!p.chunked || batch < 1) return p;
   const int q = dtype == SF_BF16 ? MathBf16::Q : MathF32::Q;
   const int units = heads / groups * ((head_dim + kSlice - 1) / kSlice);
-  p.waves = units >= 3 ? 4 : units;
-  p.split.blocks = (units + p.waves - 1) / p.waves;
+  p.split.blocks = (units + kWaves - 1) / kWaves;
   // Segments: enough workgroups for two on a CU, with at least four chunks each.
   const int64_t chunks = (max_len + q - 1) / q;
   const int64_t base = batch * groups * p.split.blocks;
@@ -644,13 +795,20 @@ ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int 
   return p;
 }
 
+bool scan_chunk_takes(const ScanArgs& a) {
+  const int64_t most = 1 << 24;
+  for (const int64_t s : {a.x_t, a.dt_t, a.b_t, a.c_t, a.y_t})
+    if (s < 0 || s > most) return false;
+  return true;
+}
+
 int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int dtype, hipStream_t stream) {
   ScanSplit sp = p.split;
   sp.parts = static_cast<float*>(workspace);
   sp.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums_at);
-  if (dtype == SF_BF16) return launch_chunk_m<__hip_bfloat16, MathBf16>(a, sp, p.waves, stream);
-  if (dtype == SF_F16) return launch_chunk_m<__half, MathF32>(a, sp, p.waves, stream);
-  return launch_chunk_m<float, MathF32>(a, sp, p.waves, stream);
+  if (dtype == SF_BF16) return launch_chunk_m<__hip_bfloat16, MathBf16>(a, sp, stream);
+  if (dtype == SF_F16) return launch_chunk_m<__half, MathF32>(a, sp, stream);
+  return launch_chunk_m<float, MathF32>(a, sp, stream);
 }
 
 }  // namespace sf

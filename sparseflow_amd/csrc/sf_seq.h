@@ -28,14 +28,15 @@ __device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]
   *reinterpret_cast<Vec<T, V>*>(p) = q;
 }
 
-// Rows [first, first + n) of the token axis that are sequence b's.
+// Rows [first, first + n) of the token axis that are sequence b's (b the same in
+// all lanes).
 __device__ __forceinline__ void seq_rows(const SeqAxis& s, int64_t b, int64_t& first, int64_t& n) {
   if (s.offsets == nullptr) {
     first = 0;
     n = s.tokens;
     return;
   }
-  const int64_t lo = s.offsets[b], hi = s.offsets[b + 1];
+  const int64_t lo = __builtin_amdgcn_readfirstlane(s.offsets[b]), hi = __builtin_amdgcn_readfirstlane(s.offsets[b + 1]);
   first = lo < 0 ? 0 : (lo > s.tokens ? s.tokens : lo);
   const int64_t end = hi > s.tokens ? s.tokens : hi;
   n = end > first ? end - first : 0;
@@ -47,8 +48,34 @@ __device__ __forceinline__ int64_t seq_slot(const SeqAxis& s, int64_t b) {
   return r >= 0 && r < s.states ? r : -1;
 }
 
-// log(1 + exp(v)), from the larger of 0 and v so that neither end overflows.
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
+// 2^v by the hardware's exponential (relative error 2^-23; results below the
+// normal range are 0).
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|), so that neither end
+// overflows and the far negative one keeps its relative accuracy.  e is
+// 2^(hi + lo) with hi + lo = -|v| log2(e) to more than 24 bits, and log1p(e) =
+// 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^15 (the next term is
+// below 2^-29 of the sum).
+__device__ __forceinline__ float softplus(float v) {
+  const float a = -fabsf(v);
+  const float hi = a * 1.44269502f, lo = fmaf(a, 1.44269502f, -hi) + a * 1.92596303e-8f;
+  const float p = exp2_hw(hi);
+  const float e = a < -120.f ? p : fmaf(p * 0.693147182f, lo, p);  // (-inf: lo is NaN)
+  const float den = 2.f + e;
+  float r = __builtin_amdgcn_rcpf(den);
+  r = fmaf(fmaf(-den, r, 1.f), r, r);
+  const float s = e * r, q = s * s;
+  float t = 1.f / 15.f;
+  t = fmaf(t, q, 1.f / 13.f);
+  t = fmaf(t, q, 1.f / 11.f);
+  t = fmaf(t, q, 1.f / 9.f);
+  t = fmaf(t, q, 1.f / 7.f);
+  t = fmaf(t, q, 1.f / 5.f);
+  t = fmaf(t, q, 1.f / 3.f);
+  t = fmaf(t * q, s, s);
+  return fmaxf(v, 0.f) + (t + t);
+}
 
 // v * sigmoid(v): 0 at the far negative end (v / inf), NaN where v is.
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
