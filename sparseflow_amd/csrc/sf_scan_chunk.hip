@@ -36,12 +36,14 @@ namespace sf {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kChunk = 32;  // tokens
 constexpr int kSlice = 32;  // columns of x of a wavefront
 constexpr int kWaves = 4;   // of a workgroup
 constexpr int kThreads = kWaves * kWave;
@@ -60,7 +62,6 @@ __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(
 struct MathBf16 {
   typedef uint16_t E;  // as in LDS
   typedef u32x4 Frag;  // pairs of bf16
-  static constexpr int Q = 64;
   static constexpr int kUnit = 8;  // elements of 16 bytes
   static constexpr int kPlanes = 3;
   static constexpr bool kPair = false;  // L as one float in the chunk
@@ -86,6 +87,19 @@ struct MathBf16 {
   static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
     return join(*reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k))),
                 *reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k + 8))));
+  }
+  // A 16 x 16 quadrant of a product of two tiles' rows, tokens ja + lane % 16 of a
+  // with jb + lane % 16 of b: 16 bytes of both for 32 of the depth.
+  template <int NP>
+  static __device__ __forceinline__ f32x4 quadrant(const E* a, const E* b, int lane) {
+    const int j = lane & 15, q = lane >> 4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int place = j * NP + unit<NP>(j, q) * 8;
+#pragma unroll
+    for (int k = 0; k < NP / 32; ++k)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(a + (place ^ (32 * k))),
+                                                    *reinterpret_cast<const bf16x8*>(b + (place ^ (32 * k))), acc, 0, 0, 0);
+    return acc;
   }
   // Tokens as depth: columns n0 + lane % 32 of tile m, tokens from 16 k.  Four
   // lanes point at a token's 16 columns, and lane l of each 16 gets column l of
@@ -122,15 +136,16 @@ struct MathBf16 {
   static __device__ __forceinline__ float get(const Frag& f, int e) {
     return e % 2 == 0 ? low_bf16(f[e / 2]) : high_bf16(f[e / 2]);
   }
-  static __device__ __forceinline__ bool finite(const Frag (&x)[Q / 16]) {
+  static __device__ __forceinline__ bool finite(const Frag (&x)[kChunk / 16]) {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 most = {0, 0};
+    uint32_t most = 0;
 #pragma unroll
-    for (int k = 0; k < Q / 16; ++k)
+    for (int k = 0; k < kChunk / 16; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu));
-    return most[0] < 0x7f80 && most[1] < 0x7f80;
+        most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                      __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu)));
+    return max(most >> 16, most & 0xffffu) < 0x7f80u;
   }
   static __device__ __forceinline__ void four(const E* p, float (&v)[4]) {
     const uint2 q = *reinterpret_cast<const uint2*>(p);
@@ -161,7 +176,6 @@ struct MathF32 {
   struct Frag {
     float e[8];
   };
-  static constexpr int Q = 32;
   static constexpr int kUnit = 4;
   static constexpr int kPlanes = 1;
   static constexpr bool kPair = true;
@@ -181,6 +195,19 @@ struct MathF32 {
     f.e[0] = lo.x, f.e[1] = lo.y, f.e[2] = lo.z, f.e[3] = lo.w;
     f.e[4] = hi.x, f.e[5] = hi.y, f.e[6] = hi.z, f.e[7] = hi.w;
     return f;
+  }
+  template <int NP>
+  static __device__ __forceinline__ f32x4 quadrant(const E* a, const E* b, int lane) {
+    const int j = lane & 15, q = lane >> 4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int place = j * NP + unit<NP>(j, q) * 4;
+#pragma unroll
+    for (int k = 0; k < NP / 16; ++k) {
+      const f32x4 av = *reinterpret_cast<const f32x4*>(a + (place ^ (16 * k))), bv = *reinterpret_cast<const f32x4*>(b + (place ^ (16 * k)));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], bv[e], acc, 0, 0, 0);
+    }
+    return acc;
   }
   template <int NP>
   static __device__ __forceinline__ int col_place(int lane) {
@@ -211,10 +238,10 @@ struct MathF32 {
     return f;
   }
   static __device__ __forceinline__ float get(const Frag& f, int e) { return f.e[e]; }
-  static __device__ __forceinline__ bool finite(const Frag (&x)[Q / 16]) {
+  static __device__ __forceinline__ bool finite(const Frag (&x)[kChunk / 16]) {
     bool ok = true;
 #pragma unroll
-    for (int k = 0; k < Q / 16; ++k)
+    for (int k = 0; k < kChunk / 16; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) ok = ok && fabsf(x[k].e[e]) < __builtin_huge_valf();
     return ok;
@@ -229,20 +256,26 @@ struct MathF32 {
   static __device__ __forceinline__ E pack(float v) { return v; }
 };
 
-// Per token of a chunk, for one head (exponents of 2).  M is the L in the middle
-// of the token's 32.
-//            factors apart         a factor per element
-//   w        2^(L_end - L) d       the same
-//   p        2^(L - M)             L
-//   q        2^(M - L) d           d
-//   r        before 32: 2^(L_31 - L) d, from 32 on: 2^(L - L_31); what L loses as one float
-template <int Q>
+// Per token of a chunk, for one head.  The state in the accumulators is 2^-K h, K
+// kept near 0 (kScaleMost), so that a chunk's decay need not be multiplied in each
+// time; K' is its value after the chunk.
+//            factors apart      a factor per element (wide)
+//   w        2^(L_end - L - K') d, both
+//   p        2^(L + K)          L
+//   q        2^(-L - K) d       d
+//   r                           what L loses as one float
 struct alignas(16) ChunkScalars {
-  float w[Q], p[Q], q[Q], r[Q];
+  float w[kChunk], p[kChunk], q[kChunk], r[kChunk];
+  float k, rescale, wide, pad;  // K; what the state is multiplied by before the chunk's part comes in
 };
+struct HeadSums {
+  double k, l;  // K, and the sum of the exponents so far
+};
+constexpr double kScaleMost = 20.0;
+constexpr float kApartMost = 100.f;  // exponents of factors apart
 
-// The sum of v over lanes 0 .. this one.
-__device__ __forceinline__ double wave_sum_up_to(double v) {
+// The sum of v over this half wavefront's lanes up to this one.
+__device__ __forceinline__ double half_sum_up_to(double v) {
   auto step = [&](auto ctrl, auto rows) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
@@ -255,7 +288,6 @@ __device__ __forceinline__ double wave_sum_up_to(double v) {
   step(std::integral_constant<int, 0x114>(), All());
   step(std::integral_constant<int, 0x118>(), All());
   step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // lane 15 to row 1, 47 to row 3
-  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // lane 31 to rows 2 and 3
   return v;
 }
 
@@ -267,14 +299,16 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
 
 template <typename M, int NP>
 struct ChunkLds {
-  static constexpr int tile = M::Q * NP * (int)sizeof(typename M::E);
-  static constexpr int tiles = M::Q == 64 ? 3 : 1;  // 32 x 32 tiles of G on and below the diagonal
-  static constexpr int x = M::Q * kSlice * (int)sizeof(typename M::E);
-  static constexpr int wave = x + (int)sizeof(ChunkScalars<M::Q>);
-  // B twice (the next chunk's arrives while this one's is read), x and the
-  // scalars of each wavefront, C, G.
-  static constexpr int c = 2 * tile + kWaves * wave, g = c + tile;
-  static constexpr int bytes(bool states) { return states ? c : g + tiles * 4096; }
+  static constexpr int tile = kChunk * NP * (int)sizeof(typename M::E);
+  // B, a slice of x for each wavefront and the scalars of up to as many heads twice
+  // (the next chunk's arrive while this one's are read), C, G.
+  static constexpr int x = 2 * tile;
+  static constexpr int x_bytes = kChunk * kSlice * (int)sizeof(typename M::E);
+  static constexpr int scalars = x + 2 * kWaves * x_bytes;
+  static constexpr int sums = scalars + 2 * kWaves * (int)sizeof(ChunkScalars);
+  static constexpr int c = sums + kWaves * (int)sizeof(HeadSums);
+  static constexpr int g = c + tile;
+  static constexpr int bytes(bool states) { return states ? c : g + kChunk * kChunk * 4; }
 };
 
 // 64 lanes' 16 bytes from base + off (bytes) to LDS at dst and on, lane by lane
@@ -324,12 +358,15 @@ __device__ __forceinline__ void stage_unit(typename M::E* to, const T* __restric
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
 // vec: rows are whole units, 16 bytes (or what makes 16 bytes in LDS) aligned.
 template <typename T, typename M, int NP, bool STATES>
-__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(ScanArgs a, ScanSplit sp, bool vec) {
+__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 4 ? 2 : 3) void k_scan_chunk(ScanArgs a,
+                                                                                                       ScanSplit sp,
+                                                                                                       bool vec) {
   typedef typename M::E E;
   typedef typename M::Frag Frag;
-  constexpr int Q = M::Q, KB = Q / 16, IT = Q / 32, NT = NP / 32;
+  constexpr int Q = kChunk, KB = Q / 16, NT = NP / 32;
   constexpr int U = M::kUnit;
-  constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits, kRounds = Q / kRows;  // of B and C
+  constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits;  // of B and C at a time
+  constexpr int kRounds = Q > kRows ? Q / kRows : 1;
   constexpr int kXUnits = kSlice / U, kXRows = kWave / kXUnits, kXRounds = Q / kXRows;
   constexpr bool kDma = sizeof(T) == sizeof(E);
   typedef ChunkLds<M, NP> Lds;
@@ -339,9 +376,10 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
   E* s_b = reinterpret_cast<E*>(lds);
   E* s_c = reinterpret_cast<E*>(lds + Lds::c);
   float* s_g = reinterpret_cast<float*>(lds + Lds::g);
-  char* s_wave = lds + 2 * Lds::tile + wave * Lds::wave;
-  E* s_x = reinterpret_cast<E*>(s_wave);
-  ChunkScalars<Q>& sc = *reinterpret_cast<ChunkScalars<Q>*>(s_wave + Lds::x);
+  char* const s_x0 = lds + Lds::x + 2 * wave * Lds::x_bytes;
+  E* s_x = reinterpret_cast<E*>(s_x0);
+  ChunkScalars* s_sc = reinterpret_cast<ChunkScalars*>(lds + Lds::scalars);
+  HeadSums* s_sums = reinterpret_cast<HeadSums*>(lds + Lds::sums);
 
   // This workgroup's sequence, segment and group; this wavefront's head and columns.
   int64_t item = a.block0 + blockIdx.x;
@@ -352,9 +390,11 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
   const int seg = (int)(item % (STATES ? sp.segments - 1 : sp.segments));
   const int64_t b = item / (STATES ? sp.segments - 1 : sp.segments);
   const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
+  const int units = per_group * slices, first_head = ub * kWaves / slices;
   const int unit = ub * kWaves + wave;
-  const bool on = unit < per_group * slices;
-  const int hd = g * per_group + (on ? unit / slices : 0);
+  const bool on = unit < units;
+  const int own = on ? unit / slices - first_head : 0;  // the head, of those of this workgroup
+  const int hd = g * per_group + first_head + own;
   const int p0 = on ? unit % slices * kSlice : 0;
   const int P = a.head_dim, N = a.state_dim;
   int64_t first, n;
@@ -365,13 +405,79 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
   // (The launcher takes token strides below 2^24 only.)
   const int x_t = (int)a.x_t, dt_t = (int)a.dt_t, b_t = (int)a.b_t, c_t = (int)a.c_t, y_t = (int)a.y_t;
   const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + (first + t0) * a.x_t + hd * a.x_h + p0;
-  const T* __restrict__ dt = static_cast<const T*>(a.dt) + b * a.dt_b + (first + t0) * a.dt_t + hd * a.dt_h;
   const T* __restrict__ B = static_cast<const T*>(a.b) + b * a.b_b + (first + t0) * a.b_t + g * a.b_g;
   const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + (first + t0) * a.c_t + g * a.c_g;
   T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + (first + t0) * a.y_t + hd * a.y_h + p0;
   const int64_t slot = seq_slot(a.seq, b);
-  const float D = a.D != nullptr ? a.D[hd] : 0.f, bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.f;
-  const double A2 = (double)a.A[hd] * 1.4426950408889634;  // exponents of 2
+  const float D = a.D != nullptr ? a.D[hd] : 0.f;
+
+  // The scalars of two heads at once, one to each half wavefront: by one wavefront
+  // for heads 0 and 1 of the workgroup, by another for 2 and 3, in turns.
+  const int heads = (min(units, (ub + 1) * kWaves) - 1) / slices - first_head + 1;
+  const int turns = heads > 2 ? 2 : 1;
+  // Whether chunk i's scalars are this wavefront's turn, and for which pair of heads (-1: not).
+  auto turn = [&](int i) {
+    const int k = (wave + 2 * kWaves - i % kWaves) % kWaves;  // 0 and 2: in turn for pair 0 and 1
+    return k == 0 ? 0 : k == 2 && turns == 2 ? 1 : -1;
+  };
+  const T* __restrict__ dts = static_cast<const T*>(a.dt) + b * a.dt_b + (first + t0) * a.dt_t;
+  T next_dt = from_f32<T>(0.f);
+  auto load_dt = [&](int i, int pair) {
+    const int hl = 2 * pair + half;
+    const int64_t t = (int64_t)i * Q + col;
+    if (hl < heads && t < t1 - t0)
+      next_dt = dts[t * dt_t + (g * per_group + first_head + hl) * a.dt_h];
+  };
+  auto write_scalars = [&](int i, int pair) {
+    const int hl = 2 * pair + half, hg = g * per_group + first_head + hl;
+    const bool there = hl < heads;
+    ChunkScalars& sc = s_sc[(i & 1) * kWaves + (there ? hl : 0)];
+    float d = 0.f;
+    double l = 0.0, k = 0.0;
+    if (there) {
+      k = s_sums[hl].k;
+      if ((int64_t)i * Q + col < t1 - t0) {
+        d = to_f32<T>(next_dt) + (a.dt_bias != nullptr ? a.dt_bias[hg] : 0.f);
+        if (a.softplus) d = softplus(d);
+        l = (double)a.A[hg] * 1.4426950408889634 * (double)d;  // an exponent of 2
+      }
+    }
+    l = half_sum_up_to(l);
+    const double end0 = lane_of(l, 31), end1 = lane_of(l, 63), end = half == 0 ? end0 : end1;
+    float p = (float)l, q = d, r = (float)(l - (double)p);
+    bool wide = M::kPair;  // a factor per element: L moves far in the chunk, or as precise as float32 is
+    if constexpr (!STATES && !M::kPair) {
+      const float off = (float)(l + k), fall = exp2_hw(-off) * d;
+      // (Also where a factor of a later token is no number: it meets zeros of G.)
+      const uint64_t no = __ballot(!(fabsf(off) < kApartMost && fabsf(fall) < __builtin_huge_valf()));
+      wide = (half == 0 ? (uint32_t)no : (uint32_t)(no >> 32)) != 0u;
+      if (!wide) {
+        p = exp2_hw(off);
+        q = fall;
+      }
+    }
+    double k_new = k + end;
+    float rescale = 1.f;
+    if (!(fabs(k_new) < kScaleMost)) {
+      const double to = end < 0.0 ? kScaleMost : 0.0;
+      rescale = exp2_hw((float)(k_new - to));
+      k_new = to;
+    }
+    if (!there) return;
+    sc.w[col] = exp2_hw((float)(end - l - k_new)) * d;
+    if constexpr (!STATES) {
+      sc.p[col] = p;
+      sc.q[col] = q;
+      if constexpr (M::kPair) sc.r[col] = r;
+    }
+    if (col == 0) {
+      sc.k = (float)k;
+      sc.rescale = rescale;
+      sc.wide = wide ? 1.f : 0.f;
+      s_sums[hl].k = k_new;
+      s_sums[hl].l += end;
+    }
+  };
 
   // The state: register r of tile nt is row p0 + col, column
   // 32 nt + 8 (r / 4) + 4 half + r % 4.
@@ -411,7 +517,6 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
         }
       }
   }
-  double l_seg = 0.0;
 
   // A whole chunk of aligned rows goes from memory to LDS while the chunk before
   // it is worked on: B to its other buffer, C and x once their readers are done.
@@ -419,28 +524,35 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
   const int bj = threadIdx.x / kRowUnits, bv = threadIdx.x % kRowUnits;
   const int xj = lane / kXUnits, xv = lane % kXUnits;
   auto ahead = [&](int64_t rest) { return kDma && vec && rest >= Q; };
+  const bool whole_n = N == NP, whole_p = p0 + kSlice <= P;
   auto load_rows = [&](const T* base, int stride, E* to) {
+    const char* from = reinterpret_cast<const char*>(base);
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int u = M::template unit<NP>(r * kRows + bj, bv);
-      if (u * U < N)
-        load_to_lds(base + (int64_t)(r * kRows) * stride, (uint32_t)(bj * stride + u * U) * (uint32_t)sizeof(T),
-                    to + (r * kThreads + wave * kWave) * U);
+      const uint32_t off = (uint32_t)(bj * stride + u * U) * (uint32_t)sizeof(T);
+      E* dst = to + (r * kThreads + wave * kWave) * U;
+      if (kRows <= Q && whole_n) load_to_lds(from, off, dst);
+      else if (u * U < N && bj < Q) load_to_lds(from, off, dst);
+      from += (uint32_t)(kRows * stride) * (uint32_t)sizeof(T);
     }
   };
-  auto load_x = [&]() {
+  auto load_x = [&](E* to) {
     if (!on) return;
+    const char* from = reinterpret_cast<const char*>(x);
 #pragma unroll
     for (int r = 0; r < kXRounds; ++r) {
       const int u = M::xat(r * kXRows + xj, xv * U) % kSlice / U;
-      if (p0 + u * U < P)
-        load_to_lds(x + (int64_t)(r * kXRows) * x_t, (uint32_t)(xj * x_t + u * U) * (uint32_t)sizeof(T),
-                    s_x + r * kWave * U);
+      const uint32_t off = (uint32_t)(xj * x_t + u * U) * (uint32_t)sizeof(T);
+      if (whole_p) load_to_lds(from, off, to + r * kWave * U);
+      else if (p0 + u * U < P) load_to_lds(from, off, to + r * kWave * U);
+      from += (uint32_t)(kXRows * x_t) * (uint32_t)sizeof(T);
     }
   };
   auto stage_rows = [&](const T* base, int stride, E* to, int len) {
     for (int r = 0; r < kRounds; ++r) {
       const int j = r * kRows + bj;
+      if (j >= Q) break;
       stage_unit<T, M>(to + j * NP + M::template unit<NP>(j, bv) * U, base + ((int64_t)j * stride + bv * U),
                        j < len ? N - bv * U : 0, vec);
     }
@@ -449,15 +561,18 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
   for (int i = threadIdx.x * 4; i < Lds::bytes(STATES) / 4; i += kThreads * 4)
     store_f32<float, 4>(reinterpret_cast<float*>(lds) + i, {0.f, 0.f, 0.f, 0.f});
   __syncthreads();
-  T ndt = from_f32<T>(0.f);
-  if (lane < left && lane < Q) ndt = dt[lane * dt_t];
   if (ahead(left)) {
     load_rows(B, b_t, s_b);
     if constexpr (!STATES) load_rows(C, c_t, s_c);
-    load_x();
+    load_x(s_x);
   }
+  if (left > 0 && turn(0) >= 0) {
+    load_dt(0, turn(0));
+    write_scalars(0, turn(0));
+  }
+  if (left > Q && turn(1) >= 0) load_dt(1, turn(1));
 
-  for (; left > 0; left -= Q) {
+  for (int i = 0; left > 0; left -= Q, ++i) {
     const int len = (int)(left < Q ? left : Q);
     if (!ahead(left)) {
       stage_rows(B, b_t, s_b, len);
@@ -468,52 +583,22 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
                          on && j < len ? P - p0 - xv * U : 0, vec);
       }
     }
-    float decay;        // 2^L_end
-    float e_mid[2] = {0.f, 0.f};  // 2^M
-    bool wide = M::kPair;  // a factor per element: L moves far within 32 tokens, or as precise as float32 is
-    {
-      float d = 0.f;
-      if (lane < len) {
-        d = to_f32<T>(ndt) + bias;
-        if (a.softplus) d = softplus(d);
-      }
-      const double l = wave_sum_up_to(lane < len ? A2 * (double)d : 0.0);
-      const double end = lane_of(l, Q - 1);
-      decay = exp2_hw((float)end);
-      l_seg += end;
-      const float w = exp2_hw((float)(end - l)) * d;
-      float p = (float)l, q = d, r = (float)(l - (double)p);
-      if constexpr (!STATES && !M::kPair) {
-        const double mid = lane_of(l, 31), m0 = lane_of(l, 15), m1 = lane_of(l, 47);
-        const float off = (float)(l - (lane < 32 ? m0 : m1));
-        wide = __ballot(!(fabsf(off) < 100.f)) != 0ull;
-        if (!wide) {
-          p = exp2_hw(off);
-          q = exp2_hw(-off) * d;
-          r = lane < 32 ? exp2_hw((float)(mid - l)) * d : exp2_hw((float)(l - mid));
-          e_mid[0] = exp2_hw((float)m0);
-          e_mid[1] = exp2_hw((float)m1);
-        }
-      }
-      if (lane < Q) {
-        sc.w[lane] = w;
-        if constexpr (!STATES) {
-          sc.p[lane] = p;
-          sc.q[lane] = q;
-          sc.r[lane] = r;
-        }
-      }
-    }
     // The steps to the next chunk.
     B += (int64_t)Q * b_t;
     C += (int64_t)Q * c_t;
     x += (int64_t)Q * x_t;
-    dt += (int64_t)Q * dt_t;
     lds_dma_wait();
     __syncthreads();
     E* s_next = reinterpret_cast<E*>(lds + Lds::tile - (reinterpret_cast<char*>(s_b) - lds));
-    if (lane < left - Q && lane < Q) ndt = dt[lane * dt_t];
-    if (ahead(left - Q)) load_rows(B, b_t, s_next);
+    E* s_xnext = reinterpret_cast<E*>(s_x0 + Lds::x_bytes - (reinterpret_cast<char*>(s_x) - s_x0));
+    if (ahead(left - Q)) {
+      load_rows(B, b_t, s_next);
+      load_x(s_xnext);
+    }
+    if (left > Q && turn(i + 1) >= 0) write_scalars(i + 1, turn(i + 1));
+    if (left > 2 * Q && turn(i + 2) >= 0) load_dt(i + 2, turn(i + 2));
+    const ChunkScalars& sc = s_sc[(i & 1) * kWaves + own];
+    const float rescale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc.rescale)));
     Frag xf[KB];
 #pragma unroll
     for (int k = 0; k < KB; ++k) xf[k] = M::xcol(s_x, k, lane);
@@ -523,141 +608,116 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
     asm volatile("" : "+v"(row_at), "+v"(col_at));
 
     if constexpr (!STATES) {
-      // ---- G = B C^T: lane = token i of C, registers = tokens j of B ----
-      if (wave < Lds::tiles) {
-        const int it = wave == 0 ? 0 : 1, jt = wave == 2 ? 1 : 0;  // (0, 0), (1, 0), (1, 1)
-        f32x16 acc;
+      // ---- G = B C^T, lane = token i of C, registers = tokens j of B: the three 16 x 16
+      // quadrants on and below the diagonal, by the wavefronts that do not write scalars ----
+      const int quad = (wave + 2 * kWaves - (i + 1) % kWaves) % kWaves - 1;  // (0, 0), (1, 0), (1, 1)
+      if (quad >= 0) {
+        const int iq = quad > 0 ? 1 : 0, jq = quad > 1 ? 1 : 0, ci = lane & 15, j0 = 4 * (lane >> 4);
+        const f32x4 acc = M::template quadrant<NP>(s_b + 16 * jq * NP, s_c + 16 * iq * NP, lane);
+        float gv[4];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-#pragma unroll
-        for (int k = 0; k < NP / 16; ++k)
-          acc = M::mma(M::row(s_b + 32 * jt * NP, row_at, k), M::row(s_c + 32 * it * NP, row_at, k), acc);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(s_g + ((wave * 4 + q) * 64 + lane) * 4) =
-              make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        for (int e = 0; e < 4; ++e) gv[e] = iq > jq || j0 + e <= ci ? acc[e] : 0.f;
+        const int j = 16 * jq + j0;
+        store_f32<float, 4>(s_g + ((j / 8) * 64 + 16 * iq + ci + 32 * ((j / 4) % 2)) * 4, gv);
       }
-      // ---- 2^L_i h C_i^T + D x: lane = token i, registers = columns p ----
-      f32x16 acc[IT];
+      // ---- h C_i^T: lane = token i, registers = columns p ----
+      f32x16 acc;
 #pragma unroll
-      for (int it = 0; it < IT; ++it)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[it][r] = 0.f;
+      for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
       for (int k = 0; k < NP / 16; ++k) {
         float hv[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) hv[e] = h[k / 2][8 * (k % 2) + e];
-        const Frag hf = M::of(hv);
-#pragma unroll
-        for (int it = 0; it < IT; ++it) acc[it] = M::mma(hf, M::row(s_c + 32 * it * NP, row_at, k), acc[it]);
+        acc = M::mma(M::of(hv), M::row(s_c, row_at, k), acc);
       }
-      float my_p[IT], my_r[IT];
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        my_p[it] = sc.p[32 * it + col];
-        my_r[it] = sc.r[32 * it + col];
-        const float my_e = wide ? exp2_hw(my_p[it]) : my_p[it] * e_mid[it];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float xq[4];
-          M::four(s_x + M::xat(32 * it + col, 8 * q + 4 * half), xq);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[it][4 * q + e] = fmaf(acc[it][4 * q + e], my_e, D * xq[e]);
-        }
-      }
+      const float my_p = sc.p[col], my_r = M::kPair ? sc.r[col] : 0.f;
+      const bool wide = __builtin_amdgcn_readfirstlane(__float_as_uint(sc.wide)) != 0u;
       __syncthreads();
       if (ahead(left - Q)) load_rows(C, c_t, s_c);
 
       // ---- x^T S: S[i][j] = G[i][j] 2^(L_i - L_j) d_j for j <= i ----
-      // The factor for token j (its p, q and r); below: j's 32 tokens are earlier ones.
-      auto factor = [&](auto apart, int it, bool below, float pj, float qj, float rj) {
-        if constexpr (decltype(apart)::value) return below ? my_r[it] * rj : my_p[it] * qj;
-        float delta = my_p[it] - pj;
-        if constexpr (M::kPair) delta += my_r[it] - rj;
+      // Factors apart: 2^(L_i + K) is multiplied in at the end; G is 0 above the diagonal.
+      const bool finite = __ballot(!M::finite(xf)) == 0ull;
+      auto factor = [&](float pj, float qj, float rj) {
+        float delta = my_p - pj;
+        if constexpr (M::kPair) delta += my_r - rj;
         return exp2_hw(delta) * qj;
       };
-      int reach = col - 4 * half;  // j <= i as a number of the fragment's place; opaque, so that the
-      asm volatile("" : "+v"(reach));  // comparisons are made here and not kept in registers
-      auto sum_near = [&](auto apart) {
-        constexpr bool kApart = decltype(apart)::value;
+      if (wide) {
+        const float f = exp2_hw(my_p + sc.k);
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
+        for (int r = 0; r < 16; ++r) acc[r] *= f;
+      }
+      if (finite && (M::kPair || !wide)) {
 #pragma unroll
-          for (int k = 0; k < 2 * (it + 1); ++k) {
-            const bool below = k / 2 < it;
-            float s[8];
+        for (int k = 0; k < KB; ++k) {
+          float s[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int j0 = 16 * k + 8 * q + 4 * half;
-              float gv[4], pv[4] = {0.f, 0.f, 0.f, 0.f}, qv[4] = {0.f, 0.f, 0.f, 0.f}, rv[4] = {0.f, 0.f, 0.f, 0.f};
-              load_f32<float, 4>(s_g + (((it + k / 2) * 4 + 2 * (k % 2) + q) * 64 + lane) * 4, gv);
-              if (!kApart) load_f32<float, 4>(sc.p + j0, pv);
-              if (!kApart || !below) load_f32<float, 4>(sc.q + j0, qv);
-              if (kApart ? below : M::kPair) load_f32<float, 4>(sc.r + j0, rv);
+          for (int q = 0; q < 2; ++q) {
+            const int j0 = 16 * k + 8 * q + 4 * half;
+            float gv[4], pv[4], qv[4], rv[4];
+            load_f32<float, 4>(s_g + ((2 * k + q) * 64 + lane) * 4, gv);
+            load_f32<float, 4>(sc.q + j0, qv);
+            if constexpr (M::kPair) {
+              load_f32<float, 4>(sc.p + j0, pv);
+              load_f32<float, 4>(sc.r + j0, rv);
+            }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = gv[e] * factor(apart, it, below, pv[e], qv[e], rv[e]);
-                s[4 * q + e] = below || 16 * (k % 2) + 8 * q + e <= reach ? v : 0.f;
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (M::kPair) {
+                const float v = gv[e] * factor(pv[e], qv[e], rv[e]);
+                s[4 * q + e] = j0 + e <= col ? v : 0.f;
+              } else {
+                s[4 * q + e] = gv[e] * qv[e];
               }
             }
-            acc[it] = M::mma(xf[k], M::of(s), acc[it]);
           }
-        }
-      };
-      if (__ballot(!M::finite(xf)) == 0ull) {
-        if constexpr (M::kPair) {
-          sum_near(std::false_type());
-        } else {
-          if (wide) sum_near(std::false_type());
-          else sum_near(std::true_type());
+          acc = M::mma(xf[k], M::of(s), acc);
         }
       } else {
-        // An x that is not finite must not meet the zeros of S: its terms one by one.
+        // Term by term: an x that is not finite must not meet the zeros of S, and a
+        // decay that leaves a float's range in the chunk has no factors apart.
+        for (int j = 0; j < Q; ++j) {
+          const float gv = s_g[((j / 8) * 64 + col + 32 * ((j / 4) % 2)) * 4 + j % 4];
+          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], M::kPair ? sc.r[j] : 0.f) : sc.q[j]);
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
-          for (int j = 0; j < 32 * (it + 1); ++j) {
-            const int tile = it + j / 32, jj = j % 32;
-            const float gv = s_g[((tile * 4 + jj / 8) * 64 + col + 32 * ((jj / 4) % 2)) * 4 + jj % 4];
-            const float s = gv * (wide ? factor(std::false_type(), it, j / 32 < it, sc.p[j], sc.q[j], sc.r[j])
-                                       : factor(std::true_type(), it, j / 32 < it, sc.p[j], sc.q[j], sc.r[j]));
+          for (int q = 0; q < 4; ++q) {
+            float xq[4];
+            M::four(s_x + M::xat(j, 8 * q + 4 * half), xq);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float xq[4];
-              M::four(s_x + M::xat(j, 8 * q + 4 * half), xq);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                acc[it][4 * q + e] = j <= 32 * it + col ? fmaf(s, xq[e], acc[it][4 * q + e]) : acc[it][4 * q + e];
-            }
+            for (int e = 0; e < 4; ++e) acc[4 * q + e] = j <= col ? fmaf(s, xq[e], acc[4 * q + e]) : acc[4 * q + e];
           }
         }
       }
+      const float f = wide ? 1.f : my_p;
 #pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        if (!on || 32 * it + col >= len) continue;
-        T* row = y + (int64_t)(32 * it) * y_t + (col * y_t + 4 * half);
+      for (int q = 0; q < 4; ++q) {
+        float xq[4];
+        M::four(s_x + M::xat(col, 8 * q + 4 * half), xq);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = p0 + 8 * q + 4 * half;
-          const float v[4] = {acc[it][4 * q], acc[it][4 * q + 1], acc[it][4 * q + 2], acc[it][4 * q + 3]};
-          if (vec) {
-            if (c < P) store_f32<T, 4>(row + 8 * q, v);
-          } else {
+        for (int e = 0; e < 4; ++e) acc[4 * q + e] = fmaf(acc[4 * q + e], f, D * xq[e]);
+      }
+      if (on && col < len) {
+        T* row = y + (col * y_t + 4 * half);
+        if (vec && whole_p) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c + e < P) row[8 * q + e] = from_f32<T>(v[e]);
-          }
+          for (int q = 0; q < 4; ++q) store_f32<T, 4>(row + 8 * q, {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (p0 + 8 * (r / 4) + 4 * half + r % 4 < P) row[8 * (r / 4) + r % 4] = from_f32<T>(acc[r]);
         }
       }
       y += (int64_t)Q * y_t;
     }
-    if (ahead(left - Q)) load_x();
-
     // ---- h <- 2^L_end h + B^T v ----
+    if (rescale != 1.f) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) h[nt][r] *= decay;
+        for (int r = 0; r < 16; ++r) h[nt][r] *= rescale;
+    }
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
       float v[8];
@@ -668,19 +728,25 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * q + e] = M::get(xf[k], 4 * q + e) * wv[e];
       }
-      Frag vf[M::kPlanes];
+      Frag vf[M::kPlanes], bt[NT];
       M::split(v, vf);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const Frag bt = M::template col<NP>(s_b, col_at, nt, k);
+      for (int nt = 0; nt < NT; ++nt) bt[nt] = M::template col<NP>(s_b, col_at, nt, k);
 #pragma unroll
-        for (int pl = 0; pl < M::kPlanes; ++pl) h[nt] = M::mma(bt, vf[pl], h[nt]);
-      }
+      for (int pl = 0; pl < M::kPlanes; ++pl)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) h[nt] = M::mma(bt[nt], vf[pl], h[nt]);
     }
     s_b = s_next;
+    s_x = s_xnext;
   }
 
   if (to != nullptr && mine) {
+    const float f = exp2_hw((float)s_sums[own].k);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) h[nt][r] *= f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -697,7 +763,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : 2) void k_scan_chunk(Scan
         }
       }
   }
-  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)l_seg;
+  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)s_sums[own].l;
 }
 
 // Segment by segment, the state that each starts from in place of the part that
@@ -775,13 +841,12 @@ ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int 
   // Fewer tokens than half a chunk: the walk token by token.
   p.chunked = max_len >= kScanChunkFrom;
   if (!p.chunked || batch < 1) return p;
-  const int q = dtype == SF_BF16 ? MathBf16::Q : MathF32::Q;
   const int units = heads / groups * ((head_dim + kSlice - 1) / kSlice);
   p.split.blocks = (units + kWaves - 1) / kWaves;
   // Segments: enough workgroups for two on a CU, with at least four chunks each.
-  const int64_t chunks = (max_len + q - 1) / q;
+  const int64_t chunks = (max_len + kChunk - 1) / kChunk;
   const int64_t base = batch * groups * p.split.blocks;
-  int64_t segs = (2 * (int64_t)num_cus() + base - 1) / base;
+  int64_t segs = (3 * (int64_t)num_cus() + base - 1) / base;
   if (segs > chunks / 4) segs = chunks / 4;
   if (segs < 1) segs = 1;
   const int64_t per = (chunks + segs - 1) / segs;
