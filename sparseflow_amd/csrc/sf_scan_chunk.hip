@@ -56,8 +56,11 @@ __device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v
 __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 // ---- the two kinds of products ------------------------------------------------
-// A fragment is a lane's 8 values of a 16-deep slice of an operand: depths
-// 4 half + {0, 1, 2, 3} and 8 + 4 half + {0, 1, 2, 3}, half = lane / 32.
+// A fragment is a lane's 8 values of a 16-deep slice of an operand: depths 8 half to
+// 8 half + 7, half = lane / 32.  A product leaves rows 8 q + 4 half + e in register
+// 4 q + e; with its rows of 4 in the order 0, 2, 1, 3 of each 16 (order4), registers
+// 8 k to 8 k + 7 are a fragment.
+__device__ __forceinline__ int order4(int b) { return (b >> 1) | ((b & 1) << 1); }
 
 struct MathBf16 {
   typedef uint16_t E;  // as in LDS
@@ -70,7 +73,7 @@ struct MathBf16 {
   // one unit of 16 rows nor a transposed one of two units of 4 rows meets a bank
   // twice.
   template <int NP>
-  static __device__ __forceinline__ int unit(int j, int u) {
+  static constexpr __device__ __forceinline__ int unit(int j, int u) {
     if constexpr (NP >= 128) return u ^ ((2 * (j & 7)) | ((j >> 3) & 1));
     else if constexpr (NP == 64) return u ^ ((2 * ((j >> 1) & 3)) | ((j >> 3) & 1));
     else return u ^ ((2 * ((j >> 2) & 1)) | ((j >> 3) & 1));
@@ -82,11 +85,10 @@ struct MathBf16 {
   // where its first ones are; the others differ in single bits of it).
   template <int NP>
   static __device__ __forceinline__ int row_place(int j, int half) {
-    return j * NP + unit<NP>(j, 0) * 8 + 4 * half;
+    return j * NP + unit<NP>(j, half) * 8;
   }
   static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
-    return join(*reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k))),
-                *reinterpret_cast<const bf16x4*>(m + (place ^ (16 * k + 8))));
+    return *reinterpret_cast<const Frag*>(m + (place ^ (16 * k)));
   }
   // A 16 x 16 quadrant of a product of two tiles' rows, tokens ja + lane % 16 of a
   // with jb + lane % 16 of b: 16 bytes of both for 32 of the depth.
@@ -101,8 +103,8 @@ struct MathBf16 {
                                                     *reinterpret_cast<const bf16x8*>(b + (place ^ (32 * k))), acc, 0, 0, 0);
     return acc;
   }
-  // Tokens as depth: columns n0 + lane % 32 of tile m, tokens from 16 k.  Four
-  // lanes point at a token's 16 columns, and lane l of each 16 gets column l of
+  // Tokens as depth: columns of tile m in the order of order4, tokens from 16 k.
+  // Four lanes point at a token's 16 columns, and lane l of each 16 gets column l of
   // the four tokens.
   static __device__ __forceinline__ bf16x4 transposed(const E* p) {
     typedef __attribute__((address_space(3))) bf16x4 Lds;
@@ -110,22 +112,25 @@ struct MathBf16 {
   }
   template <int NP>
   static __device__ __forceinline__ int col_place(int lane) {
-    const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3), j = 4 * half + (s >> 2);
+    const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * order4(s & 3), j = 8 * half + (s >> 2);
     return j * NP + unit<NP>(j, n >> 3) * 8 + (n & 7);
   }
+  // (Four tokens on: only the bits of j & 4 differ.)
   template <int NP>
   static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
-    return join(transposed(m + (place ^ (32 * nt)) + 16 * k * NP), transposed(m + (place ^ (32 * nt + 8)) + (16 * k + 8) * NP));
+    constexpr int next = unit<NP>(4, 0) * 8;
+    return join(transposed(m + (place ^ (32 * nt)) + 16 * k * NP),
+                transposed(m + (place ^ (32 * nt) ^ next) + (16 * k + 4) * NP));
   }
-  // The same of a slice of x, rows of 64 bytes: 4 rows are read at once transposed,
-  // 16 as rows.
+  // The same of a slice of x, rows of 64 bytes, its columns in their own order: 4
+  // rows are read at once transposed, 16 as rows.
   static __device__ __forceinline__ int xat(int j, int c) {
     return j * kSlice + ((c >> 3) ^ ((j >> 2) & 3)) * 8 + (c & 7);
   }
   static __device__ __forceinline__ Frag xcol(const E* x, int k, int lane) {
     const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3);
-    const int j = 16 * k + 4 * half + (s >> 2);
-    return join(transposed(x + xat(j, n)), transposed(x + xat(j + 8, n)));
+    const int j = 16 * k + 8 * half + (s >> 2);
+    return join(transposed(x + xat(j, n)), transposed(x + xat(j + 4, n)));
   }
   static __device__ __forceinline__ Frag of(const float (&v)[8]) {
     Frag f;
@@ -147,8 +152,8 @@ struct MathBf16 {
                                                                       __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu)));
     return max(most >> 16, most & 0xffffu) < 0x7f80u;
   }
-  static __device__ __forceinline__ void four(const E* p, float (&v)[4]) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
+  typedef uint2 Quad;  // four elements
+  static __device__ __forceinline__ void four(Quad q, float (&v)[4]) {
     v[0] = low_bf16(q.x), v[1] = high_bf16(q.x), v[2] = low_bf16(q.y), v[3] = high_bf16(q.y);
   }
   // v as a sum of kPlanes fragments.
@@ -181,19 +186,17 @@ struct MathF32 {
   static constexpr bool kPair = true;
 
   template <int NP>
-  static __device__ __forceinline__ int unit(int j, int u) {
+  static constexpr __device__ __forceinline__ int unit(int j, int u) {
     return u ^ (j & 7);
   }
   template <int NP>
   static __device__ __forceinline__ int row_place(int j, int half) {
-    return j * NP + unit<NP>(j, half) * 4;
+    return j * NP + unit<NP>(j, 2 * half) * 4;
   }
   static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
     Frag f;
-    const float4 lo = *reinterpret_cast<const float4*>(m + (place ^ (16 * k)));
-    const float4 hi = *reinterpret_cast<const float4*>(m + (place ^ (16 * k + 8)));
-    f.e[0] = lo.x, f.e[1] = lo.y, f.e[2] = lo.z, f.e[3] = lo.w;
-    f.e[4] = hi.x, f.e[5] = hi.y, f.e[6] = hi.z, f.e[7] = hi.w;
+    load_f32<float, 4>(m + (place ^ (16 * k)), *reinterpret_cast<float(*)[4]>(f.e));
+    load_f32<float, 4>(m + (place ^ (16 * k + 4)), *reinterpret_cast<float(*)[4]>(f.e + 4));
     return f;
   }
   template <int NP>
@@ -211,14 +214,14 @@ struct MathF32 {
   }
   template <int NP>
   static __device__ __forceinline__ int col_place(int lane) {
-    const int half = lane >> 5, n = lane & 31;
-    return 4 * half * NP + (n ^ (16 * half));
+    const int half = lane >> 5, n = (lane & 19) + 4 * order4((lane >> 2) & 3);
+    return 8 * half * NP + n;
   }
   template <int NP>
   static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = m[(place ^ (32 * nt + 4 * (e & 3))) + (16 * k + 8 * (e >> 2) + (e & 3)) * NP];
+    for (int e = 0; e < 8; ++e) f.e[e] = m[(place ^ (32 * nt + 4 * e)) + (16 * k + e) * NP];
     return f;
   }
   static __device__ __forceinline__ int xat(int j, int c) {
@@ -228,7 +231,7 @@ struct MathF32 {
     const int half = lane >> 5;
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = x[xat(16 * k + 8 * (e >> 2) + 4 * half + (e & 3), lane & 31)];
+    for (int e = 0; e < 8; ++e) f.e[e] = x[xat(16 * k + 8 * half + e, lane & 31)];
     return f;
   }
   static __device__ __forceinline__ Frag of(const float (&v)[8]) {
@@ -246,7 +249,11 @@ struct MathF32 {
       for (int e = 0; e < 8; ++e) ok = ok && fabsf(x[k].e[e]) < __builtin_huge_valf();
     return ok;
   }
-  static __device__ __forceinline__ void four(const E* p, float (&v)[4]) { load_f32<float, 4>(p, v); }
+  typedef f32x4 Quad;
+  static __device__ __forceinline__ void four(Quad q, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = q[e];
+  }
   static __device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[kPlanes]) { f[0] = of(v); }
   static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
 #pragma unroll
@@ -268,10 +275,7 @@ struct alignas(16) ChunkScalars {
   float w[kChunk], p[kChunk], q[kChunk], r[kChunk];
   float k, rescale, wide, pad;  // K; what the state is multiplied by before the chunk's part comes in
 };
-struct HeadSums {
-  double k, l;  // K, and the sum of the exponents so far
-};
-constexpr double kScaleMost = 20.0;
+constexpr double kScaleMost = 20.0, kScaleFrom = 16.0;  // (a chunk that decays nothing leaves K alone)
 constexpr float kApartMost = 100.f;  // exponents of factors apart
 
 // The sum of v over this half wavefront's lanes up to this one.
@@ -291,6 +295,14 @@ __device__ __forceinline__ double half_sum_up_to(double v) {
   return v;
 }
 
+// A value that is the same in all lanes, held once for them.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+__device__ __forceinline__ double uniform(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
 __device__ __forceinline__ double lane_of(double v, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v);
   const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
@@ -300,15 +312,14 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
 template <typename M, int NP>
 struct ChunkLds {
   static constexpr int tile = kChunk * NP * (int)sizeof(typename M::E);
-  // B, a slice of x for each wavefront and the scalars of up to as many heads twice
-  // (the next chunk's arrive while this one's are read), C, G.
-  static constexpr int x = 2 * tile;
   static constexpr int x_bytes = kChunk * kSlice * (int)sizeof(typename M::E);
-  static constexpr int scalars = x + 2 * kWaves * x_bytes;
-  static constexpr int sums = scalars + 2 * kWaves * (int)sizeof(ChunkScalars);
-  static constexpr int c = sums + kWaves * (int)sizeof(HeadSums);
-  static constexpr int g = c + tile;
-  static constexpr int bytes(bool states) { return states ? c : g + kChunk * kChunk * 4; }
+  // B, and a slice of x for each wavefront, for this chunk and `depth - 1` after it
+  // that are on their way; the scalars of two chunks for each wavefront; C, G.
+  static constexpr int x(int depth) { return depth * tile; }
+  static constexpr int scalars(int depth) { return x(depth) + depth * kWaves * x_bytes; }
+  static constexpr int c(int depth) { return scalars(depth) + 2 * kWaves * (int)sizeof(ChunkScalars); }
+  static constexpr int g(int depth) { return c(depth) + tile; }
+  static constexpr int bytes(int depth, bool states) { return states ? c(depth) : g(depth) + kChunk * kChunk * 4; }
 };
 
 // 64 lanes' 16 bytes from base + off (bytes) to LDS at dst and on, lane by lane
@@ -322,6 +333,13 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, cons
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(l) : "m0", "memory");
 }
 #pragma clang diagnostic pop
+
+// Waits until at most KEEP of this wavefront's latest memory operations are not
+// done (they are done in their order).
+template <int KEEP>
+__device__ __forceinline__ void wait_memory() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory");
+}
 
 // kUnit elements of a row into LDS by way of registers; what lies outside becomes 0.
 template <typename T, typename M>
@@ -369,17 +387,17 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
   constexpr int kRounds = Q > kRows ? Q / kRows : 1;
   constexpr int kXUnits = kSlice / U, kXRows = kWave / kXUnits, kXRounds = Q / kXRows;
   constexpr bool kDma = sizeof(T) == sizeof(E);
+  // (Three workgroups fit a CU with either.)
+  constexpr int kDepth = STATES && sizeof(E) == 2 && NP <= 128 ? 3 : 2;
   typedef ChunkLds<M, NP> Lds;
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  E* s_b = reinterpret_cast<E*>(lds);
-  E* s_c = reinterpret_cast<E*>(lds + Lds::c);
-  float* s_g = reinterpret_cast<float*>(lds + Lds::g);
-  char* const s_x0 = lds + Lds::x + 2 * wave * Lds::x_bytes;
-  E* s_x = reinterpret_cast<E*>(s_x0);
-  ChunkScalars* s_sc = reinterpret_cast<ChunkScalars*>(lds + Lds::scalars);
-  HeadSums* s_sums = reinterpret_cast<HeadSums*>(lds + Lds::sums);
+  E* const s_b0 = reinterpret_cast<E*>(lds);
+  E* const s_x0 = reinterpret_cast<E*>(lds + Lds::x(kDepth) + wave * kDepth * Lds::x_bytes);
+  ChunkScalars* s_sc = reinterpret_cast<ChunkScalars*>(lds + Lds::scalars(kDepth)) + 2 * wave;
+  E* s_c = reinterpret_cast<E*>(lds + Lds::c(kDepth));
+  float* const s_g = reinterpret_cast<float*>(lds + Lds::g(kDepth));
 
   // This workgroup's sequence, segment and group; this wavefront's head and columns.
   int64_t item = a.block0 + blockIdx.x;
@@ -390,11 +408,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
   const int seg = (int)(item % (STATES ? sp.segments - 1 : sp.segments));
   const int64_t b = item / (STATES ? sp.segments - 1 : sp.segments);
   const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
-  const int units = per_group * slices, first_head = ub * kWaves / slices;
   const int unit = ub * kWaves + wave;
-  const bool on = unit < units;
-  const int own = on ? unit / slices - first_head : 0;  // the head, of those of this workgroup
-  const int hd = g * per_group + first_head + own;
+  const bool on = unit < per_group * slices;
+  const int hd = g * per_group + (on ? unit / slices : 0);
   const int p0 = on ? unit % slices * kSlice : 0;
   const int P = a.head_dim, N = a.state_dim;
   int64_t first, n;
@@ -409,78 +425,70 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
   const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + (first + t0) * a.c_t + g * a.c_g;
   T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + (first + t0) * a.y_t + hd * a.y_h + p0;
   const int64_t slot = seq_slot(a.seq, b);
-  const float D = a.D != nullptr ? a.D[hd] : 0.f;
+  const float D = uniform(a.D != nullptr ? a.D[hd] : 0.f);
 
-  // The scalars of two heads at once, one to each half wavefront: by one wavefront
-  // for heads 0 and 1 of the workgroup, by another for 2 and 3, in turns.
-  const int heads = (min(units, (ub + 1) * kWaves) - 1) / slices - first_head + 1;
-  const int turns = heads > 2 ? 2 : 1;
-  // Whether chunk i's scalars are this wavefront's turn, and for which pair of heads (-1: not).
-  auto turn = [&](int i) {
-    const int k = (wave + 2 * kWaves - i % kWaves) % kWaves;  // 0 and 2: in turn for pair 0 and 1
-    return k == 0 ? 0 : k == 2 && turns == 2 ? 1 : -1;
-  };
-  const T* __restrict__ dts = static_cast<const T*>(a.dt) + b * a.dt_b + (first + t0) * a.dt_t;
+  // The scalars of two chunks at once, one to each half wavefront.
+  const T* __restrict__ dt = static_cast<const T*>(a.dt) + b * a.dt_b + (first + t0) * a.dt_t + hd * a.dt_h;
+  const float bias = uniform(a.dt_bias != nullptr ? a.dt_bias[hd] : 0.f);
+  const double A2 = uniform((double)a.A[hd] * 1.4426950408889634);  // exponents of 2
+  double k_state = 0.0, l_seg = 0.0;  // (l_seg: the sum of the exponents)
   T next_dt = from_f32<T>(0.f);
-  auto load_dt = [&](int i, int pair) {
-    const int hl = 2 * pair + half;
-    const int64_t t = (int64_t)i * Q + col;
-    if (hl < heads && t < t1 - t0)
-      next_dt = dts[t * dt_t + (g * per_group + first_head + hl) * a.dt_h];
+  // rest: tokens from the first of the two chunks on.
+  auto load_dt = [&](const T* from, int64_t rest) {
+    if (lane < rest) next_dt = from[lane * dt_t];
   };
-  auto write_scalars = [&](int i, int pair) {
-    const int hl = 2 * pair + half, hg = g * per_group + first_head + hl;
-    const bool there = hl < heads;
-    ChunkScalars& sc = s_sc[(i & 1) * kWaves + (there ? hl : 0)];
+  auto write_scalars = [&](int64_t rest) {
     float d = 0.f;
-    double l = 0.0, k = 0.0;
-    if (there) {
-      k = s_sums[hl].k;
-      if ((int64_t)i * Q + col < t1 - t0) {
-        d = to_f32<T>(next_dt) + (a.dt_bias != nullptr ? a.dt_bias[hg] : 0.f);
-        if (a.softplus) d = softplus(d);
-        l = (double)a.A[hg] * 1.4426950408889634 * (double)d;  // an exponent of 2
+    if (lane < rest) {
+      d = to_f32<T>(next_dt) + bias;
+      if (a.softplus) d = softplus(d);
+    }
+    const double l = half_sum_up_to(lane < rest ? A2 * (double)d : 0.0);
+    const double end[2] = {lane_of(l, 31), lane_of(l, 63)};
+    double k[3] = {k_state, 0.0, 0.0};
+    float rescale[2] = {1.f, 1.f};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      k[c + 1] = k[c] + end[c];
+      if constexpr (STATES) l_seg = uniform(l_seg + end[c]);
+      if (!(fabs(k[c + 1]) < kScaleMost)) {
+        const double to = end[c] < 0.0 ? kScaleFrom : 0.0;
+        rescale[c] = exp2_hw((float)(k[c + 1] - to));
+        k[c + 1] = to;
       }
     }
-    l = half_sum_up_to(l);
-    const double end0 = lane_of(l, 31), end1 = lane_of(l, 63), end = half == 0 ? end0 : end1;
-    float p = (float)l, q = d, r = (float)(l - (double)p);
-    bool wide = M::kPair;  // a factor per element: L moves far in the chunk, or as precise as float32 is
-    if constexpr (!STATES && !M::kPair) {
-      const float off = (float)(l + k), fall = exp2_hw(-off) * d;
-      // (Also where a factor of a later token is no number: it meets zeros of G.)
-      const uint64_t no = __ballot(!(fabsf(off) < kApartMost && fabsf(fall) < __builtin_huge_valf()));
-      wide = (half == 0 ? (uint32_t)no : (uint32_t)(no >> 32)) != 0u;
-      if (!wide) {
-        p = exp2_hw(off);
-        q = fall;
-      }
-    }
-    double k_new = k + end;
-    float rescale = 1.f;
-    if (!(fabs(k_new) < kScaleMost)) {
-      const double to = end < 0.0 ? kScaleMost : 0.0;
-      rescale = exp2_hw((float)(k_new - to));
-      k_new = to;
-    }
-    if (!there) return;
-    sc.w[col] = exp2_hw((float)(end - l - k_new)) * d;
+    k_state = uniform(k[2]);
+    ChunkScalars& sc = s_sc[half];
+    sc.w[col] = exp2_hw((float)((half == 0 ? end[0] - k[1] : end[1] - k[2]) - l)) * d;
+    float wide = 0.f;
     if constexpr (!STATES) {
+      float p = (float)l, q = d;
+      if constexpr (M::kPair) {
+        wide = 1.f;
+        sc.r[col] = (float)(l - (double)p);
+      } else {
+        const float off = (float)(l + (half == 0 ? k[0] : k[1])), fall = exp2_hw(-off) * d;
+        // (Also where a factor of a later token is no number: it meets zeros of G.)
+        const uint64_t no = __ballot(!(fabsf(off) < kApartMost && fabsf(fall) < __builtin_huge_valf()));
+        if ((half == 0 ? (uint32_t)no : (uint32_t)(no >> 32)) != 0u) {
+          wide = 1.f;
+        } else {
+          p = exp2_hw(off);
+          q = fall;
+        }
+      }
       sc.p[col] = p;
       sc.q[col] = q;
-      if constexpr (M::kPair) sc.r[col] = r;
     }
     if (col == 0) {
-      sc.k = (float)k;
-      sc.rescale = rescale;
-      sc.wide = wide ? 1.f : 0.f;
-      s_sums[hl].k = k_new;
-      s_sums[hl].l += end;
+      sc.k = (float)(half == 0 ? k[0] : k[1]);
+      sc.rescale = half == 0 ? rescale[0] : rescale[1];
+      sc.wide = wide;
     }
   };
 
   // The state: register r of tile nt is row p0 + col, column
-  // 32 nt + 8 (r / 4) + 4 half + r % 4.
+  // 32 nt + 16 (r / 8) + 8 half + r % 8.
   f32x16 h[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -491,21 +499,17 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
   const bool vec_n = N % 4 == 0;
   const int64_t plane = (int64_t)P * N;
   const float* from = nullptr;
-  float* to = nullptr;
-  if constexpr (STATES) {
-    to = sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane;
-  } else {
+  if constexpr (!STATES) {
     from = sp.segments > 1 ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
            : a.h0 != nullptr && slot >= 0 ? a.h0 + (slot * a.heads + hd) * plane
                                           : nullptr;
-    if (seg == sp.segments - 1 && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
   }
   if (from != nullptr && mine) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n0 = 32 * nt + 8 * q + 4 * half;
+        const int n0 = 32 * nt + 16 * (q / 2) + 8 * half + 4 * (q % 2);
         const float* src = from + (int64_t)p * N + n0;
         if (vec_n && n0 < N) {
           const float4 v = *reinterpret_cast<const float4*>(src);
@@ -558,67 +562,82 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
     }
   };
   int64_t left = t1 - t0;  // tokens from this chunk on
-  for (int i = threadIdx.x * 4; i < Lds::bytes(STATES) / 4; i += kThreads * 4)
+  for (int i = threadIdx.x * 4; i < Lds::bytes(kDepth, STATES) / 4; i += kThreads * 4)
     store_f32<float, 4>(reinterpret_cast<float*>(lds) + i, {0.f, 0.f, 0.f, 0.f});
   __syncthreads();
-  if (ahead(left)) {
-    load_rows(B, b_t, s_b);
-    if constexpr (!STATES) load_rows(C, c_t, s_c);
-    load_x(s_x);
+#pragma unroll
+  for (int c = 0; c < kDepth - 1; ++c) {
+    if (ahead(left - c * Q)) {
+      load_rows(B, b_t, s_b0 + c * Q * NP);
+      if (c == 0 && !STATES) load_rows(C, c_t, s_c);
+      load_x(s_x0 + c * Q * kSlice);
+    }
+    B += (int64_t)Q * b_t;
+    x += (int64_t)Q * x_t;
   }
-  if (left > 0 && turn(0) >= 0) {
-    load_dt(0, turn(0));
-    write_scalars(0, turn(0));
-  }
-  if (left > Q && turn(1) >= 0) load_dt(1, turn(1));
+  load_dt(dt, left);
+  write_scalars(left);
+  // Every wavefront issues as many memory operations to a chunk as any: the latest
+  // may be left under way at the next.
+  const bool counted = kDma && vec && on && whole_n && whole_p && kRows <= Q;
 
   for (int i = 0; left > 0; left -= Q, ++i) {
     const int len = (int)(left < Q ? left : Q);
+    const int at = i % kDepth, at_last = (i + kDepth - 1) % kDepth;
+    const E* s_b = s_b0 + at * Q * NP;
+    const E* s_x = s_x0 + at * Q * kSlice;
     if (!ahead(left)) {
-      stage_rows(B, b_t, s_b, len);
+      const T* b_now = B - (int64_t)(kDepth - 1) * Q * b_t;
+      const T* x_now = x - (int64_t)(kDepth - 1) * Q * x_t;
+      stage_rows(b_now, b_t, s_b0 + at * Q * NP, len);
       if constexpr (!STATES) stage_rows(C, c_t, s_c, len);
       for (int r = 0; r < kXRounds; ++r) {
         const int j = r * kXRows + xj;
-        stage_unit<T, M>(s_x + M::xat(j, xv * U), x + ((int64_t)j * x_t + xv * U),
+        stage_unit<T, M>(s_x0 + at * Q * kSlice + M::xat(j, xv * U), x_now + ((int64_t)j * x_t + xv * U),
                          on && j < len ? P - p0 - xv * U : 0, vec);
       }
+    }
+    // This chunk has arrived.  Issued after it: the chunk before's y (four stores), or
+    // the next chunk's B and x.
+    if (counted && (STATES ? kDepth == 3 && ahead(left - Q) : i > 0)) wait_memory<STATES ? kRounds + kXRounds : 4>();
+    else wait_memory<0>();
+    __syncthreads();
+    if (ahead(left - (kDepth - 1) * Q)) {
+      load_rows(B, b_t, s_b0 + at_last * Q * NP);
+      load_x(s_x0 + at_last * Q * kSlice);
     }
     // The steps to the next chunk.
     B += (int64_t)Q * b_t;
     C += (int64_t)Q * c_t;
     x += (int64_t)Q * x_t;
-    lds_dma_wait();
-    __syncthreads();
-    E* s_next = reinterpret_cast<E*>(lds + Lds::tile - (reinterpret_cast<char*>(s_b) - lds));
-    E* s_xnext = reinterpret_cast<E*>(s_x0 + Lds::x_bytes - (reinterpret_cast<char*>(s_x) - s_x0));
-    if (ahead(left - Q)) {
-      load_rows(B, b_t, s_next);
-      load_x(s_xnext);
+    if (i % 2 == 0) {
+      dt += (int64_t)(2 * Q) * dt_t;
+      load_dt(dt, left - 2 * Q);
     }
-    if (left > Q && turn(i + 1) >= 0) write_scalars(i + 1, turn(i + 1));
-    if (left > 2 * Q && turn(i + 2) >= 0) load_dt(i + 2, turn(i + 2));
-    const ChunkScalars& sc = s_sc[(i & 1) * kWaves + own];
-    const float rescale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc.rescale)));
+    const ChunkScalars& sc = s_sc[i & 1];
+    const float rescale = uniform(sc.rescale);
+    // (Opaque: places of single reads and comparisons are made from these when they
+    // are wanted.  Kept in registers from chunk to chunk they would spill, and a
+    // reload waits for all of the loads ahead: 283 -> 358 us.)
+    int row_at = M::template row_place<NP>(col, half), col_at = M::template col_place<NP>(lane);
+    int ln = lane;
+    asm volatile("" : "+v"(row_at), "+v"(col_at), "+v"(ln));
+
     Frag xf[KB];
 #pragma unroll
-    for (int k = 0; k < KB; ++k) xf[k] = M::xcol(s_x, k, lane);
-    // (Opaque: the places of single reads are made from these when they are read,
-    // not kept in registers from chunk to chunk.)
-    int row_at = M::template row_place<NP>(col, half), col_at = M::template col_place<NP>(lane);
-    asm volatile("" : "+v"(row_at), "+v"(col_at));
-
+    for (int k = 0; k < KB; ++k) xf[k] = M::xcol(s_x, k, ln);
     if constexpr (!STATES) {
+      // Element (i, j) of G: the 8 tokens j of a fragment lie together.
+      auto g_at = [&](int i, int j) { return s_g + ((j / 8) * 32 + i) * 8 + j % 8; };
       // ---- G = B C^T, lane = token i of C, registers = tokens j of B: the three 16 x 16
-      // quadrants on and below the diagonal, by the wavefronts that do not write scalars ----
-      const int quad = (wave + 2 * kWaves - (i + 1) % kWaves) % kWaves - 1;  // (0, 0), (1, 0), (1, 1)
-      if (quad >= 0) {
-        const int iq = quad > 0 ? 1 : 0, jq = quad > 1 ? 1 : 0, ci = lane & 15, j0 = 4 * (lane >> 4);
-        const f32x4 acc = M::template quadrant<NP>(s_b + 16 * jq * NP, s_c + 16 * iq * NP, lane);
+      // quadrants on and below the diagonal ----
+      if (wave < 3) {
+        const int iq = wave > 0 ? 1 : 0, jq = wave > 1 ? 1 : 0, ci = ln & 15, j0 = 4 * (ln >> 4);
+        const f32x4 acc = M::template quadrant<NP>(s_b + 16 * jq * NP, s_c + 16 * iq * NP, ln);
         float gv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) gv[e] = iq > jq || j0 + e <= ci ? acc[e] : 0.f;
-        const int j = 16 * jq + j0;
-        store_f32<float, 4>(s_g + ((j / 8) * 64 + 16 * iq + ci + 32 * ((j / 4) % 2)) * 4, gv);
+        store_f32<float, 4>(g_at(16 * iq + ci, 16 * jq + j0), gv);
       }
       // ---- h C_i^T: lane = token i, registers = columns p ----
       f32x16 acc;
@@ -631,8 +650,11 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         for (int e = 0; e < 8; ++e) hv[e] = h[k / 2][8 * (k % 2) + e];
         acc = M::mma(M::of(hv), M::row(s_c, row_at, k), acc);
       }
+      typename M::Quad xr[4];  // this token's x, for D
+#pragma unroll
+      for (int q = 0; q < 4; ++q) xr[q] = *reinterpret_cast<const typename M::Quad*>(s_x + M::xat(ln & 31, 8 * q + 4 * (ln >> 5)));
       const float my_p = sc.p[col], my_r = M::kPair ? sc.r[col] : 0.f;
-      const bool wide = __builtin_amdgcn_readfirstlane(__float_as_uint(sc.wide)) != 0u;
+      const bool wide = uniform(sc.wide) != 0.f;
       __syncthreads();
       if (ahead(left - Q)) load_rows(C, c_t, s_c);
 
@@ -655,9 +677,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
           float s[8];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int j0 = 16 * k + 8 * q + 4 * half;
+            const int j0 = 16 * k + 8 * half + 4 * q;
             float gv[4], pv[4], qv[4], rv[4];
-            load_f32<float, 4>(s_g + ((2 * k + q) * 64 + lane) * 4, gv);
+            load_f32<float, 4>(g_at(ln & 31, 16 * k + 8 * (ln >> 5) + 4 * q), gv);
             load_f32<float, 4>(sc.q + j0, qv);
             if constexpr (M::kPair) {
               load_f32<float, 4>(sc.p + j0, pv);
@@ -679,12 +701,12 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         // Term by term: an x that is not finite must not meet the zeros of S, and a
         // decay that leaves a float's range in the chunk has no factors apart.
         for (int j = 0; j < Q; ++j) {
-          const float gv = s_g[((j / 8) * 64 + col + 32 * ((j / 4) % 2)) * 4 + j % 4];
+          const float gv = *g_at(col, j);
           const float s = gv * (wide ? factor(sc.p[j], sc.q[j], M::kPair ? sc.r[j] : 0.f) : sc.q[j]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float xq[4];
-            M::four(s_x + M::xat(j, 8 * q + 4 * half), xq);
+            M::four(*reinterpret_cast<const typename M::Quad*>(s_x + M::xat(j, 8 * q + 4 * half)), xq);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[4 * q + e] = j <= col ? fmaf(s, xq[e], acc[4 * q + e]) : acc[4 * q + e];
           }
@@ -694,7 +716,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float xq[4];
-        M::four(s_x + M::xat(col, 8 * q + 4 * half), xq);
+        M::four(xr[q], xq);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[4 * q + e] = fmaf(acc[4 * q + e], f, D * xq[e]);
       }
@@ -706,7 +728,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (p0 + 8 * (r / 4) + 4 * half + r % 4 < P) row[8 * (r / 4) + r % 4] = from_f32<T>(acc[r]);
+            if (p0 + 8 * (r / 4) + 4 * (ln >> 5) + r % 4 < P) row[8 * (r / 4) + r % 4] = from_f32<T>(acc[r]);
         }
       }
       y += (int64_t)Q * y_t;
@@ -724,7 +746,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float wv[4];
-        load_f32<float, 4>(sc.w + 16 * k + 8 * q + 4 * half, wv);
+        load_f32<float, 4>(sc.w + 16 * k + 8 * half + 4 * q, wv);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * q + e] = M::get(xf[k], 4 * q + e) * wv[e];
       }
@@ -737,12 +759,14 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) h[nt] = M::mma(bt[nt], vf[pl], h[nt]);
     }
-    s_b = s_next;
-    s_x = s_xnext;
+    if (i % 2 == 1 && left > Q) write_scalars(left - Q);
   }
 
+  float* to = nullptr;
+  if (STATES) to = sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane;
+  else if (seg == sp.segments - 1 && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
   if (to != nullptr && mine) {
-    const float f = exp2_hw((float)s_sums[own].k);
+    const float f = exp2_hw((float)k_state);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -751,7 +775,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n0 = 32 * nt + 8 * q + 4 * half;
+        const int n0 = 32 * nt + 16 * (q / 2) + 8 * half + 4 * (q % 2);
         float* dst = to + (int64_t)p * N + n0;
         if (vec_n && n0 < N) {
           *reinterpret_cast<float4*>(dst) =
@@ -763,7 +787,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         }
       }
   }
-  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)s_sums[own].l;
+  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)l_seg;
 }
 
 // Segment by segment, the state that each starts from in place of the part that
@@ -799,7 +823,8 @@ int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
                    aligned_to(a.b, U * sizeof(T)) && aligned_to(a.c, U * sizeof(T)) && aligned_to(a.y, U * sizeof(T));
   const int64_t blocks = a.seq.batch * (STATES ? sp.segments - 1 : sp.segments) * a.groups * sp.blocks;
   return launch_blocks(a, &ScanArgs::block0, blocks, [&](const ScanArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_scan_chunk<T, M, NP, STATES>), dim3(n), dim3(kThreads), Lds::bytes(STATES), stream, la, sp, vec);
+    hipLaunchKernelGGL((k_scan_chunk<T, M, NP, STATES>), dim3(n), dim3(kThreads), Lds::bytes(STATES && sizeof(typename M::E) == 2 && NP <= 128 ? 3 : 2, STATES), stream,
+                       la, sp, vec);
   });
 }
 
