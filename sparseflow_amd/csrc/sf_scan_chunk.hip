@@ -16,11 +16,14 @@
 // state's the h of the second.  B and x are also needed with tokens along the
 // registers: they are read from LDS transposed.
 //
-// Rounding.  bf16: C, B and x are exact; S and h are rounded to bf16 as operands
-// of y, which is rounded to bf16 itself.  v is split into three bf16 parts (its 24
-// bits), so that the state, which is summed up over all tokens, stays a float32
-// one.  float32 and f16 inputs use the float32 matrix instructions.  L is summed in
-// 64 bits: differences of it are exponents.
+// All of it runs on the bf16 instructions, whatever the inputs: x, B and C are taken
+// apart into bf16 parts (bf16 one, f16 two, float32 three: all of their bits), S and h
+// into as many, and a product of two sums of parts leaves out the terms below the last
+// part (three products for f16 and six for float32, a sixth of the time that the
+// float32 instructions take).  So S and h are rounded to 8 bits for bf16 outputs and to
+// 16 for f16 ones, which have 8 and 11 themselves.  v is split into three parts, its 24
+// bits, always: the state is summed up over all tokens and stays a float32 one.  L is
+// summed in 64 bits: differences of it are exponents.
 //
 // Few heads and long sequences: the token axis is cut into segments.  A first
 // pass walks each segment from a zero state for its own part of the state
@@ -55,213 +58,111 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 __device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// ---- the two kinds of products ------------------------------------------------
-// A fragment is a lane's 8 values of a 16-deep slice of an operand: depths 8 half to
-// 8 half + 7, half = lane / 32.  A product leaves rows 8 q + 4 half + e in register
-// 4 q + e; with its rows of 4 in the order 0, 2, 1, 3 of each 16 (order4), registers
-// 8 k to 8 k + 7 are a fragment.
+// ---- fragments ------------------------------------------------------------------
+// A fragment is a lane's 8 values of a 16-deep slice of an operand, as bf16: depths
+// 8 half to 8 half + 7, half = lane / 32.  A product leaves rows 8 q + 4 half + e in
+// register 4 q + e; with its rows of 4 in the order 0, 2, 1, 3 of each 16 (order4),
+// registers 8 k to 8 k + 7 are a fragment.
+typedef u32x4 Frag;  // pairs of bf16
 __device__ __forceinline__ int order4(int b) { return (b >> 1) | ((b & 1) << 1); }
 
-struct MathBf16 {
-  typedef uint16_t E;  // as in LDS
-  typedef u32x4 Frag;  // pairs of bf16
-  static constexpr int kUnit = 8;  // elements of 16 bytes
-  static constexpr int kPlanes = 3;
-  static constexpr bool kPair = false;  // L as one float in the chunk
+// Place of 16-byte unit u (8 elements) in token j's row of a tile [32][NP]: spread so
+// that neither a read of one unit of 16 rows nor a transposed one of two units of 4
+// rows meets a bank twice.
+template <int NP>
+constexpr __device__ __forceinline__ int unit_place(int j, int u) {
+  if constexpr (NP >= 128) return u ^ ((2 * (j & 7)) | ((j >> 3) & 1));
+  else if constexpr (NP == 64) return u ^ ((2 * ((j >> 1) & 3)) | ((j >> 3) & 1));
+  else return u ^ ((2 * ((j >> 2) & 1)) | ((j >> 3) & 1));
+}
 
-  // Place of 16-byte unit u in token j's row: spread so that neither a read of
-  // one unit of 16 rows nor a transposed one of two units of 4 rows meets a bank
-  // twice.
-  template <int NP>
-  static constexpr __device__ __forceinline__ int unit(int j, int u) {
-    if constexpr (NP >= 128) return u ^ ((2 * (j & 7)) | ((j >> 3) & 1));
-    else if constexpr (NP == 64) return u ^ ((2 * ((j >> 1) & 3)) | ((j >> 3) & 1));
-    else return u ^ ((2 * ((j >> 2) & 1)) | ((j >> 3) & 1));
-  }
-  static __device__ __forceinline__ Frag join(bf16x4 lo, bf16x4 hi) {
-    return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  // Tokens as lanes: token j's row of tile m [.][NP], depths from 16 k (place:
-  // where its first ones are; the others differ in single bits of it).
-  template <int NP>
-  static __device__ __forceinline__ int row_place(int j, int half) {
-    return j * NP + unit<NP>(j, half) * 8;
-  }
-  static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
-    return *reinterpret_cast<const Frag*>(m + (place ^ (16 * k)));
-  }
-  // A 16 x 16 quadrant of a product of two tiles' rows, tokens ja + lane % 16 of a
-  // with jb + lane % 16 of b: 16 bytes of both for 32 of the depth.
-  template <int NP>
-  static __device__ __forceinline__ f32x4 quadrant(const E* a, const E* b, int lane) {
-    const int j = lane & 15, q = lane >> 4;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const int place = j * NP + unit<NP>(j, q) * 8;
+// Tokens as lanes: token j's row, depths from 16 k (place: where its first ones are;
+// the others differ in single bits of it).
+template <int NP>
+__device__ __forceinline__ int row_place(int j, int half) {
+  return j * NP + unit_place<NP>(j, half) * 8;
+}
+__device__ __forceinline__ Frag row_frag(const uint16_t* m, int place, int k) {
+  return *reinterpret_cast<const Frag*>(m + (place ^ (16 * k)));
+}
+
+// Tokens as depth: columns in the order of order4, tokens from 16 k.  Four lanes
+// point at a token's 16 columns, and lane l of each 16 gets column l of the four
+// tokens.
+__device__ __forceinline__ Frag join(bf16x4 lo, bf16x4 hi) {
+  return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ bf16x4 transposed(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) bf16x4 Lds;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<uint16_t*>(p)));
+}
+template <int NP>
+__device__ __forceinline__ int col_place(int lane) {
+  const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * order4(s & 3), j = 8 * half + (s >> 2);
+  return j * NP + unit_place<NP>(j, n >> 3) * 8 + (n & 7);
+}
+// (Four tokens on: only the bits of j & 4 differ.)
+template <int NP>
+__device__ __forceinline__ Frag col_frag(const uint16_t* m, int place, int nt, int k) {
+  constexpr int next = unit_place<NP>(4, 0) * 8;
+  return join(transposed(m + (place ^ (32 * nt)) + 16 * k * NP),
+              transposed(m + (place ^ (32 * nt) ^ next) + (16 * k + 4) * NP));
+}
+// The same of a slice of x, rows of 64 bytes, its columns in their own order: 4 rows
+// are read at once transposed, 16 as rows.
+__device__ __forceinline__ int x_place(int j, int c) {
+  return j * kSlice + ((c >> 3) ^ ((j >> 2) & 3)) * 8 + (c & 7);
+}
+__device__ __forceinline__ Frag x_frag(const uint16_t* x, int k, int lane) {
+  const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3);
+  const int j = 16 * k + 8 * half + (s >> 2);
+  return join(transposed(x + x_place(j, n)), transposed(x + x_place(j + 4, n)));
+}
+
+__device__ __forceinline__ float get(const Frag& f, int e) {
+  return e % 2 == 0 ? low_bf16(f[e / 2]) : high_bf16(f[e / 2]);
+}
+
+// v as a sum of PL bf16 values: PL = 3 are all of its 24 bits.
+template <int PL>
+__device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[PL]) {
 #pragma unroll
-    for (int k = 0; k < NP / 32; ++k)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(a + (place ^ (32 * k))),
-                                                    *reinterpret_cast<const bf16x8*>(b + (place ^ (32 * k))), acc, 0, 0, 0);
-    return acc;
-  }
-  // Tokens as depth: columns of tile m in the order of order4, tokens from 16 k.
-  // Four lanes point at a token's 16 columns, and lane l of each 16 gets column l of
-  // the four tokens.
-  static __device__ __forceinline__ bf16x4 transposed(const E* p) {
-    typedef __attribute__((address_space(3))) bf16x4 Lds;
-    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<E*>(p)));
-  }
-  template <int NP>
-  static __device__ __forceinline__ int col_place(int lane) {
-    const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * order4(s & 3), j = 8 * half + (s >> 2);
-    return j * NP + unit<NP>(j, n >> 3) * 8 + (n & 7);
-  }
-  // (Four tokens on: only the bits of j & 4 differ.)
-  template <int NP>
-  static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
-    constexpr int next = unit<NP>(4, 0) * 8;
-    return join(transposed(m + (place ^ (32 * nt)) + 16 * k * NP),
-                transposed(m + (place ^ (32 * nt) ^ next) + (16 * k + 4) * NP));
-  }
-  // The same of a slice of x, rows of 64 bytes, its columns in their own order: 4
-  // rows are read at once transposed, 16 as rows.
-  static __device__ __forceinline__ int xat(int j, int c) {
-    return j * kSlice + ((c >> 3) ^ ((j >> 2) & 3)) * 8 + (c & 7);
-  }
-  static __device__ __forceinline__ Frag xcol(const E* x, int k, int lane) {
-    const int half = lane >> 5, s = lane & 15, n = (lane & 16) + 4 * (s & 3);
-    const int j = 16 * k + 8 * half + (s >> 2);
-    return join(transposed(x + xat(j, n)), transposed(x + xat(j + 4, n)));
-  }
-  static __device__ __forceinline__ Frag of(const float (&v)[8]) {
-    Frag f;
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    return f;
-  }
-  static __device__ __forceinline__ float get(const Frag& f, int e) {
-    return e % 2 == 0 ? low_bf16(f[e / 2]) : high_bf16(f[e / 2]);
-  }
-  static __device__ __forceinline__ bool finite(const Frag (&x)[kChunk / 16]) {
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    uint32_t most = 0;
-#pragma unroll
-    for (int k = 0; k < kChunk / 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
-                                                                      __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu)));
-    return max(most >> 16, most & 0xffffu) < 0x7f80u;
-  }
-  typedef uint2 Quad;  // four elements
-  static __device__ __forceinline__ void four(Quad q, float (&v)[4]) {
-    v[0] = low_bf16(q.x), v[1] = high_bf16(q.x), v[2] = low_bf16(q.y), v[3] = high_bf16(q.y);
-  }
-  // v as a sum of kPlanes fragments.
-  static __device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[kPlanes]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a = v[2 * i], b = v[2 * i + 1];
-#pragma unroll
-      for (int p = 0; p < kPlanes; ++p) {
-        const uint32_t w = pack_bf16(a, b);
-        f[p][i] = w;
-        a -= low_bf16(w);
-        b -= high_bf16(w);
-      }
+    for (int p = 0; p < PL; ++p) {
+      const uint32_t w = pack_bf16(a, b);
+      f[p][i] = w;
+      a -= low_bf16(w);
+      b -= high_bf16(w);
     }
   }
-  static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ E pack(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
-};
+}
 
-struct MathF32 {
-  typedef float E;
-  struct Frag {
-    float e[8];
-  };
-  static constexpr int kUnit = 4;
-  static constexpr int kPlanes = 1;
-  static constexpr bool kPair = true;
+// Whether all of a slice's x (their first parts) are finite.
+__device__ __forceinline__ bool all_finite(uint32_t most) { return max(most >> 16, most & 0xffffu) < 0x7f80u; }
+__device__ __forceinline__ uint32_t most_of(uint32_t most, uint32_t pair) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                __builtin_bit_cast(u16x2, pair & 0x7fff7fffu)));
+}
 
-  template <int NP>
-  static constexpr __device__ __forceinline__ int unit(int j, int u) {
-    return u ^ (j & 7);
-  }
-  template <int NP>
-  static __device__ __forceinline__ int row_place(int j, int half) {
-    return j * NP + unit<NP>(j, 2 * half) * 4;
-  }
-  static __device__ __forceinline__ Frag row(const E* m, int place, int k) {
-    Frag f;
-    load_f32<float, 4>(m + (place ^ (16 * k)), *reinterpret_cast<float(*)[4]>(f.e));
-    load_f32<float, 4>(m + (place ^ (16 * k + 4)), *reinterpret_cast<float(*)[4]>(f.e + 4));
-    return f;
-  }
-  template <int NP>
-  static __device__ __forceinline__ f32x4 quadrant(const E* a, const E* b, int lane) {
-    const int j = lane & 15, q = lane >> 4;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const int place = j * NP + unit<NP>(j, q) * 4;
+__device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Frag& a, const Frag& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The product of two sums of parts, without the terms below the last part's (PL
+// parts of a value have its last bits at 2^-8 PL of it).
+template <int PL>
+__device__ __forceinline__ f32x16 mma_parts(const Frag (&a)[PL], const Frag (&b)[PL], f32x16 c) {
 #pragma unroll
-    for (int k = 0; k < NP / 16; ++k) {
-      const f32x4 av = *reinterpret_cast<const f32x4*>(a + (place ^ (16 * k))), bv = *reinterpret_cast<const f32x4*>(b + (place ^ (16 * k)));
+  for (int i = 0; i < PL; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], bv[e], acc, 0, 0, 0);
-    }
-    return acc;
-  }
-  template <int NP>
-  static __device__ __forceinline__ int col_place(int lane) {
-    const int half = lane >> 5, n = (lane & 19) + 4 * order4((lane >> 2) & 3);
-    return 8 * half * NP + n;
-  }
-  template <int NP>
-  static __device__ __forceinline__ Frag col(const E* m, int place, int nt, int k) {
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = m[(place ^ (32 * nt + 4 * e)) + (16 * k + e) * NP];
-    return f;
-  }
-  static __device__ __forceinline__ int xat(int j, int c) {
-    return j * kSlice + ((c >> 2) ^ ((j >> 1) & 7)) * 4 + (c & 3);
-  }
-  static __device__ __forceinline__ Frag xcol(const E* x, int k, int lane) {
-    const int half = lane >> 5;
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = x[xat(16 * k + 8 * half + e, lane & 31)];
-    return f;
-  }
-  static __device__ __forceinline__ Frag of(const float (&v)[8]) {
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f.e[e] = v[e];
-    return f;
-  }
-  static __device__ __forceinline__ float get(const Frag& f, int e) { return f.e[e]; }
-  static __device__ __forceinline__ bool finite(const Frag (&x)[kChunk / 16]) {
-    bool ok = true;
-#pragma unroll
-    for (int k = 0; k < kChunk / 16; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ok = ok && fabsf(x[k].e[e]) < __builtin_huge_valf();
-    return ok;
-  }
-  typedef f32x4 Quad;
-  static __device__ __forceinline__ void four(Quad q, float (&v)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = q[e];
-  }
-  static __device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[kPlanes]) { f[0] = of(v); }
-  static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.e[e], b.e[e], c, 0, 0, 0);
-    return c;
-  }
-  static __device__ __forceinline__ E pack(float v) { return v; }
-};
+    for (int j = 0; i + j < PL; ++j) c = mma(a[i], b[j], c);
+  return c;
+}
 
 // Per token of a chunk, for one head.  The state in the accumulators is 2^-K h, K
 // kept near 0 (kScaleMost), so that a chunk's decay need not be multiplied in each
@@ -273,7 +174,6 @@ struct MathF32 {
 //   r                           what L loses as one float
 struct alignas(16) ChunkScalars {
   float w[kChunk], p[kChunk], q[kChunk], r[kChunk];
-  float k, rescale, wide, pad;  // K; what the state is multiplied by before the chunk's part comes in
 };
 constexpr double kScaleMost = 20.0, kScaleFrom = 16.0;  // (a chunk that decays nothing leaves K alone)
 constexpr float kApartMost = 100.f;  // exponents of factors apart
@@ -309,10 +209,10 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-template <typename M, int NP>
+template <int PL, int NP>
 struct ChunkLds {
-  static constexpr int tile = kChunk * NP * (int)sizeof(typename M::E);
-  static constexpr int x_bytes = kChunk * kSlice * (int)sizeof(typename M::E);
+  static constexpr int tile = PL * kChunk * NP * 2;
+  static constexpr int x_bytes = PL * kChunk * kSlice * 2;
   // B, and a slice of x for each wavefront, for this chunk and `depth - 1` after it
   // that are on their way; the scalars of two chunks for each wavefront; C, G.
   static constexpr int x(int depth) { return depth * tile; }
@@ -321,6 +221,13 @@ struct ChunkLds {
   static constexpr int g(int depth) { return c(depth) + tile; }
   static constexpr int bytes(int depth, bool states) { return states ? c(depth) : g(depth) + kChunk * kChunk * 4; }
 };
+
+// Chunks in LDS at a time: by way of registers one; straight into LDS two, or three
+// where as many workgroups fit a CU with them.
+template <int NP, bool DIRECT, bool STATES>
+constexpr int chunk_depth() {
+  return !DIRECT ? 1 : STATES && NP <= 128 ? 3 : 2;
+}
 
 // 64 lanes' 16 bytes from base + off (bytes) to LDS at dst and on, lane by lane
 // (lanes that are off leave theirs as it was).  In asm because the compiler would
@@ -341,62 +248,74 @@ __device__ __forceinline__ void wait_memory() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory");
 }
 
-// kUnit elements of a row into LDS by way of registers; what lies outside becomes 0.
-template <typename T, typename M>
-__device__ __forceinline__ void stage_unit(typename M::E* to, const T* __restrict__ from, int left, bool vec) {
-  constexpr int U = M::kUnit;
-  if constexpr (sizeof(T) == 2 && sizeof(typename M::E) == 2) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (vec) {
-      if (left > 0) v = *reinterpret_cast<const uint4*>(from);
-    } else {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(from);
-      uint32_t e[U];
+// 8 elements of a row on their way to LDS; what lies outside becomes 0.  vec: rows
+// are whole units, aligned to 16 bytes.
+template <typename T>
+__device__ __forceinline__ void load_unit(const T* __restrict__ from, int left, bool vec, uint32_t (&v)[2 * sizeof(T)]) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) e[i] = i < left ? p[i] : 0u;
-      v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) v[i] = 0u;
+  if (vec) {
+    if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(from)[i];
+        v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+      }
     }
-    *reinterpret_cast<uint4*>(to) = v;
+  } else if constexpr (sizeof(T) == 2) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) v[e / 2] |= (uint32_t)p[e] << (16 * (e % 2));
   } else {
-    float v[U];
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(from);
 #pragma unroll
-    for (int i = 0; i < U; ++i) v[i] = 0.f;
-    if (vec) {
-      if (left > 0) load_f32<T, U>(from, v);
-    } else {
+    for (int e = 0; e < 8; ++e)
+      if (e < left) v[e] = p[e];
+  }
+}
+
+// ... and into LDS as PL parts, `apart` elements from one to the next.
+template <typename T, int PL>
+__device__ __forceinline__ void store_unit(uint16_t* to, int apart, const uint32_t (&v)[2 * sizeof(T)]) {
+  if constexpr (std::is_same<T, __hip_bfloat16>::value) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+  } else {
+    float f[8];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (i < left) v[i] = to_f32<T>(from[i]);
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (sizeof(T) == 4) f[e] = __uint_as_float(v[e]);
+      else f[e] = __half2float(__ushort_as_half((unsigned short)(v[e / 2] >> (16 * (e % 2)))));
     }
-    store_f32<float, U>(reinterpret_cast<float*>(to), v);
+    Frag p[PL];
+    split(f, p);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) *reinterpret_cast<Frag*>(to + i * apart) = p[i];
   }
 }
 
 // STATES: a segment's own part of the state, from a zero state, to `parts`, with
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
-// vec: rows are whole units, 16 bytes (or what makes 16 bytes in LDS) aligned.
-template <typename T, typename M, int NP, bool STATES>
-__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 4 ? 2 : 3) void k_scan_chunk(ScanArgs a,
-                                                                                                       ScanSplit sp,
-                                                                                                       bool vec) {
-  typedef typename M::E E;
-  typedef typename M::Frag Frag;
-  constexpr int Q = kChunk, KB = Q / 16, NT = NP / 32;
-  constexpr int U = M::kUnit;
+// PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
+// which go straight into LDS.
+template <typename T, int PL, int NP, bool DIRECT, bool STATES>
+__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_scan_chunk(ScanArgs a, ScanSplit sp,
+                                                                                   bool vec) {
+  constexpr int Q = kChunk, KB = Q / 16, NT = NP / 32, U = 8;
   constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits;  // of B and C at a time
   constexpr int kRounds = Q > kRows ? Q / kRows : 1;
   constexpr int kXUnits = kSlice / U, kXRows = kWave / kXUnits, kXRounds = Q / kXRows;
-  constexpr bool kDma = sizeof(T) == sizeof(E);
-  // (Three workgroups fit a CU with either.)
-  constexpr int kDepth = STATES && sizeof(E) == 2 && NP <= 128 ? 3 : 2;
-  typedef ChunkLds<M, NP> Lds;
+  constexpr int kDepth = chunk_depth<NP, DIRECT, STATES>();
+  constexpr int kTile = Q * NP, kX = Q * kSlice;  // elements of a part
+  constexpr bool kPair = PL == 3;                 // exponents to more than a float's bits
+  typedef ChunkLds<PL, NP> Lds;
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  E* const s_b0 = reinterpret_cast<E*>(lds);
-  E* const s_x0 = reinterpret_cast<E*>(lds + Lds::x(kDepth) + wave * kDepth * Lds::x_bytes);
+  uint16_t* const s_b0 = reinterpret_cast<uint16_t*>(lds);
+  uint16_t* const s_x0 = reinterpret_cast<uint16_t*>(lds + Lds::x(kDepth) + wave * kDepth * Lds::x_bytes);
   ChunkScalars* s_sc = reinterpret_cast<ChunkScalars*>(lds + Lds::scalars(kDepth)) + 2 * wave;
-  E* s_c = reinterpret_cast<E*>(lds + Lds::c(kDepth));
+  uint16_t* s_c = reinterpret_cast<uint16_t*>(lds + Lds::c(kDepth));
   float* const s_g = reinterpret_cast<float*>(lds + Lds::g(kDepth));
 
   // This workgroup's sequence, segment and group; this wavefront's head and columns.
@@ -432,6 +351,10 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
   const float bias = uniform(a.dt_bias != nullptr ? a.dt_bias[hd] : 0.f);
   const double A2 = uniform((double)a.A[hd] * 1.4426950408889634);  // exponents of 2
   double k_state = 0.0, l_seg = 0.0;  // (l_seg: the sum of the exponents)
+  // Of each of the two: K; what the state is multiplied by before the chunk's part
+  // comes in; whether the factors are an element's.
+  float k_of[2], rescale_of[2];
+  bool wide_of[2];
   T next_dt = from_f32<T>(0.f);
   // rest: tokens from the first of the two chunks on.
   auto load_dt = [&](const T* from, int64_t rest) {
@@ -446,44 +369,39 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
     const double l = half_sum_up_to(lane < rest ? A2 * (double)d : 0.0);
     const double end[2] = {lane_of(l, 31), lane_of(l, 63)};
     double k[3] = {k_state, 0.0, 0.0};
-    float rescale[2] = {1.f, 1.f};
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      k_of[c] = uniform((float)k[c]);
+      rescale_of[c] = 1.f;
       k[c + 1] = k[c] + end[c];
       if constexpr (STATES) l_seg = uniform(l_seg + end[c]);
       if (!(fabs(k[c + 1]) < kScaleMost)) {
         const double to = end[c] < 0.0 ? kScaleFrom : 0.0;
-        rescale[c] = exp2_hw((float)(k[c + 1] - to));
+        rescale_of[c] = uniform(exp2_hw((float)(k[c + 1] - to)));
         k[c + 1] = to;
       }
     }
     k_state = uniform(k[2]);
     ChunkScalars& sc = s_sc[half];
     sc.w[col] = exp2_hw((float)((half == 0 ? end[0] - k[1] : end[1] - k[2]) - l)) * d;
-    float wide = 0.f;
     if constexpr (!STATES) {
       float p = (float)l, q = d;
-      if constexpr (M::kPair) {
-        wide = 1.f;
+      if constexpr (kPair) {
+        wide_of[0] = wide_of[1] = true;
         sc.r[col] = (float)(l - (double)p);
       } else {
         const float off = (float)(l + (half == 0 ? k[0] : k[1])), fall = exp2_hw(-off) * d;
         // (Also where a factor of a later token is no number: it meets zeros of G.)
         const uint64_t no = __ballot(!(fabsf(off) < kApartMost && fabsf(fall) < __builtin_huge_valf()));
-        if ((half == 0 ? (uint32_t)no : (uint32_t)(no >> 32)) != 0u) {
-          wide = 1.f;
-        } else {
+        wide_of[0] = (uint32_t)no != 0u;
+        wide_of[1] = (uint32_t)(no >> 32) != 0u;
+        if (half == 0 ? !wide_of[0] : !wide_of[1]) {
           p = exp2_hw(off);
           q = fall;
         }
       }
       sc.p[col] = p;
       sc.q[col] = q;
-    }
-    if (col == 0) {
-      sc.k = (float)(half == 0 ? k[0] : k[1]);
-      sc.rescale = half == 0 ? rescale[0] : rescale[1];
-      sc.wide = wide;
     }
   };
 
@@ -511,121 +429,150 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
       for (int q = 0; q < 4; ++q) {
         const int n0 = 32 * nt + 16 * (q / 2) + 8 * half + 4 * (q % 2);
         const float* src = from + (int64_t)p * N + n0;
-        if (vec_n && n0 < N) {
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          h[nt][4 * q] = v.x, h[nt][4 * q + 1] = v.y, h[nt][4 * q + 2] = v.z, h[nt][4 * q + 3] = v.w;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (vec_n) {
+          if (n0 < N) load_f32<float, 4>(src, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (n0 + e < N) h[nt][4 * q + e] = src[e];
+            if (n0 + e < N) v[e] = src[e];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[nt][4 * q + e] = v[e];
       }
   }
 
-  // A whole chunk of aligned rows goes from memory to LDS while the chunk before
-  // it is worked on: B to its other buffer, C and x once their readers are done.
-  // Other chunks are staged by way of registers when their turn comes.
   const int bj = threadIdx.x / kRowUnits, bv = threadIdx.x % kRowUnits;
   const int xj = lane / kXUnits, xv = lane % kXUnits;
-  auto ahead = [&](int64_t rest) { return kDma && vec && rest >= Q; };
   const bool whole_n = N == NP, whole_p = p0 + kSlice <= P;
-  auto load_rows = [&](const T* base, int stride, E* to) {
+  // DIRECT: a whole chunk goes from memory to LDS while chunks before it are worked on:
+  // B and x to a buffer of their own, C once its readers are done.  (The last chunk, if
+  // it is not whole, is staged by way of registers when its turn comes.)
+  auto ahead = [&](int64_t rest) { return DIRECT && rest >= Q; };
+  auto load_rows = [&](const T* base, int stride, uint16_t* to) {
     const char* from = reinterpret_cast<const char*>(base);
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int u = M::template unit<NP>(r * kRows + bj, bv);
+      const int u = unit_place<NP>(r * kRows + bj, bv);
       const uint32_t off = (uint32_t)(bj * stride + u * U) * (uint32_t)sizeof(T);
-      E* dst = to + (r * kThreads + wave * kWave) * U;
+      uint16_t* dst = to + (r * kThreads + wave * kWave) * U;
       if (kRows <= Q && whole_n) load_to_lds(from, off, dst);
       else if (u * U < N && bj < Q) load_to_lds(from, off, dst);
       from += (uint32_t)(kRows * stride) * (uint32_t)sizeof(T);
     }
   };
-  auto load_x = [&](E* to) {
+  auto load_x = [&](uint16_t* to) {
     if (!on) return;
     const char* from = reinterpret_cast<const char*>(x);
 #pragma unroll
     for (int r = 0; r < kXRounds; ++r) {
-      const int u = M::xat(r * kXRows + xj, xv * U) % kSlice / U;
+      const int u = x_place(r * kXRows + xj, xv * U) % kSlice / U;
       const uint32_t off = (uint32_t)(xj * x_t + u * U) * (uint32_t)sizeof(T);
       if (whole_p) load_to_lds(from, off, to + r * kWave * U);
       else if (p0 + u * U < P) load_to_lds(from, off, to + r * kWave * U);
       from += (uint32_t)(kXRows * x_t) * (uint32_t)sizeof(T);
     }
   };
-  auto stage_rows = [&](const T* base, int stride, E* to, int len) {
+  // By way of registers: the next chunk's B, C and x wait in them.
+  constexpr int kWords = 2 * (int)sizeof(T);
+  uint32_t nb[kRounds][kWords], nc[STATES ? 1 : kRounds][kWords], nx[kXRounds][kWords];
+  auto fetch = [&](const T* b_from, const T* c_from, const T* x_from, int len, bool vec) {
+#pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int j = r * kRows + bj;
-      if (j >= Q) break;
-      stage_unit<T, M>(to + j * NP + M::template unit<NP>(j, bv) * U, base + ((int64_t)j * stride + bv * U),
-                       j < len ? N - bv * U : 0, vec);
+      load_unit<T>(b_from + ((int64_t)(r * kRows) * b_t + (bj * b_t + bv * U)), j < len ? N - bv * U : 0, vec, nb[r]);
+      if constexpr (!STATES)
+        load_unit<T>(c_from + ((int64_t)(r * kRows) * c_t + (bj * c_t + bv * U)), j < len ? N - bv * U : 0, vec, nc[r]);
     }
+#pragma unroll
+    for (int r = 0; r < kXRounds; ++r)
+      load_unit<T>(x_from + ((int64_t)(r * kXRows) * x_t + (xj * x_t + xv * U)),
+                   on && r * kXRows + xj < len ? P - p0 - xv * U : 0, vec, nx[r]);
+  };
+  auto unload = [&](uint16_t* to_b, uint16_t* to_x) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int j = r * kRows + bj;
+      if (kRows > Q && j >= Q) break;
+      const int at = j * NP + unit_place<NP>(j, bv) * U;
+      store_unit<T, PL>(to_b + at, kTile, nb[r]);
+      if constexpr (!STATES) store_unit<T, PL>(s_c + at, kTile, nc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kXRounds; ++r) store_unit<T, PL>(to_x + x_place(r * kXRows + xj, xv * U), kX, nx[r]);
   };
   int64_t left = t1 - t0;  // tokens from this chunk on
   for (int i = threadIdx.x * 4; i < Lds::bytes(kDepth, STATES) / 4; i += kThreads * 4)
     store_f32<float, 4>(reinterpret_cast<float*>(lds) + i, {0.f, 0.f, 0.f, 0.f});
   __syncthreads();
+  if constexpr (DIRECT) {
 #pragma unroll
-  for (int c = 0; c < kDepth - 1; ++c) {
-    if (ahead(left - c * Q)) {
-      load_rows(B, b_t, s_b0 + c * Q * NP);
-      if (c == 0 && !STATES) load_rows(C, c_t, s_c);
-      load_x(s_x0 + c * Q * kSlice);
+    for (int c = 0; c < kDepth - 1; ++c) {
+      if (ahead(left - c * Q)) {
+        load_rows(B, b_t, s_b0 + c * kTile);
+        if (c == 0 && !STATES) load_rows(C, c_t, s_c);
+        load_x(s_x0 + c * kX);
+      }
+      B += (int64_t)Q * b_t;
+      x += (int64_t)Q * x_t;
     }
-    B += (int64_t)Q * b_t;
-    x += (int64_t)Q * x_t;
+  } else if (left > 0) {
+    fetch(B, C, x, (int)(left < Q ? left : Q), vec);
   }
   load_dt(dt, left);
   write_scalars(left);
   // Every wavefront issues as many memory operations to a chunk as any: the latest
   // may be left under way at the next.
-  const bool counted = kDma && vec && on && whole_n && whole_p && kRows <= Q;
+  const bool counted = DIRECT && on && whole_n && whole_p && kRows <= Q;
 
   for (int i = 0; left > 0; left -= Q, ++i) {
     const int len = (int)(left < Q ? left : Q);
     const int at = i % kDepth, at_last = (i + kDepth - 1) % kDepth;
-    const E* s_b = s_b0 + at * Q * NP;
-    const E* s_x = s_x0 + at * Q * kSlice;
-    if (!ahead(left)) {
-      const T* b_now = B - (int64_t)(kDepth - 1) * Q * b_t;
-      const T* x_now = x - (int64_t)(kDepth - 1) * Q * x_t;
-      stage_rows(b_now, b_t, s_b0 + at * Q * NP, len);
-      if constexpr (!STATES) stage_rows(C, c_t, s_c, len);
-      for (int r = 0; r < kXRounds; ++r) {
-        const int j = r * kXRows + xj;
-        stage_unit<T, M>(s_x0 + at * Q * kSlice + M::xat(j, xv * U), x_now + ((int64_t)j * x_t + xv * U),
-                         on && j < len ? P - p0 - xv * U : 0, vec);
+    const uint16_t* s_b = s_b0 + at * PL * kTile;
+    const uint16_t* s_x = s_x0 + at * PL * kX;
+    if constexpr (DIRECT) {
+      if (!ahead(left)) {
+        fetch(B - (int64_t)(kDepth - 1) * Q * b_t, C, x - (int64_t)(kDepth - 1) * Q * x_t, len, true);
+        unload(s_b0 + at * kTile, s_x0 + at * kX);
       }
-    }
-    // This chunk has arrived.  Issued after it: the chunk before's y (four stores), or
-    // the next chunk's B and x.
-    if (counted && (STATES ? kDepth == 3 && ahead(left - Q) : i > 0)) wait_memory<STATES ? kRounds + kXRounds : 4>();
-    else wait_memory<0>();
-    __syncthreads();
-    if (ahead(left - (kDepth - 1) * Q)) {
-      load_rows(B, b_t, s_b0 + at_last * Q * NP);
-      load_x(s_x0 + at_last * Q * kSlice);
+      // This chunk has arrived.  Issued after it: the chunk before's y (four stores), or
+      // the next chunk's B and x.
+      if (counted && (STATES ? kDepth == 3 && ahead(left - Q) : i > 0)) wait_memory<STATES ? kRounds + kXRounds : 4>();
+      else wait_memory<0>();
+      __syncthreads();
+      if (ahead(left - (kDepth - 1) * Q)) {
+        load_rows(B, b_t, s_b0 + at_last * kTile);
+        load_x(s_x0 + at_last * kX);
+      }
+    } else {
+      if (i > 0) __syncthreads();  // the chunk before's readers
+      unload(s_b0, s_x0);
+      __syncthreads();
     }
     // The steps to the next chunk.
     B += (int64_t)Q * b_t;
     C += (int64_t)Q * c_t;
     x += (int64_t)Q * x_t;
+    if constexpr (!DIRECT) {
+      if (left > Q) fetch(B, C, x, (int)(left - Q < Q ? left - Q : Q), vec);
+    }
     if (i % 2 == 0) {
       dt += (int64_t)(2 * Q) * dt_t;
       load_dt(dt, left - 2 * Q);
     }
     const ChunkScalars& sc = s_sc[i & 1];
-    const float rescale = uniform(sc.rescale);
+    const float rescale = i % 2 == 0 ? rescale_of[0] : rescale_of[1];
     // (Opaque: places of single reads and comparisons are made from these when they
     // are wanted.  Kept in registers from chunk to chunk they would spill, and a
     // reload waits for all of the loads ahead: 283 -> 358 us.)
-    int row_at = M::template row_place<NP>(col, half), col_at = M::template col_place<NP>(lane);
-    int ln = lane;
+    int row_at = row_place<NP>(col, half), col_at = col_place<NP>(lane), ln = lane;
     asm volatile("" : "+v"(row_at), "+v"(col_at), "+v"(ln));
-
-    Frag xf[KB];
+    Frag xf[KB][PL];
 #pragma unroll
-    for (int k = 0; k < KB; ++k) xf[k] = M::xcol(s_x, k, ln);
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int pl = 0; pl < PL; ++pl) xf[k][pl] = x_frag(s_x + pl * kX, k, ln);
+
     if constexpr (!STATES) {
       // Element (i, j) of G: the 8 tokens j of a fragment lie together.
       auto g_at = [&](int i, int j) { return s_g + ((j / 8) * 32 + i) * 8 + j % 8; };
@@ -633,7 +580,21 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
       // quadrants on and below the diagonal ----
       if (wave < 3) {
         const int iq = wave > 0 ? 1 : 0, jq = wave > 1 ? 1 : 0, ci = ln & 15, j0 = 4 * (ln >> 4);
-        const f32x4 acc = M::template quadrant<NP>(s_b + 16 * jq * NP, s_c + 16 * iq * NP, ln);
+        const int place = ci * NP + unit_place<NP>(ci, ln >> 4) * 8;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NP / 32; ++k) {
+          Frag bf[PL], cf[PL];
+#pragma unroll
+          for (int pl = 0; pl < PL; ++pl) {
+            bf[pl] = *reinterpret_cast<const Frag*>(s_b + pl * kTile + 16 * jq * NP + (place ^ (32 * k)));
+            cf[pl] = *reinterpret_cast<const Frag*>(s_c + pl * kTile + 16 * iq * NP + (place ^ (32 * k)));
+          }
+#pragma unroll
+          for (int u = 0; u < PL; ++u)
+#pragma unroll
+            for (int v = 0; u + v < PL; ++v) acc = mma16(bf[u], cf[v], acc);
+        }
         float gv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) gv[e] = iq > jq || j0 + e <= ci ? acc[e] : 0.f;
@@ -648,65 +609,92 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         float hv[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) hv[e] = h[k / 2][8 * (k % 2) + e];
-        acc = M::mma(M::of(hv), M::row(s_c, row_at, k), acc);
-      }
-      typename M::Quad xr[4];  // this token's x, for D
+        Frag hf[PL], cf[PL];
+        split(hv, hf);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) xr[q] = *reinterpret_cast<const typename M::Quad*>(s_x + M::xat(ln & 31, 8 * q + 4 * (ln >> 5)));
-      const float my_p = sc.p[col], my_r = M::kPair ? sc.r[col] : 0.f;
-      const bool wide = uniform(sc.wide) != 0.f;
+        for (int pl = 0; pl < PL; ++pl) cf[pl] = row_frag(s_c + pl * kTile, row_at, k);
+        acc = mma_parts(hf, cf, acc);
+      }
+      // This token's x, for D.
+      auto own_x = [&](int q, float (&v)[4]) {
+        v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+        for (int pl = PL - 1; pl >= 0; --pl) {
+          const uint2 u = *reinterpret_cast<const uint2*>(s_x + pl * kX + x_place(ln & 31, 8 * q + 4 * (ln >> 5)));
+          v[0] += low_bf16(u.x), v[1] += high_bf16(u.x), v[2] += low_bf16(u.y), v[3] += high_bf16(u.y);
+        }
+      };
+      uint2 xr[PL == 1 ? 4 : 1];  // (one part: read before the barrier)
+      if constexpr (PL == 1) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          xr[q] = *reinterpret_cast<const uint2*>(s_x + x_place(ln & 31, 8 * q + 4 * (ln >> 5)));
+      }
+      const float my_p = sc.p[col], my_r = kPair ? sc.r[col] : 0.f;
+      const bool wide = kPair || (i % 2 == 0 ? wide_of[0] : wide_of[1]);
       __syncthreads();
       if (ahead(left - Q)) load_rows(C, c_t, s_c);
 
       // ---- x^T S: S[i][j] = G[i][j] 2^(L_i - L_j) d_j for j <= i ----
       // Factors apart: 2^(L_i + K) is multiplied in at the end; G is 0 above the diagonal.
-      const bool finite = __ballot(!M::finite(xf)) == 0ull;
+      uint32_t most = 0;
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = most_of(most, xf[k][0][e]);
+      const bool finite = __ballot(!all_finite(most)) == 0ull;
       auto factor = [&](float pj, float qj, float rj) {
         float delta = my_p - pj;
-        if constexpr (M::kPair) delta += my_r - rj;
+        if constexpr (kPair) delta += my_r - rj;
         return exp2_hw(delta) * qj;
       };
       if (wide) {
-        const float f = exp2_hw(my_p + sc.k);
+        const float f = exp2_hw(my_p + (i % 2 == 0 ? k_of[0] : k_of[1]));
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] *= f;
       }
-      if (finite && (M::kPair || !wide)) {
+      if (finite && (kPair || !wide)) {
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
           float s[8];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int j0 = 16 * k + 8 * half + 4 * q;
+            const int j0 = 16 * k + 8 * (ln >> 5) + 4 * q;
             float gv[4], pv[4], qv[4], rv[4];
-            load_f32<float, 4>(g_at(ln & 31, 16 * k + 8 * (ln >> 5) + 4 * q), gv);
+            load_f32<float, 4>(g_at(ln & 31, j0), gv);
             load_f32<float, 4>(sc.q + j0, qv);
-            if constexpr (M::kPair) {
+            if constexpr (kPair) {
               load_f32<float, 4>(sc.p + j0, pv);
               load_f32<float, 4>(sc.r + j0, rv);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if constexpr (M::kPair) {
+              if constexpr (kPair) {
                 const float v = gv[e] * factor(pv[e], qv[e], rv[e]);
-                s[4 * q + e] = j0 + e <= col ? v : 0.f;
+                s[4 * q + e] = j0 + e <= (ln & 31) ? v : 0.f;
               } else {
                 s[4 * q + e] = gv[e] * qv[e];
               }
             }
           }
-          acc = M::mma(xf[k], M::of(s), acc);
+          Frag sf[PL];
+          split(s, sf);
+          acc = mma_parts(xf[k], sf, acc);
         }
       } else {
         // Term by term: an x that is not finite must not meet the zeros of S, and a
         // decay that leaves a float's range in the chunk has no factors apart.
         for (int j = 0; j < Q; ++j) {
           const float gv = *g_at(col, j);
-          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], M::kPair ? sc.r[j] : 0.f) : sc.q[j]);
+          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], kPair ? sc.r[j] : 0.f) : sc.q[j]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float xq[4];
-            M::four(*reinterpret_cast<const typename M::Quad*>(s_x + M::xat(j, 8 * q + 4 * half)), xq);
+            float xq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int pl = PL - 1; pl >= 0; --pl) {
+              const uint2 u = *reinterpret_cast<const uint2*>(s_x + pl * kX + x_place(j, 8 * q + 4 * half));
+              xq[0] += low_bf16(u.x), xq[1] += high_bf16(u.x), xq[2] += low_bf16(u.y), xq[3] += high_bf16(u.y);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[4 * q + e] = j <= col ? fmaf(s, xq[e], acc[4 * q + e]) : acc[4 * q + e];
           }
@@ -716,13 +704,14 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float xq[4];
-        M::four(xr[q], xq);
+        if constexpr (PL == 1) xq[0] = low_bf16(xr[q].x), xq[1] = high_bf16(xr[q].x), xq[2] = low_bf16(xr[q].y), xq[3] = high_bf16(xr[q].y);
+        else own_x(q, xq);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[4 * q + e] = fmaf(acc[4 * q + e], f, D * xq[e]);
       }
       if (on && col < len) {
         T* row = y + (col * y_t + 4 * half);
-        if (vec && whole_p) {
+        if ((DIRECT || vec) && whole_p) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) store_f32<T, 4>(row + 8 * q, {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
         } else {
@@ -733,6 +722,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
       }
       y += (int64_t)Q * y_t;
     }
+
     // ---- h <- 2^L_end h + B^T v ----
     if (rescale != 1.f) {
 #pragma unroll
@@ -748,16 +738,26 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
         float wv[4];
         load_f32<float, 4>(sc.w + 16 * k + 8 * half + 4 * q, wv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = M::get(xf[k], 4 * q + e) * wv[e];
+        for (int e = 0; e < 4; ++e) {
+          float xv = get(xf[k][PL - 1], 4 * q + e);
+#pragma unroll
+          for (int pl = PL - 2; pl >= 0; --pl) xv += get(xf[k][pl], 4 * q + e);
+          v[4 * q + e] = xv * wv[e];
+        }
       }
-      Frag vf[M::kPlanes], bt[NT];
-      M::split(v, vf);
+      Frag vf[3];
+      split(v, vf);
+      // (All 24 bits of v against the parts of B, largest terms first.)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) bt[nt] = M::template col<NP>(s_b, col_at, nt, k);
+      for (int pl = 0; pl < PL; ++pl) {
+        Frag bt[NT];
 #pragma unroll
-      for (int pl = 0; pl < M::kPlanes; ++pl)
+        for (int nt = 0; nt < NT; ++nt) bt[nt] = col_frag<NP>(s_b + pl * kTile, col_at, nt, k);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) h[nt] = M::mma(bt[nt], vf[pl], h[nt]);
+        for (int u = 0; u + pl < 3; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) h[nt] = mma(bt[nt], vf[u], h[nt]);
+      }
     }
     if (i % 2 == 1 && left > Q) write_scalars(left - Q);
   }
@@ -770,20 +770,18 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : sizeof(typename M::E) == 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) h[nt][r] *= f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n0 = 32 * nt + 16 * (q / 2) + 8 * half + 4 * (q % 2);
         float* dst = to + (int64_t)p * N + n0;
-        if (vec_n && n0 < N) {
-          *reinterpret_cast<float4*>(dst) =
-              make_float4(h[nt][4 * q], h[nt][4 * q + 1], h[nt][4 * q + 2], h[nt][4 * q + 3]);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = h[nt][4 * q + e] * f;
+        if (vec_n) {
+          if (n0 < N) store_f32<float, 4>(dst, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (n0 + e < N) dst[e] = h[nt][4 * q + e];
+            if (n0 + e < N) dst[e] = v[e];
         }
       }
   }
@@ -812,27 +810,23 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
   }
 }
 
-template <typename T, typename M, int NP, bool STATES>
-int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
-  typedef ChunkLds<M, NP> Lds;
-  const int rc = set_lds_limit_once<k_scan_chunk<T, M, NP, STATES>>(kMaxLdsBytes);
+template <typename T, int PL, int NP, bool DIRECT, bool STATES>
+int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
+  const int rc = set_lds_limit_once<k_scan_chunk<T, PL, NP, DIRECT, STATES>>(kMaxLdsBytes);
   if (rc != (int)hipSuccess) return rc;
-  constexpr int U = M::kUnit;
-  const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g | a.y_b | a.y_t | a.y_h;
-  const bool vec = strides % U == 0 && a.head_dim % U == 0 && a.state_dim % U == 0 && aligned_to(a.x, U * sizeof(T)) &&
-                   aligned_to(a.b, U * sizeof(T)) && aligned_to(a.c, U * sizeof(T)) && aligned_to(a.y, U * sizeof(T));
+  constexpr int lds = ChunkLds<PL, NP>::bytes(chunk_depth<NP, DIRECT, STATES>(), STATES);
+  static_assert(lds <= kMaxLdsBytes, "a workgroup's LDS");
   const int64_t blocks = a.seq.batch * (STATES ? sp.segments - 1 : sp.segments) * a.groups * sp.blocks;
   return launch_blocks(a, &ScanArgs::block0, blocks, [&](const ScanArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_scan_chunk<T, M, NP, STATES>), dim3(n), dim3(kThreads), Lds::bytes(STATES && sizeof(typename M::E) == 2 && NP <= 128 ? 3 : 2, STATES), stream,
-                       la, sp, vec);
+    hipLaunchKernelGGL((k_scan_chunk<T, PL, NP, DIRECT, STATES>), dim3(n), dim3(kThreads), lds, stream, la, sp, vec);
   });
 }
 
-template <typename T, typename M, int NP>
-int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
+template <typename T, int PL, int NP, bool DIRECT>
+int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
   if (sp.segments > 1) {
     timing_begin(K_SCAN_PARTS, stream);
-    int rc = launch_chunk_k<T, M, NP, true>(a, sp, stream);
+    int rc = launch_chunk_k<T, PL, NP, DIRECT, true>(a, sp, vec, stream);
     if (rc == (int)hipSuccess) {
       const int64_t plane = (int64_t)a.head_dim * a.state_dim;
       const int64_t blocks = (plane + kChainThreads - 1) / kChainThreads;
@@ -844,17 +838,17 @@ int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
     if (rc != (int)hipSuccess) return rc;
   }
   timing_begin(K_SCAN_CHUNK, stream);
-  const int rc = launch_chunk_k<T, M, NP, false>(a, sp, stream);
+  const int rc = launch_chunk_k<T, PL, NP, DIRECT, false>(a, sp, vec, stream);
   timing_end(K_SCAN_CHUNK, stream);
   return rc;
 }
 
-template <typename T, typename M>
-int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
-  if (a.state_dim <= 32) return launch_chunk_n<T, M, 32>(a, sp, stream);
-  if (a.state_dim <= 64) return launch_chunk_n<T, M, 64>(a, sp, stream);
-  if (a.state_dim <= 128) return launch_chunk_n<T, M, 128>(a, sp, stream);
-  return launch_chunk_n<T, M, 256>(a, sp, stream);
+template <typename T, int PL, bool DIRECT>
+int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
+  if (a.state_dim <= 32) return launch_chunk_n<T, PL, 32, DIRECT>(a, sp, vec, stream);
+  if (a.state_dim <= 64) return launch_chunk_n<T, PL, 64, DIRECT>(a, sp, vec, stream);
+  if (a.state_dim <= 128) return launch_chunk_n<T, PL, 128, DIRECT>(a, sp, vec, stream);
+  return launch_chunk_n<T, PL, 256, DIRECT>(a, sp, vec, stream);
 }
 
 size_t align16(size_t v) { return (v + 15) / 16 * 16; }
@@ -868,10 +862,12 @@ ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int 
   if (!p.chunked || batch < 1) return p;
   const int units = heads / groups * ((head_dim + kSlice - 1) / kSlice);
   p.split.blocks = (units + kWaves - 1) / kWaves;
-  // Segments: enough workgroups for two on a CU, with at least four chunks each.
+  // Segments: enough workgroups for all that fit the CUs at once, with at least four
+  // chunks each.
+  const int64_t fit = state_dim > 128 ? 1 : dtype == SF_BF16 ? 3 : 2;
   const int64_t chunks = (max_len + kChunk - 1) / kChunk;
   const int64_t base = batch * groups * p.split.blocks;
-  int64_t segs = (3 * (int64_t)num_cus() + base - 1) / base;
+  int64_t segs = (fit * num_cus() + base - 1) / base;
   if (segs > chunks / 4) segs = chunks / 4;
   if (segs < 1) segs = 1;
   const int64_t per = (chunks + segs - 1) / segs;
@@ -896,9 +892,13 @@ int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int
   ScanSplit sp = p.split;
   sp.parts = static_cast<float*>(workspace);
   sp.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums_at);
-  if (dtype == SF_BF16) return launch_chunk_m<__hip_bfloat16, MathBf16>(a, sp, stream);
-  if (dtype == SF_F16) return launch_chunk_m<__half, MathF32>(a, sp, stream);
-  return launch_chunk_m<float, MathF32>(a, sp, stream);
+  const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g | a.y_b | a.y_t | a.y_h;
+  const bool vec = strides % 8 == 0 && a.head_dim % 8 == 0 && a.state_dim % 8 == 0 && aligned_to(a.x, 16) &&
+                   aligned_to(a.b, 16) && aligned_to(a.c, 16) && aligned_to(a.y, 16);
+  if (dtype == SF_F32) return launch_chunk_m<float, 3, false>(a, sp, vec, stream);
+  if (dtype == SF_F16) return launch_chunk_m<__half, 2, false>(a, sp, vec, stream);
+  if (vec) return launch_chunk_m<__hip_bfloat16, 1, true>(a, sp, vec, stream);
+  return launch_chunk_m<__hip_bfloat16, 1, false>(a, sp, vec, stream);
 }
 
 }  // namespace sf
