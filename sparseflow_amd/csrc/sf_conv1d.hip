@@ -2,17 +2,18 @@
 //   y[t, c] = act(bias[c] + sum_k w[c, k] u[t - K + 1 + k, c])
 // (u before the sequence's start: the state, or zeros).
 //
-// A thread owns V neighbouring channels and a run of kRun tokens: the last
-// K - 1 inputs stay in registers as the run is walked, every input of the run is
-// one load of 16 bytes, and the K - 1 before it are read again (from the cache:
-// a neighbouring thread's run).  Bound by HBM: x in, y out.
+// A thread owns V neighbouring channels and a run of tokens: the last K - 1 inputs
+// stay in registers as the run is walked, every input of the run is one load of 16
+// bytes, kBatch of them under way at a time, and the K - 1 before the run are read
+// again (from the cache: a neighbouring thread's run).  Bound by HBM: x in, y out.
 #include "sf_seq.h"
+#include "sf_tile.h"
 
 namespace sf {
 
 namespace {
 
-constexpr int kRun = 16;  // tokens of a thread
+constexpr int kBatch = 8;  // tokens loaded at a time
 constexpr int kThreads = 256;
 
 template <typename T, int V, bool VEC>
@@ -27,7 +28,7 @@ __device__ __forceinline__ void conv_load(const T* __restrict__ p, int ch, int c
 
 template <typename T, int K, int V, bool VEC>
 __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv, int blocks_per_seq, int runs,
-                                                            int keep) {
+                                                            int length, int keep) {
   const int64_t block = a.block0 + blockIdx.x;
   const int64_t b = block / blocks_per_seq;
   const int64_t item = (block - b * blocks_per_seq) * kThreads + threadIdx.x;
@@ -36,10 +37,10 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
   const int ch = (int)(item - (int64_t)run * cv) * V;
   int64_t first, n;
   seq_rows(a.seq, b, first, n);
-  const int64_t t0 = (int64_t)run * kRun;
+  const int64_t t0 = (int64_t)run * length;
   if (t0 >= n && run > 0) return;
   // (max_len sizes the launch: where a sequence is longer, its last run goes on.)
-  const int64_t t1 = run == runs - 1 ? n : (t0 + kRun < n ? t0 + kRun : n);
+  const int64_t t1 = run == runs - 1 ? n : (t0 + length < n ? t0 + length : n);
   const bool last = t1 == n;
   const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + first * a.x_t;
   T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + first * a.y_t;
@@ -76,8 +77,10 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
       for (int i = 0; i < V; ++i) u[k][i] = 0.f;
     }
   }
-  for (int64_t t = t0; t < t1; ++t) {
-    conv_load<T, V, VEC>(x + t * a.x_t, ch, a.channels, u[K - 1]);
+  const T* __restrict__ xt = x + t0 * a.x_t;
+  T* __restrict__ yt = y + t0 * a.y_t + ch;
+  // One token: u's last input has come in.
+  auto token = [&]() {
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -86,12 +89,33 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
       for (int k = 0; k < K; ++k) s[i] = fmaf(w[k][i], u[k][i], s[i]);
       if (a.act == SF_ACT_SILU) s[i] = silu(s[i]);
     }
-    if constexpr (VEC) store_f32<T, V>(y + t * a.y_t + ch, s);
-    else y[t * a.y_t + ch] = from_f32<T>(s[0]);
+    if constexpr (VEC) store_f32<T, V>(yt, s);
+    else *yt = from_f32<T>(s[0]);
+    yt += a.y_t;
 #pragma unroll
     for (int k = 0; k + 1 < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) u[k][i] = u[k + 1][i];
+  };
+  int64_t left = t1 - t0;
+  for (; left >= kBatch; left -= kBatch) {
+    Vec<T, V> in[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      in[j] = *reinterpret_cast<const Vec<T, V>*>(xt + ch);
+      xt += a.x_t;
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[K - 1][i] = to_f32<T>(in[j].e[i]);
+      token();
+    }
+  }
+  for (; left > 0; --left) {
+    conv_load<T, V, VEC>(xt, ch, a.channels, u[K - 1]);
+    xt += a.x_t;
+    token();
   }
   if (last && keep && slot >= 0) {
     T* after = static_cast<T*>(a.after) + slot * (K - 1) * (int64_t)a.channels;
@@ -130,7 +154,11 @@ __global__ __launch_bounds__(kThreads) void k_conv1d_state(Conv1dArgs a, int blo
 template <typename T, int K, int V, bool VEC>
 int launch_conv1d_v(const Conv1dArgs& a, hipStream_t stream) {
   const int cv = a.channels / V;
-  const int64_t runs = a.max_len > kRun ? (a.max_len + kRun - 1) / kRun : 1;
+  // Runs as long as leave a few wavefronts for every SIMD (16 tokens read 3 / 16 of
+  // their inputs twice, 64 less than a twentieth).
+  int length = 64;
+  while (length > 8 && a.seq.batch * cv * ((a.max_len + length - 1) / length) < (int64_t)num_cus() * 4 * 4 * kWave) length /= 2;
+  const int64_t runs = a.max_len > length ? (a.max_len + length - 1) / length : 1;
   const int64_t per_seq = (runs * cv + kThreads - 1) / kThreads;
   // In place: a step's thread holds all that it overwrites; in a prompt the
   // thread that writes a state is not the one that read it, unless there is one
@@ -141,7 +169,7 @@ int launch_conv1d_v(const Conv1dArgs& a, hipStream_t stream) {
   const bool apart = keep && runs > 1 && a.before != nullptr && p0 < p1 + pool && p1 < p0 + pool;
   int rc = launch_blocks(a, &Conv1dArgs::block0, a.seq.batch * per_seq, [&](const Conv1dArgs& la, unsigned n) {
     hipLaunchKernelGGL((k_causal_conv1d<T, K, V, VEC>), dim3(n), dim3(kThreads), 0, stream, la, cv, (int)per_seq,
-                       (int)runs, keep && !apart ? 1 : 0);
+                       (int)runs, length, keep && !apart ? 1 : 0);
   });
   if (rc != (int)hipSuccess || !apart) return rc;
   const int64_t blocks = (a.channels + kThreads - 1) / kThreads;

@@ -2,8 +2,9 @@
 // each row:
 //   t = act(gate) x (gate first), t *= w / rms(t) over each group, t *= act(gate),
 //   r = residual + scale t, h = r w' / rms(r)
-// A row is held in registers by LT threads, E elements in each as vectors of V:
-// read once, two sums over it, written once.  Bound by HBM.
+// A row is held in registers by LT threads, vectors of V elements: x, gate and residual
+// are all loaded before the first sum, and h is written after the second.  Bound by
+// HBM.  Short rows (4 vectors a lane) are a wavefront's, whose sums need no barrier.
 //
 // Groups are rows of their own where no norm of the whole row follows; otherwise
 // a workgroup holds the row and the groups' sums meet in LDS.
@@ -37,7 +38,9 @@ __device__ __forceinline__ float row_sum(float v, float* s_part) {
 }
 
 // sub: groups that are rows of their own (1: the whole row).  GROUPED: groups
-// inside the row (LT = the workgroup, group % V == 0).
+// inside the row (LT = the workgroup, group % V == 0).  (Workgroups that go row after
+// row with their weights in registers were no faster: 226 against 214 us at
+// 32768 x 2048, f16 with a float32 residual.)
 template <typename T, typename TR, int LT, int V, int NV, bool GROUPED>
 __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormArgs a, int sub) {
   constexpr int kRowsPerBlock = (LT > kBlock ? LT : kBlock) / LT;
@@ -46,28 +49,31 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
   const int width = a.dim / sub;
   const int64_t item = (a.item0 + blockIdx.x) * kRowsPerBlock + threadIdx.x / LT;
   if (item >= a.outer * a.inner * sub) return;  // (LT > 64 has one row to a workgroup)
-  const int64_t row = item / sub;
-  const int c0 = (int)(item - row * sub) * width;
-  const int64_t o = row / a.inner, i = row - o * a.inner;
+  const int64_t row = sub == 1 ? item : item / sub;
+  const int c0 = sub == 1 ? 0 : (int)(item - row * sub) * width;
+  const int64_t o = a.outer == 1 ? 0 : row / a.inner, i = row - o * a.inner;
   const T* __restrict__ x = static_cast<const T*>(a.x) + o * a.x_o + i * a.x_i + c0;
+  const T* __restrict__ g = static_cast<const T*>(a.gate) + o * a.g_o + i * a.g_i + c0;
+  const TR* __restrict__ res = static_cast<const TR*>(a.res) + o * a.res_o + i * a.res_i + c0;
+  Vec<T, V> gv[NV];
+  Vec<TR, V> rv[NV];
   float t[NV][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * LT + lt) * V;
 #pragma unroll
     for (int e = 0; e < V; ++e) t[k][e] = 0.f;
-    if (c < width) load_f32<T, V>(x + c, t[k]);
+    if (c >= width) continue;
+    load_f32<T, V>(x + c, t[k]);
+    if (a.gate != nullptr) gv[k] = *reinterpret_cast<const Vec<T, V>*>(g + c);
+    if (a.res != nullptr) rv[k] = *reinterpret_cast<const Vec<TR, V>*>(res + c);
   }
   auto gate = [&]() {
-    const T* __restrict__ g = static_cast<const T*>(a.gate) + o * a.g_o + i * a.g_i + c0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * LT + lt) * V;
-      if (c >= width) continue;
-      float v[V];
-      load_f32<T, V>(g + c, v);
+      if ((k * LT + lt) * V >= width) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) t[k][e] *= act_of(a.act, v[e]);
+      for (int e = 0; e < V; ++e) t[k][e] *= act_of(a.act, to_f32<T>(gv[k].e[e]));
     }
   };
   auto squares = [&]() {
@@ -91,12 +97,12 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
         if (k * LT + lt < vecs) s_group[k * LT + lt] = s;
       }
       __syncthreads();
-      for (int g = threadIdx.x / kWave; g < groups; g += LT / kWave) {
+      for (int q = threadIdx.x / kWave; q < groups; q += LT / kWave) {
         float s = 0.f;
-        for (int v = lane_id(); v < per; v += kWave) s += s_group[g * per + v];
+        for (int v = lane_id(); v < per; v += kWave) s += s_group[q * per + v];
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-        if (lane_id() == 0) s_group[vecs + g] = 1.f / sqrtf(s / (float)a.group + a.eps);
+        if (lane_id() == 0) s_group[vecs + q] = 1.f / sqrtf(s / (float)a.group + a.eps);
       }
       __syncthreads();
 #pragma unroll
@@ -123,32 +129,28 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
     }
   }
   if (a.gate != nullptr && !a.gate_first) gate();
-  const TR* __restrict__ res = a.res == nullptr ? nullptr : static_cast<const TR*>(a.res) + o * a.res_o + i * a.res_i + c0;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * LT + lt) * V;
     if (c >= width) continue;
-    float v[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = 0.f;
-    if (res != nullptr) load_f32<TR, V>(res + c, v);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float f = a.scale_w != nullptr ? a.scale * a.scale_w[c0 + c + e] : a.scale;
-      t[k][e] = res != nullptr ? fmaf(f, t[k][e], v[e]) : f * t[k][e];
+      t[k][e] = a.res != nullptr ? fmaf(f, t[k][e], to_f32<TR>(rv[k].e[e])) : f * t[k][e];
     }
     if (a.r != nullptr) store_f32<TR, V>(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0 + c, t[k]);
   }
-  if (a.pre_w == nullptr) return;
-  const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
-  T* __restrict__ h = static_cast<T*>(a.h) + o * a.h_o + i * a.h_i;
+  if (a.pre_w != nullptr) {
+    const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
+    T* __restrict__ h = static_cast<T*>(a.h) + o * a.h_o + i * a.h_i;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * LT + lt) * V;
-    if (c >= width) continue;
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LT + lt) * V;
+      if (c >= width) continue;
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[k][e] *= f * a.pre_w[c0 + c + e];
-    store_f32<T, V>(h + c0 + c, t[k]);
+      for (int e = 0; e < V; ++e) t[k][e] *= f * a.pre_w[c0 + c + e];
+      store_f32<T, V>(h + c0 + c, t[k]);
+    }
   }
 }
 
@@ -166,6 +168,7 @@ int launch_norm_k(const NormArgs& a, int sub, hipStream_t stream) {
   });
 }
 
+// M vectors a thread hold the widest row that 1024 threads take.
 template <typename T, typename TR, int V, int M>
 int launch_norm_v(const NormArgs& a, hipStream_t stream) {
   const bool grouped = a.post_w != nullptr && a.group != a.dim;
@@ -175,20 +178,26 @@ int launch_norm_v(const NormArgs& a, hipStream_t stream) {
   }
   const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
   if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false>(a, sub, stream);
-  if (width <= 64 * V * M) return launch_norm_k<T, TR, 64, V, M, false>(a, sub, stream);
+  if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false>(a, sub, stream);
+  if (width <= 64 * V * 4) return launch_norm_k<T, TR, 64, V, 4, false>(a, sub, stream);
+  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false>(a, sub, stream);
   if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false>(a, sub, stream);
   return launch_norm_k<T, TR, 1024, V, M, false>(a, sub, stream);
 }
 
 template <typename T, typename TR>
 int launch_norm_t(const NormArgs& a, hipStream_t stream) {
-  constexpr int V = 4;
+  // 16 bytes of the widest type.
+  constexpr int V = 16 / (sizeof(T) > sizeof(TR) ? sizeof(T) : sizeof(TR));
   const int64_t strides = a.x_o | a.x_i | a.r_o | a.r_i | a.h_o | a.h_i |
                           (a.gate != nullptr ? a.g_o | a.g_i : 0) | (a.res != nullptr ? a.res_o | a.res_i : 0);
   const bool vec = a.dim % V == 0 && a.group % V == 0 && strides % V == 0 && aligned_to(a.x, V * sizeof(T)) &&
                    aligned_to(a.gate, V * sizeof(T)) && aligned_to(a.h, V * sizeof(T)) &&
-                   aligned_to(a.res, V * sizeof(TR)) && aligned_to(a.r, V * sizeof(TR));
-  return vec ? launch_norm_v<T, TR, V, 4>(a, stream) : launch_norm_v<T, TR, 1, 16>(a, stream);
+                   aligned_to(a.res, 16) && aligned_to(a.r, 16);
+  return vec ? launch_norm_v<T, TR, V, 16 / V>(a, stream) : launch_norm_v<T, TR, 1, 16>(a, stream);
 }
 
 template <typename T>

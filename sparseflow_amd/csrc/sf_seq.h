@@ -7,9 +7,9 @@
 namespace sf {
 namespace {
 
-// V elements of T, loaded and stored at once (p aligned to all of them).
+// V elements of T, loaded and stored at once (p aligned to all of them, or to 16 bytes).
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Vec {
+struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
   T e[V];
 };
 
@@ -77,9 +77,14 @@ __device__ __forceinline__ float softplus(float v) {
   return fmaxf(v, 0.f) + (t + t);
 }
 
-// v * sigmoid(v): 0 at the far negative end (v / inf), NaN where v is.
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
-__device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
+// sigmoid(v) and v sigmoid(v) by the hardware's exponential and reciprocal: each is
+// good to a unit in the last place, and the exponent's rounding costs |v| of them in
+// 1 + exp(-v) where that still counts.  (With expf and a division the convolution of
+// bf16 rows was bound by arithmetic: 183 us for 2 x 16384 x 4352, against 130.)
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + exp2_hw(v * -1.44269502f));
+}
+__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
 }  // namespace
 
