@@ -8,11 +8,31 @@ slots: row b)."""
 
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import Callable, List, Optional, Tuple
 
 import torch
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def signature(*tensors: Optional[torch.Tensor]) -> tuple:
+    """Everything about a call's tensors but their addresses and values."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+class Plans(dict):
+    """What a checked call with a signature comes to.  A decoding loop repeats its
+    calls, and checking the tensors of one again costs as much as launching it
+    (a step of the scan: 14 us with, 9 without)."""
+
+    MOST = 4096
+
+    def make(self, key: tuple, check: Callable, *args):
+        plan = check(*args)
+        if len(self) >= self.MOST:
+            self.clear()
+        self[key] = plan
+        return plan
 
 
 def check_input(t: torch.Tensor, name: str) -> None:

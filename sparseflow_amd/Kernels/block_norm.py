@@ -19,25 +19,20 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _lib
-from ._sequences import FLOATS, check_input, check_param, last_contiguous
+from ._sequences import Plans, check_input, check_param, last_contiguous, signature
+
+_plans = Plans()
 
 MAX_DIM = 16384
 
 
-def _rows(t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[torch.Tensor, Tuple[int, int]]:
-    """A tensor that the kernel reads in place (broadcast to `shape`), and its
-    (outer, inner) strides; more than two leading axes that are no one stride
-    become a copy."""
+def _rows(t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[torch.Tensor, ...]:
+    """A tensor broadcast to `shape`, as up to three axes that the kernel reads in
+    place: a copy where its strides allow no such view."""
     if t.shape != shape:
         t = t.expand(shape)
     t = last_contiguous(t)
-    if t.dim() == 1:
-        return t, (0, 0)
-    if t.dim() == 2:
-        return t, (0, t.stride(0))
-    if t.dim() > 3:
-        t = t.reshape(-1, t.shape[-2], t.shape[-1])
-    return t, (t.stride(0), t.stride(1))
+    return (t.reshape(-1, t.shape[-2], t.shape[-1]) if t.dim() > 3 else t,)
 
 
 def _host(x, gate, act, gate_first, post_weight, group, residual, scale, pre_weight, eps):
@@ -78,6 +73,52 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
     "sigmoid" or None.  r has the residual's type (without one, x's).  out (h)
     and residual_out (r) may be given, and may be x and the residual.
     """
+    scale_weight = scale if isinstance(scale, torch.Tensor) else None
+    factor = 1.0 if scale is None or scale_weight is not None else float(scale)
+    key = (signature(x, gate, post_weight, residual, scale_weight, pre_weight, out, residual_out), activation, gate_first,
+           group_size, factor, eps)
+    plan = _plans.get(key) or _plans.make(key, _check, x, gate, activation, gate_first, post_weight, group_size, residual,
+                                          scale_weight, factor, pre_weight, eps, out, residual_out)
+    group, r_type, desc = plan
+    if not x.is_cuda:
+        r, h = _host(x, gate, activation, gate_first, post_weight, group, residual, scale, pre_weight, eps)
+        if r.shape != x.shape:
+            raise ValueError(f"gate or residual does not broadcast to {tuple(x.shape)}")
+        r = r.to(r_type) if residual_out is None else residual_out.copy_(r)
+        if h is not None:
+            h = h.to(x.dtype) if out is None else out.copy_(h)
+        return r, h
+    shape = x.shape
+    if desc is None:
+        # An input that the kernel does not read in place, or one to broadcast.
+        x, gate, residual = (None if t is None else _rows(t, shape)[0] for t in (x, gate, residual))
+        r, h = block_norm_forward(x, gate, activation, gate_first, post_weight, group_size, residual, scale, pre_weight, eps,
+                                  None if out is None else out.view(x.shape),
+                                  None if residual_out is None else residual_out.view(x.shape))
+        return (r.view(shape) if residual_out is None else residual_out,
+                None if h is None else h.view(shape) if out is None else out)
+    r = torch.empty(shape, dtype=r_type, device=x.device) if residual_out is None else residual_out
+    h = None
+    if pre_weight is not None:
+        h = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
+    _lib.block_norm(desc, x, gate, post_weight, residual, scale_weight, pre_weight, r, h)
+    return r, h
+
+
+def _in_place(t: Optional[torch.Tensor], shape: torch.Size) -> Optional[Tuple[int, int]]:
+    """The (outer, inner) strides of a tensor of up to three axes that the kernel
+    reads in place."""
+    if t is None:
+        return 0, 0
+    if t.shape != shape or t.dim() > 3 or (t.stride(-1) != 1 and t.shape[-1] != 1):
+        return None
+    return (0, 0) if t.dim() == 1 else (0, t.stride(0)) if t.dim() == 2 else (t.stride(0), t.stride(1))
+
+
+def _check(x, gate, activation, gate_first, post_weight, group_size, residual, scale_weight, factor, pre_weight, eps, out,
+           residual_out):
+    """-> (group size, the type of r, the descriptor of a device call or None where
+    an input has to be laid out first)."""
     check_input(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x is {tuple(x.shape)}: (..., dim) is wanted")
@@ -91,7 +132,6 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
                          "wanted")
     check_param(post_weight, x, "post_weight", (dim,))
     check_param(pre_weight, x, "pre_weight", (dim,))
-    scale_weight = scale if isinstance(scale, torch.Tensor) else None
     check_param(scale_weight, x, "scale", (dim,))
     group = dim if group_size is None else int(group_size)
     if group < 1 or dim % group != 0:
@@ -101,37 +141,19 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
         if t is not None and (t.shape != shape or t.dtype != dtype or t.device != x.device):
             raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {tuple(shape)} {dtype} on "
                              f"{x.device} is wanted")
+        if t is not None and x.is_cuda and (_in_place(t, shape) is None if t.dim() <= 3 else not t.is_contiguous()):
+            raise ValueError(f"{name}: a contiguous last axis is wanted (over more than three axes: all of them)")
     if out is not None and pre_weight is None:
         raise ValueError("out without pre_weight: there is no second norm to write")
     if dim > MAX_DIM:
         raise _lib.UnsupportedError(f"dim {dim} is over {MAX_DIM}")
-    if not x.is_cuda:
-        r, h = _host(x, gate, activation, gate_first, post_weight, group, residual, scale, pre_weight, eps)
-        if r.shape != shape:
-            raise ValueError(f"gate or residual does not broadcast to {tuple(shape)}")
-        r = r.to(r_type) if residual_out is None else residual_out.copy_(r)
-        if h is not None:
-            h = h.to(x.dtype) if out is None else out.copy_(h)
-        return r, h
-    x, xs = _rows(x, shape)
-    gs = ps = hs = (0, 0)
-    if gate is not None:
-        gate, gs = _rows(gate, shape)
-    if residual is not None:
-        residual, ps = _rows(residual, shape)
-    r = torch.empty(shape, dtype=r_type, device=x.device) if residual_out is None else residual_out
-    h = None
-    if pre_weight is not None:
-        h = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
-    rv, rs = _rows(r, shape)
-    hv = None
-    if h is not None:
-        hv, hs = _rows(h, shape)
-    if rv.data_ptr() != r.data_ptr() or (h is not None and hv.data_ptr() != h.data_ptr()):
-        raise ValueError("out, residual_out: a contiguous last axis and at most two leading strides are wanted")
-    inner = 1 if x.dim() == 1 else int(x.shape[-2])
-    outer = int(x.shape[0]) if x.dim() == 3 else 1
-    desc = _lib.norm_desc(outer, inner, xs, gs, ps, rs, hs, dim, group, x.dtype, r_type, activation, bool(gate_first),
-                          float(eps), 1.0 if scale is None or scale_weight is not None else float(scale))
-    _lib.block_norm(desc, x, gate, post_weight, residual, scale_weight, pre_weight, rv, hv)
-    return r, h
+    strides = [_in_place(t, shape) for t in (x, gate, residual)]
+    if not x.is_cuda or None in strides:
+        return group, r_type, None
+    # (New outputs have the default strides.)
+    plain = _in_place(torch.empty(shape, device="meta"), shape)
+    outputs = [plain if t is None else _in_place(t, shape) for t in (residual_out, out)]
+    inner = 1 if x.dim() == 1 else int(shape[-2])
+    outer = int(shape[0]) if x.dim() == 3 else 1
+    return group, r_type, _lib.norm_desc(outer, inner, *strides, *outputs, dim, group, x.dtype, r_type, activation,
+                                         bool(gate_first), float(eps), factor)

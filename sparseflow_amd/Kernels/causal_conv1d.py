@@ -16,8 +16,10 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ._sequences import check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
-    last_contiguous
+from ._sequences import Plans, check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
+    last_contiguous, signature
+
+_prompts, _steps = Plans(), Plans()
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, bias, activation) -> Tuple[int, int]:
@@ -58,6 +60,33 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
     before, nothing kept); they may be one tensor.  max_len, the longest
     sequence, sizes the launch of a packed call (default: all its tokens).
     """
+    if x.is_cuda:
+        x = last_contiguous(x)
+    key = (signature(x, weight, bias, initial_state, offsets, slots, out, final_state), activation, max_len)
+    plan = _prompts.get(key) or _prompts.make(key, _check_prompt, x, weight, bias, activation, initial_state, offsets,
+                                              max_len, slots, out, final_state)
+    shape, desc = plan
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if final_state is None:
+        final_state = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if not x.is_cuda:
+        keep = shape[1]
+        rows = host_slots(shape[0], final_state.shape[0], slots)
+        for b, (xs, ys) in enumerate(zip(host_spans(x, offsets), host_spans(out, offsets))):
+            before = initial_state[rows[b]] if initial_state is not None and rows[b] >= 0 \
+                else x.new_zeros(keep, x.shape[-1])
+            u = torch.cat([before, xs])
+            ys.copy_(_host_conv(u, weight, bias, activation))
+            if rows[b] >= 0:
+                final_state[rows[b]] = u[u.shape[0] - keep:]
+        return out, final_state
+    _lib.causal_conv1d(desc, x, weight, bias, offsets, slots, initial_state, out, final_state)
+    return out, final_state
+
+
+def _check_prompt(x, weight, bias, activation, initial_state, offsets, max_len, slots, out, final_state):
+    """-> (the states' shape, the descriptor of a device call)."""
     if x.dim() != (3 if offsets is None else 2):
         raise ValueError(f"x is {tuple(x.shape)}: (batch, tokens, C), or (total, C) with offsets, is wanted")
     ch, k = _check(x, weight, bias, activation)
@@ -73,33 +102,21 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
         raise ValueError("slots without final_state: the pool that keeps the states is wanted")
     if initial_state is not None and final_state is not None and initial_state.shape != final_state.shape:
         raise ValueError("initial_state and final_state have different numbers of rows")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
+    if out is not None:
         check_like(out, x, "out", tuple(x.shape))
         if out.stride(-1) != 1 and ch > 1:
             raise ValueError("out: a contiguous last axis is wanted")
-    if final_state is None:
-        final_state = torch.empty((batch, k - 1, ch), dtype=x.dtype, device=x.device)
     if not x.is_cuda:
-        rows = host_slots(batch, final_state.shape[0], slots)
-        for b, (xs, ys) in enumerate(zip(host_spans(x, offsets), host_spans(out, offsets))):
-            before = initial_state[rows[b]] if initial_state is not None and rows[b] >= 0 else x.new_zeros(k - 1, ch)
-            u = torch.cat([before, xs])
-            ys.copy_(_host_conv(u, weight, bias, activation))
-            if rows[b] >= 0:
-                final_state[rows[b]] = u[u.shape[0] - (k - 1):]
-        return out, final_state
-    x = last_contiguous(x)
+        return (batch, k - 1, ch), None
+    rows = batch if final_state is None else int(final_state.shape[0])
+    # (A new out has the default strides.)
+    ys = torch.empty(x.shape, device="meta").stride() if out is None else out.stride()
     if offsets is None:
-        max_len = tokens
-        xs, ys = (x.stride(0), x.stride(1)), (out.stride(0), out.stride(1))
+        longest, xs, ys = tokens, x.stride()[:2], ys[:2]
     else:
-        max_len = tokens if max_len is None else min(max(int(max_len), 0), tokens)
-        xs, ys = (0, x.stride(0)), (0, out.stride(0))
-    desc = _lib.conv1d_desc(batch, tokens, max_len, int(final_state.shape[0]), xs, ys, ch, k, x.dtype, activation)
-    _lib.causal_conv1d(desc, x, weight, bias, offsets, slots, initial_state, out, final_state)
-    return out, final_state
+        longest = tokens if max_len is None else min(max(int(max_len), 0), tokens)
+        xs, ys = (0, x.stride(0)), (0, ys[0])
+    return (rows, k - 1, ch), _lib.conv1d_desc(batch, tokens, longest, rows, xs, ys, ch, k, x.dtype, activation)
 
 
 def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
@@ -111,20 +128,14 @@ def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     (int32 [batch], no two alike), moves on by the token in place.  A slot
     outside the pool: y is zero there and no state changes.
     """
-    if x.dim() != 2:
-        raise ValueError(f"x is {tuple(x.shape)}: (batch, C) is wanted")
-    ch, k = _check(x, weight, bias, activation)
-    batch = int(x.shape[0])
-    check_index(slots, x, "slots", batch)
-    check_pool(state, x, "state", (k - 1, ch), x.dtype, batch, slots)
+    if x.is_cuda:
+        x = last_contiguous(x)
+    key = (signature(state, x, weight, bias, slots, out), activation)
+    plan = _steps.get(key) or _steps.make(key, _check_step, state, x, weight, bias, activation, slots, out)
     if out is None:
-        out = torch.empty((batch, ch), dtype=x.dtype, device=x.device)
-    else:
-        check_like(out, x, "out", (batch, ch))
-        if out.stride(-1) != 1 and ch > 1:
-            raise ValueError("out: a contiguous last axis is wanted")
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if not x.is_cuda:
-        for b, row in enumerate(host_slots(batch, state.shape[0], slots)):
+        for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
             if row < 0:
                 out[b] = 0
                 continue
@@ -132,8 +143,23 @@ def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
             out[b] = _host_conv(u, weight, bias, activation)[0].to(x.dtype)
             state[row] = u[1:]
         return out
-    x = last_contiguous(x)
-    desc = _lib.conv1d_desc(batch, 1, 1, int(state.shape[0]), (x.stride(0), 0), (out.stride(0), 0), ch, k, x.dtype,
-                            activation)
-    _lib.causal_conv1d_step(desc, state, x, weight, bias, slots, out)
+    _lib.causal_conv1d_step(plan[0], state, x, weight, bias, slots, out)
     return out
+
+
+def _check_step(state, x, weight, bias, activation, slots, out):
+    """-> (the descriptor of a device call,)."""
+    if x.dim() != 2:
+        raise ValueError(f"x is {tuple(x.shape)}: (batch, C) is wanted")
+    ch, k = _check(x, weight, bias, activation)
+    batch = int(x.shape[0])
+    check_index(slots, x, "slots", batch)
+    check_pool(state, x, "state", (k - 1, ch), x.dtype, batch, slots)
+    if out is not None:
+        check_like(out, x, "out", (batch, ch))
+        if out.stride(-1) != 1 and ch > 1:
+            raise ValueError("out: a contiguous last axis is wanted")
+    if not x.is_cuda:
+        return (None,)
+    ys = ch if out is None else out.stride(0)
+    return (_lib.conv1d_desc(batch, 1, 1, int(state.shape[0]), (x.stride(0), 0), (ys, 0), ch, k, x.dtype, activation),)

@@ -18,8 +18,10 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ._sequences import check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
-    last_contiguous
+from ._sequences import Plans, check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
+    last_contiguous, signature
+
+_prompts, _steps = Plans(), Plans()
 
 
 def _check(x, dt, A, B, C, D, dt_bias) -> Tuple[int, int, int, int]:
@@ -74,6 +76,38 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     (default: all its tokens).  workspace optionally holds the scratch between
     calls (uint8; a new one where it is too small).
     """
+    if x.is_cuda:
+        x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
+    key = (signature(x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, out, final_state), max_len, dt_softplus)
+    plan = _prompts.get(key) or _prompts.make(key, _check_prompt, x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state,
+                                              offsets, max_len, slots, out, final_state)
+    shape, desc = plan
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if final_state is None:
+        final_state = torch.empty(shape, dtype=torch.float32, device=x.device)
+    if not x.is_cuda:
+        H, P, N = shape[1:]
+        rows = host_slots(shape[0], final_state.shape[0], slots)
+        spans = zip(*(host_spans(t, offsets) for t in (x, dt, B, C, out)))
+        for b, (xs, ds, bs, cs, ys) in enumerate(spans):
+            h = torch.zeros(H, P, N) if initial_state is None or rows[b] < 0 else initial_state[rows[b]].clone()
+            for t in range(xs.shape[0]):
+                ys[t] = _host_token(h, xs[t], ds[t], A, bs[t], cs[t], D, dt_bias, dt_softplus).to(x.dtype)
+            if rows[b] >= 0:
+                final_state[rows[b]] = h
+        return out, final_state
+    need = desc[2]
+    if need == 0:
+        workspace = None
+    elif workspace is None or workspace.device != x.device or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _lib.selective_scan(desc, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, out, final_state, workspace)
+    return out, final_state
+
+
+def _check_prompt(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state, offsets, max_len, slots, out, final_state):
+    """-> (the states' shape, the descriptor of a device call)."""
     if x.dim() != (4 if offsets is None else 3):
         raise ValueError(f"x is {tuple(x.shape)}: (batch, tokens, H, P), or (total, H, P) with offsets, is wanted")
     H, P, G, N = _check(x, dt, A, B, C, D, dt_bias)
@@ -89,41 +123,23 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
         raise ValueError("slots without final_state: the pool that keeps the states is wanted")
     if initial_state is not None and final_state is not None and initial_state.shape != final_state.shape:
         raise ValueError("initial_state and final_state have different numbers of rows")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
+    if out is not None:
         check_like(out, x, "out", tuple(x.shape))
         if out.stride(-1) != 1 and P > 1:
             raise ValueError("out: a contiguous last axis is wanted")
-    if final_state is None:
-        final_state = torch.empty((batch, H, P, N), dtype=torch.float32, device=x.device)
+    shape = (batch, H, P, N) if final_state is None else tuple(final_state.shape)
     if not x.is_cuda:
-        rows = host_slots(batch, final_state.shape[0], slots)
-        spans = zip(*(host_spans(t, offsets) for t in (x, dt, B, C, out)))
-        for b, (xs, ds, bs, cs, ys) in enumerate(spans):
-            h = torch.zeros(H, P, N) if initial_state is None or rows[b] < 0 else initial_state[rows[b]].clone()
-            for t in range(xs.shape[0]):
-                ys[t] = _host_token(h, xs[t], ds[t], A, bs[t], cs[t], D, dt_bias, dt_softplus).to(x.dtype)
-            if rows[b] >= 0:
-                final_state[rows[b]] = h
-        return out, final_state
-    x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
+        return (batch, H, P, N), None
+    # (A new out has the default strides.)
+    ys = torch.empty(x.shape, device="meta").stride() if out is None else out.stride()
     if offsets is None:
-        max_len = tokens
-        strides = (x.stride()[:3], dt.stride(), B.stride()[:3], C.stride()[:3], out.stride()[:3])
+        longest = tokens
+        strides = (x.stride()[:3], dt.stride(), B.stride()[:3], C.stride()[:3], ys[:3])
     else:
-        max_len = tokens if max_len is None else min(max(int(max_len), 0), tokens)
+        longest = tokens if max_len is None else min(max(int(max_len), 0), tokens)
         strides = ((0,) + x.stride()[:2], (0,) + dt.stride(), (0,) + B.stride()[:2], (0,) + C.stride()[:2],
-                   (0,) + out.stride()[:2])
-    desc = _lib.scan_desc(batch, tokens, max_len, int(final_state.shape[0]), *strides, H, P, G, N, x.dtype,
-                          bool(dt_softplus))
-    need = desc[2]
-    if need == 0:
-        workspace = None
-    elif workspace is None or workspace.device != x.device or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _lib.selective_scan(desc, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, out, final_state, workspace)
-    return out, final_state
+                   (0,) + ys[:2])
+    return shape, _lib.scan_desc(batch, tokens, longest, shape[0], *strides, H, P, G, N, x.dtype, bool(dt_softplus))
 
 
 def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
@@ -137,28 +153,38 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
     the token in place.  A slot outside the pool: y is zero there and no state
     changes.
     """
+    if x.is_cuda:
+        x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
+    key = (signature(state, x, dt, A, B, C, D, dt_bias, slots, out), dt_softplus)
+    plan = _steps.get(key) or _steps.make(key, _check_step, state, x, dt, A, B, C, D, dt_bias, dt_softplus, slots, out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not x.is_cuda:
+        for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
+            if row < 0:
+                out[b] = 0
+            else:
+                out[b] = _host_token(state[row], x[b], dt[b], A, B[b], C[b], D, dt_bias, dt_softplus).to(x.dtype)
+        return out
+    _lib.selective_scan_step(plan[0], state, x, dt, A, B, C, D, dt_bias, slots, out)
+    return out
+
+
+def _check_step(state, x, dt, A, B, C, D, dt_bias, dt_softplus, slots, out):
+    """-> (the descriptor of a device call,)."""
     if x.dim() != 3:
         raise ValueError(f"x is {tuple(x.shape)}: (batch, H, P) is wanted")
     H, P, G, N = _check(x, dt, A, B, C, D, dt_bias)
     batch = int(x.shape[0])
     check_index(slots, x, "slots", batch)
     check_pool(state, x, "state", (H, P, N), torch.float32, batch, slots)
-    if out is None:
-        out = torch.empty((batch, H, P), dtype=x.dtype, device=x.device)
-    else:
+    if out is not None:
         check_like(out, x, "out", (batch, H, P))
         if out.stride(-1) != 1 and P > 1:
             raise ValueError("out: a contiguous last axis is wanted")
     if not x.is_cuda:
-        for b, row in enumerate(host_slots(batch, state.shape[0], slots)):
-            if row < 0:
-                out[b] = 0
-            else:
-                out[b] = _host_token(state[row], x[b], dt[b], A, B[b], C[b], D, dt_bias, dt_softplus).to(x.dtype)
-        return out
-    x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
-    pair = lambda t: (t.stride(0), 0, t.stride(1))  # noqa: E731
-    desc = _lib.scan_desc(batch, 1, 1, int(state.shape[0]), pair(x), pair(dt), pair(B), pair(C), pair(out), H, P, G, N,
-                          x.dtype, bool(dt_softplus))
-    _lib.selective_scan_step(desc, state, x, dt, A, B, C, D, dt_bias, slots, out)
-    return out
+        return (None,)
+    pair = lambda s: (s[0], 0, s[1])  # noqa: E731
+    ys = (H * P, P) if out is None else out.stride()
+    return (_lib.scan_desc(batch, 1, 1, int(state.shape[0]), pair(x.stride()), pair(dt.stride()), pair(B.stride()),
+                           pair(C.stride()), pair(ys), H, P, G, N, x.dtype, bool(dt_softplus)),)
