@@ -35,6 +35,7 @@ def _rows(t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[torch.Tensor, ...]:
     return (t.reshape(-1, t.shape[-2], t.shape[-1]) if t.dim() > 3 else t,)
 
 
+@torch.no_grad()
 def _host(x, gate, act, gate_first, post_weight, group, residual, scale, pre_weight, eps):
     def norm(t, w, size):
         g = t.unflatten(-1, (-1, size))

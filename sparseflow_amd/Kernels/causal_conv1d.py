@@ -71,16 +71,17 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
     if final_state is None:
         final_state = torch.empty(shape, dtype=x.dtype, device=x.device)
     if not x.is_cuda:
-        keep = shape[1]
-        rows = host_slots(shape[0], final_state.shape[0], slots)
-        for b, (xs, ys) in enumerate(zip(host_spans(x, offsets), host_spans(out, offsets))):
-            before = initial_state[rows[b]] if initial_state is not None and rows[b] >= 0 \
-                else x.new_zeros(keep, x.shape[-1])
-            u = torch.cat([before, xs])
-            ys.copy_(_host_conv(u, weight, bias, activation))
-            if rows[b] >= 0:
-                final_state[rows[b]] = u[u.shape[0] - keep:]
-        return out, final_state
+        with torch.no_grad():
+            keep = shape[1]
+            rows = host_slots(shape[0], final_state.shape[0], slots)
+            for b, (xs, ys) in enumerate(zip(host_spans(x, offsets), host_spans(out, offsets))):
+                before = initial_state[rows[b]] if initial_state is not None and rows[b] >= 0 \
+                    else x.new_zeros(keep, x.shape[-1])
+                u = torch.cat([before, xs])
+                ys.copy_(_host_conv(u, weight, bias, activation))
+                if rows[b] >= 0:
+                    final_state[rows[b]] = u[u.shape[0] - keep:]
+            return out, final_state
     _lib.causal_conv1d(desc, x, weight, bias, offsets, slots, initial_state, out, final_state)
     return out, final_state
 
@@ -135,14 +136,15 @@ def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if not x.is_cuda:
-        for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
-            if row < 0:
-                out[b] = 0
-                continue
-            u = torch.cat([state[row], x[b:b + 1]])
-            out[b] = _host_conv(u, weight, bias, activation)[0].to(x.dtype)
-            state[row] = u[1:]
-        return out
+        with torch.no_grad():
+            for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
+                if row < 0:
+                    out[b] = 0
+                    continue
+                u = torch.cat([state[row], x[b:b + 1]])
+                out[b] = _host_conv(u, weight, bias, activation)[0].to(x.dtype)
+                state[row] = u[1:]
+            return out
     _lib.causal_conv1d_step(plan[0], state, x, weight, bias, slots, out)
     return out
 

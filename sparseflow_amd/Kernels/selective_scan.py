@@ -87,16 +87,17 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     if final_state is None:
         final_state = torch.empty(shape, dtype=torch.float32, device=x.device)
     if not x.is_cuda:
-        H, P, N = shape[1:]
-        rows = host_slots(shape[0], final_state.shape[0], slots)
-        spans = zip(*(host_spans(t, offsets) for t in (x, dt, B, C, out)))
-        for b, (xs, ds, bs, cs, ys) in enumerate(spans):
-            h = torch.zeros(H, P, N) if initial_state is None or rows[b] < 0 else initial_state[rows[b]].clone()
-            for t in range(xs.shape[0]):
-                ys[t] = _host_token(h, xs[t], ds[t], A, bs[t], cs[t], D, dt_bias, dt_softplus).to(x.dtype)
-            if rows[b] >= 0:
-                final_state[rows[b]] = h
-        return out, final_state
+        with torch.no_grad():
+            H, P, N = shape[1:]
+            rows = host_slots(shape[0], final_state.shape[0], slots)
+            spans = zip(*(host_spans(t, offsets) for t in (x, dt, B, C, out)))
+            for b, (xs, ds, bs, cs, ys) in enumerate(spans):
+                h = torch.zeros(H, P, N) if initial_state is None or rows[b] < 0 else initial_state[rows[b]].clone()
+                for t in range(xs.shape[0]):
+                    ys[t] = _host_token(h, xs[t], ds[t], A, bs[t], cs[t], D, dt_bias, dt_softplus).to(x.dtype)
+                if rows[b] >= 0:
+                    final_state[rows[b]] = h
+            return out, final_state
     need = desc[2]
     if need == 0:
         workspace = None
@@ -160,12 +161,13 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if not x.is_cuda:
-        for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
-            if row < 0:
-                out[b] = 0
-            else:
-                out[b] = _host_token(state[row], x[b], dt[b], A, B[b], C[b], D, dt_bias, dt_softplus).to(x.dtype)
-        return out
+        with torch.no_grad():
+            for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
+                if row < 0:
+                    out[b] = 0
+                else:
+                    out[b] = _host_token(state[row], x[b], dt[b], A, B[b], C[b], D, dt_bias, dt_softplus).to(x.dtype)
+            return out
     _lib.selective_scan_step(plan[0], state, x, dt, A, B, C, D, dt_bias, slots, out)
     return out
 
