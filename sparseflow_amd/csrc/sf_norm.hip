@@ -179,7 +179,7 @@ int launch_norm_v(const NormArgs& a, hipStream_t stream) {
   const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
   if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false>(a, sub, stream);
   if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false>(a, sub, stream);
-  if (width <= 64 * V * 4) return launch_norm_k<T, TR, 64, V, 4, false>(a, sub, stream);
+  if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false>(a, sub, stream);
   if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false>(a, sub, stream);
   if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false>(a, sub, stream);
   if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false>(a, sub, stream);
