@@ -818,7 +818,6 @@ static sf::ScanArgs scan_args(const sf_scan_desc* d, const void* x, const void* 
   a.h0 = h0;
   a.h1 = h1;
   a.y = y;
-  a.max_len = step ? 1 : offsets == nullptr ? d->tokens : d->max_len;
   const int64_t dense = offsets == nullptr ? 1 : 0, walk = step ? 0 : 1;
   a.x_b = d->x_strides[0] * dense;
   a.x_t = d->x_strides[1] * walk;
@@ -841,12 +840,13 @@ static sf::ScanArgs scan_args(const sf_scan_desc* d, const void* x, const void* 
   a.state_dim = d->state_dim;
   a.softplus = d->dt_softplus != 0;
   a.step = step ? 1 : 0;
+  a.state_vec = d->state_dim % 4 == 0 && sf::aligned_to(h0, 16) && sf::aligned_to(h1, 16);
   return a;
 }
 
 static sf::ScanPlan plan_of(const sf_scan_desc* d) {
-  return sf::scan_plan(d->batch, d->max_len < d->tokens ? d->max_len : d->tokens, d->heads, d->head_dim, d->groups,
-                       d->state_dim, d->dtype);
+  return sf::scan_plan(d->batch, d->tokens, d->max_len < d->tokens ? d->max_len : d->tokens, d->heads, d->head_dim,
+                       d->groups, d->state_dim, d->dtype);
 }
 
 size_t sf_selective_scan_workspace_size(const sf_scan_desc* d) {
@@ -865,6 +865,8 @@ int sf_selective_scan(const sf_scan_desc* d, const void* x, const void* dt, cons
   const sf::ScanPlan plan = plan_of(d);
   if (workspace_bytes < plan.bytes || (plan.bytes > 0 && workspace == nullptr))
     return fail(SF_ERR_WORKSPACE, "workspace too small");
+  if (plan.bytes > 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(SF_ERR_WORKSPACE, "workspace is not aligned to 16 bytes");
   const sf::ScanArgs a =
       scan_args(d, x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, y, final_state, false);
   const int e = plan.chunked && sf::scan_chunk_takes(a)

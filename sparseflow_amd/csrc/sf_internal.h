@@ -274,6 +274,8 @@ struct SeqAxis {
   int64_t batch, tokens, states;
 };
 
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 struct Conv1dArgs {
   SeqAxis seq;
   const void* x;
@@ -302,18 +304,21 @@ struct ScanArgs {
   const float* h0;
   float* h1;
   void* y;
-  int64_t max_len;
   // Strides (elements) of sequence, token and head / group; packed: *_b = 0.
   int64_t x_b, x_t, x_h, dt_b, dt_t, dt_h, b_b, b_t, b_g, c_b, c_t, c_g, y_b, y_t, y_h;
   int64_t block0;
   int heads, head_dim, groups, state_dim, softplus;
   int step;
+  int state_vec;  // rows of the states in units of 16 bytes
 };
 constexpr int kScanMaxState = 256;
 int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);
 
 // Prompts chunk by chunk: how the work is cut.
-constexpr int kScanChunkFrom = 24;  // longest sequence from which chunks are used
+// The longest sequence from which chunks are used (bf16 and float32, 64 sequences of 24
+// heads x 64, N 128: of 4 tokens 26 and 38 us, token by token 32 and 25; of 8 tokens 27
+// and 37, token by token 50 and 39; a chunk's time is that of a whole one).
+constexpr int kScanChunkFrom = 8;
 struct ScanSplit {
   float* parts;  // [batch, segments, heads, head_dim, state_dim]
   float* sums;   // [batch, segments, heads] exponents
@@ -327,7 +332,7 @@ struct ScanPlan {
   size_t sums_at;  // bytes into the workspace
   size_t bytes;    // of workspace
 };
-ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype);
+ScanPlan scan_plan(int64_t batch, int64_t tokens, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype);
 bool scan_chunk_takes(const ScanArgs& a);  // its token strides are within the kernel's range
 int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int dtype, hipStream_t stream);
 

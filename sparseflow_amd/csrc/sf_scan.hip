@@ -138,9 +138,8 @@ int launch_seq_r(const ScanArgs& a, hipStream_t stream) {
 
 template <typename T, int TN>
 int launch_seq_n(const ScanArgs& a, hipStream_t stream) {
-  const bool vec = a.state_dim % 4 == 0 && ((a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g) % 4) == 0 &&
-                   aligned_to(a.b, 4 * sizeof(T)) && aligned_to(a.c, 4 * sizeof(T)) && aligned_to(a.h0, 16) &&
-                   aligned_to(a.h1, 16);
+  const bool vec = a.state_vec != 0 && ((a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g) % 4) == 0 &&
+                   aligned_to(a.b, 4 * sizeof(T)) && aligned_to(a.c, 4 * sizeof(T));
   // As many rows to a thread as the head has.
   constexpr int kRows = kThreads / TN;
   const int r = (a.head_dim + kRows - 1) / kRows;

@@ -294,6 +294,13 @@ __device__ __forceinline__ void store_unit(uint16_t* to, int apart, const uint32
   }
 }
 
+// The last segment of a sequence of n tokens: it takes the tokens beyond the longest
+// sequence that the call was cut for, too.
+__device__ __forceinline__ int last_segment(const ScanSplit& sp, int64_t n) {
+  const int64_t s = (n + (int64_t)sp.chunks * kChunk - 1) / ((int64_t)sp.chunks * kChunk) - 1;
+  return (int)(s < 0 ? 0 : s >= sp.segments ? sp.segments - 1 : s);
+}
+
 // STATES: a segment's own part of the state, from a zero state, to `parts`, with
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
 // PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
@@ -319,24 +326,28 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   float* const s_g = reinterpret_cast<float*>(lds + Lds::g(kDepth));
 
   // This workgroup's sequence, segment and group; this wavefront's head and columns.
+  const int segs = STATES ? sp.segments - 1 : sp.segments;
+  // (In the order of the launch: given to the XCDs so that those of one sequence and
+  // group share an L2 for B and C, ragged calls take up to a third longer.)
   int64_t item = a.block0 + blockIdx.x;
   const int ub = (int)(item % sp.blocks);
   item /= sp.blocks;
   const int g = (int)(item % a.groups);
   item /= a.groups;
-  const int seg = (int)(item % (STATES ? sp.segments - 1 : sp.segments));
-  const int64_t b = item / (STATES ? sp.segments - 1 : sp.segments);
+  const int seg = (int)(item % segs);
+  const int64_t b = item / segs;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int last = last_segment(sp, n);
+  if (STATES ? seg >= last : seg > last) return;
   const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
   const int unit = ub * kWaves + wave;
   const bool on = unit < per_group * slices;
   const int hd = g * per_group + (on ? unit / slices : 0);
   const int p0 = on ? unit % slices * kSlice : 0;
   const int P = a.head_dim, N = a.state_dim;
-  int64_t first, n;
-  seq_rows(a.seq, b, first, n);
   const int64_t per_seg = (int64_t)sp.chunks * Q;
-  int64_t t0 = seg * per_seg, t1 = t0 + per_seg;
-  if (t1 > n || (!STATES && seg == sp.segments - 1)) t1 = n;
+  const int64_t t0 = seg * per_seg, t1 = seg == last ? n : t0 + per_seg;
   // (The launcher takes token strides below 2^24 only.)
   const int x_t = (int)a.x_t, dt_t = (int)a.dt_t, b_t = (int)a.b_t, c_t = (int)a.c_t, y_t = (int)a.y_t;
   const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + (first + t0) * a.x_t + hd * a.x_h + p0;
@@ -414,11 +425,11 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
     for (int r = 0; r < 16; ++r) h[nt][r] = 0.f;
   const int p = p0 + col;
   const bool mine = on && p < P;
-  const bool vec_n = N % 4 == 0;
+  const bool vec_n = a.state_vec != 0;
   const int64_t plane = (int64_t)P * N;
   const float* from = nullptr;
   if constexpr (!STATES) {
-    from = sp.segments > 1 ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
+    from = seg > 0 ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
            : a.h0 != nullptr && slot >= 0 ? a.h0 + (slot * a.heads + hd) * plane
                                           : nullptr;
   }
@@ -764,7 +775,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
 
   float* to = nullptr;
   if (STATES) to = sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane;
-  else if (seg == sp.segments - 1 && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
+  else if (seg == last && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
   if (to != nullptr && mine) {
     const float f = exp2_hw((float)k_state);
 #pragma unroll
@@ -788,8 +799,8 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)l_seg;
 }
 
-// Segment by segment, the state that each starts from in place of the part that
-// the first pass left there.
+// Segment by segment, the state that the next one starts from, in the place of that
+// one's own part.
 constexpr int kChainThreads = 256;
 __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSplit sp, int blocks) {
   int64_t item = a.block0 + blockIdx.x;
@@ -800,13 +811,22 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
   const int64_t plane = (int64_t)a.head_dim * a.state_dim;
   const int64_t e = (int64_t)part * kChainThreads + threadIdx.x;
   if (e >= plane) return;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int last = last_segment(sp, n);
   const int64_t slot = seq_slot(a.seq, b);
   float h = a.h0 != nullptr && slot >= 0 ? a.h0[(slot * a.heads + hd) * plane + e] : 0.f;
-  for (int s = 0; s < sp.segments; ++s) {
-    float* at = sp.parts + ((b * sp.segments + s) * a.heads + hd) * plane + e;
-    const float own = s + 1 < sp.segments ? *at : 0.f;
-    *at = h;
-    if (s + 1 < sp.segments) h = fmaf(h, exp2f(sp.sums[(b * sp.segments + s) * a.heads + hd]), own);
+  float* at = sp.parts + (b * sp.segments * a.heads + hd) * plane + e;
+  const float* sum = sp.sums + b * sp.segments * a.heads + hd;
+  float own = last > 0 ? *at : 0.f;
+  for (int s = 0; s < last; ++s) {
+    float* const next = at + a.heads * plane;
+    const float next_own = s + 1 < last ? *next : 0.f;
+    h = fmaf(h, exp2f(*sum), own);
+    *next = h;
+    own = next_own;
+    at = next;
+    sum += a.heads;
   }
 }
 
@@ -855,20 +875,24 @@ size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 
 }  // namespace
 
-ScanPlan scan_plan(int64_t batch, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype) {
+ScanPlan scan_plan(int64_t batch, int64_t tokens, int64_t max_len, int heads, int head_dim, int groups, int state_dim, int dtype) {
   ScanPlan p{};
-  // Fewer tokens than half a chunk: the walk token by token.
   p.chunked = max_len >= kScanChunkFrom;
   if (!p.chunked || batch < 1) return p;
   const int units = heads / groups * ((head_dim + kSlice - 1) / kSlice);
   p.split.blocks = (units + kWaves - 1) / kWaves;
-  // Segments: enough workgroups for all that fit the CUs at once, with at least four
-  // chunks each.
+  // Segments: as many as the CUs hold workgroups for at once (fit: of a CU), since one
+  // more makes all wait for a second turn (32 x 1024 tokens of f16, 24 heads x 64, N 128:
+  // 334 us as 768 workgroups, 245 as 384), and of two chunks or more (1 x 512 of bf16, 16
+  // heads: 52 us whole, 43 in segments of four, 39 of two; under 8 chunks the passes'
+  // launches cost what they save: 1 x 200 of bf16, 8 heads x 32, 20 us whole, 25 cut).
+  // In a packed call the sequences are taken to fill their tokens with their longest.
   const int64_t fit = state_dim > 128 ? 1 : dtype == SF_BF16 ? 3 : 2;
   const int64_t chunks = (max_len + kChunk - 1) / kChunk;
-  const int64_t base = batch * groups * p.split.blocks;
-  int64_t segs = (fit * num_cus() + base - 1) / base;
-  if (segs > chunks / 4) segs = chunks / 4;
+  int64_t full = batch;
+  if (max_len < tokens && (tokens + max_len - 1) / max_len < full) full = (tokens + max_len - 1) / max_len;
+  int64_t segs = chunks < 8 ? 1 : fit * num_cus() / (full * groups * p.split.blocks);
+  if (segs > chunks / 2) segs = chunks / 2;
   if (segs < 1) segs = 1;
   const int64_t per = (chunks + segs - 1) / segs;
   p.split.chunks = (int)per;

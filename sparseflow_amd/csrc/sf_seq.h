@@ -102,6 +102,4 @@ int launch_blocks(Args a, int64_t Args::*first, int64_t blocks, Launch&& launch)
   return (int)hipSuccess;
 }
 
-inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
 }  // namespace sf

@@ -223,6 +223,39 @@ def test_scan_packed(dtype, lens, hint):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens,P,N", [([1200, 0, 31, 700], 64, 128), ([0, 999], 40, 256)])
+def test_scan_packed_is_split_with_states_at_any_address(dtype, lens, P, N):
+    announce(f"scan split {dtype} {lens} P={P} N={N}")
+    H, G = 2, 1
+    g = _gen(sum(lens) + P)
+    off = [0]
+    for v in lens:
+        off.append(off[-1] + v)
+    x, dt, A, B, C, D, bias = _scan_inputs(g, (off[-1],), H, P, G, N, dtype)
+    h0 = _randn(g, len(lens), H, P, N)
+    # (States that begin one float after a multiple of 16 bytes.)
+    kept, before = (torch.zeros(h0.numel() + 1, device=DEV)[1:].view(h0.shape) for _ in range(2))
+    before.copy_(h0)
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C, D, bias), initial_state=before, final_state=kept,
+                                      offsets=torch.tensor(off, dtype=torch.int32, device=DEV), max_len=max(lens))
+    assert state is kept and torch.equal(before.cpu(), h0)
+    for i, v in enumerate(lens):
+        at = slice(off[i], off[i + 1])
+        _scan_check(y[at], kept[i], x[at], dt[at], A, B[at], C[at], D, bias, True, h0[i], dtype, f"sequence {i} of {v}")
+
+
+def test_scan_workspace_is_reused_or_refused():
+    g = _gen(8)
+    x, dt, A, B, C, D, bias = _dev(*_scan_inputs(g, (1, 600), 1, 32, 1, 32, F32))
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device=DEV)
+    want = selective_scan_forward(x, dt, A, B, C, D, bias)
+    got = selective_scan_forward(x, dt, A, B, C, D, bias, workspace=ws)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(_lib.SparseFlowLibError, match="16 bytes"):
+        selective_scan_forward(x, dt, A, B, C, D, bias, workspace=ws[1:])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("H,P,G,N", [(3, 64, 1, 64), (8, 64, 1, 128), (4, 20, 2, 24), (3, 7, 1, 5), (2, 128, 1, 256),
                                      (4, 33, 4, 100)])
 def test_scan_step(dtype, H, P, G, N):
