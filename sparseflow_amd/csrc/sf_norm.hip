@@ -4,7 +4,10 @@
 //   r = residual + scale t, h = r w' / rms(r)
 // A row is held in registers by LT threads, vectors of V elements: x, gate and residual
 // are all loaded before the first sum, and h is written after the second.  Bound by
-// HBM.  Short rows (4 vectors a lane) are a wavefront's, whose sums need no barrier.
+// HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 152 us, 5.3 TB/s; 32768 x 2048
+// f16 with gate, float32 residual and h (940 MB) 207 us, 4.5 TB/s.  Short rows (up to 3
+// vectors a lane) are a wavefront's, whose sums need no barrier: 32768 x 384 float32 25
+// us, as a workgroup's 37; of 768 53 and 57; of four vectors, 2048 bf16, 86 and 77.
 //
 // Groups are rows of their own where no norm of the whole row follows; otherwise
 // a workgroup holds the row and the groups' sums meet in LDS.
@@ -41,7 +44,7 @@ __device__ __forceinline__ float row_sum(float v, float* s_part) {
 // inside the row (LT = the workgroup, group % V == 0).  (Workgroups that go row after
 // row with their weights in registers were no faster: 226 against 214 us at
 // 32768 x 2048, f16 with a float32 residual.)
-template <typename T, typename TR, int LT, int V, int NV, bool GROUPED>
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormArgs a, int sub) {
   constexpr int kRowsPerBlock = (LT > kBlock ? LT : kBlock) / LT;
   __shared__ float s_part[LT / kWave];
@@ -64,9 +67,9 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
 #pragma unroll
     for (int e = 0; e < V; ++e) t[k][e] = 0.f;
     if (c >= width) continue;
-    load_f32<T, V>(x + c, t[k]);
-    if (a.gate != nullptr) gv[k] = *reinterpret_cast<const Vec<T, V>*>(g + c);
-    if (a.res != nullptr) rv[k] = *reinterpret_cast<const Vec<TR, V>*>(res + c);
+    load_f32<T, V, ONCE>(x + c, t[k]);
+    if (a.gate != nullptr) gv[k] = load_vec<T, V, ONCE>(g + c);
+    if (a.res != nullptr) rv[k] = load_vec<TR, V, ONCE>(res + c);
   }
   auto gate = [&]() {
 #pragma unroll
@@ -154,38 +157,38 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
   }
 }
 
-template <typename T, typename TR, int LT, int V, int NV, bool GROUPED>
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, bool ONCE>
 int launch_norm_k(const NormArgs& a, int sub, hipStream_t stream) {
   constexpr int threads = LT > kBlock ? LT : kBlock, rows = threads / LT;
   const int64_t items = a.outer * a.inner * sub;
   const size_t lds = GROUPED ? (size_t)(a.dim / V + a.dim / a.group) * sizeof(float) : 0;
   if (lds > 48 * 1024) {
-    const int rc = set_lds_limit_once<k_block_norm<T, TR, LT, V, NV, GROUPED>>(kMaxLdsBytes - 1024);
+    const int rc = set_lds_limit_once<k_block_norm<T, TR, LT, V, NV, GROUPED, ONCE>>(kMaxLdsBytes - 1024);
     if (rc != (int)hipSuccess) return rc;
   }
   return launch_blocks(a, &NormArgs::item0, (items + rows - 1) / rows, [&](const NormArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_block_norm<T, TR, LT, V, NV, GROUPED>), dim3(n), dim3(threads), lds, stream, la, sub);
+    hipLaunchKernelGGL((k_block_norm<T, TR, LT, V, NV, GROUPED, ONCE>), dim3(n), dim3(threads), lds, stream, la, sub);
   });
 }
 
 // M vectors a thread hold the widest row that 1024 threads take.
-template <typename T, typename TR, int V, int M>
+template <typename T, typename TR, int V, int M, bool ONCE>
 int launch_norm_v(const NormArgs& a, hipStream_t stream) {
   const bool grouped = a.post_w != nullptr && a.group != a.dim;
   if (grouped && a.pre_w != nullptr) {
-    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true>(a, 1, stream);
-    return launch_norm_k<T, TR, 1024, V, M, true>(a, 1, stream);
+    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true, ONCE>(a, 1, stream);
+    return launch_norm_k<T, TR, 1024, V, M, true, ONCE>(a, 1, stream);
   }
   const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
-  if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false>(a, sub, stream);
-  if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false>(a, sub, stream);
-  if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false>(a, sub, stream);
-  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false>(a, sub, stream);
-  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false>(a, sub, stream);
-  return launch_norm_k<T, TR, 1024, V, M, false>(a, sub, stream);
+  if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false, ONCE>(a, sub, stream);
+  if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false, ONCE>(a, sub, stream);
+  if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false, ONCE>(a, sub, stream);
+  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false, false>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false, ONCE>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false, ONCE>(a, sub, stream);
+  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false, ONCE>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false, ONCE>(a, sub, stream);
+  return launch_norm_k<T, TR, 1024, V, M, false, ONCE>(a, sub, stream);
 }
 
 template <typename T, typename TR>
@@ -197,7 +200,10 @@ int launch_norm_t(const NormArgs& a, hipStream_t stream) {
   const bool vec = a.dim % V == 0 && a.group % V == 0 && strides % V == 0 && aligned_to(a.x, V * sizeof(T)) &&
                    aligned_to(a.gate, V * sizeof(T)) && aligned_to(a.h, V * sizeof(T)) &&
                    aligned_to(a.res, 16) && aligned_to(a.r, 16);
-  return vec ? launch_norm_v<T, TR, V, 16 / V>(a, stream) : launch_norm_v<T, TR, 1, 16>(a, stream);
+  if (!vec) return launch_norm_v<T, TR, 1, 16, false>(a, stream);
+  const int64_t bytes = (a.gate != nullptr ? 2 : 1) * (int64_t)sizeof(T) + (a.res != nullptr ? (int64_t)sizeof(TR) : 0);
+  return read_once(a.outer * a.inner * a.dim * bytes) ? launch_norm_v<T, TR, V, 16 / V, true>(a, stream)
+                                                      : launch_norm_v<T, TR, V, 16 / V, false>(a, stream);
 }
 
 template <typename T>

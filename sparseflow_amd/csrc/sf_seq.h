@@ -13,9 +13,28 @@ struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
   T e[V];
 };
 
-template <typename T, int V>
+// V elements at p.  ONCE: read once, and more than the caches hold (read_once): they do
+// not keep it.
+template <typename T, int V, bool ONCE>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* __restrict__ p) {
+  constexpr int bytes = V * sizeof(T);
+  if constexpr (!ONCE) {
+    return *reinterpret_cast<const Vec<T, V>*>(p);
+  } else if constexpr (bytes % 16 == 0) {
+    typedef uint32_t U __attribute__((ext_vector_type(4)));
+    U u[bytes / 16];
+#pragma unroll
+    for (int i = 0; i < bytes / 16; ++i) u[i] = __builtin_nontemporal_load(reinterpret_cast<const U*>(p) + i);
+    return __builtin_bit_cast(Vec<T, V>, u);
+  } else {
+    static_assert(bytes == 8, "8 or 16 bytes");
+    typedef uint32_t U __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(Vec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const U*>(p)));
+  }
+}
+template <typename T, int V, bool ONCE = false>
 __device__ __forceinline__ void load_f32(const T* __restrict__ p, float (&v)[V]) {
-  const Vec<T, V> q = *reinterpret_cast<const Vec<T, V>*>(p);
+  const Vec<T, V> q = load_vec<T, V, ONCE>(p);
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = to_f32<T>(q.e[i]);
 }
@@ -26,6 +45,12 @@ __device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]
 #pragma unroll
   for (int i = 0; i < V; ++i) q.e[i] = from_f32<T>(v[i]);
   *reinterpret_cast<Vec<T, V>*>(p) = q;
+}
+
+// A store of data that the caches are not to keep (16 bytes).
+__device__ __forceinline__ void store_once(float* __restrict__ p, const float (&v)[4]) {
+  typedef float F __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(F{v[0], v[1], v[2], v[3]}, reinterpret_cast<F*>(p));
 }
 
 // Rows [first, first + n) of the token axis that are sequence b's (b the same in
@@ -87,6 +112,14 @@ __device__ __forceinline__ float sigmoid(float v) {
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
 }  // namespace
+
+// Whether a kernel that reads `bytes` once leaves them out of the caches: half of what
+// the memory side's holds, so that less than that still lies there from the kernel that
+// wrote it, or for the next.  Kept and left out: norm of 32768 x 1024 float32 (134 MB) 75
+// and 64 us, of 32768 x 384 25 and 29, of 32768 x 2048 f16 with gate and float32 residual
+// 215 and 207; states of 1 GB and 100 MB a step's 210 and 192, 38 and 40.  (The
+// convolution reads a run's last tokens again: 2 x 16384 x 4352 bf16 130 and 136.)
+inline bool read_once(int64_t bytes) { return bytes >= (int64_t)128 << 20; }
 
 // A launch holds fewer than 2^32 threads: `blocks` workgroups in as many
 // launches as that takes, block0 being the first of each.
