@@ -840,7 +840,6 @@ static sf::ScanArgs scan_args(const sf_scan_desc* d, const void* x, const void* 
   a.state_dim = d->state_dim;
   a.softplus = d->dt_softplus != 0;
   a.step = step ? 1 : 0;
-  a.state_vec = d->state_dim % 4 == 0 && sf::aligned_to(h0, 16) && sf::aligned_to(h1, 16);
   return a;
 }
 

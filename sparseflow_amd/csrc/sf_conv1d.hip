@@ -6,9 +6,9 @@
 // stay in registers as the run is walked, every input of the run is one load of 16
 // bytes, kBatch of them under way at a time, and the K - 1 before the run are read
 // again (from the cache: a neighbouring thread's run).  Bound by HBM: x in, y out;
-// 2 x 16384 x 4352 bf16, K = 4: 130 us, 4.4 TB/s; with single elements (odd channels)
-// ragged sequences of 17,300 x 1037 float32: 40 us, 3.6 TB/s; one token of 256 x 2304: 10
-// us, a call's own time.
+// 2 x 16384 x 4352 bf16, K = 4: 130 us, 4.4 TB/s; ragged sequences of 17,300 x 1037
+// float32, whose rows begin anywhere: 39 us, 3.4 TB/s; one token of 256 x 2304: 10 us, a
+// call's own time.
 #include "sf_seq.h"
 #include "sf_tile.h"
 
@@ -19,17 +19,7 @@ namespace {
 constexpr int kBatch = 8;  // tokens loaded at a time
 constexpr int kThreads = 256;
 
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void conv_load(const T* __restrict__ p, int ch, int channels, float (&v)[V]) {
-  if constexpr (VEC) {
-    load_f32<T, V>(p + ch, v);
-  } else {
-    static_assert(V == 1, "scalar form");
-    v[0] = to_f32<T>(p[ch]);
-  }
-}
-
-template <typename T, int K, int V, bool VEC>
+template <typename T, int K, int V>
 __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv, int blocks_per_seq, int runs,
                                                             int length, int keep) {
   const int64_t block = a.block0 + blockIdx.x;
@@ -37,7 +27,8 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
   const int64_t item = (block - b * blocks_per_seq) * kThreads + threadIdx.x;
   const int run = (int)(item / cv);
   if (run >= runs) return;
-  const int ch = (int)(item - (int64_t)run * cv) * V;
+  // (A row's last thread takes its last V channels, some of them another's too.)
+  const int ch = min((int)(item - (int64_t)run * cv) * V, a.channels - V);
   int64_t first, n;
   seq_rows(a.seq, b, first, n);
   const int64_t t0 = (int64_t)run * length;
@@ -55,8 +46,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = 0.f;
-    if constexpr (VEC) store_f32<T, V>(y + ch, z);
-    else y[ch] = from_f32<T>(0.f);
+    store_any_f32<T, V>(y + ch, z);
     return;
   }
   float w[K][V], bias[V];
@@ -72,15 +62,15 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
   for (int k = 0; k < K - 1; ++k) {
     const int64_t t = t0 - (K - 1) + k;
     if (t >= 0) {
-      conv_load<T, V, VEC>(x + t * a.x_t, ch, a.channels, u[k]);
+      load_any_f32<T, V>(x + t * a.x_t + ch, u[k]);
     } else if (before != nullptr) {
-      conv_load<T, V, VEC>(before + (t + K - 1) * (int64_t)a.channels, ch, a.channels, u[k]);
+      load_any_f32<T, V>(before + (t + K - 1) * (int64_t)a.channels + ch, u[k]);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) u[k][i] = 0.f;
     }
   }
-  const T* __restrict__ xt = x + t0 * a.x_t;
+  const T* __restrict__ xt = x + t0 * a.x_t + ch;
   T* __restrict__ yt = y + t0 * a.y_t + ch;
   // One token: u's last input has come in.
   auto token = [&]() {
@@ -92,8 +82,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
       for (int k = 0; k < K; ++k) s[i] = fmaf(w[k][i], u[k][i], s[i]);
       if (a.act == SF_ACT_SILU) s[i] = silu(s[i]);
     }
-    if constexpr (VEC) store_f32<T, V>(yt, s);
-    else *yt = from_f32<T>(s[0]);
+    store_any_f32<T, V>(yt, s);
     yt += a.y_t;
 #pragma unroll
     for (int k = 0; k + 1 < K; ++k)
@@ -105,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
     Vec<T, V> in[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      in[j] = *reinterpret_cast<const Vec<T, V>*>(xt + ch);
+      in[j] = load_any<T, V>(xt);
       xt += a.x_t;
     }
 #pragma unroll
@@ -116,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
     }
   }
   for (; left > 0; --left) {
-    conv_load<T, V, VEC>(xt, ch, a.channels, u[K - 1]);
+    load_any_f32<T, V>(xt, u[K - 1]);
     xt += a.x_t;
     token();
   }
@@ -124,8 +113,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
     T* after = static_cast<T*>(a.after) + slot * (K - 1) * (int64_t)a.channels;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-      if constexpr (VEC) store_f32<T, V>(after + (int64_t)k * a.channels + ch, u[k]);
-      else after[(int64_t)k * a.channels + ch] = from_f32<T>(u[k][0]);
+      store_any_f32<T, V>(after + (int64_t)k * a.channels + ch, u[k]);
     }
   }
 }
@@ -154,9 +142,9 @@ __global__ __launch_bounds__(kThreads) void k_conv1d_state(Conv1dArgs a, int blo
   for (int k = 0; k < m; ++k) after[(int64_t)k * a.channels + ch] = v[k];
 }
 
-template <typename T, int K, int V, bool VEC>
+template <typename T, int K, int V>
 int launch_conv1d_v(const Conv1dArgs& a, hipStream_t stream) {
-  const int cv = a.channels / V;
+  const int cv = (a.channels + V - 1) / V;
   // Runs as long as leave a few wavefronts for every SIMD (8 tokens read 3 / 8 of their
   // inputs twice, 64 less than a twentieth): 2 x 16384 x 4352 bf16 takes 132 us in runs of
   // 64 and 170 in runs of 8, 2048 x 1024 24 us in runs of 64 and 9 in runs of 8.
@@ -166,13 +154,13 @@ int launch_conv1d_v(const Conv1dArgs& a, hipStream_t stream) {
   const int64_t per_seq = (runs * cv + kThreads - 1) / kThreads;
   // In place: a step's thread holds all that it overwrites; in a prompt the
   // thread that writes a state is not the one that read it, unless there is one
-  // run.
+  // run and no channel has two threads.
   const size_t pool = (size_t)a.seq.states * (K - 1) * a.channels * sizeof(T);
   const char *p0 = static_cast<const char*>(a.before), *p1 = static_cast<const char*>(a.after);
   const bool keep = a.after != nullptr && K > 1;
-  const bool apart = keep && runs > 1 && a.before != nullptr && p0 < p1 + pool && p1 < p0 + pool;
+  const bool apart = keep && (runs > 1 || a.channels % V != 0) && a.before != nullptr && p0 < p1 + pool && p1 < p0 + pool;
   int rc = launch_blocks(a, &Conv1dArgs::block0, a.seq.batch * per_seq, [&](const Conv1dArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_causal_conv1d<T, K, V, VEC>), dim3(n), dim3(kThreads), 0, stream, la, cv, (int)per_seq,
+    hipLaunchKernelGGL((k_causal_conv1d<T, K, V>), dim3(n), dim3(kThreads), 0, stream, la, cv, (int)per_seq,
                        (int)runs, length, keep && !apart ? 1 : 0);
   });
   if (rc != (int)hipSuccess || !apart) return rc;
@@ -184,11 +172,10 @@ int launch_conv1d_v(const Conv1dArgs& a, hipStream_t stream) {
 
 template <typename T, int K>
 int launch_conv1d_k(const Conv1dArgs& a, hipStream_t stream) {
+  // 16 bytes an access, at any address.  A step in place has one thread to a channel.
   constexpr int V = 16 / sizeof(T);
-  // 16-byte accesses: every row of x, y and the states starts at a multiple.
-  const bool vec = a.channels % V == 0 && ((a.x_b | a.x_t | a.y_b | a.y_t) % V) == 0 && aligned_to(a.x, 16) &&
-                   aligned_to(a.y, 16) && aligned_to(a.before, 16) && aligned_to(a.after, 16);
-  return vec ? launch_conv1d_v<T, K, V, true>(a, stream) : launch_conv1d_v<T, K, 1, false>(a, stream);
+  return a.channels % V == 0 || (a.channels > V && !a.step) ? launch_conv1d_v<T, K, V>(a, stream)
+                                                            : launch_conv1d_v<T, K, 1>(a, stream);
 }
 
 template <typename T>

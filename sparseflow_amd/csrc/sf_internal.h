@@ -309,7 +309,6 @@ struct ScanArgs {
   int64_t block0;
   int heads, head_dim, groups, state_dim, softplus;
   int step;
-  int state_vec;  // rows of the states in units of 16 bytes
 };
 constexpr int kScanMaxState = 256;
 int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);

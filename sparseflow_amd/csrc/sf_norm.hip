@@ -67,9 +67,9 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
 #pragma unroll
     for (int e = 0; e < V; ++e) t[k][e] = 0.f;
     if (c >= width) continue;
-    load_f32<T, V, ONCE>(x + c, t[k]);
-    if (a.gate != nullptr) gv[k] = load_vec<T, V, ONCE>(g + c);
-    if (a.res != nullptr) rv[k] = load_vec<TR, V, ONCE>(res + c);
+    load_any_f32<T, V, ONCE>(x + c, t[k]);
+    if (a.gate != nullptr) gv[k] = load_any<T, V, ONCE>(g + c);
+    if (a.res != nullptr) rv[k] = load_any<TR, V, ONCE>(res + c);
   }
   auto gate = [&]() {
 #pragma unroll
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
       const float f = a.scale_w != nullptr ? a.scale * a.scale_w[c0 + c + e] : a.scale;
       t[k][e] = a.res != nullptr ? fmaf(f, t[k][e], to_f32<TR>(rv[k].e[e])) : f * t[k][e];
     }
-    if (a.r != nullptr) store_f32<TR, V>(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0 + c, t[k]);
+    if (a.r != nullptr) store_any_f32<TR, V>(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0 + c, t[k]);
   }
   if (a.pre_w != nullptr) {
     const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
       if (c >= width) continue;
 #pragma unroll
       for (int e = 0; e < V; ++e) t[k][e] *= f * a.pre_w[c0 + c + e];
-      store_f32<T, V>(h + c0 + c, t[k]);
+      store_any_f32<T, V>(h + c0 + c, t[k]);
     }
   }
 }
@@ -195,12 +195,7 @@ template <typename T, typename TR>
 int launch_norm_t(const NormArgs& a, hipStream_t stream) {
   // 16 bytes of the widest type.
   constexpr int V = 16 / (sizeof(T) > sizeof(TR) ? sizeof(T) : sizeof(TR));
-  const int64_t strides = a.x_o | a.x_i | a.r_o | a.r_i | a.h_o | a.h_i |
-                          (a.gate != nullptr ? a.g_o | a.g_i : 0) | (a.res != nullptr ? a.res_o | a.res_i : 0);
-  const bool vec = a.dim % V == 0 && a.group % V == 0 && strides % V == 0 && aligned_to(a.x, V * sizeof(T)) &&
-                   aligned_to(a.gate, V * sizeof(T)) && aligned_to(a.h, V * sizeof(T)) &&
-                   aligned_to(a.res, 16) && aligned_to(a.r, 16);
-  if (!vec) return launch_norm_v<T, TR, 1, 16, false>(a, stream);
+  if (a.dim % V != 0 || a.group % V != 0) return launch_norm_v<T, TR, 1, 16, false>(a, stream);
   const int64_t bytes = (a.gate != nullptr ? 2 : 1) * (int64_t)sizeof(T) + (a.res != nullptr ? (int64_t)sizeof(TR) : 0);
   return read_once(a.outer * a.inner * a.dim * bytes) ? launch_norm_v<T, TR, V, 16 / V, true>(a, stream)
                                                       : launch_norm_v<T, TR, V, 16 / V, false>(a, stream);

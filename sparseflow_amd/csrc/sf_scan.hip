@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_seq(ScanArgs a, int slices) {
     if (a.h0 != nullptr && slot >= 0 && p < P) {
       const float* row = a.h0 + head_row + (int64_t)p * N;
       if constexpr (VEC) {
-        if (n0 < N) load_f32<float, 4, ONCE>(row + n0, h[r]);
+        if (n0 < N) load_any_f32<float, 4, ONCE>(row + n0, h[r]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -65,29 +65,34 @@ __global__ __launch_bounds__(kThreads) void k_scan_seq(ScanArgs a, int slices) {
     }
   }
   for (int64_t t = 0; t < n; ++t) {
-    float bv[4] = {0.f, 0.f, 0.f, 0.f}, cv[4] = {0.f, 0.f, 0.f, 0.f};
+    // (All of a token's loads before the first use: rows and columns past the end read
+    // the last ones, and go nowhere.)
+    T xr[R], br[4], cr[4];
+    Vec<T, 4> bq, cq;
+    const T dr = dt[t * a.dt_t];
     if constexpr (VEC) {
-      if (n0 < N) {
-        load_f32<T, 4>(B + t * a.b_t + n0, bv);
-        load_f32<T, 4>(C + t * a.c_t + n0, cv);
-      }
+      bq = load_any<T, 4>(B + t * a.b_t + min(n0, N - 4));
+      cq = load_any<T, 4>(C + t * a.c_t + min(n0, N - 4));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n0 + i < N) {
-          bv[i] = to_f32<T>(B[t * a.b_t + n0 + i]);
-          cv[i] = to_f32<T>(C[t * a.c_t + n0 + i]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        br[i] = B[t * a.b_t + min(n0 + i, N - 1)];
+        cr[i] = C[t * a.c_t + min(n0 + i, N - 1)];
+      }
     }
-    float d = to_f32<T>(dt[t * a.dt_t]) + bias;
+#pragma unroll
+    for (int r = 0; r < R; ++r) xr[r] = x[t * a.x_t + min(p0 + r * kRows, P - 1)];
+    float bv[4], cv[4], xv[R], s[R];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bv[i] = to_f32<T>(VEC ? bq.e[i] : br[i]);
+      cv[i] = to_f32<T>(VEC ? cq.e[i] : cr[i]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) xv[r] = to_f32<T>(xr[r]);
+    float d = to_f32<T>(dr) + bias;
     if (a.softplus) d = softplus(d);
     const float decay = expf(A * d);
-    float xv[R], s[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int p = p0 + r * kRows;
-      xv[r] = p < P ? to_f32<T>(x[t * a.x_t + p]) : 0.f;
-    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float u = d * xv[r];
@@ -118,9 +123,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_seq(ScanArgs a, int slices) {
       if (p >= P) continue;
       float* row = a.h1 + head_row + (int64_t)p * N;
       if constexpr (VEC) {
-        if (n0 >= N) continue;
-        if constexpr (ONCE) store_once(row + n0, h[r]);
-        else store_f32<float, 4>(row + n0, h[r]);
+        if (n0 < N) store_any_f32<float, 4, ONCE>(row + n0, h[r]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -141,8 +144,7 @@ int launch_seq_r(const ScanArgs& a, hipStream_t stream) {
 
 template <typename T, int TN>
 int launch_seq_n(const ScanArgs& a, hipStream_t stream) {
-  const bool vec = a.state_vec != 0 && ((a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g) % 4) == 0 &&
-                   aligned_to(a.b, 4 * sizeof(T)) && aligned_to(a.c, 4 * sizeof(T));
+  const bool vec = a.state_dim % 4 == 0;
   // As many rows to a thread as the head has, up to 8 (a step of 256 sequences, 64 heads x
   // 64, N 128: 212 us, with two rows 218, with one 316).
   constexpr int kRows = kThreads / TN;

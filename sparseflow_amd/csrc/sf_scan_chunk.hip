@@ -25,6 +25,11 @@
 // bits, always: the state is summed up over all tokens and stays a float32 one.  L is
 // summed in 64 bits: differences of it are exponents.
 //
+// Bound by the chain of products and the waits between them, not by memory: 2 x 16384
+// tokens, 64 heads x 64, N 128, bf16 (562 MB, 241 GFLOP of products) take 389 us, 620
+// TFLOP/s and 1.4 TB/s, 280 of them the main pass; rows at any address, by way of
+// registers, a quarter more; 23 ragged sequences of up to 1500 of f16, 24 heads, 195 us.
+//
 // Few heads and long sequences: the token axis is cut into segments.  A first
 // pass walks each segment from a zero state for its own part of the state
 // (the last product alone), a second one chains the parts, and the main pass
@@ -248,19 +253,16 @@ __device__ __forceinline__ void wait_memory() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory");
 }
 
-// 8 elements of a row on their way to LDS; what lies outside becomes 0.  vec: rows
-// are whole units, aligned to 16 bytes.
+// 8 elements of a row on their way to LDS; what lies outside becomes 0.
 template <typename T>
-__device__ __forceinline__ void load_unit(const T* __restrict__ from, int left, bool vec, uint32_t (&v)[2 * sizeof(T)]) {
+__device__ __forceinline__ void load_unit(const T* __restrict__ from, int left, uint32_t (&v)[2 * sizeof(T)]) {
 #pragma unroll
   for (int i = 0; i < (int)(2 * sizeof(T)); ++i) v[i] = 0u;
-  if (vec) {
-    if (left > 0) {
+  if (left >= 8) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(from)[i];
-        v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
-      }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const AnyX4 q = reinterpret_cast<const AnyX4*>(from)[i];
+      v[4 * i] = q[0], v[4 * i + 1] = q[1], v[4 * i + 2] = q[2], v[4 * i + 3] = q[3];
     }
   } else if constexpr (sizeof(T) == 2) {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(from);
@@ -306,8 +308,7 @@ __device__ __forceinline__ int last_segment(const ScanSplit& sp, int64_t n) {
 // PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
 // which go straight into LDS.
 template <typename T, int PL, int NP, bool DIRECT, bool STATES>
-__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_scan_chunk(ScanArgs a, ScanSplit sp,
-                                                                                   bool vec) {
+__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_scan_chunk(ScanArgs a, ScanSplit sp) {
   constexpr int Q = kChunk, KB = Q / 16, NT = NP / 32, U = 8;
   constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits;  // of B and C at a time
   constexpr int kRounds = Q > kRows ? Q / kRows : 1;
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
     for (int r = 0; r < 16; ++r) h[nt][r] = 0.f;
   const int p = p0 + col;
   const bool mine = on && p < P;
-  const bool vec_n = a.state_vec != 0;
+  const bool vec_n = N % 4 == 0;
   const int64_t plane = (int64_t)P * N;
   const float* from = nullptr;
   if constexpr (!STATES) {
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
         const float* src = from + (int64_t)p * N + n0;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (vec_n) {
-          if (n0 < N) load_f32<float, 4>(src, v);
+          if (n0 < N) load_any_f32<float, 4>(src, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -487,18 +488,18 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   // By way of registers: the next chunk's B, C and x wait in them.
   constexpr int kWords = 2 * (int)sizeof(T);
   uint32_t nb[kRounds][kWords], nc[STATES ? 1 : kRounds][kWords], nx[kXRounds][kWords];
-  auto fetch = [&](const T* b_from, const T* c_from, const T* x_from, int len, bool vec) {
+  auto fetch = [&](const T* b_from, const T* c_from, const T* x_from, int len) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int j = r * kRows + bj;
-      load_unit<T>(b_from + ((int64_t)(r * kRows) * b_t + (bj * b_t + bv * U)), j < len ? N - bv * U : 0, vec, nb[r]);
+      load_unit<T>(b_from + ((int64_t)(r * kRows) * b_t + (bj * b_t + bv * U)), j < len ? N - bv * U : 0, nb[r]);
       if constexpr (!STATES)
-        load_unit<T>(c_from + ((int64_t)(r * kRows) * c_t + (bj * c_t + bv * U)), j < len ? N - bv * U : 0, vec, nc[r]);
+        load_unit<T>(c_from + ((int64_t)(r * kRows) * c_t + (bj * c_t + bv * U)), j < len ? N - bv * U : 0, nc[r]);
     }
 #pragma unroll
     for (int r = 0; r < kXRounds; ++r)
       load_unit<T>(x_from + ((int64_t)(r * kXRows) * x_t + (xj * x_t + xv * U)),
-                   on && r * kXRows + xj < len ? P - p0 - xv * U : 0, vec, nx[r]);
+                   on && r * kXRows + xj < len ? P - p0 - xv * U : 0, nx[r]);
   };
   auto unload = [&](uint16_t* to_b, uint16_t* to_x) {
 #pragma unroll
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
       x += (int64_t)Q * x_t;
     }
   } else if (left > 0) {
-    fetch(B, C, x, (int)(left < Q ? left : Q), vec);
+    fetch(B, C, x, (int)(left < Q ? left : Q));
   }
   load_dt(dt, left);
   write_scalars(left);
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
     const uint16_t* s_x = s_x0 + at * PL * kX;
     if constexpr (DIRECT) {
       if (!ahead(left)) {
-        fetch(B - (int64_t)(kDepth - 1) * Q * b_t, C, x - (int64_t)(kDepth - 1) * Q * x_t, len, true);
+        fetch(B - (int64_t)(kDepth - 1) * Q * b_t, C, x - (int64_t)(kDepth - 1) * Q * x_t, len);
         unload(s_b0 + at * kTile, s_x0 + at * kX);
       }
       // This chunk has arrived.  Issued after it: the chunk before's y (four stores), or
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
     C += (int64_t)Q * c_t;
     x += (int64_t)Q * x_t;
     if constexpr (!DIRECT) {
-      if (left > Q) fetch(B, C, x, (int)(left - Q < Q ? left - Q : Q), vec);
+      if (left > Q) fetch(B, C, x, (int)(left - Q < Q ? left - Q : Q));
     }
     if (i % 2 == 0) {
       dt += (int64_t)(2 * Q) * dt_t;
@@ -722,9 +723,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
       }
       if (on && col < len) {
         T* row = y + (col * y_t + 4 * half);
-        if ((DIRECT || vec) && whole_p) {
+        if (whole_p) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) store_f32<T, 4>(row + 8 * q, {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
+          for (int q = 0; q < 4; ++q) store_any_f32<T, 4>(row + 8 * q, {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -788,7 +789,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = h[nt][4 * q + e] * f;
         if (vec_n) {
-          if (n0 < N) store_f32<float, 4>(dst, v);
+          if (n0 < N) store_any_f32<float, 4>(dst, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -831,22 +832,22 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
 }
 
 template <typename T, int PL, int NP, bool DIRECT, bool STATES>
-int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
+int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   const int rc = set_lds_limit_once<k_scan_chunk<T, PL, NP, DIRECT, STATES>>(kMaxLdsBytes);
   if (rc != (int)hipSuccess) return rc;
   constexpr int lds = ChunkLds<PL, NP>::bytes(chunk_depth<NP, DIRECT, STATES>(), STATES);
   static_assert(lds <= kMaxLdsBytes, "a workgroup's LDS");
   const int64_t blocks = a.seq.batch * (STATES ? sp.segments - 1 : sp.segments) * a.groups * sp.blocks;
   return launch_blocks(a, &ScanArgs::block0, blocks, [&](const ScanArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_scan_chunk<T, PL, NP, DIRECT, STATES>), dim3(n), dim3(kThreads), lds, stream, la, sp, vec);
+    hipLaunchKernelGGL((k_scan_chunk<T, PL, NP, DIRECT, STATES>), dim3(n), dim3(kThreads), lds, stream, la, sp);
   });
 }
 
 template <typename T, int PL, int NP, bool DIRECT>
-int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
+int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   if (sp.segments > 1) {
     timing_begin(K_SCAN_PARTS, stream);
-    int rc = launch_chunk_k<T, PL, NP, DIRECT, true>(a, sp, vec, stream);
+    int rc = launch_chunk_k<T, PL, NP, DIRECT, true>(a, sp, stream);
     if (rc == (int)hipSuccess) {
       const int64_t plane = (int64_t)a.head_dim * a.state_dim;
       const int64_t blocks = (plane + kChainThreads - 1) / kChainThreads;
@@ -858,17 +859,17 @@ int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t
     if (rc != (int)hipSuccess) return rc;
   }
   timing_begin(K_SCAN_CHUNK, stream);
-  const int rc = launch_chunk_k<T, PL, NP, DIRECT, false>(a, sp, vec, stream);
+  const int rc = launch_chunk_k<T, PL, NP, DIRECT, false>(a, sp, stream);
   timing_end(K_SCAN_CHUNK, stream);
   return rc;
 }
 
 template <typename T, int PL, bool DIRECT>
-int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, bool vec, hipStream_t stream) {
-  if (a.state_dim <= 32) return launch_chunk_n<T, PL, 32, DIRECT>(a, sp, vec, stream);
-  if (a.state_dim <= 64) return launch_chunk_n<T, PL, 64, DIRECT>(a, sp, vec, stream);
-  if (a.state_dim <= 128) return launch_chunk_n<T, PL, 128, DIRECT>(a, sp, vec, stream);
-  return launch_chunk_n<T, PL, 256, DIRECT>(a, sp, vec, stream);
+int launch_chunk_m(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
+  if (a.state_dim <= 32) return launch_chunk_n<T, PL, 32, DIRECT>(a, sp, stream);
+  if (a.state_dim <= 64) return launch_chunk_n<T, PL, 64, DIRECT>(a, sp, stream);
+  if (a.state_dim <= 128) return launch_chunk_n<T, PL, 128, DIRECT>(a, sp, stream);
+  return launch_chunk_n<T, PL, 256, DIRECT>(a, sp, stream);
 }
 
 size_t align16(size_t v) { return (v + 15) / 16 * 16; }
@@ -916,13 +917,13 @@ int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int
   ScanSplit sp = p.split;
   sp.parts = static_cast<float*>(workspace);
   sp.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums_at);
-  const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g | a.y_b | a.y_t | a.y_h;
-  const bool vec = strides % 8 == 0 && a.head_dim % 8 == 0 && a.state_dim % 8 == 0 && aligned_to(a.x, 16) &&
-                   aligned_to(a.b, 16) && aligned_to(a.c, 16) && aligned_to(a.y, 16);
-  if (dtype == SF_F32) return launch_chunk_m<float, 3, false>(a, sp, vec, stream);
-  if (dtype == SF_F16) return launch_chunk_m<__half, 2, false>(a, sp, vec, stream);
-  if (vec) return launch_chunk_m<__hip_bfloat16, 1, true>(a, sp, vec, stream);
-  return launch_chunk_m<__hip_bfloat16, 1, false>(a, sp, vec, stream);
+  if (dtype == SF_F32) return launch_chunk_m<float, 3, false>(a, sp, stream);
+  if (dtype == SF_F16) return launch_chunk_m<__half, 2, false>(a, sp, stream);
+  const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g;
+  const bool units = strides % 8 == 0 && a.head_dim % 8 == 0 && a.state_dim % 8 == 0 && aligned_to(a.x, 16) &&
+                     aligned_to(a.b, 16) && aligned_to(a.c, 16);
+  if (units) return launch_chunk_m<__hip_bfloat16, 1, true>(a, sp, stream);
+  return launch_chunk_m<__hip_bfloat16, 1, false>(a, sp, stream);
 }
 
 }  // namespace sf

@@ -7,34 +7,60 @@
 namespace sf {
 namespace {
 
-// V elements of T, loaded and stored at once (p aligned to all of them, or to 16 bytes).
+// V elements of T, loaded and stored at once.
 template <typename T, int V>
 struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
   T e[V];
 };
 
-// V elements at p.  ONCE: read once, and more than the caches hold (read_once): they do
-// not keep it.
-template <typename T, int V, bool ONCE>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* __restrict__ p) {
-  constexpr int bytes = V * sizeof(T);
-  if constexpr (!ONCE) {
-    return *reinterpret_cast<const Vec<T, V>*>(p);
-  } else if constexpr (bytes % 16 == 0) {
-    typedef uint32_t U __attribute__((ext_vector_type(4)));
-    U u[bytes / 16];
+// 16 and 8 bytes at the address of any 16-bit element.
+typedef uint32_t AnyX4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t AnyX2 __attribute__((ext_vector_type(2), aligned(2)));
+
+// V elements at p, aligned to one element only: global memory takes 8 and 16 bytes at
+// any address.  ONCE: read once, and more than the caches hold (read_once): they do not
+// keep it.
+template <typename T, int V, bool ONCE = false>
+__device__ __forceinline__ Vec<T, V> load_any(const T* __restrict__ p) {
+  Vec<T, V> q;
+  if constexpr (ONCE && sizeof(q) % 16 == 0) {
+    AnyX4 u[sizeof(q) / 16];
 #pragma unroll
-    for (int i = 0; i < bytes / 16; ++i) u[i] = __builtin_nontemporal_load(reinterpret_cast<const U*>(p) + i);
-    return __builtin_bit_cast(Vec<T, V>, u);
+    for (int i = 0; i < (int)sizeof(q) / 16; ++i) u[i] = __builtin_nontemporal_load(reinterpret_cast<const AnyX4*>(p) + i);
+    __builtin_memcpy(&q, u, sizeof(q));
+  } else if constexpr (ONCE && sizeof(q) == 8) {
+    const AnyX2 u = __builtin_nontemporal_load(reinterpret_cast<const AnyX2*>(p));
+    __builtin_memcpy(&q, &u, sizeof(q));
   } else {
-    static_assert(bytes == 8, "8 or 16 bytes");
-    typedef uint32_t U __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(Vec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const U*>(p)));
+    __builtin_memcpy(&q, p, sizeof(q));
   }
+  return q;
 }
 template <typename T, int V, bool ONCE = false>
+__device__ __forceinline__ void load_any_f32(const T* __restrict__ p, float (&v)[V]) {
+  const Vec<T, V> q = load_any<T, V, ONCE>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_f32<T>(q.e[i]);
+}
+template <typename T, int V, bool ONCE = false>
+__device__ __forceinline__ void store_any_f32(T* __restrict__ p, const float (&v)[V]) {
+  Vec<T, V> q;
+#pragma unroll
+  for (int i = 0; i < V; ++i) q.e[i] = from_f32<T>(v[i]);
+  if constexpr (ONCE) {
+    static_assert(sizeof(q) == 16, "one access");
+    AnyX4 u;
+    __builtin_memcpy(&u, &q, sizeof(q));
+    __builtin_nontemporal_store(u, reinterpret_cast<AnyX4*>(p));
+  } else {
+    __builtin_memcpy(p, &q, sizeof(q));
+  }
+}
+
+// Aligned to all of them, or to 16 bytes.
+template <typename T, int V>
 __device__ __forceinline__ void load_f32(const T* __restrict__ p, float (&v)[V]) {
-  const Vec<T, V> q = load_vec<T, V, ONCE>(p);
+  const Vec<T, V> q = *reinterpret_cast<const Vec<T, V>*>(p);
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = to_f32<T>(q.e[i]);
 }
@@ -45,12 +71,6 @@ __device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]
 #pragma unroll
   for (int i = 0; i < V; ++i) q.e[i] = from_f32<T>(v[i]);
   *reinterpret_cast<Vec<T, V>*>(p) = q;
-}
-
-// A store of data that the caches are not to keep (16 bytes).
-__device__ __forceinline__ void store_once(float* __restrict__ p, const float (&v)[4]) {
-  typedef float F __attribute__((ext_vector_type(4)));
-  __builtin_nontemporal_store(F{v[0], v[1], v[2], v[3]}, reinterpret_cast<F*>(p));
 }
 
 // Rows [first, first + n) of the token axis that are sequence b's (b the same in

@@ -127,6 +127,28 @@ def test_conv_strided_views_pool_in_place_and_step():
     assert torch.equal(step_pool[[0, 2, 3, 4, 5]], before[[0, 2, 3, 4, 5]])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,c", [(1, 13), (6, 37), (90, 1037), (40, 3), (50, 64)])
+def test_conv_odd_rows_at_any_address_and_in_place(dtype, n, c):
+    announce(f"conv odd rows {dtype} n={n} c={c}")
+    g = _gen(n + c)
+    k, off = 4, 3
+    wide = _randn(g, 2, n, c + off, dtype=dtype).to(DEV)
+    x = wide[..., off:]
+    w, b = _randn(g, c, k).to(DEV), _randn(g, c).to(DEV)
+    pool = torch.zeros(1 + 2 * (k - 1) * c, dtype=dtype, device=DEV)[1:].view(2, k - 1, c)
+    pool.copy_(_randn(g, 2, k - 1, c, dtype=dtype))
+    start = pool.clone()
+    y, kept = causal_conv1d_forward(x, w, b, activation="silu", initial_state=pool, final_state=pool)
+    assert kept is pool
+    for i in range(2):
+        _conv_check(y[i], pool[i], x[i], w, b, "silu", start[i], dtype, f"sequence {i}")
+    stepped = start.clone()
+    for t in range(min(n, 9)):
+        yt = causal_conv1d_step(stepped, x[:, t], w, b, activation="silu")
+        assert torch.equal(yt, y[:, t])
+
+
 # ---- selective scan -----------------------------------------------------------
 
 
@@ -319,6 +341,24 @@ def test_scan_bad_values_reach_later_tokens_only(dtype, bad, where):
     assert torch.equal(torch.isfinite(state[0].double().cpu()), torch.isfinite(h))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,H,P,G,N", [(5, 3, 64, 1, 64), (75, 4, 64, 2, 128), (700, 2, 40, 1, 96), (40, 2, 36, 1, 20)])
+def test_scan_rows_at_any_address(dtype, n, H, P, G, N):
+    announce(f"scan odd rows {dtype} n={n} H={H} P={P} G={G} N={N}")
+    g = _gen(n + P)
+    _, dt, A, _, _, D, bias = _scan_inputs(g, (2, n), H, P, G, N, dtype)
+    row = _randn(g, 2, n, 1 + H * P + 2 * G * N, dtype=dtype)  # an odd number of elements from row to row
+    x = row[..., 1:1 + H * P].unflatten(-1, (H, P))
+    B, C = (row[..., 1 + H * P + i * G * N:1 + H * P + (i + 1) * G * N].unflatten(-1, (G, N)) for i in range(2))
+    h0 = _randn(g, 2, H, P, N)
+    out = torch.zeros(2, n, H * P + 3, dtype=dtype, device=DEV)[..., 1:1 + H * P].unflatten(-1, (H, P))
+    y, state = selective_scan_forward(_on_device(x), _on_device(dt), A.to(DEV), _on_device(B), _on_device(C), D.to(DEV),
+                                      bias.to(DEV), initial_state=h0.to(DEV), out=out)
+    assert y is out and not out._base[..., 0].any() and not out._base[..., 1 + H * P:].any()
+    for b in range(2):
+        _scan_check(y[b], state[b], x[b], dt[b], A, B[b], C[b], D, bias, True, h0[b], dtype, f"sequence {b}")
+
+
 def test_scan_without_softplus_and_strides_of_its_own():
     announce("scan no softplus, head-major views")
     H, P, G, N, n = 4, 32, 2, 32, 100
@@ -368,6 +408,20 @@ def test_block_norm(dtype, res, rows, dim, form):
     if h is not None:
         rms = torch.sqrt(rr.square().mean(-1, keepdim=True) + eps)
         _within(h, hh, 2 * f * (mag / rms * pre + hh.abs()) + HALF_ULP[dtype] * hh.abs() + 2.0 ** -25, "h")
+
+
+@pytest.mark.parametrize("dtype,res", [(F32, F32), (F16, F16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("rows,dim", [(3, 64), (2, 1024), (5, 104)])
+def test_block_norm_rows_at_any_address(dtype, res, rows, dim):
+    announce(f"norm odd rows {dtype} {res} {rows}x{dim}")
+    g = _gen(rows + dim)
+    x, gate = (_randn(g, rows, dim + 1, dtype=dtype).to(DEV)[:, 1:] for _ in range(2))
+    residual = _randn(g, rows, dim + 3, dtype=res).to(DEV)[:, 3:]
+    w, pre = torch.rand(dim, generator=g) + 0.5, torch.rand(dim, generator=g) + 0.5
+    kw = dict(post_weight=w.to(DEV), group_size=dim // 8, pre_weight=pre.to(DEV))
+    r, h = block_norm_forward(x, gate, residual=residual, **kw)
+    r2, h2 = block_norm_forward(x.contiguous(), gate.contiguous(), residual=residual.contiguous(), **kw)
+    assert torch.equal(r, r2) and torch.equal(h, h2)
 
 
 def test_block_norm_strides_broadcasts_and_in_place():
