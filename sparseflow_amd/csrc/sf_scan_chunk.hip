@@ -803,29 +803,37 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
 // Segment by segment, the state that the next one starts from, in the place of that
 // one's own part.
 constexpr int kChainThreads = 256;
+template <int V>
 __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSplit sp, int blocks) {
   int64_t item = a.block0 + blockIdx.x;
   const int part = (int)(item % blocks);
   item /= blocks;
   const int hd = (int)(item % a.heads);
   const int64_t b = item / a.heads;
-  const int64_t plane = (int64_t)a.head_dim * a.state_dim;
-  const int64_t e = (int64_t)part * kChainThreads + threadIdx.x;
-  if (e >= plane) return;
   int64_t first, n;
   seq_rows(a.seq, b, first, n);
   const int last = last_segment(sp, n);
+  const int64_t plane = (int64_t)a.head_dim * a.state_dim;
+  const int64_t e = ((int64_t)part * kChainThreads + threadIdx.x) * V;
+  if (last == 0 || e >= plane) return;
   const int64_t slot = seq_slot(a.seq, b);
-  float h = a.h0 != nullptr && slot >= 0 ? a.h0[(slot * a.heads + hd) * plane + e] : 0.f;
+  float h[V] = {};
+  if (a.h0 != nullptr && slot >= 0) load_any_f32<float, V>(a.h0 + (slot * a.heads + hd) * plane + e, h);
   float* at = sp.parts + (b * sp.segments * a.heads + hd) * plane + e;
   const float* sum = sp.sums + b * sp.segments * a.heads + hd;
-  float own = last > 0 ? *at : 0.f;
+  float own[V];
+  load_any_f32<float, V>(at, own);
   for (int s = 0; s < last; ++s) {
     float* const next = at + a.heads * plane;
-    const float next_own = s + 1 < last ? *next : 0.f;
-    h = fmaf(h, exp2f(*sum), own);
-    *next = h;
-    own = next_own;
+    float next_own[V] = {};
+    if (s + 1 < last) load_any_f32<float, V>(next, next_own);
+    const float decay = exp2f(*sum);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      h[i] = fmaf(h[i], decay, own[i]);
+      own[i] = next_own[i];
+    }
+    store_any_f32<float, V>(next, h);
     at = next;
     sum += a.heads;
   }
@@ -843,17 +851,22 @@ int launch_chunk_k(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   });
 }
 
+template <int V>
+int launch_chain(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
+  constexpr int each = kChainThreads * V;
+  const int64_t blocks = ((int64_t)a.head_dim * a.state_dim + each - 1) / each;
+  return launch_blocks(a, &ScanArgs::block0, a.seq.batch * a.heads * blocks, [&](const ScanArgs& la, unsigned n) {
+    hipLaunchKernelGGL(k_scan_chain<V>, dim3(n), dim3(kChainThreads), 0, stream, la, sp, (int)blocks);
+  });
+}
+
 template <typename T, int PL, int NP, bool DIRECT>
 int launch_chunk_n(const ScanArgs& a, const ScanSplit& sp, hipStream_t stream) {
   if (sp.segments > 1) {
     timing_begin(K_SCAN_PARTS, stream);
     int rc = launch_chunk_k<T, PL, NP, DIRECT, true>(a, sp, stream);
     if (rc == (int)hipSuccess) {
-      const int64_t plane = (int64_t)a.head_dim * a.state_dim;
-      const int64_t blocks = (plane + kChainThreads - 1) / kChainThreads;
-      rc = launch_blocks(a, &ScanArgs::block0, a.seq.batch * a.heads * blocks, [&](const ScanArgs& la, unsigned n) {
-        hipLaunchKernelGGL(k_scan_chain, dim3(n), dim3(kChainThreads), 0, stream, la, sp, (int)blocks);
-      });
+      rc = a.state_dim % 4 == 0 ? launch_chain<4>(a, sp, stream) : launch_chain<1>(a, sp, stream);
     }
     timing_end(K_SCAN_PARTS, stream);
     if (rc != (int)hipSuccess) return rc;
