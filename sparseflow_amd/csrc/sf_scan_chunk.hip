@@ -898,14 +898,22 @@ ScanPlan scan_plan(int64_t batch, int64_t tokens, int64_t max_len, int heads, in
   // Segments: as many as the CUs hold workgroups for at once (fit: of a CU), since one
   // more makes all wait for a second turn (32 x 1024 tokens of f16, 24 heads x 64, N 128:
   // 334 us as 768 workgroups, 245 as 384), and of two chunks or more (1 x 512 of bf16, 16
-  // heads: 52 us whole, 43 in segments of four, 39 of two; under 8 chunks the passes'
-  // launches cost what they save: 1 x 200 of bf16, 8 heads x 32, 20 us whole, 25 cut).
-  // In a packed call the sequences are taken to fill their tokens with their longest.
+  // heads: 43 us in segments of four, 39 of two).  In a packed call the sequences are
+  // taken to fill their tokens with their longest.
+  // Whole, a call of up to a workgroup to a CU takes a time per chunk; cut, one per chunk
+  // and workgroup that comes to the same near a workgroup for each of 7/8 of the CUs, and
+  // for the passes and their launches the time of 14 chunks (bf16), 8 (f16) or 6
+  // (float32).  Whole and cut, us, 24 heads x 64, N 128: bf16 2 x 512 52 and 45, 5 x 512 53
+  // and 58, 8 x 1024 96 and 88, 16 x 1024 96 and 114, 16 x 4096 352 and 305, 21 x 4096 356
+  // and 378; f16 5 x 512 79 and 63, 11 x 512 78 and 88, 11 x 1024 144 and 132, 16 x 1024 146
+  // and 163; float32 8 x 256 58 and 65, 8 x 512 104 and 92, 16 x 512 106 and 136.
   const int64_t fit = state_dim > 128 ? 1 : dtype == SF_BF16 ? 3 : 2;
-  const int64_t chunks = (max_len + kChunk - 1) / kChunk;
+  const int64_t passes = dtype == SF_BF16 ? 14 : dtype == SF_F16 ? 8 : 6;
+  const int64_t chunks = (max_len + kChunk - 1) / kChunk, cus = num_cus();
   int64_t full = batch;
   if (max_len < tokens && (tokens + max_len - 1) / max_len < full) full = (tokens + max_len - 1) / max_len;
-  int64_t segs = chunks < 8 ? 1 : fit * num_cus() / (full * groups * p.split.blocks);
+  const int64_t base = full * groups * p.split.blocks;
+  int64_t segs = chunks * (7 * cus - 8 * base) > passes * 7 * cus ? fit * cus / base : 1;
   if (segs > chunks / 2) segs = chunks / 2;
   if (segs < 1) segs = 1;
   const int64_t per = (chunks + segs - 1) / segs;
