@@ -5,7 +5,7 @@
 // A row is held in registers by LT threads, vectors of V elements: x, gate and residual
 // are all loaded before the first sum, and h is written after the second.  Bound by
 // HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 152 us, 5.3 TB/s; 32768 x 2048
-// f16 with gate, float32 residual and h (940 MB) 207 us, 4.5 TB/s.  Short rows (up to 3
+// f16 with gate, float32 residual and h (940 MB) 180 us, 5.2 TB/s.  Short rows (up to 3
 // vectors a lane) are a wavefront's, whose sums need no barrier: 32768 x 384 float32 25
 // us, as a workgroup's 37; of 768 53 and 57; of four vectors, 2048 bf16, 86 and 77.
 //
@@ -13,11 +13,17 @@
 // a workgroup holds the row and the groups' sums meet in LDS.
 #include "sf_seq.h"
 
+#include <type_traits>
+
 namespace sf {
 
 namespace {
 
 constexpr int kBlock = 256;
+// Rows of whole vectors; those whose inputs the caches are not to keep; rows that end
+// inside a vector (32768 x 2047 bf16: 141 us, by single elements 238; the checks for it
+// would cost whole rows, 2048, 92 against 70).
+constexpr int kPlain = 0, kOnce = 1, kRagged = 2;
 
 __device__ __forceinline__ float act_of(int act, float v) {
   return act == SF_ACT_SILU ? silu(v) : act == SF_ACT_SIGMOID ? sigmoid(v) : v;
@@ -44,8 +50,9 @@ __device__ __forceinline__ float row_sum(float v, float* s_part) {
 // inside the row (LT = the workgroup, group % V == 0).  (Workgroups that go row after
 // row with their weights in registers were no faster: 226 against 214 us at
 // 32768 x 2048, f16 with a float32 residual.)
-template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, bool ONCE>
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, int MODE>
 __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormArgs a, int sub) {
+  constexpr bool ONCE = MODE == kOnce, RAGGED = MODE == kRagged;
   constexpr int kRowsPerBlock = (LT > kBlock ? LT : kBlock) / LT;
   __shared__ float s_part[LT / kWave];
   const int lt = threadIdx.x % LT;
@@ -67,6 +74,17 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
 #pragma unroll
     for (int e = 0; e < V; ++e) t[k][e] = 0.f;
     if (c >= width) continue;
+    if (RAGGED && c + V > width) {
+      // The end of a row that is not whole vectors: zeros behind it.
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int at = min(c + e, width - 1);
+        if (c + e < width) t[k][e] = to_f32<T>(x[at]);
+        if (a.gate != nullptr) gv[k].e[e] = g[at];
+        if (a.res != nullptr) rv[k].e[e] = res[at];
+      }
+      continue;
+    }
     load_any_f32<T, V, ONCE>(x + c, t[k]);
     if (a.gate != nullptr) gv[k] = load_any<T, V, ONCE>(g + c);
     if (a.res != nullptr) rv[k] = load_any<TR, V, ONCE>(res + c);
@@ -79,8 +97,39 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
       for (int e = 0; e < V; ++e) t[k][e] *= act_of(a.act, to_f32<T>(gv[k].e[e]));
     }
   };
+  // The weights of a vector's columns (behind the row's end the last one).
+  auto weights = [&](const float* __restrict__ w, int c, float (&v)[V]) {
+    if (!RAGGED || c + V <= width) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = w[c0 + c + e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = w[c0 + min(c + e, width - 1)];
+    }
+  };
+  auto store = [&](auto* __restrict__ p, int c, const float (&v)[V]) {
+    typedef std::remove_reference_t<decltype(*p)> E;
+    if (!RAGGED || c + V <= width) {
+      store_any_f32<E, V>(p + c, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c + e < width) p[c + e] = from_f32<E>(v[e]);
+    }
+  };
   auto squares = [&]() {
     float s = 0.f;
+    if constexpr (RAGGED) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * LT + lt) * V;
+        if (c < width && c + V > width) {
+          // (What a gate or weight that is not finite made of the zeros.)
+#pragma unroll
+          for (int e = 0; e < V; ++e) t[k][e] = c + e < width ? t[k][e] : 0.f;
+        }
+      }
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -127,8 +176,10 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
     for (int k = 0; k < NV; ++k) {
       const int c = (k * LT + lt) * V;
       if (c >= width) continue;
+      float w[V];
+      weights(a.post_w, c, w);
 #pragma unroll
-      for (int e = 0; e < V; ++e) t[k][e] *= a.post_w[c0 + c + e];
+      for (int e = 0; e < V; ++e) t[k][e] *= w[e];
     }
   }
   if (a.gate != nullptr && !a.gate_first) gate();
@@ -136,12 +187,14 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
   for (int k = 0; k < NV; ++k) {
     const int c = (k * LT + lt) * V;
     if (c >= width) continue;
+    float w[V] = {};
+    if (a.scale_w != nullptr) weights(a.scale_w, c, w);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float f = a.scale_w != nullptr ? a.scale * a.scale_w[c0 + c + e] : a.scale;
+      const float f = a.scale_w != nullptr ? a.scale * w[e] : a.scale;
       t[k][e] = a.res != nullptr ? fmaf(f, t[k][e], to_f32<TR>(rv[k].e[e])) : f * t[k][e];
     }
-    if (a.r != nullptr) store_any_f32<TR, V>(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0 + c, t[k]);
+    if (a.r != nullptr) store(static_cast<TR*>(a.r) + o * a.r_o + i * a.r_i + c0, c, t[k]);
   }
   if (a.pre_w != nullptr) {
     const float f = 1.f / sqrtf(row_sum<LT>(squares(), s_part) / (float)width + a.eps);
@@ -150,55 +203,60 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
     for (int k = 0; k < NV; ++k) {
       const int c = (k * LT + lt) * V;
       if (c >= width) continue;
+      float w[V];
+      weights(a.pre_w, c, w);
 #pragma unroll
-      for (int e = 0; e < V; ++e) t[k][e] *= f * a.pre_w[c0 + c + e];
-      store_any_f32<T, V>(h + c0 + c, t[k]);
+      for (int e = 0; e < V; ++e) t[k][e] *= f * w[e];
+      store(h + c0, c, t[k]);
     }
   }
 }
 
-template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, bool ONCE>
+template <typename T, typename TR, int LT, int V, int NV, bool GROUPED, int MODE>
 int launch_norm_k(const NormArgs& a, int sub, hipStream_t stream) {
   constexpr int threads = LT > kBlock ? LT : kBlock, rows = threads / LT;
   const int64_t items = a.outer * a.inner * sub;
   const size_t lds = GROUPED ? (size_t)(a.dim / V + a.dim / a.group) * sizeof(float) : 0;
   if (lds > 48 * 1024) {
-    const int rc = set_lds_limit_once<k_block_norm<T, TR, LT, V, NV, GROUPED, ONCE>>(kMaxLdsBytes - 1024);
+    const int rc = set_lds_limit_once<k_block_norm<T, TR, LT, V, NV, GROUPED, MODE>>(kMaxLdsBytes - 1024);
     if (rc != (int)hipSuccess) return rc;
   }
   return launch_blocks(a, &NormArgs::item0, (items + rows - 1) / rows, [&](const NormArgs& la, unsigned n) {
-    hipLaunchKernelGGL((k_block_norm<T, TR, LT, V, NV, GROUPED, ONCE>), dim3(n), dim3(threads), lds, stream, la, sub);
+    hipLaunchKernelGGL((k_block_norm<T, TR, LT, V, NV, GROUPED, MODE>), dim3(n), dim3(threads), lds, stream, la, sub);
   });
 }
 
 // M vectors a thread hold the widest row that 1024 threads take.
-template <typename T, typename TR, int V, int M, bool ONCE>
+template <typename T, typename TR, int V, int M, int MODE>
 int launch_norm_v(const NormArgs& a, hipStream_t stream) {
   const bool grouped = a.post_w != nullptr && a.group != a.dim;
-  if (grouped && a.pre_w != nullptr) {
-    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true, ONCE>(a, 1, stream);
-    return launch_norm_k<T, TR, 1024, V, M, true, ONCE>(a, 1, stream);
+  if (MODE != kRagged && grouped && a.pre_w != nullptr) {
+    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true, MODE>(a, 1, stream);
+    return launch_norm_k<T, TR, 1024, V, M, true, MODE>(a, 1, stream);
   }
   const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
-  if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false, ONCE>(a, sub, stream);
-  if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false, ONCE>(a, sub, stream);
-  if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false, ONCE>(a, sub, stream);
-  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false, false>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false, ONCE>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false, ONCE>(a, sub, stream);
-  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false, ONCE>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false, ONCE>(a, sub, stream);
-  return launch_norm_k<T, TR, 1024, V, M, false, ONCE>(a, sub, stream);
+  if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false, MODE>(a, sub, stream);
+  if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false, MODE>(a, sub, stream);
+  if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false, MODE>(a, sub, stream);
+  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false, kPlain>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false, MODE>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false, MODE>(a, sub, stream);
+  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false, MODE>(a, sub, stream);
+  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false, MODE>(a, sub, stream);
+  return launch_norm_k<T, TR, 1024, V, M, false, MODE>(a, sub, stream);
 }
 
 template <typename T, typename TR>
 int launch_norm_t(const NormArgs& a, hipStream_t stream) {
   // 16 bytes of the widest type.
   constexpr int V = 16 / (sizeof(T) > sizeof(TR) ? sizeof(T) : sizeof(TR));
-  if (a.dim % V != 0 || a.group % V != 0) return launch_norm_v<T, TR, 1, 16, false>(a, stream);
+  // Groups inside a row that are not whole vectors: single elements.
+  if (a.post_w != nullptr && a.pre_w != nullptr && a.group != a.dim && a.group % V != 0)
+    return launch_norm_v<T, TR, 1, 16, kPlain>(a, stream);
   const int64_t bytes = (a.gate != nullptr ? 2 : 1) * (int64_t)sizeof(T) + (a.res != nullptr ? (int64_t)sizeof(TR) : 0);
-  return read_once(a.outer * a.inner * a.dim * bytes) ? launch_norm_v<T, TR, V, 16 / V, true>(a, stream)
-                                                      : launch_norm_v<T, TR, V, 16 / V, false>(a, stream);
+  if ((a.post_w != nullptr ? a.group : a.dim) % V != 0) return launch_norm_v<T, TR, V, 16 / V, kRagged>(a, stream);
+  return read_once(a.outer * a.inner * a.dim * bytes) ? launch_norm_v<T, TR, V, 16 / V, kOnce>(a, stream)
+                                                      : launch_norm_v<T, TR, V, 16 / V, kPlain>(a, stream);
 }
 
 template <typename T>
