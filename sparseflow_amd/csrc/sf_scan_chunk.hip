@@ -33,7 +33,9 @@
 // Few heads and long sequences: the token axis is cut into segments.  A first
 // pass walks each segment from a zero state for its own part of the state
 // (the last product alone), a second one chains the parts, and the main pass
-// starts each segment from its true state.
+// starts each segment from its true state.  Of such a sequence the main pass does not
+// read the states that the call began with: it writes the final ones, maybe to the same
+// rows, and its workgroups are in no order.
 #include "sf_seq.h"
 #include "sf_tile.h"
 
@@ -430,9 +432,12 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   const int64_t plane = (int64_t)P * N;
   const float* from = nullptr;
   if constexpr (!STATES) {
-    from = seg > 0 ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
-           : a.h0 != nullptr && slot >= 0 ? a.h0 + (slot * a.heads + hd) * plane
-                                          : nullptr;
+    // (Of a sequence that is cut, segment 0 starts from the chain's copy too: the last
+    // segment may write the pool's row before segment 0 would have read it.)
+    const bool start = a.h0 != nullptr && slot >= 0;
+    from = seg > 0 || (start && last > 0) ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
+           : start ? a.h0 + (slot * a.heads + hd) * plane
+                   : nullptr;
   }
   if (from != nullptr && mine) {
 #pragma unroll
@@ -801,7 +806,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
 }
 
 // Segment by segment, the state that the next one starts from, in the place of that
-// one's own part.
+// one's own part; the first one's, from the pool, in the place of its own.
 constexpr int kChainThreads = 256;
 template <int V>
 __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSplit sp, int blocks) {
@@ -818,11 +823,14 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
   if (last == 0 || e >= plane) return;
   const int64_t slot = seq_slot(a.seq, b);
   float h[V] = {};
-  if (a.h0 != nullptr && slot >= 0) load_any_f32<float, V>(a.h0 + (slot * a.heads + hd) * plane + e, h);
   float* at = sp.parts + (b * sp.segments * a.heads + hd) * plane + e;
   const float* sum = sp.sums + b * sp.segments * a.heads + hd;
   float own[V];
   load_any_f32<float, V>(at, own);
+  if (a.h0 != nullptr && slot >= 0) {
+    load_any_f32<float, V>(a.h0 + (slot * a.heads + hd) * plane + e, h);
+    store_any_f32<float, V>(at, h);
+  }
   for (int s = 0; s < last; ++s) {
     float* const next = at + a.heads * plane;
     float next_own[V] = {};
