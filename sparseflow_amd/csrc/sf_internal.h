@@ -319,11 +319,12 @@ int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);
 // and 37, token by token 50 and 39; a chunk's time is that of a whole one).
 constexpr int kScanChunkFrom = 8;
 struct ScanSplit {
-  float* parts;  // [batch, segments, heads, head_dim, state_dim]
-  float* sums;   // [batch, segments, heads] exponents
-  int segments;  // of the token axis
-  int chunks;    // of a segment
-  int blocks;    // workgroups per (sequence, segment, group)
+  float* parts;   // [rows, heads, head_dim, state_dim], a row to each segment of a cut sequence
+  float* sums;    // [rows, heads] exponents
+  int segments;   // of the token axis, at most
+  int chunks;     // of a segment
+  int blocks;     // workgroups per (sequence, segment, group)
+  int by_tokens;  // a sequence's first row: by where its tokens begin, otherwise by its number
 };
 struct ScanPlan {
   ScanSplit split;

@@ -305,6 +305,16 @@ __device__ __forceinline__ int last_segment(const ScanSplit& sp, int64_t n) {
   return (int)(s < 0 ? 0 : s >= sp.segments ? sp.segments - 1 : s);
 }
 
+// The workspace's row of the first segment of a cut sequence whose tokens begin at
+// `first`.  By tokens: it has more than a segment's tokens, n > s, so that the next cut
+// one begins floor(n / s) >= 1 segments on or later, and 2 floor(n / s) >= ceil(n / s)
+// rows are its own.  (A packed call of one long sequence and many short ones has many
+// segments times many sequences, hardly any of which are cut: of 16384 tokens and 255
+// times 16, 64 heads x 64, N 128, 6.4 GB by their numbers, 63 MB by tokens.)
+__device__ __forceinline__ int64_t first_row(const ScanSplit& sp, int64_t b, int64_t first) {
+  return sp.by_tokens ? first / ((int64_t)sp.chunks * kChunk) * 2 : b * sp.segments;
+}
+
 // STATES: a segment's own part of the state, from a zero state, to `parts`, with
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
 // PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
@@ -357,7 +367,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   const T* __restrict__ B = static_cast<const T*>(a.b) + b * a.b_b + (first + t0) * a.b_t + g * a.b_g;
   const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + (first + t0) * a.c_t + g * a.c_g;
   T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + (first + t0) * a.y_t + hd * a.y_h + p0;
-  const int64_t slot = seq_slot(a.seq, b);
+  const int64_t slot = seq_slot(a.seq, b), row0 = first_row(sp, b, first);
   const float D = uniform(a.D != nullptr ? a.D[hd] : 0.f);
 
   // The scalars of two chunks at once, one to each half wavefront.
@@ -435,7 +445,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
     // (Of a sequence that is cut, segment 0 starts from the chain's copy too: the last
     // segment may write the pool's row before segment 0 would have read it.)
     const bool start = a.h0 != nullptr && slot >= 0;
-    from = seg > 0 || (start && last > 0) ? sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane
+    from = seg > 0 || (start && last > 0) ? sp.parts + ((row0 + seg) * a.heads + hd) * plane
            : start ? a.h0 + (slot * a.heads + hd) * plane
                    : nullptr;
   }
@@ -780,7 +790,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   }
 
   float* to = nullptr;
-  if (STATES) to = sp.parts + ((b * sp.segments + seg) * a.heads + hd) * plane;
+  if (STATES) to = sp.parts + ((row0 + seg) * a.heads + hd) * plane;
   else if (seg == last && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
   if (to != nullptr && mine) {
     const float f = exp2_hw((float)k_state);
@@ -802,7 +812,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
         }
       }
   }
-  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(b * sp.segments + seg) * a.heads + hd] = (float)l_seg;
+  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(row0 + seg) * a.heads + hd] = (float)l_seg;
 }
 
 // Segment by segment, the state that the next one starts from, in the place of that
@@ -823,8 +833,9 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
   if (last == 0 || e >= plane) return;
   const int64_t slot = seq_slot(a.seq, b);
   float h[V] = {};
-  float* at = sp.parts + (b * sp.segments * a.heads + hd) * plane + e;
-  const float* sum = sp.sums + b * sp.segments * a.heads + hd;
+  const int64_t row0 = first_row(sp, b, first);
+  float* at = sp.parts + (row0 * a.heads + hd) * plane + e;
+  const float* sum = sp.sums + row0 * a.heads + hd;
   float own[V];
   load_any_f32<float, V>(at, own);
   if (a.h0 != nullptr && slot >= 0) {
@@ -928,7 +939,10 @@ ScanPlan scan_plan(int64_t batch, int64_t tokens, int64_t max_len, int heads, in
   p.split.chunks = (int)per;
   p.split.segments = (int)((chunks + per - 1) / per);
   if (p.split.segments > 1) {
-    const size_t rows = (size_t)batch * p.split.segments * heads;
+    // (max_len < tokens: a packed call, batch sequences of `tokens` tokens in all.)
+    const int64_t by_number = batch * p.split.segments, by_tokens = tokens / (per * kChunk) * 2 + 2;
+    p.split.by_tokens = max_len < tokens && by_tokens < by_number ? 1 : 0;
+    const size_t rows = (size_t)(p.split.by_tokens ? by_tokens : by_number) * heads;
     p.sums_at = align16(rows * head_dim * state_dim * sizeof(float));
     p.bytes = p.sums_at + align16(rows * sizeof(float));
   }
@@ -944,6 +958,8 @@ bool scan_chunk_takes(const ScanArgs& a) {
 
 int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int dtype, hipStream_t stream) {
   ScanSplit sp = p.split;
+  // (A descriptor of dense sequences whose max_len is not their tokens: not cut.)
+  if (a.seq.offsets == nullptr && sp.by_tokens) sp.segments = 1;
   sp.parts = static_cast<float*>(workspace);
   sp.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums_at);
   if (dtype == SF_F32) return launch_chunk_m<float, 3, false>(a, sp, stream);

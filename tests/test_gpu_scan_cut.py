@@ -103,3 +103,27 @@ def test_the_module_continues_long_prompts(dtype):
                                                  initial_state=before)
             assert torch.equal(y, want)
         assert torch.equal(after, m.state)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens", [[5000] + [3, 0, 40, 1] * 40, [7, 3000, 0, 65, 129, 97, 33, 64, 2, 1025, 130, 131, 63] * 2,
+                                  [100] * 30 + [2000], [4000] + [70] * 50])
+def test_packed_long_among_short(dtype, lens):
+    """The segments of cut sequences next to each other do not share workspace."""
+    announce(f"scan packed long among short {dtype} {len(lens)} of up to {max(lens)}")
+    H, P, G, N = 2, 32, 1, 16
+    off = [0]
+    for v in lens:
+        off.append(off[-1] + v)
+    args = _inputs((off[-1],), H, P, G, N, dtype, len(lens))
+    pool = torch.randn(len(lens), H, P, N, generator=torch.Generator().manual_seed(2)).to(DEV)
+    y, start = _both_ways(args, pool, offsets=torch.tensor(off, dtype=torch.int32, device=DEV), max_len=max(lens))
+    x, dt, A, B, C = (t.cpu() for t in args)
+    for i, n in enumerate(lens):
+        at = slice(off[i], off[i + 1])
+        ref, h, ym, hm = ora.scan(x[at], dt[at], A, B[at], C[at], None, None, True, start[i].cpu())
+        f = (4 * n + 300) * 2.0 ** -24
+        half_ulp, inner = {F32: (2.0 ** -24, 0), F16: (2.0 ** -11, 2.0 ** -15), BF16: (2.0 ** -8, 2.0 ** -8)}[dtype]
+        assert bool(((pool[i].double().cpu() - h).abs() <= f * hm).all()), f"state {i} of {n}"
+        assert bool(((y[at].double().cpu() - ref).abs() <= (f + inner) * ym + half_ulp * ref.abs() + 2.0 ** -25).all()), \
+            f"sequence {i} of {n}"
