@@ -18,12 +18,14 @@
 //
 // All of it runs on the bf16 instructions, whatever the inputs: x, B and C are taken
 // apart into bf16 parts (bf16 one, f16 two, float32 three: all of their bits), S and h
-// into as many, and a product of two sums of parts leaves out the terms below the last
-// part (three products for f16 and six for float32, a sixth of the time that the
-// float32 instructions take).  So S and h are rounded to 8 bits for bf16 outputs and to
-// 16 for f16 ones, which have 8 and 11 themselves.  v is split into three parts, its 24
-// bits, always: the state is summed up over all tokens and stays a float32 one.  L is
-// summed in 64 bits: differences of it are exponents.
+// into two, two and three, and a product of two sums of parts leaves out the terms below
+// the last part (two products for bf16, three for f16 and six for float32, a sixth of
+// the time that the float32 instructions take).  So S and h are rounded to 16 bits for
+// bf16 and f16 outputs, which have 8 and 11 themselves: what y loses is its own rounding
+// (as one part for bf16, y was off by more than that where its terms cancel: the kernels
+// of 2 x 16384 tokens took 482 us, and take 550).  v is split into three parts, its 24 bits, always: the state is summed up
+// over all tokens and stays a float32 one.  L is summed in 64 bits: differences of it
+// are exponents.
 //
 // Bound by the chain of products and the waits between them, not by memory: 2 x 16384
 // tokens, 64 heads x 64, N 128, bf16 (562 MB, 241 GFLOP of products) take 389 us, 620
@@ -160,14 +162,15 @@ __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
 __device__ __forceinline__ f32x4 mma16(const Frag& a, const Frag& b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// The product of two sums of parts, without the terms below the last part's (PL
-// parts of a value have its last bits at 2^-8 PL of it).
-template <int PL>
-__device__ __forceinline__ f32x16 mma_parts(const Frag (&a)[PL], const Frag (&b)[PL], f32x16 c) {
+// The product of two sums of parts, without the terms below the last part's (P
+// parts of a value have its last bits at 2^-8 P of it).
+template <int PA, int PB>
+__device__ __forceinline__ f32x16 mma_parts(const Frag (&a)[PA], const Frag (&b)[PB], f32x16 c) {
 #pragma unroll
-  for (int i = 0; i < PL; ++i)
+  for (int i = 0; i < PA; ++i)
 #pragma unroll
-    for (int j = 0; i + j < PL; ++j) c = mma(a[i], b[j], c);
+    for (int j = 0; j < PB; ++j)
+      if (i + j < (PA > PB ? PA : PB)) c = mma(a[i], b[j], c);
   return c;
 }
 
@@ -320,7 +323,7 @@ __device__ __forceinline__ int64_t first_row(const ScanSplit& sp, int64_t b, int
 // PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
 // which go straight into LDS.
 template <typename T, int PL, int NP, bool DIRECT, bool STATES>
-__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_scan_chunk(ScanArgs a, ScanSplit sp) {
+__global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !STATES) ? 2 : 3) void k_scan_chunk(ScanArgs a, ScanSplit sp) {
   constexpr int Q = kChunk, KB = Q / 16, NT = NP / 32, U = 8;
   constexpr int kRowUnits = NP / U, kRows = kThreads / kRowUnits;  // of B and C at a time
   constexpr int kRounds = Q > kRows ? Q / kRows : 1;
@@ -328,6 +331,8 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   constexpr int kDepth = chunk_depth<NP, DIRECT, STATES>();
   constexpr int kTile = Q * NP, kX = Q * kSlice;  // elements of a part
   constexpr bool kPair = PL == 3;                 // exponents to more than a float's bits
+  constexpr int SP = PL > 2 ? PL : 2;             // parts of S and h
+  constexpr bool kTight = PL == 1 && NP == 128 && !STATES;  // registers for three workgroups a CU, and none to spare
   typedef ChunkLds<PL, NP> Lds;
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), half = lane >> 5, col = lane & 31;
@@ -469,8 +474,12 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
       }
   }
 
-  const int bj = threadIdx.x / kRowUnits, bv = threadIdx.x % kRowUnits;
-  const int xj = lane / kXUnits, xv = lane % kXUnits;
+  // (Opaque where registers are tight, so that what is made of it is not kept in them.)
+  auto thread = []() {
+    int t = threadIdx.x;
+    if constexpr (kTight) asm volatile("" : "+v"(t));
+    return t;
+  };
   const bool whole_n = N == NP, whole_p = p0 + kSlice <= P;
   // DIRECT: a whole chunk goes from memory to LDS while chunks before it are worked on:
   // B and x to a buffer of their own, C once its readers are done.  (The last chunk, if
@@ -478,6 +487,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   auto ahead = [&](int64_t rest) { return DIRECT && rest >= Q; };
   auto load_rows = [&](const T* base, int stride, uint16_t* to) {
     const char* from = reinterpret_cast<const char*>(base);
+    const int bj = thread() / kRowUnits, bv = thread() % kRowUnits;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int u = unit_place<NP>(r * kRows + bj, bv);
@@ -491,6 +501,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   auto load_x = [&](uint16_t* to) {
     if (!on) return;
     const char* from = reinterpret_cast<const char*>(x);
+    const int xj = thread() % kWave / kXUnits, xv = thread() % kXUnits;
 #pragma unroll
     for (int r = 0; r < kXRounds; ++r) {
       const int u = x_place(r * kXRows + xj, xv * U) % kSlice / U;
@@ -504,6 +515,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
   constexpr int kWords = 2 * (int)sizeof(T);
   uint32_t nb[kRounds][kWords], nc[STATES ? 1 : kRounds][kWords], nx[kXRounds][kWords];
   auto fetch = [&](const T* b_from, const T* c_from, const T* x_from, int len) {
+    const int bj = thread() / kRowUnits, bv = thread() % kRowUnits, xj = thread() % kWave / kXUnits, xv = thread() % kXUnits;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int j = r * kRows + bj;
@@ -517,6 +529,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
                    on && r * kXRows + xj < len ? P - p0 - xv * U : 0, nx[r]);
   };
   auto unload = [&](uint16_t* to_b, uint16_t* to_x) {
+    const int bj = thread() / kRowUnits, bv = thread() % kRowUnits, xj = thread() % kWave / kXUnits, xv = thread() % kXUnits;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int j = r * kRows + bj;
@@ -636,7 +649,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
         float hv[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) hv[e] = h[k / 2][8 * (k % 2) + e];
-        Frag hf[PL], cf[PL];
+        Frag hf[SP], cf[PL];
         split(hv, hf);
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) cf[pl] = row_frag(s_c + pl * kTile, row_at, k);
@@ -651,8 +664,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
           v[0] += low_bf16(u.x), v[1] += high_bf16(u.x), v[2] += low_bf16(u.y), v[3] += high_bf16(u.y);
         }
       };
-      uint2 xr[PL == 1 ? 4 : 1];  // (one part: read before the barrier)
-      if constexpr (PL == 1) {
+      constexpr bool kEarly = PL == 1 && !kTight;
+      uint2 xr[kEarly ? 4 : 1];  // (one part: read before the barrier)
+      if constexpr (kEarly) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           xr[q] = *reinterpret_cast<const uint2*>(s_x + x_place(ln & 31, 8 * q + 4 * (ln >> 5)));
@@ -704,7 +718,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
               }
             }
           }
-          Frag sf[PL];
+          Frag sf[SP];
           split(s, sf);
           acc = mma_parts(xf[k], sf, acc);
         }
@@ -731,7 +745,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 ? 2 : 3) void k_sc
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float xq[4];
-        if constexpr (PL == 1) xq[0] = low_bf16(xr[q].x), xq[1] = high_bf16(xr[q].x), xq[2] = low_bf16(xr[q].y), xq[3] = high_bf16(xr[q].y);
+        if constexpr (kEarly) xq[0] = low_bf16(xr[q].x), xq[1] = high_bf16(xr[q].x), xq[2] = low_bf16(xr[q].y), xq[3] = high_bf16(xr[q].y);
         else own_x(q, xq);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[4 * q + e] = fmaf(acc[4 * q + e], f, D * xq[e]);
