@@ -415,9 +415,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
     sc.w[col] = exp2_hw((float)((half == 0 ? end[0] - k[1] : end[1] - k[2]) - l)) * d;
     if constexpr (!STATES) {
       float p = (float)l, q = d;
+      sc.r[col] = (float)(l - (double)p);
       if constexpr (kPair) {
         wide_of[0] = wide_of[1] = true;
-        sc.r[col] = (float)(l - (double)p);
       } else {
         const float off = (float)(l + (half == 0 ? k[0] : k[1])), fall = exp2_hw(-off) * d;
         // (Also where a factor of a later token is no number: it meets zeros of G.)
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
         for (int q = 0; q < 4; ++q)
           xr[q] = *reinterpret_cast<const uint2*>(s_x + x_place(ln & 31, 8 * q + 4 * (ln >> 5)));
       }
-      const float my_p = sc.p[col], my_r = kPair ? sc.r[col] : 0.f;
+      const float my_p = sc.p[col];
       const bool wide = kPair || (i % 2 == 0 ? wide_of[0] : wide_of[1]);
       __syncthreads();
       if (ahead(left - Q)) load_rows(C, c_t, s_c);
@@ -684,11 +684,8 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = most_of(most, xf[k][0][e]);
       const bool finite = __ballot(!all_finite(most)) == 0ull;
-      auto factor = [&](float pj, float qj, float rj) {
-        float delta = my_p - pj;
-        if constexpr (kPair) delta += my_r - rj;
-        return exp2_hw(delta) * qj;
-      };
+      const float my_r = kPair || wide ? sc.r[col] : 0.f;
+      auto factor = [&](float pj, float qj, float rj) { return exp2_hw((my_p - pj) + (my_r - rj)) * qj; };
       if (wide) {
         const float f = exp2_hw(my_p + (i % 2 == 0 ? k_of[0] : k_of[1]));
 #pragma unroll
@@ -727,7 +724,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
         // decay that leaves a float's range in the chunk has no factors apart.
         for (int j = 0; j < Q; ++j) {
           const float gv = *g_at(col, j);
-          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], kPair ? sc.r[j] : 0.f) : sc.q[j]);
+          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], sc.r[j]) : sc.q[j]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float xq[4] = {0.f, 0.f, 0.f, 0.f};

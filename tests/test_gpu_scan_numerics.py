@@ -62,3 +62,27 @@ def test_outputs_are_rounded_once(dtype, n, H, P, G, N, offset):
     ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, True, h0[0])
     _within(y[0], ref, _bound(n, ref, ym, dtype), "y")
     _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_decays_after_one_large_step(dtype, offset):
+    """A step that forgets everything leaves exponents of a million behind it in its
+    chunk; the decays of the tokens after it are differences of those."""
+    announce(f"scan one large step {dtype} offset={offset}")
+    n, H, P, G, N = 64, 2, 32, 1, 32
+    g = _gen(50)
+    x, B, C = (torch.rand(s, generator=g).to(dtype) for s in ((1, n, H, P + offset), (1, n, G, N), (1, n, G, N)))
+    x = x[..., offset:]
+    dt = torch.full((1, n, H), 1.0 / 128).to(dtype)
+    dt[0, 5], dt[0, 40] = 60000.0, 2000.0
+    A = torch.tensor([-16.0, -7.3])
+    y, state = selective_scan_forward(torch.as_strided(x._base.to(DEV) if offset else x.to(DEV), x.shape, x.stride(),
+                                                       x.storage_offset()), *_dev(dt, A, B, C), dt_softplus=False)
+    ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, torch.zeros(H, P, N))
+    # (What is over the format's range is infinite; no result is within 2^-12 of its end.)
+    over = ref.to(dtype).isinf()
+    assert bool(((ref / torch.finfo(dtype).max - 1).abs() > 2.0 ** -12).all())
+    assert torch.equal(y[0].isinf().cpu(), over)
+    _within(torch.where(over.to(DEV), 0, y[0]), torch.where(over, 0, ref), _bound(n, ref, ym, dtype), "y")
+    _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
