@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_seq(ScanArgs a, int slices) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int p = p0 + r * kRows;
-      if (nl == 0 && p < P) y[t * a.y_t + p] = from_f32<T>(fmaf(D, xv[r], s[r]));
+      if (nl == 0 && p < P) y[t * a.y_t + p] = from_f32<T>(a.D != nullptr ? fmaf(D, xv[r], s[r]) : s[r]);
     }
   }
   if (a.h1 != nullptr && slot >= 0) {

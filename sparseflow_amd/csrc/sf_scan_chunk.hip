@@ -32,6 +32,10 @@
 // TFLOP/s and 1.4 TB/s, 280 of them the main pass; rows at any address, by way of
 // registers, a quarter more; 23 ragged sequences of up to 1500 of f16, 24 heads, 190 us.
 //
+// Where products are not finite, a wavefront does its segment again, token by token:
+// infinities, NaN and results near the ends of a float's range are those of the
+// recurrence.
+//
 // Few heads and long sequences: the token axis is cut into segments.  A first
 // pass walks each segment from a zero state for its own part of the state
 // (the last product alone), a second one chains the parts, and the main pass
@@ -148,12 +152,11 @@ __device__ __forceinline__ void split(const float (&v)[8], Frag (&f)[PL]) {
   }
 }
 
-// Whether all of a slice's x (their first parts) are finite.
-__device__ __forceinline__ bool all_finite(uint32_t most) { return max(most >> 16, most & 0xffffu) < 0x7f80u; }
-__device__ __forceinline__ uint32_t most_of(uint32_t most, uint32_t pair) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
-                                                                __builtin_bit_cast(u16x2, pair & 0x7fff7fffu)));
+// z (0 or NaN), or NaN if any of v is not finite.
+__device__ __forceinline__ float not_finite(const f32x16& v, float z) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z = fmaf(v[r], 0.f, z);
+  return z;
 }
 
 __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
@@ -175,8 +178,8 @@ __device__ __forceinline__ f32x16 mma_parts(const Frag (&a)[PA], const Frag (&b)
 }
 
 // Per token of a chunk, for one head.  The state in the accumulators is 2^-K h, K
-// kept near 0 (kScaleMost), so that a chunk's decay need not be multiplied in each
-// time; K' is its value after the chunk.
+// between 0 and kScaleMost (the range that it costs is at the small end), so that a
+// chunk's decay need not be multiplied in each time; K' is its value after the chunk.
 //            factors apart      a factor per element (wide)
 //   w        2^(L_end - L - K') d, both
 //   p        2^(L + K)          L
@@ -318,6 +321,40 @@ __device__ __forceinline__ int64_t first_row(const ScanSplit& sp, int64_t b, int
   return sp.by_tokens ? first / ((int64_t)sp.chunks * kChunk) * 2 : b * sp.segments;
 }
 
+// A workgroup's sequence, segment (tokens t0 to t1 of the sequence) and group; a
+// wavefront's head and columns.
+struct ChunkWork {
+  int64_t b, first, t0, t1, slot, row0;  // (row0: first_row)
+  int g, seg, last, hd, p0;
+  bool on, idle;  // whether the wavefront has columns; whether there is no such segment
+};
+template <bool STATES>
+__device__ __forceinline__ ChunkWork chunk_work(const ScanArgs& a, const ScanSplit& sp, int64_t item, int wave) {
+  ChunkWork w;
+  const int segs = STATES ? sp.segments - 1 : sp.segments;
+  const int ub = (int)(item % sp.blocks);
+  item /= sp.blocks;
+  w.g = (int)(item % a.groups);
+  item /= a.groups;
+  w.seg = (int)(item % segs);
+  w.b = item / segs;
+  int64_t n;
+  seq_rows(a.seq, w.b, w.first, n);
+  w.last = last_segment(sp, n);
+  w.idle = STATES ? w.seg >= w.last : w.seg > w.last;
+  const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
+  const int unit = ub * kWaves + wave;
+  w.on = unit < per_group * slices;
+  w.hd = w.g * per_group + (w.on ? unit / slices : 0);
+  w.p0 = w.on ? unit % slices * kSlice : 0;
+  const int64_t per_seg = (int64_t)sp.chunks * kChunk;
+  w.t0 = w.seg * per_seg;
+  w.t1 = w.seg == w.last ? n : w.t0 + per_seg;
+  w.slot = seq_slot(a.seq, w.b);
+  w.row0 = first_row(sp, w.b, w.first);
+  return w;
+}
+
 // STATES: a segment's own part of the state, from a zero state, to `parts`, with
 // the sum of its exponents to `sums`.  Otherwise y, from the segment's true state.
 // PL: bf16 parts of an element of x, B and C.  DIRECT: rows of whole aligned units,
@@ -343,36 +380,19 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   uint16_t* s_c = reinterpret_cast<uint16_t*>(lds + Lds::c(kDepth));
   float* const s_g = reinterpret_cast<float*>(lds + Lds::g(kDepth));
 
-  // This workgroup's sequence, segment and group; this wavefront's head and columns.
-  const int segs = STATES ? sp.segments - 1 : sp.segments;
   // (In the order of the launch: given to the XCDs so that those of one sequence and
   // group share an L2 for B and C, ragged calls take up to a third longer.)
-  int64_t item = a.block0 + blockIdx.x;
-  const int ub = (int)(item % sp.blocks);
-  item /= sp.blocks;
-  const int g = (int)(item % a.groups);
-  item /= a.groups;
-  const int seg = (int)(item % segs);
-  const int64_t b = item / segs;
-  int64_t first, n;
-  seq_rows(a.seq, b, first, n);
-  const int last = last_segment(sp, n);
-  if (STATES ? seg >= last : seg > last) return;
-  const int per_group = a.heads / a.groups, slices = (a.head_dim + kSlice - 1) / kSlice;
-  const int unit = ub * kWaves + wave;
-  const bool on = unit < per_group * slices;
-  const int hd = g * per_group + (on ? unit / slices : 0);
-  const int p0 = on ? unit % slices * kSlice : 0;
-  const int P = a.head_dim, N = a.state_dim;
-  const int64_t per_seg = (int64_t)sp.chunks * Q;
-  const int64_t t0 = seg * per_seg, t1 = seg == last ? n : t0 + per_seg;
+  const ChunkWork work = chunk_work<STATES>(a, sp, a.block0 + blockIdx.x, wave);
+  if (work.idle) return;
+  const int64_t b = work.b, first = work.first, t0 = work.t0, t1 = work.t1;
+  const int g = work.g, hd = work.hd, p0 = work.p0, P = a.head_dim, N = a.state_dim;
+  const bool on = work.on;
   // (The launcher takes token strides below 2^24 only.)
   const int x_t = (int)a.x_t, dt_t = (int)a.dt_t, b_t = (int)a.b_t, c_t = (int)a.c_t, y_t = (int)a.y_t;
   const T* __restrict__ x = static_cast<const T*>(a.x) + b * a.x_b + (first + t0) * a.x_t + hd * a.x_h + p0;
   const T* __restrict__ B = static_cast<const T*>(a.b) + b * a.b_b + (first + t0) * a.b_t + g * a.b_g;
   const T* __restrict__ C = static_cast<const T*>(a.c) + b * a.c_b + (first + t0) * a.c_t + g * a.c_g;
   T* __restrict__ y = static_cast<T*>(a.y) + b * a.y_b + (first + t0) * a.y_t + hd * a.y_h + p0;
-  const int64_t slot = seq_slot(a.seq, b), row0 = first_row(sp, b, first);
   const float D = uniform(a.D != nullptr ? a.D[hd] : 0.f);
 
   // The scalars of two chunks at once, one to each half wavefront.
@@ -404,7 +424,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
       rescale_of[c] = 1.f;
       k[c + 1] = k[c] + end[c];
       if constexpr (STATES) l_seg = uniform(l_seg + end[c]);
-      if (!(fabs(k[c + 1]) < kScaleMost)) {
+      if (!(k[c + 1] >= 0.0 && k[c + 1] < kScaleMost)) {
         const double to = end[c] < 0.0 ? kScaleFrom : 0.0;
         rescale_of[c] = uniform(exp2_hw((float)(k[c + 1] - to)));
         k[c + 1] = to;
@@ -445,15 +465,16 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   const bool mine = on && p < P;
   const bool vec_n = N % 4 == 0;
   const int64_t plane = (int64_t)P * N;
-  const float* from = nullptr;
-  if constexpr (!STATES) {
-    // (Of a sequence that is cut, segment 0 starts from the chain's copy too: the last
-    // segment may write the pool's row before segment 0 would have read it.)
-    const bool start = a.h0 != nullptr && slot >= 0;
-    from = seg > 0 || (start && last > 0) ? sp.parts + ((row0 + seg) * a.heads + hd) * plane
-           : start ? a.h0 + (slot * a.heads + hd) * plane
-                   : nullptr;
-  }
+  // The state that a segment starts from.  (Of a sequence that is cut, segment 0's is the
+  // chain's copy too: the last segment may write the pool's row before segment 0 would
+  // have read it.)
+  auto start_of = [&](const ChunkWork& w, const ScanArgs& args, const ScanSplit& split) -> const float* {
+    const bool kept = args.h0 != nullptr && w.slot >= 0;
+    return w.seg > 0 || (kept && w.last > 0) ? split.parts + ((w.row0 + w.seg) * args.heads + w.hd) * plane
+           : kept                            ? args.h0 + (w.slot * args.heads + w.hd) * plane
+                                             : nullptr;
+  };
+  const float* const from = STATES ? nullptr : start_of(work, a, sp);
   if (from != nullptr && mine) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -565,6 +586,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   // may be left under way at the next.
   const bool counted = DIRECT && on && whole_n && whole_p && kRows <= Q;
 
+  float bad = 0.f;  // not 0 (NaN) where products have not been finite
   for (int i = 0; left > 0; left -= Q, ++i) {
     const int len = (int)(left < Q ? left : Q);
     const int at = i % kDepth, at_last = (i + kDepth - 1) % kDepth;
@@ -671,27 +693,21 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
         for (int q = 0; q < 4; ++q)
           xr[q] = *reinterpret_cast<const uint2*>(s_x + x_place(ln & 31, 8 * q + 4 * (ln >> 5)));
       }
-      const float my_p = sc.p[col];
+      const float my_p = sc.p[ln & 31];
       const bool wide = kPair || (i % 2 == 0 ? wide_of[0] : wide_of[1]);
       __syncthreads();
       if (ahead(left - Q)) load_rows(C, c_t, s_c);
 
       // ---- x^T S: S[i][j] = G[i][j] 2^(L_i - L_j) d_j for j <= i ----
       // Factors apart: 2^(L_i + K) is multiplied in at the end; G is 0 above the diagonal.
-      uint32_t most = 0;
-#pragma unroll
-      for (int k = 0; k < KB; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = most_of(most, xf[k][0][e]);
-      const bool finite = __ballot(!all_finite(most)) == 0ull;
-      const float my_r = kPair || wide ? sc.r[col] : 0.f;
+      const float my_r = kPair || wide ? sc.r[ln & 31] : 0.f;
       auto factor = [&](float pj, float qj, float rj) { return exp2_hw((my_p - pj) + (my_r - rj)) * qj; };
       if (wide) {
         const float f = exp2_hw(my_p + (i % 2 == 0 ? k_of[0] : k_of[1]));
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] *= f;
       }
-      if (finite && (kPair || !wide)) {
+      if (kPair || !wide) {
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
           float s[8];
@@ -720,24 +736,25 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
           acc = mma_parts(xf[k], sf, acc);
         }
       } else {
-        // Term by term: an x that is not finite must not meet the zeros of S, and a
-        // decay that leaves a float's range in the chunk has no factors apart.
+        // Term by term: a decay that leaves a float's range in the chunk has no factors
+        // apart.
         for (int j = 0; j < Q; ++j) {
-          const float gv = *g_at(col, j);
-          const float s = gv * (wide ? factor(sc.p[j], sc.q[j], sc.r[j]) : sc.q[j]);
+          const float gv = *g_at(ln & 31, j);
+          const float s = gv * factor(sc.p[j], sc.q[j], sc.r[j]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float xq[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int pl = PL - 1; pl >= 0; --pl) {
-              const uint2 u = *reinterpret_cast<const uint2*>(s_x + pl * kX + x_place(j, 8 * q + 4 * half));
+              const uint2 u = *reinterpret_cast<const uint2*>(s_x + pl * kX + x_place(j, 8 * q + 4 * (ln >> 5)));
               xq[0] += low_bf16(u.x), xq[1] += high_bf16(u.x), xq[2] += low_bf16(u.y), xq[3] += high_bf16(u.y);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[4 * q + e] = j <= col ? fmaf(s, xq[e], acc[4 * q + e]) : acc[4 * q + e];
+            for (int e = 0; e < 4; ++e) acc[4 * q + e] = j <= (ln & 31) ? fmaf(s, xq[e], acc[4 * q + e]) : acc[4 * q + e];
           }
         }
       }
+      bad = not_finite(acc, bad);
       const float f = wide ? 1.f : my_p;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -747,8 +764,8 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[4 * q + e] = fmaf(acc[4 * q + e], f, D * xq[e]);
       }
-      if (on && col < len) {
-        T* row = y + (col * y_t + 4 * half);
+      if (on && (ln & 31) < len) {
+        T* row = y + ((ln & 31) * y_t + 4 * (ln >> 5));
         if (whole_p) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) store_any_f32<T, 4>(row + 8 * q, {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
@@ -774,7 +791,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float wv[4];
-        load_f32<float, 4>(sc.w + 16 * k + 8 * half + 4 * q, wv);
+        load_f32<float, 4>(sc.w + 16 * k + 8 * (ln >> 5) + 4 * q, wv);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float xv = get(xf[k][PL - 1], 4 * q + e);
@@ -800,17 +817,93 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
     if (i % 2 == 1 && left > Q) write_scalars(left - Q);
   }
 
+  if constexpr (STATES) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) bad = not_finite(h[nt], bad);
+  }
+  // (Found again, and from the arguments themselves: kept over the chunks, all of this
+  // takes registers from them.)
+  struct Args {
+    ScanArgs a;
+    ScanSplit sp;
+  };
+  typedef const __attribute__((address_space(4))) Args* ArgsAt;
+  ArgsAt args = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const ScanArgs& ea = ((const Args*)args)->a;
+  const ScanSplit& esp = ((const Args*)args)->sp;
+  const ChunkWork end = chunk_work<STATES>(ea, esp, ea.block0 + blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  if (end.on && __ballot(bad != 0.f) != 0ull) {
+    // The recurrence itself, token by token, from the segment's start.  The products meet
+    // zeros that it does not have (of S, of an exact number's lower parts, of padding), and
+    // leave a float's range where factors apart or a part's rounding do: where they are not
+    // finite they do not say what the result is.  2 x 16384 tokens, 64 heads x 64, N 128,
+    // with an infinity in one head take 8 ms.  (The y stored so far are in place before they
+    // are written again.)
+    wait_memory<0>();
+    int64_t t = end.t0;
+    const int64_t row = end.first + t;
+    const T* b_from = static_cast<const T*>(ea.b) + end.b * ea.b_b + row * ea.b_t + end.g * ea.b_g;
+    const T* c_from = static_cast<const T*>(ea.c) + end.b * ea.c_b + row * ea.c_t + end.g * ea.c_g;
+    const T* x_from = static_cast<const T*>(ea.x) + end.b * ea.x_b + row * ea.x_t + end.hd * ea.x_h + min(end.p0 + col, P - 1);
+    const T* dt_from = static_cast<const T*>(ea.dt) + end.b * ea.dt_b + row * ea.dt_t + end.hd * ea.dt_h;
+    T* y_to = static_cast<T*>(ea.y) + end.b * ea.y_b + row * ea.y_t + end.hd * ea.y_h + end.p0 + col;
+    const float rate = ea.A[end.hd], skip = ea.D != nullptr ? ea.D[end.hd] : 0.f;
+    const float shift = ea.dt_bias != nullptr ? ea.dt_bias[end.hd] : 0.f;
+    const float* start = STATES ? nullptr : start_of(end, ea, esp);
+    float hv[NT * 16];
+#pragma unroll
+    for (int r = 0; r < NT * 16; ++r) {
+      const int n = 32 * (r / 16) + 16 * (r / 8 % 2) + 8 * half + r % 8;
+      hv[r] = start != nullptr ? start[(int64_t)min(end.p0 + col, P - 1) * N + min(n, N - 1)] : 0.f;
+    }
+    for (; t < end.t1; ++t) {
+      float d = to_f32<T>(*dt_from) + shift;
+      if (ea.softplus) d = softplus(d);
+      const float decay = expf(rate * d), xv = to_f32<T>(*x_from), u = d * xv;
+      float s = 0.f;
+      int at = 8 * half;  // (opaque: what is made of it is not kept over the tokens)
+      asm volatile("" : "+v"(at));
+#pragma unroll
+      for (int q = 0; q < 4 * NT; ++q) {
+        const int n = 32 * (q / 4) + 16 * (q / 2 % 2) + 4 * (q % 2) + at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int from = min(n + e, N - 1);
+          float& now = hv[4 * q + e];
+          now = fmaf(decay, now, u * to_f32<T>(b_from[from]));
+          // (Columns past the end go nowhere.)
+          if constexpr (!STATES)
+            s += __uint_as_float(__float_as_uint(now * to_f32<T>(c_from[from])) & (uint32_t)((n + e - N) >> 31));
+        }
+        if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (!STATES) {
+        s += __shfl_xor(s, 32, kWave);
+        if (half == 0 && end.p0 + col < P) *y_to = from_f32<T>(ea.D != nullptr ? fmaf(skip, xv, s) : s);
+        c_from += ea.c_t;
+        y_to += ea.y_t;
+      }
+      b_from += ea.b_t;
+      x_from += ea.x_t;
+      dt_from += ea.dt_t;
+    }
+#pragma unroll
+    for (int r = 0; r < NT * 16; ++r) h[r / 16][r % 16] = hv[r];
+    k_state = 0.0;
+  }
   float* to = nullptr;
-  if (STATES) to = sp.parts + ((row0 + seg) * a.heads + hd) * plane;
-  else if (seg == last && a.h1 != nullptr && slot >= 0) to = a.h1 + (slot * a.heads + hd) * plane;
-  if (to != nullptr && mine) {
+  if (STATES) to = esp.parts + ((end.row0 + end.seg) * ea.heads + end.hd) * plane;
+  else if (end.seg == end.last && ea.h1 != nullptr && end.slot >= 0) to = ea.h1 + (end.slot * ea.heads + end.hd) * plane;
+  const int p_end = end.p0 + col;
+  if (to != nullptr && end.on && p_end < P) {
     const float f = exp2_hw((float)k_state);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n0 = 32 * nt + 16 * (q / 2) + 8 * half + 4 * (q % 2);
-        float* dst = to + (int64_t)p * N + n0;
+        float* dst = to + (int64_t)p_end * N + n0;
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = h[nt][4 * q + e] * f;
@@ -823,7 +916,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
         }
       }
   }
-  if (STATES && on && p0 == 0 && lane == 0) sp.sums[(row0 + seg) * a.heads + hd] = (float)l_seg;
+  if (STATES && end.on && end.p0 == 0 && lane == 0) esp.sums[(end.row0 + end.seg) * ea.heads + end.hd] = (float)l_seg;
 }
 
 // Segment by segment, the state that the next one starts from, in the place of that
@@ -858,9 +951,11 @@ __global__ __launch_bounds__(kChainThreads) void k_scan_chain(ScanArgs a, ScanSp
     float next_own[V] = {};
     if (s + 1 < last) load_any_f32<float, V>(next, next_own);
     const float decay = exp2f(*sum);
+    // (Infinity times each of a segment's decays stays so, though their product is 0.)
+    const bool stays = decay == 0.f && *sum > -__builtin_huge_valf();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      h[i] = fmaf(h[i], decay, own[i]);
+      h[i] = stays && fabsf(h[i]) == __builtin_huge_valf() ? h[i] + own[i] : fmaf(h[i], decay, own[i]);
       own[i] = next_own[i];
     }
     store_any_f32<float, V>(next, h);

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import state_space as ora
-from sparseflow_amd.Kernels.selective_scan import selective_scan_forward
+from sparseflow_amd.Kernels.selective_scan import selective_scan_forward, selective_scan_step
 from tests.gpu_helpers import DEV, announce
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +86,135 @@ def test_decays_after_one_large_step(dtype, offset):
     assert torch.equal(y[0].isinf().cpu(), over)
     _within(torch.where(over.to(DEV), 0, y[0]), torch.where(over, 0, ref), _bound(n, ref, ym, dtype), "y")
     _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [70, 1500])
+def test_large_results_with_fast_decay(dtype, n):
+    """Terms of 2^40 that a chunk decays by 2^-90: finite, whatever factors the decays
+    are taken apart into.  (1500 tokens of one head are cut into segments.)"""
+    announce(f"scan large results {dtype} n={n}")
+    H, P, G, N = 1, 32, 1, 32
+    g = _gen(60)
+    x, B, C = ((torch.randn(s, generator=g) * 2.0 ** 12).to(dtype) for s in ((1, n, H, P), (1, n, G, N), (1, n, G, N)))
+    dt = torch.full((1, n, H), 2.0).to(dtype)
+    A = torch.tensor([-0.98])
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False)
+    ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, torch.zeros(H, P, N))
+    assert float(ref.abs().max()) > 2.0 ** 38
+    _within(y[0], ref, _bound(n, ref, ym, dtype), "y")
+    _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rate", [-0.02, -0.5, 0.0])
+@pytest.mark.parametrize("n", [40, 100])
+def test_states_near_the_largest_float(dtype, rate, n):
+    announce(f"scan large states {dtype} rate={rate} n={n}")
+    H, P, G, N = 2, 32, 1, 32
+    g = _gen(61)
+    x, dt, B = _randn(g, 1, n, H, P, dtype=dtype), torch.full((1, n, H), 1.0).to(dtype), _randn(g, 1, n, G, N, dtype=dtype)
+    C = torch.zeros(1, n, G, N, dtype=dtype)
+    A, h0 = torch.full((H,), rate), _randn(g, 1, H, P, N) * 2.0 ** 118
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False, initial_state=h0.to(DEV))
+    ref, h, _, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, h0[0])
+    assert torch.isfinite(state).all() and not y.any()
+    _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+def test_inputs_and_states_near_the_largest_float32():
+    """Above 3.39e38 a float32 rounds to infinity in bf16."""
+    announce("scan float32 inputs near the largest float")
+    n, H, P, G, N, most = 50, 2, 32, 1, 32, 3.4e38
+    g = _gen(62)
+    x, dt, A = _randn(g, 1, n, H, P), torch.full((1, n, H), 1.0), torch.tensor([-0.1, -3.0])
+    B, C = _randn(g, 1, n, G, N), _randn(g, 1, n, G, N)
+    x[0, 20, 0, 3], B[0, 20] = most, B[0, 20] * 1e-30
+    h0 = _randn(g, 1, H, P, N)
+    h0[0, 1, 5, 7], C[0, 0] = most, C[0, 0] * 1e-30
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False, initial_state=h0.to(DEV))
+    ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, h0[0])
+    ok = ym < 2.0 ** 127
+    assert bool(ok[:, 0].all()) and bool(ok[0].all()) and torch.isfinite(y[0].cpu()[ok]).all()
+    _within(torch.where(ok, y[0].double().cpu(), ref), ref, _bound(n, ref, ym, F32), "y")
+    _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+def _same_values(got, want, what):
+    got = got.detach().double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: {int((torch.isnan(got) != torch.isnan(want)).sum())} NaN"
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), f"{what}: infinities"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("where", ["x", "B", "C", "state", "several"])
+@pytest.mark.parametrize("n,at,step", [(20, 0, 0.25), (100, 77, 0.25), (1500, 300, 0.25), (1500, 300, 4.0)])
+def test_infinities_are_those_of_the_recurrence(dtype, where, n, at, step):
+    """(1500 tokens of two heads are cut into segments.)"""
+    announce(f"scan infinities in {where} {dtype} n={n} step={step}")
+    H, P, G, N = 2, 40, 2, 48
+    g = _gen(63)
+    x = _randn(g, 1, n, H, P, dtype=dtype)
+    B, C = ((torch.rand(1, n, G, N, generator=g) + 0.25).to(dtype) for _ in range(2))
+    # (1.0: exact in one part, whose other parts are zeros.)
+    B[..., ::3], C[..., ::2] = 1.0, 1.0
+    dt, A = torch.full((1, n, H), step).to(dtype), torch.tensor([-0.125, -1.0])
+    h0, inf = _randn(g, 1, H, P, N), float("inf")
+    if where in ("x", "several"):
+        x[0, at, 1, 3], x[0, at, 1, 33] = inf, -inf
+    if where in ("B", "several"):
+        B[0, at, 1, 5] = inf
+    if where in ("C", "several"):
+        C[0, at, 1, 6] = -inf
+    if where == "state":
+        h0[0, 1, 2, 4], h0[0, 1, 3] = inf, -inf
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False, initial_state=h0.to(DEV))
+    ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, h0[0])
+    _same_values(y[0], ref, "y")
+    _same_values(state[0], h, "state")
+    ok, fine = torch.isfinite(ref), torch.isfinite(h)
+    assert bool(ok[:, 0].all()) and not bool(ok[:, 1].all())
+    for got, want, bound, keep in ((y[0], ref, _bound(n, ref, ym, dtype), ok),
+                                   (state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, fine)):
+        _within(torch.where(keep.to(DEV), got, 0), torch.where(keep, want, 0), torch.where(keep, bound, 0), "finite ones")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_large_term_after_a_slow_decay(dtype):
+    """2^118 comes in when the chunks before have decayed the state by 2^-17."""
+    announce(f"scan large term after slow decay {dtype}")
+    n, H, P, G, N = 90, 1, 32, 1, 32
+    g = _gen(64)
+    x, B = _randn(g, 1, n, H, P, dtype=dtype), _randn(g, 1, n, G, N, dtype=dtype)
+    C = (torch.randn(1, n, G, N, generator=g) * 2.0 ** -40).to(dtype)
+    x[0, 80] *= 2.0 ** 60
+    B[0, 80] *= 2.0 ** 58
+    dt, A = torch.ones(1, n, H, dtype=dtype), torch.tensor([-0.1317])
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False)
+    ref, h, ym, hm = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, torch.zeros(H, P, N))
+    _within(y[0], ref, _bound(n, ref, ym, dtype), "y")
+    _within(state[0], h, (4 * n + 300) * 2.0 ** -24 * hm, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [1, 5])
+def test_infinities_token_by_token(dtype, n):
+    """Without D an infinite x is not multiplied by a zero one."""
+    announce(f"scan infinities token by token {dtype} n={n}")
+    H, P, G, N, inf = 2, 40, 1, 48, float("inf")
+    g = _gen(65)
+    x = _randn(g, 2, n, H, P, dtype=dtype)
+    B, C = ((torch.rand(2, n, G, N, generator=g) + 0.25).to(dtype) for _ in range(2))
+    dt, A, h0 = torch.full((2, n, H), 0.25).to(dtype), torch.tensor([-0.125, -1.0]), _randn(g, 2, H, P, N)
+    x[0, 0, 1, 3], x[1, n - 1, 0, 39] = inf, -inf
+    y, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False, initial_state=h0.to(DEV))
+    for b in range(2):
+        ref, h, _, _ = ora.scan(x[b], dt[b], A, B[b], C[b], None, None, False, h0[b])
+        assert not torch.isnan(ref).any()
+        _same_values(y[b], ref, "y")
+        _same_values(state[b], h, "state")
+    if n == 1:
+        pool = h0.to(DEV)
+        step = selective_scan_step(pool, *_dev(x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0]), dt_softplus=False)
+        assert torch.equal(step, y[:, 0]) and torch.equal(pool, state)
