@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kThreads) void k_causal_conv1d(Conv1dArgs a, int cv
       s[i] = bias[i];
 #pragma unroll
       for (int k = 0; k < K; ++k) s[i] = fmaf(w[k][i], u[k][i], s[i]);
-      if (a.act == SF_ACT_SILU) s[i] = silu(s[i]);
+      if (a.act == SF_ACT_SILU) s[i] = silu<sizeof(T) == 4>(s[i]);
     }
     store_any_f32<T, V>(yt, s);
     yt += a.y_t;

@@ -25,8 +25,9 @@ constexpr int kBlock = 256;
 // would cost whole rows, 2048, 92 against 70).
 constexpr int kPlain = 0, kOnce = 1, kRagged = 2;
 
+template <bool F32>
 __device__ __forceinline__ float act_of(int act, float v) {
-  return act == SF_ACT_SILU ? silu(v) : act == SF_ACT_SIGMOID ? sigmoid(v) : v;
+  return act == SF_ACT_SILU ? silu<F32>(v) : act == SF_ACT_SIGMOID ? sigmoid<F32>(v) : v;
 }
 
 // The sum of v over the LT threads of a row (in an order of its own for every
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(LT > kBlock ? LT : kBlock) void k_block_norm(NormAr
     for (int k = 0; k < NV; ++k) {
       if ((k * LT + lt) * V >= width) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) t[k][e] *= act_of(a.act, to_f32<T>(gv[k].e[e]));
+      for (int e = 0; e < V; ++e) t[k][e] *= act_of<sizeof(TR) == 4>(a.act, to_f32<T>(gv[k].e[e]));
     }
   };
   // The weights of a vector's columns (behind the row's end the last one).

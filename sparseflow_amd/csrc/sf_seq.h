@@ -123,13 +123,23 @@ __device__ __forceinline__ float softplus(float v) {
 }
 
 // sigmoid(v) and v sigmoid(v) by the hardware's exponential and reciprocal: each is
-// good to a unit in the last place, and the exponent's rounding costs |v| of them in
-// 1 + exp(-v) where that still counts.  (With expf and a division the convolution of
-// bf16 rows was bound by arithmetic: 183 us for 2 x 16384 x 4352, against 130.)
+// good to a unit in the last place.  (With expf and a division the convolution of bf16
+// rows was bound by arithmetic: 183 us for 2 x 16384 x 4352, against 130.)  The
+// exponent's rounding costs up to |v| units in 1 + exp(-v) where v < 0: with F32, for
+// results that are float32, what it loses is made good (e = 2^(hi + lo), as above); 16-bit
+// ones have none of those bits.
+template <bool F32>
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + exp2_hw(v * -1.44269502f));
+  const float hi = v * -1.44269502f;
+  float e = exp2_hw(hi);
+  if constexpr (F32) {
+    const float lo = fmaf(v, -1.44269502f, -hi) + v * -1.92596303e-8f;
+    e = fabsf(hi) < 127.f ? fmaf(e * 0.693147182f, lo, e) : e;  // (past it e is 0, huge or no number)
+  }
+  return __builtin_amdgcn_rcpf(1.f + e);
 }
-__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
+template <bool F32>
+__device__ __forceinline__ float silu(float v) { return v * sigmoid<F32>(v); }
 
 }  // namespace
 

@@ -1,0 +1,54 @@
+"""The causal convolution and the block norm on the GPU at their edges, against the
+64-bit oracle."""
+
+import pytest
+import torch
+
+from oracle import state_space as ora
+from sparseflow_amd.Kernels.block_norm import block_norm_forward
+from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
+from tests.gpu_helpers import DEV, announce
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _gates(dtype=F32):
+    v = torch.cat([torch.linspace(-87, 20, 4091), torch.tensor([0.0, -0.0, 1e-8, -1e-8, 60.0])])
+    return v.to(dtype)
+
+
+def _close_to_a_few_units(got, want, what):
+    # The exponential and the reciprocal are good to 2 half units each, and the sum, the
+    # product and the correction to one: 7, and 10 are allowed.
+    got = got.detach().double().cpu()
+    off = (got - want).abs() - (10 * 2.0 ** -24 * want.abs() + 2.0 ** -126)
+    assert bool((off <= 0).all()), f"{what}: worst {float(((got - want).abs() / want.abs().clamp(min=1e-300)).max()) * 2 ** 24:.3g} half units"
+
+
+def test_float32_silu_of_the_convolution_to_its_last_bits():
+    announce("conv silu float32")
+    v = _gates()
+    x, w = v.expand(3, -1).contiguous()[None], torch.ones(v.numel(), 1)
+    y, _ = causal_conv1d_forward(x.to(DEV), w.to(DEV), activation="silu")
+    want = ora.silu(v.double()).expand(1, 3, -1)
+    _close_to_a_few_units(y, want, "prompt")
+    step = causal_conv1d_step(torch.empty(3, 0, v.numel(), device=DEV), x[0].to(DEV), w.to(DEV), activation="silu")
+    _close_to_a_few_units(step, want[0], "step")
+    out = causal_conv1d_forward(torch.tensor([[[float("-inf"), float("inf"), -1e30, 1e30]]], device=DEV),
+                                torch.ones(4, 1, device=DEV), activation="silu")[0].flatten().tolist()
+    assert out[0] != out[0] and out[1] == float("inf") and out[2] == 0 and out[3] == torch.tensor(1e30).item()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_gates_of_float32_results_to_their_last_bits(dtype, act):
+    announce(f"norm gate {act} {dtype} to float32")
+    g = _gates(dtype)
+    x, residual = torch.ones(2, g.numel(), dtype=dtype), torch.zeros(2, g.numel())
+    r, _ = block_norm_forward(x.to(DEV), gate=g.expand(2, -1).contiguous().to(DEV), activation=act,
+                              residual=residual.to(DEV))
+    assert r.dtype == F32
+    v = g.double()
+    _close_to_a_few_units(r, (ora.silu(v) if act == "silu" else torch.sigmoid(v)).expand(2, -1), act)
