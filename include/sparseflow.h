@@ -444,7 +444,8 @@ int sf_spike_attention(const void* q, const void* k, const void* v,
  * pool: the sequence starts from a zero state and its state is not kept, and a
  * step leaves the pool as it is and writes zeros to y.  initial_state NULL: a
  * zero state.  final_state NULL: the state is not kept.  Both may be the same
- * pool. */
+ * pool; apart from that, and a step's y that may be its x, nothing written shares
+ * memory with what is read. */
 
 #define SF_ACT_NONE 0
 #define SF_ACT_SILU 1
@@ -519,8 +520,8 @@ int sf_selective_scan_step(const sf_scan_desc* desc, float* state,
  * gate, post_weight, residual, scale_weight [dim] and pre_weight [dim] may be
  * NULL (weights are f32).  x, gate and h have `dtype`, residual and r
  * `residual_dtype` (`dtype` or f32); h is taken from the f32 value of r.  r_out
- * may be NULL where pre_weight is given, h_out where it is not; r_out may be the
- * residual and h_out may be x.  Element (o, i, c) of a tensor sits at
+ * may be NULL where pre_weight is given, h_out where it is not; each may be one of
+ * x, gate and residual (with its strides), else they share no memory.  Element (o, i, c) of a tensor sits at
  * o * strides[0] + i * strides[1] + c (a stride of inputs may be 0).
  * dim <= 16384, group_size divides dim; f32 sums. */
 typedef struct sf_norm_desc {

@@ -74,6 +74,45 @@ def check_pool(t: Optional[torch.Tensor], x: torch.Tensor, name: str, row: Tuple
                          f"({rows}, {', '.join(map(str, row))}) {dtype} on {x.device} is wanted")
 
 
+def check_out(t: Optional[torch.Tensor], name: str) -> None:
+    if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} is an expanded tensor: elements of its own are wanted")
+
+
+def _reach(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to the end of its last."""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    return (1 + sum([(n - 1) * s for n, s in zip(t.shape, t.stride())])) * t.element_size()
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether elements of a and b share memory.  (Views of one buffer that lie side by
+    side along any of its axes do not.)"""
+    by = b.data_ptr() - a.data_ptr()
+    if by >= _reach(a) or -by >= _reach(b) or a.numel() == 0 or b.numel() == 0:
+        return False
+    # Modulo a step that all longer ones are multiples of: what the shorter ones reach.
+    axes = [[(s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n > 1] for t in (a, b)]
+    for step in {s for own in axes for s, _ in own if s > 0}:
+        if any(s > step and s % step for own in axes for s, _ in own):
+            continue
+        inner = [t.element_size() + sum([s * (n - 1) for s, n in own if s < step]) for t, own in zip((a, b), axes)]
+        if by % step >= inner[0] and by % step + inner[1] <= step:
+            return False
+    return True
+
+
+def check_apart(written: torch.Tensor, name: str, others: dict, same: Tuple[str, ...] = ()) -> None:
+    """What a call writes shares no memory with what it reads; those of `same` it may be."""
+    for other, t in others.items():
+        if t is None or not overlap(written, t):
+            continue
+        if other not in same or t.data_ptr() != written.data_ptr() or t.shape != written.shape or t.dtype != written.dtype \
+                or any(a != b and n > 1 for a, b, n in zip(t.stride(), written.stride(), t.shape)):
+            raise ValueError(f"{name} shares memory with {other}")
+
+
 def last_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 

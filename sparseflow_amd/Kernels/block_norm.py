@@ -19,7 +19,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _lib
-from ._sequences import Plans, check_input, check_param, last_contiguous, signature
+from ._sequences import Plans, check_apart, check_input, check_out, check_param, last_contiguous, signature
 
 _plans = Plans()
 
@@ -72,7 +72,8 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
     post_weight, pre_weight float32 [dim]; scale a number or float32 [dim];
     group_size (of the first norm) divides dim; activation of the gate "silu",
     "sigmoid" or None.  r has the residual's type (without one, x's).  out (h)
-    and residual_out (r) may be given, and may be x and the residual.
+    and residual_out (r) may be given, and each may be one of x, gate and residual;
+    else they share no memory with those, nor with each other.
     """
     scale_weight = scale if isinstance(scale, torch.Tensor) else None
     factor = 1.0 if scale is None or scale_weight is not None else float(scale)
@@ -81,6 +82,12 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
     plan = _plans.get(key) or _plans.make(key, _check, x, gate, activation, gate_first, post_weight, group_size, residual,
                                           scale_weight, factor, pre_weight, eps, out, residual_out)
     group, r_type, desc = plan
+    if out is not None or residual_out is not None:
+        inputs = {"x": x, "gate": gate, "residual": residual}
+        if out is not None:
+            check_apart(out, "out", {**inputs, "residual_out": residual_out}, same=tuple(inputs))
+        if residual_out is not None:
+            check_apart(residual_out, "residual_out", inputs, same=tuple(inputs))
     if not x.is_cuda:
         r, h = _host(x, gate, activation, gate_first, post_weight, group, residual, scale, pre_weight, eps)
         if r.shape != x.shape:
@@ -142,6 +149,7 @@ def _check(x, gate, activation, gate_first, post_weight, group_size, residual, s
         if t is not None and (t.shape != shape or t.dtype != dtype or t.device != x.device):
             raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {tuple(shape)} {dtype} on "
                              f"{x.device} is wanted")
+        check_out(t, name)
         if t is not None and x.is_cuda and (_in_place(t, shape) is None if t.dim() <= 3 else not t.is_contiguous()):
             raise ValueError(f"{name}: a contiguous last axis is wanted (over more than three axes: all of them)")
     if out is not None and pre_weight is None:

@@ -16,8 +16,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ._sequences import Plans, check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
-    last_contiguous, signature
+from ._sequences import Plans, check_apart, check_index, check_input, check_like, check_out, check_param, check_pool, \
+    host_slots, host_spans, last_contiguous, signature
 
 _prompts, _steps = Plans(), Plans()
 
@@ -58,7 +58,8 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
     initial_state, final_state [batch, K - 1, C] in x's type, or pools
     [rows, K - 1, C] with slots (int32 [batch]; a slot outside the pool: zeros
     before, nothing kept); they may be one tensor.  max_len, the longest
-    sequence, sizes the launch of a packed call (default: all its tokens).
+    sequence, sizes the launch of a packed call (default: all its tokens).  Apart
+    from that, what is written shares no memory with what is read.
     """
     if x.is_cuda:
         x = last_contiguous(x)
@@ -68,8 +69,13 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
     shape, desc = plan
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        check_apart(out, "out", {"x": x, "initial_state": initial_state, "final_state": final_state})
     if final_state is None:
         final_state = torch.empty(shape, dtype=x.dtype, device=x.device)
+    else:
+        check_apart(final_state, "final_state", {"x": x} if final_state is initial_state else
+                    {"x": x, "initial_state": initial_state}, same=("initial_state",))
     if not x.is_cuda:
         with torch.no_grad():
             keep = shape[1]
@@ -105,6 +111,7 @@ def _check_prompt(x, weight, bias, activation, initial_state, offsets, max_len, 
         raise ValueError("initial_state and final_state have different numbers of rows")
     if out is not None:
         check_like(out, x, "out", tuple(x.shape))
+        check_out(out, "out")
         if out.stride(-1) != 1 and ch > 1:
             raise ValueError("out: a contiguous last axis is wanted")
     if not x.is_cuda:
@@ -127,7 +134,7 @@ def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
 
     state [batch, K - 1, C] in x's type, or a pool [rows, K - 1, C] with slots
     (int32 [batch], no two alike), moves on by the token in place.  A slot
-    outside the pool: y is zero there and no state changes.
+    outside the pool: y is zero there and no state changes.  out may be x.
     """
     if x.is_cuda:
         x = last_contiguous(x)
@@ -135,6 +142,8 @@ def causal_conv1d_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     plan = _steps.get(key) or _steps.make(key, _check_step, state, x, weight, bias, activation, slots, out)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        check_apart(out, "out", {"x": x, "state": state}, same=("x",))
     if not x.is_cuda:
         with torch.no_grad():
             for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
@@ -159,6 +168,7 @@ def _check_step(state, x, weight, bias, activation, slots, out):
     check_pool(state, x, "state", (k - 1, ch), x.dtype, batch, slots)
     if out is not None:
         check_like(out, x, "out", (batch, ch))
+        check_out(out, "out")
         if out.stride(-1) != 1 and ch > 1:
             raise ValueError("out: a contiguous last axis is wanted")
     if not x.is_cuda:

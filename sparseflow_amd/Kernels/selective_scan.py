@@ -18,8 +18,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ._sequences import Plans, check_index, check_input, check_like, check_param, check_pool, host_slots, host_spans, \
-    last_contiguous, signature
+from ._sequences import Plans, check_apart, check_index, check_input, check_like, check_out, check_param, check_pool, \
+    host_slots, host_spans, last_contiguous, signature
 
 _prompts, _steps = Plans(), Plans()
 
@@ -74,7 +74,8 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     [batch]; a slot outside the pool: a zero state, not kept); they may be one
     tensor.  max_len, the longest sequence, sizes the launch of a packed call
     (default: all its tokens).  workspace optionally holds the scratch between
-    calls (uint8; a new one where it is too small).
+    calls (contiguous, uint8; a new one where it is too small).  Apart from the
+    states, what is written shares no memory with what is read.
     """
     if x.is_cuda:
         x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
@@ -84,8 +85,15 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     shape, desc = plan
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        check_apart(out, "out", {"x": x, "dt": dt, "B": B, "C": C, "initial_state": initial_state, "final_state": final_state})
     if final_state is None:
         final_state = torch.empty(shape, dtype=torch.float32, device=x.device)
+    elif final_state is not initial_state:
+        check_apart(final_state, "final_state", {"x": x, "dt": dt, "B": B, "C": C, "initial_state": initial_state},
+                    same=("initial_state",))
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError(f"workspace has strides {tuple(workspace.stride())}: a contiguous one is wanted")
     if not x.is_cuda:
         with torch.no_grad():
             H, P, N = shape[1:]
@@ -126,6 +134,7 @@ def _check_prompt(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state, offset
         raise ValueError("initial_state and final_state have different numbers of rows")
     if out is not None:
         check_like(out, x, "out", tuple(x.shape))
+        check_out(out, "out")
         if out.stride(-1) != 1 and P > 1:
             raise ValueError("out: a contiguous last axis is wanted")
     shape = (batch, H, P, N) if final_state is None else tuple(final_state.shape)
@@ -152,7 +161,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
     dt [batch, H], B and C [batch, G, N]; state float32 [batch, H, P, N], or a
     pool [rows, H, P, N] with slots (int32 [batch], no two alike), moves on by
     the token in place.  A slot outside the pool: y is zero there and no state
-    changes.
+    changes.  out may be x.
     """
     if x.is_cuda:
         x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
@@ -160,6 +169,8 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
     plan = _steps.get(key) or _steps.make(key, _check_step, state, x, dt, A, B, C, D, dt_bias, dt_softplus, slots, out)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        check_apart(out, "out", {"x": x, "dt": dt, "B": B, "C": C, "state": state}, same=("x",))
     if not x.is_cuda:
         with torch.no_grad():
             for b, row in enumerate(host_slots(x.shape[0], state.shape[0], slots)):
@@ -182,6 +193,7 @@ def _check_step(state, x, dt, A, B, C, D, dt_bias, dt_softplus, slots, out):
     check_pool(state, x, "state", (H, P, N), torch.float32, batch, slots)
     if out is not None:
         check_like(out, x, "out", (batch, H, P))
+        check_out(out, "out")
         if out.stride(-1) != 1 and P > 1:
             raise ValueError("out: a contiguous last axis is wanted")
     if not x.is_cuda:

@@ -7,6 +7,7 @@ import torch
 from oracle import state_space as ora
 from sparseflow_amd.Kernels.block_norm import block_norm_forward
 from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
+from sparseflow_amd.Kernels.selective_scan import selective_scan_forward
 from tests.gpu_helpers import DEV, announce
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +53,38 @@ def test_gates_of_float32_results_to_their_last_bits(dtype, act):
     assert r.dtype == F32
     v = g.double()
     _close_to_a_few_units(r, (ora.silu(v) if act == "silu" else torch.sigmoid(v)).expand(2, -1), act)
+
+
+def test_outputs_that_overlap_inputs_are_refused():
+    announce("overlapping outputs")
+    x, w = torch.randn(2, 90, 48, device=DEV), torch.randn(48, 4, device=DEV)
+    with pytest.raises(ValueError, match="shares memory with x"):
+        causal_conv1d_forward(x, w, out=x)
+    B, dt, A = torch.randn(2, 90, 1, 8, device=DEV), torch.randn(2, 90, 3, device=DEV), -torch.ones(3, device=DEV)
+    xs = x.unflatten(-1, (3, 16))
+    with pytest.raises(ValueError, match="shares memory with x"):
+        selective_scan_forward(xs, dt, A, B, B, out=xs)
+    pool = torch.zeros(3, 3, 16, 8, device=DEV)
+    with pytest.raises(ValueError, match="shares memory with initial_state"):
+        selective_scan_forward(xs, dt, A, B, B, initial_state=pool[:2], final_state=pool[1:])
+    with pytest.raises(ValueError, match="workspace"):
+        selective_scan_forward(xs, dt, A, B, B, workspace=torch.zeros(1, device=DEV).expand(1 << 20))
+    wide = torch.randn(2, 90, 96, device=DEV)
+    want = causal_conv1d_forward(wide[..., :48].contiguous(), w)[0]
+    got = causal_conv1d_forward(wide[..., :48], w, out=wide[..., 48:])[0]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,group", [(64, 64), (2048, 256), (999, 999), (4096, 4096)])
+def test_a_norms_outputs_may_be_its_inputs(dtype, dim, group):
+    announce(f"norm in place {dtype} {dim}")
+    g = torch.Generator().manual_seed(dim)
+    x, gate, residual = (torch.randn(37, dim, generator=g).to(dtype).to(DEV) for _ in range(3))
+    post, pre = (torch.rand(dim, generator=g).to(DEV) for _ in range(2))
+    kw = dict(post_weight=post, group_size=group, pre_weight=pre)
+    want = block_norm_forward(x, gate=gate, residual=residual, **kw)
+    for out, residual_out in (("x", "residual"), ("residual", "x"), ("gate", "residual"), ("x", "gate")):
+        t = {"x": x.clone(), "gate": gate.clone(), "residual": residual.clone()}
+        got = block_norm_forward(t["x"], gate=t["gate"], residual=t["residual"], out=t[out], residual_out=t[residual_out], **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

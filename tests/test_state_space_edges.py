@@ -5,6 +5,9 @@ import pytest
 import torch
 
 from sparseflow_amd import _lib
+from sparseflow_amd.Kernels.block_norm import block_norm_forward
+from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
+from sparseflow_amd.Kernels.selective_scan import selective_scan_forward, selective_scan_step
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
@@ -16,3 +19,86 @@ def test_a_scans_workspace_is_of_the_sequences_that_are_cut(dtype, each):
     desc = _lib.scan_desc(short + 1, tokens, long, short + 1, *[(0, 1, 1)] * 5, H, P, 1, N, dtype, True)
     data = tokens * 2 * H * P * dtype.itemsize + 2 * (short + 1) * H * P * N * 4
     assert 0 < desc[2] < data // 4, f"{desc[2]} bytes of workspace for {data} of data"
+
+
+def _conv(n=6, c=4):
+    return torch.randn(2, n, c), torch.randn(c, 3)
+
+
+def _scan(n=5, H=2, P=4, G=1, N=3):
+    return [torch.randn(2, n, H, P), torch.randn(2, n, H), -torch.rand(H), torch.randn(2, n, G, N), torch.randn(2, n, G, N)]
+
+
+def test_a_convolutions_outputs_share_no_memory_with_its_inputs():
+    x, w = _conv()
+    buffer = torch.randn(2, 9, 4)
+    pools = torch.zeros(3, 2, 4)
+    flat = torch.zeros(40)
+    for kw in (dict(x=x, out=x), dict(x=buffer[:, :6], out=buffer[:, 1:7]), dict(x=buffer[:, :6], out=buffer[:, 3:]),
+               dict(x=x, initial_state=pools[:2], final_state=pools[1:]),
+               dict(x=x, initial_state=flat[:16].view(2, 2, 4), final_state=flat[1:17].view(2, 2, 4)),
+               dict(x=x, out=torch.zeros(1, 6, 4).expand(2, 6, 4))):
+        with pytest.raises(ValueError, match="memory|expanded"):
+            causal_conv1d_forward(**kw, weight=w)
+    want, _ = causal_conv1d_forward(x, w)
+    # Side by side in one buffer, along any axis, is apart.
+    for place in (torch.zeros(2, 12, 4), torch.zeros(2, 6, 8), torch.zeros(4, 6, 4), torch.zeros(2, 6, 2, 4)):
+        a, b = {(2, 12, 4): (place[:, :6], place[:, 6:]), (2, 6, 8): (place[..., :4], place[..., 4:]),
+                (4, 6, 4): (place[:2], place[2:]), (2, 6, 2, 4): (place[:, :, 0], place[:, :, 1])}[tuple(place.shape)]
+        for i, o in ((a, b), (b, a)):
+            i.copy_(x)
+            assert torch.equal(causal_conv1d_forward(i, w, out=o)[0], want) and torch.equal(i, x)
+    state = torch.zeros(2, 2, 4)
+    y, kept = causal_conv1d_forward(x, w, initial_state=state, final_state=state)
+    assert kept is state and torch.equal(y, want)
+    xt, s1, s2 = x[:, 0].clone(), state.clone(), state.clone()
+    want = causal_conv1d_step(s1, xt, w)
+    got = causal_conv1d_step(s2, xt, w, out=xt)
+    assert got is xt and torch.equal(got, want) and torch.equal(s1, s2)
+    with pytest.raises(ValueError, match="memory"):
+        causal_conv1d_step(state, xt, w, out=state[:, 0])
+
+
+def test_a_scans_outputs_share_no_memory_with_its_inputs():
+    x, dt, A, B, C = _scan()
+    buffer, states = torch.randn(2, 5, 2, 12), torch.zeros(3, 2, 4, 3)
+    for kw in (dict(x=x, out=x), dict(x=buffer[..., :4], out=buffer[..., 3:7]),
+               dict(x=x, initial_state=states[:2], final_state=states[1:]), dict(x=x, workspace=torch.zeros(1).expand(1 << 20)),
+               dict(x=x, out=torch.zeros(1, 5, 2, 4).expand(2, 5, 2, 4))):
+        with pytest.raises(ValueError, match="memory|expanded|contiguous"):
+            selective_scan_forward(**{**dict(dt=dt, A=A, B=B, C=C), **kw})
+    wide = torch.zeros(2, 5, 8)
+    with pytest.raises(ValueError, match="shares memory with B"):
+        selective_scan_forward(x, dt, A, wide[..., 2:5].unsqueeze(2), C, out=wide.unflatten(-1, (2, 4)))
+    want, last = selective_scan_forward(x, dt, A, B, C)
+    row = torch.zeros(2, 5, 8 + 8 + 6)
+    xs, out = row[..., :8].unflatten(-1, (2, 4)), row[..., 8:16].unflatten(-1, (2, 4))
+    Bs, Cs = row[..., 16:19].unsqueeze(2), row[..., 19:].unsqueeze(2)
+    xs.copy_(x), Bs.copy_(B), Cs.copy_(C)
+    assert torch.equal(selective_scan_forward(xs, dt, A, Bs, Cs, out=out)[0], want)
+    assert torch.equal(xs, x) and torch.equal(Bs, B) and torch.equal(Cs, C)
+    s1, s2, xt = torch.zeros(2, 2, 4, 3), torch.zeros(2, 2, 4, 3), x[:, 0].clone()
+    want = selective_scan_step(s1, xt, dt[:, 0], A, B[:, 0], C[:, 0])
+    assert torch.equal(selective_scan_step(s2, xt, dt[:, 0], A, B[:, 0], C[:, 0], out=xt), want) and torch.equal(s1, s2)
+    with pytest.raises(ValueError, match="memory"):
+        selective_scan_step(s1, x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], out=s1.view(-1)[:16].view(2, 2, 4))
+
+
+def test_a_norms_outputs_are_its_inputs_or_apart():
+    x, residual, w = torch.randn(3, 5, 8), torch.randn(3, 5, 8), torch.rand(8)
+    want_r, want_h = block_norm_forward(x, gate=x, residual=residual, pre_weight=w)
+    for out, residual_out in (("x", "residual"), ("residual", "x"), (None, "x"), ("x", None)):
+        t = {"x": x.clone(), "residual": residual.clone(), None: None}
+        r, h = block_norm_forward(t["x"], gate=t["x"], residual=t["residual"], pre_weight=w, out=t[out],
+                                  residual_out=t[residual_out])
+        assert torch.equal(r, want_r) and torch.equal(h, want_h)
+    one = x[:1].clone()  # (strides of an axis of one do not matter)
+    r, h = block_norm_forward(one, pre_weight=w, out=one.as_strided((1, 5, 8), (7, 8, 1)))
+    assert torch.equal(one, block_norm_forward(x[:1], pre_weight=w)[1])
+    buffer = torch.randn(4, 5, 8)
+    row = torch.randn(5, 8)
+    for kw in (dict(x=buffer[:3], out=buffer[1:]), dict(x=buffer[:3], residual_out=buffer[1:]),
+               dict(x=x, gate=row.expand(3, 5, 8), out=row.expand(3, 5, 8)),
+               dict(x=x, out=buffer[:3], residual_out=buffer[:3]), dict(x=x, out=buffer[:3], residual_out=buffer[1:])):
+        with pytest.raises(ValueError, match="memory|expanded"):
+            block_norm_forward(**kw, pre_weight=w)
