@@ -156,7 +156,7 @@ class WeightLayout:
         self._value = None
 
     def __call__(self, param: torch.Tensor):
-        key = (param._version, param.data_ptr(), param.device)
+        key = (param._version, param.data_ptr(), param.device, param.dtype)
         if self._value is None or key != self._key:
             self._value = self._build(param)
             self._key = key

@@ -4,7 +4,8 @@ selective scan and the block norm.
 CausalConv1d and SelectiveScan are stateful like the neurons (neuron.py): a
 forward continues each sequence from where the last one left it, in state rows of
 their own, until reset().  A prompt of one token runs the single-token kernels.
-Inference only."""
+Parameters of another type than the kernels' float32 (a model in 16 bits) are cast
+when they change.  Inference only."""
 
 from __future__ import annotations
 
@@ -18,6 +19,16 @@ from ..Kernels.block_norm import block_norm_forward
 from ..Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
 from ..Kernels.selective_scan import selective_scan_forward, selective_scan_step
 from ._runtime import WeightLayout
+
+
+class _Float32:
+    """A parameter as the kernels take it."""
+
+    def __init__(self):
+        self._cast = WeightLayout(lambda p: p.detach().float().contiguous())
+
+    def __call__(self, param: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        return param if param is None or (param.dtype == torch.float32 and param.is_contiguous()) else self._cast(param)
 
 
 class _Stateful(nn.Module):
@@ -43,12 +54,14 @@ class CausalConv1d(_Stateful):
         self.weight = nn.Parameter(torch.empty(self.channels, self.kernel_size))
         self.bias = nn.Parameter(torch.zeros(self.channels)) if bias else None
         nn.init.uniform_(self.weight, -self.kernel_size ** -0.5, self.kernel_size ** -0.5)
+        self._weight, self._bias = _Float32(), _Float32()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         state = self._state_for((x.shape[0], self.kernel_size - 1, self.channels), x.dtype, x.device)
+        weight, bias = self._weight(self.weight), self._bias(self.bias)
         if state is not None and x.shape[1] == 1:
-            return causal_conv1d_step(state, x[:, 0], self.weight, self.bias, activation=self.activation)[:, None]
-        y, self.state = causal_conv1d_forward(x, self.weight, self.bias, activation=self.activation, initial_state=state,
+            return causal_conv1d_step(state, x[:, 0], weight, bias, activation=self.activation)[:, None]
+        y, self.state = causal_conv1d_forward(x, weight, bias, activation=self.activation, initial_state=state,
                                               final_state=state)
         return y
 
@@ -71,15 +84,14 @@ class SelectiveScan(_Stateful):
         self.D = nn.Parameter(torch.ones(self.heads))
         self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
         self._rates = WeightLayout(lambda a: -torch.exp(a.detach().float()))
+        self._D, self._dt_bias = _Float32(), _Float32()
 
     def forward(self, x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.Tensor) -> torch.Tensor:
-        A = self._rates(self.A_log)
+        A, D, dt_bias = self._rates(self.A_log), self._D(self.D), self._dt_bias(self.dt_bias)
         state = self._state_for((x.shape[0], self.heads, self.head_dim, self.state_dim), torch.float32, x.device)
         if state is not None and x.shape[1] == 1:
-            return selective_scan_step(state, x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], D=self.D,
-                                       dt_bias=self.dt_bias)[:, None]
-        y, self.state = selective_scan_forward(x, dt, A, B, C, D=self.D, dt_bias=self.dt_bias, initial_state=state,
-                                               final_state=state)
+            return selective_scan_step(state, x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], D=D, dt_bias=dt_bias)[:, None]
+        y, self.state = selective_scan_forward(x, dt, A, B, C, D=D, dt_bias=dt_bias, initial_state=state, final_state=state)
         return y
 
     def extra_repr(self) -> str:
@@ -99,12 +111,13 @@ class BlockNorm(nn.Module):
         self.post_weight = nn.Parameter(torch.ones(self.dim)) if post else None
         self.pre_weight = nn.Parameter(torch.ones(self.dim)) if pre else None
         self.scale = nn.Parameter(torch.full((self.dim,), float(scale))) if scale is not None else None
+        self._post, self._pre, self._scale = _Float32(), _Float32(), _Float32()
 
     def forward(self, x: torch.Tensor, gate: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         return block_norm_forward(x, gate=gate, activation=self.activation, gate_first=self.gate_first,
-                                  post_weight=self.post_weight, group_size=self.group_size, residual=residual,
-                                  scale=self.scale, pre_weight=self.pre_weight, eps=self.eps)
+                                  post_weight=self._post(self.post_weight), group_size=self.group_size, residual=residual,
+                                  scale=self._scale(self.scale), pre_weight=self._pre(self.pre_weight), eps=self.eps)
 
     def extra_repr(self) -> str:
         return f"dim={self.dim}, group_size={self.group_size}, gate_first={self.gate_first}, eps={self.eps}"

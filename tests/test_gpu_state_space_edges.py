@@ -8,6 +8,7 @@ from oracle import state_space as ora
 from sparseflow_amd.Kernels.block_norm import block_norm_forward
 from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
 from sparseflow_amd.Kernels.selective_scan import selective_scan_forward
+from sparseflow_amd.Models import spiking_ssm_tiny
 from tests.gpu_helpers import DEV, announce
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,19 @@ def test_a_norms_outputs_may_be_its_inputs(dtype, dim, group):
         t = {"x": x.clone(), "gate": gate.clone(), "residual": residual.clone()}
         got = block_norm_forward(t["x"], gate=t["gate"], residual=t["residual"], out=t[out], residual_out=t[residual_out], **kw)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_model_in_16_bits(dtype):
+    announce(f"spiking ssm in {dtype}")
+    torch.manual_seed(4)
+    m = spiking_ssm_tiny(vocab=32, v_threshold=0.5).eval().to(DEV).to(dtype)
+    ids = torch.randint(0, 32, (2, 40), device=DEV)
+    with torch.no_grad():
+        b, x = m.blocks[0], torch.randn(2, 40, m.blocks[0].mixed, device=DEV).to(dtype)
+        want, _ = causal_conv1d_forward(x, b.conv.weight.float(), b.conv.bias.float(), activation="silu")
+        assert torch.equal(b.conv(x), want)
+        b.conv.reset()
+        logits, more = m(ids), m(ids[:, :1])
+    assert logits.shape == (2, 40, 32) and more.shape == (2, 1, 32) and logits.dtype == dtype
+    assert torch.isfinite(logits).all() and torch.isfinite(more).all()

@@ -8,6 +8,8 @@ from sparseflow_amd import _lib
 from sparseflow_amd.Kernels.block_norm import block_norm_forward
 from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
 from sparseflow_amd.Kernels.selective_scan import selective_scan_forward, selective_scan_step
+from sparseflow_amd.Models import spiking_ssm_tiny
+from sparseflow_amd.Ops import BlockNorm, CausalConv1d, SelectiveScan
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
@@ -102,3 +104,39 @@ def test_a_norms_outputs_are_its_inputs_or_apart():
                dict(x=x, out=buffer[:3], residual_out=buffer[:3]), dict(x=x, out=buffer[:3], residual_out=buffer[1:])):
         with pytest.raises(ValueError, match="memory|expanded"):
             block_norm_forward(**kw, pre_weight=w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_modules_in_16_bits(dtype):
+    torch.manual_seed(3)
+    conv, scan = CausalConv1d(8).to(dtype), SelectiveScan(2, 4, 3).to(dtype)
+    norm = BlockNorm(8, post=True, pre=True, scale=0.5).to(dtype)
+    x = torch.randn(2, 5, 8).to(dtype)
+    dt, B = torch.randn(2, 5, 2).to(dtype), torch.randn(2, 5, 1, 3).to(dtype)
+    for _ in range(2):
+        y = conv(x)
+        assert torch.equal(y, causal_conv1d_forward(x, conv.weight.float(), conv.bias.float(), activation="silu")[0])
+        y = scan(x.unflatten(-1, (2, 4)), dt, B, B)
+        want, _ = selective_scan_forward(x.unflatten(-1, (2, 4)), dt, -torch.exp(scan.A_log.float()), B, B, D=scan.D.float(),
+                                         dt_bias=scan.dt_bias.float())
+        assert y.dtype == dtype and torch.equal(y, want)
+        r, h = norm(x, residual=x)
+        want = block_norm_forward(x, post_weight=norm.post_weight.float(), residual=x, scale=norm.scale.float(),
+                                  pre_weight=norm.pre_weight.float(), eps=norm.eps)
+        assert torch.equal(r, want[0]) and torch.equal(h, want[1])
+        # (A token after the prompt, and weights that have changed.)
+        assert conv(x[:, :1]).shape == (2, 1, 8) and scan(x[:, :1].unflatten(-1, (2, 4)), dt[:, :1], B[:, :1], B[:, :1]).dtype == dtype
+        conv.reset(), scan.reset()
+        with torch.no_grad():
+            for p in (*conv.parameters(), *scan.parameters(), *norm.parameters()):
+                p.add_(0.5)
+
+
+def test_a_model_in_16_bits():
+    torch.manual_seed(4)
+    m = spiking_ssm_tiny(vocab=32, v_threshold=0.5).eval().to(torch.bfloat16)
+    ids = torch.randint(0, 32, (2, 6))
+    with torch.no_grad():
+        logits = m(ids)
+        more = m(ids[:, :1])
+    assert logits.shape == (2, 6, 32) and more.shape == (2, 1, 32) and torch.isfinite(logits).all()
