@@ -77,6 +77,9 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
     """
     scale_weight = scale if isinstance(scale, torch.Tensor) else None
     factor = 1.0 if scale is None or scale_weight is not None else float(scale)
+    eps, gate_first = float(eps), bool(gate_first)
+    if group_size is not None:
+        group_size = int(group_size)
     key = (signature(x, gate, post_weight, residual, scale_weight, pre_weight, out, residual_out), activation, gate_first,
            group_size, factor, eps)
     plan = _plans.get(key) or _plans.make(key, _check, x, gate, activation, gate_first, post_weight, group_size, residual,
@@ -141,7 +144,7 @@ def _check(x, gate, activation, gate_first, post_weight, group_size, residual, s
     check_param(post_weight, x, "post_weight", (dim,))
     check_param(pre_weight, x, "pre_weight", (dim,))
     check_param(scale_weight, x, "scale", (dim,))
-    group = dim if group_size is None else int(group_size)
+    group = dim if group_size is None else group_size
     if group < 1 or dim % group != 0:
         raise ValueError(f"group_size {group} does not divide {dim}")
     r_type = x.dtype if residual is None else residual.dtype

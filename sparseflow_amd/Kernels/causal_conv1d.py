@@ -63,6 +63,8 @@ def causal_conv1d_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[
     """
     if x.is_cuda:
         x = last_contiguous(x)
+    if max_len is not None:
+        max_len = int(max_len)
     key = (signature(x, weight, bias, initial_state, offsets, slots, out, final_state), activation, max_len)
     plan = _prompts.get(key) or _prompts.make(key, _check_prompt, x, weight, bias, activation, initial_state, offsets,
                                               max_len, slots, out, final_state)

@@ -79,6 +79,9 @@ def selective_scan_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     """
     if x.is_cuda:
         x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
+    if max_len is not None:
+        max_len = int(max_len)
+    dt_softplus = bool(dt_softplus)
     key = (signature(x, dt, A, B, C, D, dt_bias, offsets, slots, initial_state, out, final_state), max_len, dt_softplus)
     plan = _prompts.get(key) or _prompts.make(key, _check_prompt, x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state,
                                               offsets, max_len, slots, out, final_state)
@@ -165,6 +168,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
     """
     if x.is_cuda:
         x, B, C = last_contiguous(x), last_contiguous(B), last_contiguous(C)
+    dt_softplus = bool(dt_softplus)
     key = (signature(state, x, dt, A, B, C, D, dt_bias, slots, out), dt_softplus)
     plan = _steps.get(key) or _steps.make(key, _check_step, state, x, dt, A, B, C, D, dt_bias, dt_softplus, slots, out)
     if out is None:

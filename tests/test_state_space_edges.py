@@ -140,3 +140,19 @@ def test_a_model_in_16_bits():
         logits = m(ids)
         more = m(ids[:, :1])
     assert logits.shape == (2, 6, 32) and more.shape == (2, 1, 32) and torch.isfinite(logits).all()
+
+
+def test_numbers_that_come_as_tensors_are_read_at_every_call():
+    x, w = torch.randn(3, 8), torch.rand(8)
+    eps, group, first = torch.tensor(1e-5), torch.tensor(8), torch.tensor(True)
+    block_norm_forward(x, post_weight=w, eps=eps, group_size=group, gate=x, gate_first=first)
+    eps.fill_(1.0), group.fill_(4), first.fill_(False)
+    got, _ = block_norm_forward(x, post_weight=w, eps=eps, group_size=group, gate=x, gate_first=first)
+    assert torch.equal(got, block_norm_forward(x, post_weight=w, eps=1.0, group_size=4, gate=x)[0])
+    xs, dt, A, B, C = _scan()
+    flat, off, longest, soft = [t.flatten(0, 1) for t in (xs, dt, B, C)], torch.tensor([0, 4, 10], dtype=torch.int32), \
+        torch.tensor(6), torch.tensor(True)
+    run = lambda most, plus: selective_scan_forward(flat[0], flat[1], A, *flat[2:], dt_softplus=plus, offsets=off, max_len=most)[0]  # noqa: E731
+    assert torch.equal(run(longest, soft), run(6, True))
+    longest.fill_(5), soft.fill_(False)
+    assert torch.equal(run(longest, soft), run(5, False))
