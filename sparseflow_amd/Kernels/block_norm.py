@@ -95,7 +95,7 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
         r, h = _host(x, gate, activation, gate_first, post_weight, group, residual, scale, pre_weight, eps)
         if r.shape != x.shape:
             raise ValueError(f"gate or residual does not broadcast to {tuple(x.shape)}")
-        r = r.to(r_type) if residual_out is None else residual_out.copy_(r)
+        r = r.to(r_type, copy=r is x) if residual_out is None else residual_out.copy_(r)
         if h is not None:
             h = h.to(x.dtype) if out is None else out.copy_(h)
         return r, h

@@ -156,3 +156,12 @@ def test_numbers_that_come_as_tensors_are_read_at_every_call():
     assert torch.equal(run(longest, soft), run(6, True))
     longest.fill_(5), soft.fill_(False)
     assert torch.equal(run(longest, soft), run(5, False))
+
+
+def test_a_norm_alone_returns_r_apart_from_x():
+    x, w = torch.randn(3, 8), torch.rand(8)
+    before = x.clone()
+    r, _ = block_norm_forward(x, pre_weight=w)
+    assert torch.equal(r, x)
+    r.zero_()
+    assert torch.equal(x, before)
