@@ -32,7 +32,7 @@ def _rows(t: torch.Tensor, shape: Tuple[int, ...]) -> Tuple[torch.Tensor, ...]:
     if t.shape != shape:
         t = t.expand(shape)
     t = last_contiguous(t)
-    return (t.reshape(-1, t.shape[-2], t.shape[-1]) if t.dim() > 3 else t,)
+    return (t.flatten(0, -3) if t.dim() > 3 else t,)
 
 
 @torch.no_grad()

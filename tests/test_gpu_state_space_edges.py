@@ -105,3 +105,12 @@ def test_a_model_in_16_bits(dtype):
         logits, more = m(ids), m(ids[:, :1])
     assert logits.shape == (2, 40, 32) and more.shape == (2, 1, 32) and logits.dtype == dtype
     assert torch.isfinite(logits).all() and torch.isfinite(more).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 8), (0, 3, 5, 8), (2, 0, 5, 8), (1, 1, 0, 2, 8), (0, 8), (3, 0, 8)])
+def test_norms_over_empty_axes(shape):
+    announce(f"norm over empty axes {shape}")
+    x, w = torch.randn(shape, device=DEV), torch.rand(8, device=DEV)
+    for gate in (None, x, torch.randn(8, device=DEV)):
+        r, h = block_norm_forward(x, gate=gate, residual=x, pre_weight=w)
+        assert r.shape == h.shape == x.shape

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from sparseflow_amd import _lib
+from sparseflow_amd.Kernels import block_norm
 from sparseflow_amd.Kernels.block_norm import block_norm_forward
 from sparseflow_amd.Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
 from sparseflow_amd.Kernels.selective_scan import selective_scan_forward, selective_scan_step
@@ -165,3 +166,13 @@ def test_a_norm_alone_returns_r_apart_from_x():
     assert torch.equal(r, x)
     r.zero_()
     assert torch.equal(x, before)
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 4), (0, 3, 5, 4), (2, 0, 5, 4), (2, 3, 5, 4), (1, 1, 0, 2, 4)])
+def test_a_norms_rows_over_empty_axes(shape):
+    """More than three axes become three, also where one of them is empty."""
+    t = torch.randn(shape)
+    rows, = block_norm._rows(t, t.shape)
+    assert rows.shape == (t[..., 0, 0].numel(), *shape[-2:]) and rows.numel() == t.numel()
+    spread, = block_norm._rows(torch.randn(shape[-1]), t.shape)
+    assert spread.shape == rows.shape
