@@ -93,8 +93,6 @@ def block_norm_forward(x: torch.Tensor, gate: Optional[torch.Tensor] = None, act
             check_apart(residual_out, "residual_out", inputs, same=tuple(inputs))
     if not x.is_cuda:
         r, h = _host(x, gate, activation, gate_first, post_weight, group, residual, scale, pre_weight, eps)
-        if r.shape != x.shape:
-            raise ValueError(f"gate or residual does not broadcast to {tuple(x.shape)}")
         r = r.to(r_type, copy=r is x) if residual_out is None else residual_out.copy_(r)
         if h is not None:
             h = h.to(x.dtype) if out is None else out.copy_(h)
@@ -141,6 +139,9 @@ def _check(x, gate, activation, gate_first, post_weight, group_size, residual, s
     if residual is not None and (residual.dtype not in (x.dtype, torch.float32) or residual.device != x.device):
         raise ValueError(f"residual is {residual.dtype} on {residual.device}: {x.dtype} or float32 on {x.device} is "
                          "wanted")
+    for t, name in ((gate, "gate"), (residual, "residual")):
+        if t is not None and (t.dim() > x.dim() or any(n not in (1, m) for n, m in zip(t.shape[::-1], shape[::-1]))):
+            raise ValueError(f"{name} is {tuple(t.shape)}: it does not broadcast to {tuple(shape)}")
     check_param(post_weight, x, "post_weight", (dim,))
     check_param(pre_weight, x, "pre_weight", (dim,))
     check_param(scale_weight, x, "scale", (dim,))

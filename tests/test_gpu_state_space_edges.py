@@ -114,3 +114,17 @@ def test_norms_over_empty_axes(shape):
     for gate in (None, x, torch.randn(8, device=DEV)):
         r, h = block_norm_forward(x, gate=gate, residual=x, pre_weight=w)
         assert r.shape == h.shape == x.shape
+
+
+def test_a_norms_inputs_broadcast_or_are_refused():
+    announce("norm broadcasts")
+    x, w = torch.randn(3, 8, device=DEV), torch.rand(8, device=DEV)
+    for shape in ((3, 7), (2, 8), (2, 3, 8), (1, 3, 8), (0, 8), (5,)):
+        for name in ("gate", "residual"):
+            with pytest.raises(ValueError, match="broadcast"):
+                block_norm_forward(x, pre_weight=w, **{name: torch.randn(shape, device=DEV)})
+    for shape in ((3, 8), (1, 8), (3, 1), (8,), (1,), ()):
+        t = torch.randn(shape, device=DEV)
+        got = block_norm_forward(x, gate=t, residual=t, pre_weight=w)
+        want = block_norm_forward(x, gate=t.expand(3, 8).contiguous(), residual=t.expand(3, 8).contiguous(), pre_weight=w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

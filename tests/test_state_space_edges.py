@@ -178,3 +178,16 @@ def test_a_norms_rows_over_empty_axes(shape):
     assert rows.shape == (math.prod(shape[:-2]), *shape[-2:])
     spread, = block_norm._rows(torch.randn(shape[-1]), t.shape)
     assert spread.shape == rows.shape
+
+
+def test_a_norms_gate_and_residual_that_do_not_broadcast_are_refused():
+    x, w = torch.randn(3, 8), torch.rand(8)
+    for shape in ((3, 7), (2, 8), (2, 3, 8), (1, 3, 8), (0, 8), (5,)):
+        for name in ("gate", "residual"):
+            with pytest.raises(ValueError, match="broadcast"):
+                block_norm_forward(x, pre_weight=w, **{name: torch.randn(shape)})
+    for shape in ((3, 8), (1, 8), (3, 1), (8,), (1,), ()):
+        t = torch.randn(shape)
+        got = block_norm_forward(x, gate=t, residual=t, pre_weight=w)
+        want = block_norm_forward(x, gate=t.expand(3, 8).contiguous(), residual=t.expand(3, 8).contiguous(), pre_weight=w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
