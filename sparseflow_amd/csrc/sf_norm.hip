@@ -228,22 +228,23 @@ int launch_norm_k(const NormArgs& a, int sub, hipStream_t stream) {
 }
 
 // M vectors a thread hold the widest row that 1024 threads take.
+// Groups inside a row that has a norm of its own, too.
 template <typename T, typename TR, int V, int M, int MODE>
-int launch_norm_v(const NormArgs& a, hipStream_t stream) {
-  const bool grouped = a.post_w != nullptr && a.group != a.dim;
-  if (MODE != kRagged && grouped && a.pre_w != nullptr) {
-    if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true, MODE>(a, 1, stream);
-    return launch_norm_k<T, TR, 1024, V, M, true, MODE>(a, 1, stream);
-  }
-  const int sub = grouped ? a.dim / a.group : 1, width = a.dim / sub;
+int launch_norm_grouped(const NormArgs& a, hipStream_t stream) {
+  if (a.dim <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, true, MODE>(a, 1, stream);
+  return launch_norm_k<T, TR, 1024, V, M, true, MODE>(a, 1, stream);
+}
+
+// Rows, or groups as rows of their own.
+template <typename T, typename TR, int V, int M, int MODE>
+int launch_norm_rows(const NormArgs& a, hipStream_t stream) {
+  const int sub = a.post_w != nullptr ? a.dim / a.group : 1, width = a.dim / sub;
   if (width <= 64 * V) return launch_norm_k<T, TR, 64, V, 1, false, MODE>(a, sub, stream);
   if (width <= 64 * V * 2) return launch_norm_k<T, TR, 64, V, 2, false, MODE>(a, sub, stream);
   if (width <= 64 * V * 3) return launch_norm_k<T, TR, 64, V, 3, false, MODE>(a, sub, stream);
-  if (V == 1 && width <= 64 * 16) return launch_norm_k<T, TR, 64, 1, 16, false, kPlain>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 1) return launch_norm_k<T, TR, 256, V, 1, false, MODE>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false, MODE>(a, sub, stream);
-  if (width <= 256 * V * M) return launch_norm_k<T, TR, 256, V, M, false, MODE>(a, sub, stream);
-  if (V > 1 && width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false, MODE>(a, sub, stream);
+  if (width <= 256 * V) return launch_norm_k<T, TR, 256, V, 1, false, MODE>(a, sub, stream);
+  if (width <= 256 * V * 2) return launch_norm_k<T, TR, 256, V, 2, false, MODE>(a, sub, stream);
+  if (width <= 256 * V * 4) return launch_norm_k<T, TR, 256, V, 4, false, MODE>(a, sub, stream);
   return launch_norm_k<T, TR, 1024, V, M, false, MODE>(a, sub, stream);
 }
 
@@ -251,13 +252,18 @@ template <typename T, typename TR>
 int launch_norm_t(const NormArgs& a, hipStream_t stream) {
   // 16 bytes of the widest type.
   constexpr int V = 16 / (sizeof(T) > sizeof(TR) ? sizeof(T) : sizeof(TR));
-  // Groups inside a row that are not whole vectors: single elements.
-  if (a.post_w != nullptr && a.pre_w != nullptr && a.group != a.dim && a.group % V != 0)
-    return launch_norm_v<T, TR, 1, 16, kPlain>(a, stream);
+  const bool grouped = a.post_w != nullptr && a.pre_w != nullptr && a.group != a.dim;
+  const bool whole = (a.post_w != nullptr ? a.group : a.dim) % V == 0;
   const int64_t bytes = (a.gate != nullptr ? 2 : 1) * (int64_t)sizeof(T) + (a.res != nullptr ? (int64_t)sizeof(TR) : 0);
-  if ((a.post_w != nullptr ? a.group : a.dim) % V != 0) return launch_norm_v<T, TR, V, 16 / V, kRagged>(a, stream);
-  return read_once(a.outer * a.inner * a.dim * bytes) ? launch_norm_v<T, TR, V, 16 / V, kOnce>(a, stream)
-                                                      : launch_norm_v<T, TR, V, 16 / V, kPlain>(a, stream);
+  const bool once = read_once(a.outer * a.inner * a.dim * bytes);
+  if (grouped) {
+    // Groups that are not whole vectors: single elements.
+    if (!whole) return launch_norm_grouped<T, TR, 1, 16, kPlain>(a, stream);
+    return once ? launch_norm_grouped<T, TR, V, 16 / V, kOnce>(a, stream)
+                : launch_norm_grouped<T, TR, V, 16 / V, kPlain>(a, stream);
+  }
+  if (!whole) return launch_norm_rows<T, TR, V, 16 / V, kRagged>(a, stream);
+  return once ? launch_norm_rows<T, TR, V, 16 / V, kOnce>(a, stream) : launch_norm_rows<T, TR, V, 16 / V, kPlain>(a, stream);
 }
 
 template <typename T>
