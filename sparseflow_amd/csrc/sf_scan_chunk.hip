@@ -827,6 +827,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
     ScanArgs a;
     ScanSplit sp;
   };
+  static_assert(alignof(ScanArgs) == alignof(ScanSplit), "the kernel's arguments, one after the other");
   typedef const __attribute__((address_space(4))) Args* ArgsAt;
   ArgsAt args = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(args));

@@ -127,3 +127,19 @@ def test_packed_long_among_short(dtype, lens):
         assert bool(((pool[i].double().cpu() - h).abs() <= f * hm).all()), f"state {i} of {n}"
         assert bool(((y[at].double().cpu() - ref).abs() <= (f + inner) * ym + half_ulp * ref.abs() + 2.0 ** -25).all()), \
             f"sequence {i} of {n}"
+
+
+@pytest.mark.parametrize("longest", [8, 200, 700])
+def test_dense_calls_whose_longest_is_not_their_tokens(longest):
+    """max_len only sizes the launch: of dense sequences too, where it should be their
+    tokens."""
+    announce(f"scan dense with max_len {longest}")
+    n, H, P, G, N = 700, 3, 32, 1, 32
+    x, dt, A, B, C = _inputs((2, n), H, P, G, N, F32, 9)
+    want, last = selective_scan_forward(x, dt, A, B, C)
+    y, state = torch.zeros_like(x), torch.zeros_like(last)
+    desc = _lib.scan_desc(2, n, longest, 2, x.stride()[:3], dt.stride(), B.stride()[:3], C.stride()[:3], y.stride()[:3], H, P, G,
+                          N, F32, True)
+    workspace = torch.empty(max(desc[2], 16), dtype=torch.uint8, device=DEV)
+    _lib.selective_scan(desc, x, dt, A, B, C, None, None, None, None, None, y, state, workspace)
+    assert torch.allclose(y, want, rtol=1e-4, atol=1e-4) and torch.allclose(state, last, rtol=1e-4, atol=1e-4)
