@@ -495,7 +495,8 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
       }
   }
 
-  // (Opaque where registers are tight, so that what is made of it is not kept in them.)
+  // (Opaque where registers are tight, so that what the last chunk, by way of registers,
+  // makes of it is not kept in them.)
   auto thread = []() {
     int t = threadIdx.x;
     if constexpr (kTight) asm volatile("" : "+v"(t));
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   auto ahead = [&](int64_t rest) { return DIRECT && rest >= Q; };
   auto load_rows = [&](const T* base, int stride, uint16_t* to) {
     const char* from = reinterpret_cast<const char*>(base);
-    const int bj = thread() / kRowUnits, bv = thread() % kRowUnits;
+    const int bj = threadIdx.x / kRowUnits, bv = threadIdx.x % kRowUnits;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int u = unit_place<NP>(r * kRows + bj, bv);
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   auto load_x = [&](uint16_t* to) {
     if (!on) return;
     const char* from = reinterpret_cast<const char*>(x);
-    const int xj = thread() % kWave / kXUnits, xv = thread() % kXUnits;
+    const int xj = threadIdx.x % kWave / kXUnits, xv = threadIdx.x % kXUnits;
 #pragma unroll
     for (int r = 0; r < kXRounds; ++r) {
       const int u = x_place(r * kXRows + xj, xv * U) % kSlice / U;
