@@ -6,7 +6,7 @@
 // stay in registers as the run is walked, every input of the run is one load of 16
 // bytes, kBatch of them under way at a time, and the K - 1 before the run are read
 // again (from the cache: a neighbouring thread's run).  Bound by HBM: x in, y out;
-// 2 x 16384 x 4352 bf16, K = 4: 130 us, 4.4 TB/s; ragged sequences of 17,300 x 1037
+// 2 x 16384 x 4352 bf16, K = 4: 130 us, 4.4 TB/s; ragged sequences of 16,064 x 1037
 // float32, whose rows begin anywhere: 39 us, 3.4 TB/s; one token of 256 x 2304: 10 us, a
 // call's own time.
 #include "sf_seq.h"

@@ -314,9 +314,9 @@ constexpr int kScanMaxState = 256;
 int launch_scan_seq(const ScanArgs& a, int dtype, hipStream_t stream);
 
 // Prompts chunk by chunk: how the work is cut.
-// The longest sequence from which chunks are used (bf16 and float32, 64 sequences of 24
-// heads x 64, N 128: of 4 tokens 26 and 38 us, token by token 32 and 25; of 8 tokens 27
-// and 37, token by token 50 and 39; a chunk's time is that of a whole one).
+// The longest sequence from which chunks are used (64 sequences of 24 heads x 64, N 128,
+// bf16, f16 and float32: of 4 tokens 29, 35 and 40 us, token by token 25; of 8 tokens the
+// same, token by token 37; a chunk's time is that of a whole one).
 constexpr int kScanChunkFrom = 8;
 struct ScanSplit {
   float* parts;   // [rows, heads, head_dim, state_dim], a row to each segment of a cut sequence

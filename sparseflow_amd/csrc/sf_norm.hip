@@ -4,8 +4,8 @@
 //   r = residual + scale t, h = r w' / rms(r)
 // A row is held in registers by LT threads, vectors of V elements: x, gate and residual
 // are all loaded before the first sum, and h is written after the second.  Bound by
-// HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 152 us, 5.3 TB/s; 32768 x 2048
-// f16 with gate, float32 residual and h (940 MB) 180 us, 5.2 TB/s.  Short rows (up to 3
+// HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 154 us, 5.2 TB/s; 32768 x 2048
+// f16 with gate, float32 residual and h (940 MB) 182 us, 5.2 TB/s.  Short rows (up to 3
 // vectors a lane) are a wavefront's, whose sums need no barrier: 32768 x 384 float32 25
 // us, as a workgroup's 37; of 768 53 and 57; of four vectors, 2048 bf16, 86 and 77.
 //
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kBlock = 256;
 // Rows of whole vectors; those whose inputs the caches are not to keep; rows that end
-// inside a vector (32768 x 2047 bf16: 141 us, by single elements 238; the checks for it
+// inside a vector (32768 x 2047 bf16: 142 us, by single elements 238; the checks for it
 // would cost whole rows, 2048, 92 against 70).
 constexpr int kPlain = 0, kOnce = 1, kRagged = 2;
 

@@ -22,15 +22,16 @@
 // the last part (two products for bf16, three for f16 and six for float32, a sixth of
 // the time that the float32 instructions take).  So S and h are rounded to 16 bits for
 // bf16 and f16 outputs, which have 8 and 11 themselves: what y loses is its own rounding
-// (as one part for bf16, y was off by more than that where its terms cancel: the kernels
-// of 2 x 16384 tokens took 482 us, and take 550).  v is split into three parts, its 24 bits, always: the state is summed up
-// over all tokens and stays a float32 one.  L is summed in 64 bits: differences of it
-// are exponents.
+// (as one part for bf16, y was off by more than that where its terms cancel; 2 x 16384
+// tokens took 390 us with one and take 440).  v is split into three parts, its 24 bits,
+// always: the state is summed up over all tokens and stays a float32 one.  L is summed
+// in 64 bits: differences of it are exponents.
 //
 // Bound by the chain of products and the waits between them, not by memory: 2 x 16384
-// tokens, 64 heads x 64, N 128, bf16 (562 MB, 241 GFLOP of products) take 389 us, 620
-// TFLOP/s and 1.4 TB/s, 280 of them the main pass; rows at any address, by way of
-// registers, a quarter more; 23 ragged sequences of up to 1500 of f16, 24 heads, 190 us.
+// tokens, 64 heads x 64, N 128, bf16 (562 MB, 290 GFLOP of products) take 440 us, 660
+// TFLOP/s and 1.3 TB/s; alone, the main pass 365 us, the segments' own parts 162, the
+// chain 16; rows at any address, by way of registers, as long; 23 ragged sequences of up
+// to 1500 of f16, 24 heads, 198 us.
 //
 // Where products are not finite, a wavefront does its segment again, token by token:
 // infinities, NaN and results near the ends of a float's range are those of the
@@ -79,9 +80,10 @@ __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(
 typedef u32x4 Frag;  // pairs of bf16
 __device__ __forceinline__ int order4(int b) { return (b >> 1) | ((b & 1) << 1); }
 
-// Place of 16-byte unit u (8 elements) in token j's row of a tile [32][NP]: spread so
-// that neither a read of one unit of 16 rows nor a transposed one of two units of 4
-// rows meets a bank twice.
+// Place of 16-byte unit u (8 elements) in token j's row of a tile [32][NP]: spread over
+// the banks, for a read of one unit of 16 rows and a transposed one of two units of 4
+// rows.  (A third of the LDS's cycles are bank conflicts all the same, counted over the
+// main pass of 2 x 16384 tokens: G's reads, 16 bytes every 32, meet theirs twice.)
 template <int NP>
 constexpr __device__ __forceinline__ int unit_place(int j, int u) {
   if constexpr (NP >= 128) return u ^ ((2 * (j & 7)) | ((j >> 3) & 1));
@@ -627,7 +629,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
     const float rescale = i % 2 == 0 ? rescale_of[0] : rescale_of[1];
     // (Opaque: places of single reads and comparisons are made from these when they
     // are wanted.  Kept in registers from chunk to chunk they would spill, and a
-    // reload waits for all of the loads ahead: 283 -> 358 us.)
+    // reload waits for all of the loads ahead: a quarter more time.)
     int row_at = row_place<NP>(col, half), col_at = col_place<NP>(lane), ln = lane;
     asm volatile("" : "+v"(row_at), "+v"(col_at), "+v"(ln));
     Frag xf[KB][PL];
@@ -1030,10 +1032,11 @@ ScanPlan scan_plan(int64_t batch, int64_t tokens, int64_t max_len, int heads, in
   // Whole, a call of up to a workgroup to a CU takes a time per chunk; cut, one per chunk
   // and workgroup that comes to the same near a workgroup for each of 7/8 of the CUs, and
   // for the passes and their launches the time of 14 chunks (bf16), 8 (f16) or 6
-  // (float32).  Whole and cut, us, 24 heads x 64, N 128: bf16 2 x 512 52 and 45, 5 x 512 53
-  // and 58, 8 x 1024 96 and 88, 16 x 1024 96 and 114, 16 x 4096 352 and 305, 21 x 4096 356
-  // and 378; f16 5 x 512 79 and 63, 11 x 512 78 and 88, 11 x 1024 144 and 132, 16 x 1024 146
-  // and 163; float32 8 x 256 58 and 65, 8 x 512 104 and 92, 16 x 512 106 and 136.
+  // (float32).  Whole and cut, us, 24 heads x 64, N 128 (other shapes of a head were not
+  // measured): bf16 2 x 512 57 and 46, 5 x 512 59 and 61, 8 x 1024 104 and 94, 16 x 1024
+  // 108 and 126, 16 x 4096 390 and 366, 21 x 4096 400 and 426; f16 5 x 512 76 and 66, 11 x
+  // 512 79 and 93, 11 x 1024 145 and 133, 16 x 1024 146 and 166; float32 8 x 256 58 and 67,
+  // 8 x 512 105 and 90, 16 x 512 108 and 128.
   const int64_t fit = state_dim > 128 ? 1 : dtype == SF_BF16 ? 3 : 2;
   const int64_t passes = dtype == SF_BF16 ? 14 : dtype == SF_F16 ? 8 : 6;
   const int64_t chunks = (max_len + kChunk - 1) / kChunk, cus = num_cus();
@@ -1072,8 +1075,9 @@ int launch_scan_chunk(const ScanArgs& a, const ScanPlan& p, void* workspace, int
   sp.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums_at);
   if (dtype == SF_F32) return launch_chunk_m<float, 3, false>(a, sp, stream);
   if (dtype == SF_F16) return launch_chunk_m<__half, 2, false>(a, sp, stream);
-  // Rows of whole aligned units: straight into LDS (2 x 16384, 64 heads x 64, N 128: 480 us
-  // as a timed run of its three kernels, by way of registers 576).
+  // Rows of whole aligned units: straight into LDS (us of a call's kernels, and by way of
+  // registers: 2 x 16384, 64 heads x 64, N 128, 535 and 590, 64 x 1024, 24 heads, 245 and
+  // 290; of N up to 64 and of 256 the same within 4%).
   const int64_t strides = a.x_b | a.x_t | a.x_h | a.b_b | a.b_t | a.b_g | a.c_b | a.c_t | a.c_g;
   const bool units = strides % 8 == 0 && a.head_dim % 8 == 0 && a.state_dim % 8 == 0 && aligned_to(a.x, 16) &&
                      aligned_to(a.b, 16) && aligned_to(a.c, 16);
