@@ -21,11 +21,19 @@ from ..Kernels.selective_scan import selective_scan_forward, selective_scan_step
 from ._runtime import WeightLayout
 
 
+def _cast(param: torch.Tensor) -> torch.Tensor:
+    return param.detach().float().contiguous()
+
+
+def _decay_rates(log: torch.Tensor) -> torch.Tensor:
+    return -torch.exp(log.detach().float())
+
+
 class _Float32:
     """A parameter as the kernels take it."""
 
     def __init__(self):
-        self._cast = WeightLayout(lambda p: p.detach().float().contiguous())
+        self._cast = WeightLayout(_cast)
 
     def __call__(self, param: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         return param if param is None or (param.dtype == torch.float32 and param.is_contiguous()) else self._cast(param)
@@ -83,7 +91,7 @@ class SelectiveScan(_Stateful):
         self.A_log = nn.Parameter(torch.log(torch.empty(self.heads).uniform_(1.0, 16.0)))
         self.D = nn.Parameter(torch.ones(self.heads))
         self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
-        self._rates = WeightLayout(lambda a: -torch.exp(a.detach().float()))
+        self._rates = WeightLayout(_decay_rates)
         self._D, self._dt_bias = _Float32(), _Float32()
 
     def forward(self, x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.Tensor) -> torch.Tensor:

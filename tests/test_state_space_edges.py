@@ -2,6 +2,7 @@
 taken for others, tensors that overlap, modules in 16 bits."""
 
 import math
+import pickle
 
 import pytest
 import torch
@@ -191,3 +192,20 @@ def test_a_norms_gate_and_residual_that_do_not_broadcast_are_refused():
         got = block_norm_forward(x, gate=t, residual=t, pre_weight=w)
         want = block_norm_forward(x, gate=t.expand(3, 8).contiguous(), residual=t.expand(3, 8).contiguous(), pre_weight=w)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_modules_are_pickled(dtype):
+    torch.manual_seed(5)
+    x, dt, B = torch.randn(2, 5, 8).to(dtype), torch.randn(2, 5, 2).to(dtype), torch.randn(2, 5, 1, 3).to(dtype)
+    for m, args in ((CausalConv1d(8).to(dtype), (x,)), (SelectiveScan(2, 4, 3).to(dtype), (x.unflatten(-1, (2, 4)), dt, B, B)),
+                    (BlockNorm(8, post=True).to(dtype), (x,)), (spiking_ssm_tiny(vocab=16).to(dtype), (torch.zeros(1, 3, dtype=torch.long),))):
+        for used in (False, True):
+            again = pickle.loads(pickle.dumps(m))
+            for mod in (*m.modules(), *again.modules()):
+                if hasattr(mod, "reset"):
+                    mod.reset()
+            with torch.no_grad():
+                got, want = again(*args), m(*args)
+            got, want = (t[0] if isinstance(t, tuple) else t for t in (got, want))
+            assert torch.equal(got, want)
