@@ -182,16 +182,24 @@ __device__ __forceinline__ f32x16 mma_parts(const Frag (&a)[PA], const Frag (&b)
 // Per token of a chunk, for one head.  The state in the accumulators is 2^-K h, K
 // between 0 and kScaleMost (the range that it costs is at the small end), so that a
 // chunk's decay need not be multiplied in each time; K' is its value after the chunk.
+// (K is taken back by whole numbers, so that the state is multiplied by powers of two.)
 //            factors apart      a factor per element (wide)
 //   w        2^(L_end - L - K') d, both
-//   p        2^(L + K)          L
+//   p        2^(L + K)          L + K
 //   q        2^(-L - K) d       d
-//   r                           what L loses as one float
+//   r                           what L + K loses as one float
 struct alignas(16) ChunkScalars {
   float w[kChunk], p[kChunk], q[kChunk], r[kChunk];
 };
 constexpr double kScaleMost = 20.0, kScaleFrom = 16.0;  // (a chunk that decays nothing leaves K alone)
 constexpr float kApartMost = 100.f;  // exponents of factors apart
+
+// 2^v of an exponent of more than a float's bits: as one float it would be rounded to
+// 2^-20 of itself from 16 on.
+__device__ __forceinline__ float exp2_of(double v) {
+  const double whole = floor(v);
+  return v < -200.0 ? 0.f : __builtin_amdgcn_ldexpf(exp2_hw((float)(v - whole)), (int)fmin(whole, 200.0));
+}
 
 // The sum of v over this half wavefront's lanes up to this one.
 __device__ __forceinline__ double half_sum_up_to(double v) {
@@ -402,9 +410,9 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   const float bias = uniform(a.dt_bias != nullptr ? a.dt_bias[hd] : 0.f);
   const double A2 = uniform((double)a.A[hd] * 1.4426950408889634);  // exponents of 2
   double k_state = 0.0, l_seg = 0.0;  // (l_seg: the sum of the exponents)
-  // Of each of the two: K; what the state is multiplied by before the chunk's part
-  // comes in; whether the factors are an element's.
-  float k_of[2], rescale_of[2];
+  // Of each of the two: what the state is multiplied by before the chunk's part comes in;
+  // whether the factors are an element's.
+  float rescale_of[2];
   bool wide_of[2];
   T next_dt = from_f32<T>(0.f);
   // rest: tokens from the first of the two chunks on.
@@ -422,26 +430,26 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
     double k[3] = {k_state, 0.0, 0.0};
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      k_of[c] = uniform((float)k[c]);
       rescale_of[c] = 1.f;
       k[c + 1] = k[c] + end[c];
       if constexpr (STATES) l_seg = uniform(l_seg + end[c]);
       if (!(k[c + 1] >= 0.0 && k[c + 1] < kScaleMost)) {
-        const double to = end[c] < 0.0 ? kScaleFrom : 0.0;
-        rescale_of[c] = uniform(exp2_hw((float)(k[c + 1] - to)));
-        k[c + 1] = to;
+        const double to = end[c] < 0.0 ? kScaleFrom : 0.0, by = floor(k[c + 1] - to);
+        rescale_of[c] = uniform(exp2_of(by));
+        k[c + 1] = fabs(by) < 1e6 ? k[c + 1] - by : to;
       }
     }
     k_state = uniform(k[2]);
     ChunkScalars& sc = s_sc[half];
-    sc.w[col] = exp2_hw((float)((half == 0 ? end[0] - k[1] : end[1] - k[2]) - l)) * d;
+    sc.w[col] = exp2_of((half == 0 ? end[0] - k[1] : end[1] - k[2]) - l) * d;
     if constexpr (!STATES) {
-      float p = (float)l, q = d;
-      sc.r[col] = (float)(l - (double)p);
+      const double lk = l + (half == 0 ? k[0] : k[1]);
+      float p = (float)lk, q = d;
+      sc.r[col] = (float)(lk - (double)p);
       if constexpr (kPair) {
         wide_of[0] = wide_of[1] = true;
       } else {
-        const float off = (float)(l + (half == 0 ? k[0] : k[1])), fall = exp2_hw(-off) * d;
+        const float off = p, fall = exp2_hw(-off) * d;
         // (Also where a factor of a later token is no number: it meets zeros of G.)
         const uint64_t no = __ballot(!(fabsf(off) < kApartMost && fabsf(fall) < __builtin_huge_valf()));
         wide_of[0] = (uint32_t)no != 0u;
@@ -706,7 +714,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
       const float my_r = kPair || wide ? sc.r[ln & 31] : 0.f;
       auto factor = [&](float pj, float qj, float rj) { return exp2_hw((my_p - pj) + (my_r - rj)) * qj; };
       if (wide) {
-        const float f = exp2_hw(my_p + (i % 2 == 0 ? k_of[0] : k_of[1]));
+        const float whole = exp2_hw(my_p), f = fmaf(whole * 0.693147182f, my_r, whole);
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] *= f;
       }
@@ -901,7 +909,7 @@ __global__ __launch_bounds__(kThreads, NP == 256 ? 1 : PL > 1 || (NP == 128 && !
   else if (end.seg == end.last && ea.h1 != nullptr && end.slot >= 0) to = ea.h1 + (end.slot * ea.heads + end.hd) * plane;
   const int p_end = end.p0 + col;
   if (to != nullptr && end.on && p_end < P) {
-    const float f = exp2_hw((float)k_state);
+    const float f = exp2_of(k_state);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -218,3 +218,23 @@ def test_infinities_token_by_token(dtype, n):
         pool = h0.to(DEV)
         step = selective_scan_step(pool, *_dev(x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0]), dt_softplus=False)
         assert torch.equal(step, y[:, 0]) and torch.equal(pool, state)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,rate", [(20, -0.3), (37, -0.05), (64, -1.0), (300, -0.02), (300, -0.4), (1500, -0.1)])
+def test_states_to_a_float32s_last_bits(dtype, n, rate):
+    """A term has a handful of roundings (step, exponential, their product with x, parts,
+    sums of eight terms and of the chunks behind it), each of 2^-24 of it at most and of
+    either sign: 2^-22 of the 2-norm is four of them in a row.  (An exponent that is
+    rounded as one float costs 2^-20 from 16 on.)"""
+    announce(f"scan states to the last bits {dtype} n={n} rate={rate}")
+    H, P, G, N = 3, 32, 1, 64
+    g = _gen(66)
+    x, B, C = _randn(g, 1, n, H, P, dtype=dtype), _randn(g, 1, n, G, N, dtype=dtype), _randn(g, 1, n, G, N, dtype=dtype)
+    dt, A = (torch.rand(1, n, H, generator=g) + 0.5).to(dtype), torch.tensor([rate, rate * 1.7, rate * 0.6])
+    h0 = _randn(g, 1, H, P, N)
+    _, state = selective_scan_forward(*_dev(x, dt, A, B, C), dt_softplus=False, initial_state=h0.to(DEV))
+    _, h, _, _ = ora.scan(x[0], dt[0], A, B[0], C[0], None, None, False, h0[0])
+    for k in range(H):
+        off = float((state[0, k].double().cpu() - h[k]).norm() / h[k].norm())
+        assert off <= 2.0 ** -22, f"head {k}: 2-norm off by {off * 2 ** 22:.2f} of what is allowed"
