@@ -4,8 +4,8 @@
 //   r = residual + scale t, h = r w' / rms(r)
 // A row is held in registers by LT threads, vectors of V elements: x, gate and residual
 // are all loaded before the first sum, and h is written after the second.  Bound by
-// HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 154 us, 5.2 TB/s; 32768 x 2048
-// f16 with gate, float32 residual and h (940 MB) 182 us, 5.2 TB/s.  Short rows (up to 3
+// HBM: 32768 x 4096 bf16, gated, groups of 512 (805 MB) 157 us, 5.1 TB/s; 32768 x 2048
+// f16 with gate, float32 residual and h (940 MB) 183 us, 5.1 TB/s.  Short rows (up to 3
 // vectors a lane) are a wavefront's, whose sums need no barrier: 32768 x 384 float32 25
 // us, as a workgroup's 37; of 768 53 and 57; of four vectors, 2048 bf16, 86 and 77.
 //

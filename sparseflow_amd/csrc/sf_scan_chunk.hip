@@ -23,15 +23,15 @@
 // the time that the float32 instructions take).  So S and h are rounded to 16 bits for
 // bf16 and f16 outputs, which have 8 and 11 themselves: what y loses is its own rounding
 // (as one part for bf16, y was off by more than that where its terms cancel; 2 x 16384
-// tokens took 390 us with one and take 440).  v is split into three parts, its 24 bits,
+// tokens took 390 us with one and take 445).  v is split into three parts, its 24 bits,
 // always: the state is summed up over all tokens and stays a float32 one.  L is summed
 // in 64 bits: differences of it are exponents.
 //
 // Bound by the chain of products and the waits between them, not by memory: 2 x 16384
-// tokens, 64 heads x 64, N 128, bf16 (562 MB, 290 GFLOP of products) take 440 us, 660
+// tokens, 64 heads x 64, N 128, bf16 (562 MB, 290 GFLOP of products) take 445 us, 650
 // TFLOP/s and 1.3 TB/s; alone, the main pass 365 us, the segments' own parts 162, the
 // chain 16; rows at any address, by way of registers, as long; 23 ragged sequences of up
-// to 1500 of f16, 24 heads, 198 us.
+// to 1500 of f16, 24 heads, 199 us.
 //
 // Where products are not finite, a wavefront does its segment again, token by token:
 // infinities, NaN and results near the ends of a float's range are those of the
