@@ -536,6 +536,111 @@ int sf_block_norm(const sf_norm_desc* desc, const void* x, const void* gate,
                   const float* scale_weight, const float* pre_weight,
                   void* r_out, void* h_out, void* stream);
 
+/* ---- microscaled 4-bit operators -------------------------------------------- */
+
+/* The format.  A row of `dim` values is blocks = ceil(dim / 32) blocks of 32, the
+ * last one padded with zeros.  A block has a scale byte b = 127 + e, which stands
+ * for 2^e (255: every value is NaN), and 16 bytes of codes, two to a byte with the
+ * first in the low half: bit 3 the sign, bits 0 - 2 an index into
+ * {0, .5, 1, 1.5, 2, 3, 4, 6}.  Quantisation: with a the largest magnitude of the
+ * block e = floor(log2 a) - 2, at least -127; each x 2^-e goes to the nearest value,
+ * halfway to the even code, past 6 to 6.  A block with an infinity or NaN has the
+ * scale 255 and codes 0.  Codes are 16-byte aligned, rows follow one another. */
+
+/* x: rows (o, i) of outer x inner at o * strides[0] + i * strides[1]. */
+int sf_mx4_quantize(const void* x, int32_t dtype, int64_t outer, int64_t inner,
+                    const int64_t* strides, int64_t dim, void* codes,
+                    void* scales, void* stream);
+/* y [rows, dim] contiguous; its type's nearest values, to even. */
+int sf_mx4_dequantize(const void* codes, const void* scales, int64_t rows,
+                      int64_t dim, void* y, int32_t dtype, void* stream);
+
+/* y[m, n] = bias[n] + sum_k x[m, k] w[n, k], w [n, blocks of k] in the format; x
+ * floats, taken as they are (x_scales NULL, element (m, k) at m * x_stride + k), or in
+ * the format (x_dtype SF_X_MX4, contiguous).  bias f32 [n] or NULL; y of y_dtype at
+ * m * y_stride + n.  Products are exact, sums f32. */
+#define SF_X_MX4 3
+typedef struct sf_mx4_linear_desc {
+  int64_t m, n, k, x_stride, y_stride;
+  int32_t x_dtype, y_dtype;
+} sf_mx4_linear_desc;
+int sf_mx4_linear(const sf_mx4_linear_desc* desc, const void* x,
+                  const void* x_scales, const void* w, const void* w_scales,
+                  const float* bias, void* y, void* stream);
+
+/* A cache of keys and values in the format: codes [pages, kv_heads, page_size,
+ * blocks of head_dim * 16] and scales [pages, kv_heads, page_size, blocks], four
+ * tensors, each page page_size tokens (a power of two up to 4096); head_dim <= 256.
+ * Token t of table row r lies in page tables[r, t / page_size]; tables int32 [rows,
+ * width], lengths int32 [rows].  An entry outside 0 .. pages - 1 is no page: nothing
+ * is written there and its tokens are seen by nobody, and neither are those past the
+ * table's width.  Sequences and slots (their rows of tables and lengths) as above;
+ * sequence b's new tokens are the last of its lengths[slot].  A sequence without a
+ * row: nothing is written, y is 0. */
+typedef struct sf_mx4_cache_desc {
+  int64_t batch, tokens, max_len, rows, width, pages;
+  int64_t q_strides[3], k_strides[3], v_strides[3], y_strides[3];
+  int32_t heads, kv_heads, head_dim, page_size, dtype;
+  float scale;
+} sf_mx4_cache_desc;
+typedef struct sf_mx4_cache {
+  void *k, *k_scales, *v, *v_scales;
+  const int32_t *tables, *lengths;
+} sf_mx4_cache;
+
+/* Quantises k and v rows [tokens, kv_heads, head_dim] into the cache.  No place is
+ * named by two tokens of a call. */
+int sf_mx4_cache_append(const sf_mx4_cache_desc* desc, const sf_mx4_cache* cache,
+                        const void* k, const void* v, const int32_t* offsets,
+                        const int32_t* slots, void* stream);
+/* y = softmax(scale q k) v per query row of q [tokens, heads, head_dim], over the
+ * cached tokens up to its own (heads / kv_heads in a row share keys and values).  A
+ * query that sees no token: 0.  The workspace is 16-byte aligned. */
+size_t sf_mx4_attention_workspace_size(const sf_mx4_cache_desc* desc);
+int sf_mx4_attention(const sf_mx4_cache_desc* desc, const sf_mx4_cache* cache,
+                     const void* q, const int32_t* offsets, const int32_t* slots,
+                     void* y, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* The pages of such a cache, or of any pools [pages, ...] (contiguous; at most 16).
+ * refs int32 [pages]: how many rows of tables use a page, 0 is free.  Row r of tables
+ * int32 [rows, width] has ceil(lengths[r] / page_size) pages in front, and -1 behind.
+ * Two rows share full pages only, or pages that neither writes to.  Requests are
+ * dealt with as one: what is freed first, then free pages, the lowest first, to the
+ * requests in turn, until one cannot have what it needs; it and those behind that
+ * need pages are refused.  granted int32 [requests]: 1, or 0 for a refused request,
+ * which changes nothing; refused too: a row outside tables, a size that is negative
+ * or wider than the table, a row that an earlier request names. */
+#define SF_MAX_POOLS 16
+typedef struct sf_pages_desc {
+  int64_t pages, rows, width, requests;
+  int32_t page_size, pools;
+  void* pool[SF_MAX_POOLS];
+  int64_t page_bytes[SF_MAX_POOLS];
+} sf_pages_desc;
+size_t sf_pages_workspace_size(int64_t pages, int64_t requests);
+/* Row rows[i] to sizes[i] tokens (0: its end).  Before it grows, a partial last page
+ * that others use too is replaced by a copy. */
+int sf_pages_resize(const sf_pages_desc* desc, int32_t* refs, int32_t* tables,
+                    int32_t* lengths, const int32_t* rows, const int32_t* sizes,
+                    int32_t* granted, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/* Row children[i], which is empty, becomes what parents[i] is: it shares the full
+ * pages and has a copy of the last, partial one. */
+int sf_pages_fork(const sf_pages_desc* desc, int32_t* refs, int32_t* tables,
+                  int32_t* lengths, const int32_t* parents,
+                  const int32_t* children, int32_t* granted, void* workspace,
+                  size_t workspace_bytes, void* stream);
+/* The n pages in use become pages 0 .. n - 1: those from n on move, in order, to the
+ * free ones below; tables and refs follow.  live int32 [1]: n. */
+int sf_pages_compact(const sf_pages_desc* desc, int32_t* refs, int32_t* tables,
+                     int32_t* live, void* workspace, size_t workspace_bytes,
+                     void* stream);
+/* Page sources[i] of every pool to page targets[i]; no target is named twice or is a
+ * source too.  A pair outside the pool is left out. */
+int sf_pages_copy(const sf_pages_desc* desc, const int32_t* sources,
+                  const int32_t* targets, void* stream);
+
 /* ---- launch plans (host only) --------------------------------------------- */
 
 /* How sf_conv2d_sparse (fused_lif = 0) or sf_conv_lif_forward (1) launches the
@@ -557,7 +662,8 @@ int sf_conv2d_launch_plan(const sf_conv_desc* desc, int32_t fused_lif,
  * "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
  * "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused",
  * "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm",
- * "scan_chunk", "scan_parts").
+ * "scan_chunk", "scan_parts", "mx4_quantize", "mx4_dequantize", "mx4_linear",
+ * "mx4_append", "mx4_attention", "pages").
  * Returns the
  * number of launches recorded for that kernel. */
 int sf_timing_enable(int32_t enable);

@@ -28,6 +28,8 @@ SF_ERR_WORKSPACE = 3
 SF_ERR_HIP = 4
 
 SF_F32, SF_F16, SF_BF16 = 0, 1, 2
+SF_X_MX4 = 3
+SF_MAX_POOLS = 16
 SF_BITMAP_PIXEL_MAJOR, SF_BITMAP_PLANES = 0, 1
 _DTYPE_CODE = {torch.float32: SF_F32, torch.float16: SF_F16, torch.bfloat16: SF_BF16}
 
@@ -94,6 +96,17 @@ EXPORTS = {
     "sf_selective_scan": (c_int, [_P] * 13 + [_P, c_size_t, _P]),
     "sf_selective_scan_step": (c_int, [_P] * 12),
     "sf_block_norm": (c_int, [_P] * 10),
+    "sf_mx4_quantize": (c_int, [_P, c_int32, c_int64, c_int64, _P, c_int64, _P, _P, _P]),
+    "sf_mx4_dequantize": (c_int, [_P, _P, c_int64, c_int64, _P, c_int32, _P]),
+    "sf_mx4_linear": (c_int, [_P] * 8),
+    "sf_mx4_cache_append": (c_int, [_P] * 7),
+    "sf_mx4_attention_workspace_size": (c_size_t, [_P]),
+    "sf_mx4_attention": (c_int, [_P] * 7 + [c_size_t, _P]),
+    "sf_pages_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "sf_pages_resize": (c_int, [_P] * 8 + [c_size_t, _P]),
+    "sf_pages_fork": (c_int, [_P] * 8 + [c_size_t, _P]),
+    "sf_pages_compact": (c_int, [_P] * 5 + [c_size_t, _P]),
+    "sf_pages_copy": (c_int, [_P] * 4),
     "sf_timing_enable": (c_int, [c_int32]),
     "sf_timing_collect": (c_int, []),
     "sf_timing_query": (c_int64, [ctypes.c_char_p, ctypes.POINTER(c_double)]),
@@ -152,6 +165,36 @@ class NormDesc(ctypes.Structure):
         ("dim", c_int32), ("group_size", c_int32), ("dtype", c_int32), ("residual_dtype", c_int32),
         ("activation", c_int32), ("gate_first", c_int32),
         ("eps", c_float), ("scale", c_float),
+    ]
+
+
+class Mx4LinearDesc(ctypes.Structure):
+    _fields_ = [
+        ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x_stride", c_int64), ("y_stride", c_int64),
+        ("x_dtype", c_int32), ("y_dtype", c_int32),
+    ]
+
+
+class Mx4CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int64), ("tokens", c_int64), ("max_len", c_int64), ("rows", c_int64), ("width", c_int64),
+        ("pages", c_int64),
+        ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3), ("y_strides", c_int64 * 3),
+        ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32), ("dtype", c_int32),
+        ("scale", c_float),
+    ]
+
+
+class Mx4CacheTensors(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("k_scales", c_void_p), ("v", c_void_p), ("v_scales", c_void_p),
+                ("tables", c_void_p), ("lengths", c_void_p)]
+
+
+class PagesDesc(ctypes.Structure):
+    _fields_ = [
+        ("pages", c_int64), ("rows", c_int64), ("width", c_int64), ("requests", c_int64),
+        ("page_size", c_int32), ("pools", c_int32),
+        ("pool", c_void_p * SF_MAX_POOLS), ("page_bytes", c_int64 * SF_MAX_POOLS),
     ]
 
 
@@ -690,13 +733,132 @@ def block_norm(desc, x: torch.Tensor, gate: Optional[torch.Tensor], post_weight:
 
 
 # ---------------------------------------------------------------------------
+# Microscaled 4-bit operators and pages
+# ---------------------------------------------------------------------------
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point `name` on torch's current stream of `device`, which need not be the current device."""
+    index = device.index
+    fn = getattr(lib(), name)
+    if index == _current_device():
+        rc = fn(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, raw_stream(index))
+    _check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _pair(a: int, b: int):
+    v = (c_int64 * 2)(a, b)
+    return v, ctypes.addressof(v)
+
+
+def mx4_quantize(x: torch.Tensor, outer: int, inner: int, strides: tuple, codes: torch.Tensor,
+                 scales: torch.Tensor) -> None:
+    _launch("sf_mx4_quantize", x.device, x.data_ptr(), _DTYPE_CODE[x.dtype], outer, inner, _pair(*strides)[1], x.shape[-1],
+            codes.data_ptr(), scales.data_ptr())
+
+
+def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, rows: int, y: torch.Tensor) -> None:
+    _launch("sf_mx4_dequantize", y.device, codes.data_ptr(), scales.data_ptr(), rows, y.shape[-1], y.data_ptr(),
+            _DTYPE_CODE[y.dtype])
+
+
+@functools.lru_cache(maxsize=1024)
+def mx4_linear_desc(m: int, n: int, k: int, x_stride: int, y_stride: int, x_dtype: Optional[torch.dtype],
+                    y_dtype: torch.dtype):
+    """(the descriptor, its address); x_dtype None: x in the format."""
+    d = Mx4LinearDesc(m, n, k, x_stride, y_stride, SF_X_MX4 if x_dtype is None else dtype_code(x_dtype),
+                      dtype_code(y_dtype))
+    return d, ctypes.addressof(d)
+
+
+def mx4_linear(desc, x: torch.Tensor, x_scales: Optional[torch.Tensor], w: torch.Tensor, w_scales: torch.Tensor,
+               bias: Optional[torch.Tensor], y: torch.Tensor) -> None:
+    _launch("sf_mx4_linear", y.device, desc[1], x.data_ptr(), _raw(x_scales), w.data_ptr(), w_scales.data_ptr(), _raw(bias),
+            y.data_ptr())
+
+
+@functools.lru_cache(maxsize=1024)
+def mx4_cache_desc(batch: int, tokens: int, max_len: int, rows: int, width: int, pages: int, q_strides: tuple,
+                   k_strides: tuple, v_strides: tuple, y_strides: tuple, heads: int, kv_heads: int, head_dim: int,
+                   page_size: int, dtype: torch.dtype, scale: float):
+    """(the descriptor, its address, the bytes of workspace of an attention with it)."""
+    d = Mx4CacheDesc(batch, tokens, max_len, rows, width, pages, q_strides, k_strides, v_strides, y_strides, heads,
+                     kv_heads, head_dim, page_size, dtype_code(dtype), scale)
+    at = ctypes.addressof(d)
+    return d, at, int(lib().sf_mx4_attention_workspace_size(at))
+
+
+def _cache(cache: tuple, tables: torch.Tensor, lengths: torch.Tensor) -> Mx4CacheTensors:
+    return Mx4CacheTensors(cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(),
+                           tables.data_ptr(), lengths.data_ptr())
+
+
+def mx4_cache_append(desc, cache: tuple, tables: torch.Tensor, lengths: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     offsets: Optional[torch.Tensor], slots: Optional[torch.Tensor]) -> None:
+    c = _cache(cache, tables, lengths)
+    _launch("sf_mx4_cache_append", k.device, desc[1], ctypes.addressof(c), k.data_ptr(), v.data_ptr(), _raw(offsets),
+            _raw(slots))
+
+
+def mx4_attention(desc, cache: tuple, tables: torch.Tensor, lengths: torch.Tensor, q: torch.Tensor,
+                  offsets: Optional[torch.Tensor], slots: Optional[torch.Tensor], y: torch.Tensor,
+                  workspace: Optional[torch.Tensor]) -> None:
+    c = _cache(cache, tables, lengths)
+    _launch("sf_mx4_attention", q.device, desc[1], ctypes.addressof(c), q.data_ptr(), _raw(offsets), _raw(slots),
+            y.data_ptr(), _raw(workspace), desc[2])
+
+
+def pages_workspace_size(pages: int, requests: int) -> int:
+    return int(lib().sf_pages_workspace_size(pages, requests))
+
+
+def _pages_desc(pages: int, tables: Optional[torch.Tensor], requests: int, page_size: int, pools) -> PagesDesc:
+    d = PagesDesc(pages, 0 if tables is None else tables.shape[0], 0 if tables is None else tables.shape[1], requests,
+                  page_size, len(pools))
+    for i, t in enumerate(pools):
+        d.pool[i] = t.data_ptr()
+        d.page_bytes[i] = t.numel() // max(1, t.shape[0]) * t.element_size()
+    return d
+
+
+def pages_resize(refs, tables, lengths, rows, sizes, page_size: int, pools, granted, workspace) -> None:
+    d = _pages_desc(refs.numel(), tables, rows.numel(), page_size, pools)
+    _launch("sf_pages_resize", refs.device, ctypes.addressof(d), refs.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+            rows.data_ptr(), sizes.data_ptr(), granted.data_ptr(), workspace.data_ptr(), workspace.numel())
+
+
+def pages_fork(refs, tables, lengths, parents, children, page_size: int, pools, granted, workspace) -> None:
+    d = _pages_desc(refs.numel(), tables, parents.numel(), page_size, pools)
+    _launch("sf_pages_fork", refs.device, ctypes.addressof(d), refs.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+            parents.data_ptr(), children.data_ptr(), granted.data_ptr(), workspace.data_ptr(), workspace.numel())
+
+
+def pages_compact(refs, tables, pools, live, workspace) -> None:
+    d = _pages_desc(refs.numel(), tables, 0, 1, pools)
+    _launch("sf_pages_compact", refs.device, ctypes.addressof(d), refs.data_ptr(), tables.data_ptr(), live.data_ptr(),
+            workspace.data_ptr(), workspace.numel())
+
+
+def pages_copy(pools, sources, targets) -> None:
+    d = _pages_desc(pools[0].shape[0], None, sources.numel(), 1, pools)
+    _launch("sf_pages_copy", sources.device, ctypes.addressof(d), sources.data_ptr(), targets.data_ptr())
+
+
+# ---------------------------------------------------------------------------
 # Per-kernel timing (bench instrumentation)
 # ---------------------------------------------------------------------------
 
 KERNEL_NAMES = ("prescan_pack", "prescan_tiles", "conv_gather", "conv_lif", "conv_rows", "conv_rows_kc", "conv_flat", "conv_px3", "conv_lif_px3",
                 "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse", "spike_attention",
                 "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma", "conv_rows_fused", "conv_dense_mfma",
-                "causal_conv1d", "scan_seq", "block_norm", "scan_chunk", "scan_parts")
+                "causal_conv1d", "scan_seq", "block_norm", "scan_chunk", "scan_parts", "mx4_quantize", "mx4_dequantize",
+                "mx4_linear", "mx4_append", "mx4_attention", "pages")
 
 
 def timing_enable(on: bool) -> None:

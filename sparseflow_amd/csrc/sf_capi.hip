@@ -257,7 +257,8 @@ const char* g_names[sf::K_COUNT] = {"prescan_pack", "prescan_tiles", "conv_gathe
                                      "lif_multistep", "prescan_rows", "linear_flat", "bmm_sparse",
                                      "spike_attention", "linear_mfma", "bmm_mfma", "conv_lif_flat", "conv_mfma",
                                      "conv_rows_fused", "conv_dense_mfma", "causal_conv1d", "scan_seq", "block_norm",
-                                     "scan_chunk", "scan_parts"};
+                                     "scan_chunk", "scan_parts", "mx4_quantize", "mx4_dequantize", "mx4_linear",
+                                     "mx4_append", "mx4_attention", "pages"};
 
 }  // namespace
 
@@ -937,6 +938,303 @@ int sf_block_norm(const sf_norm_desc* d, const void* x, const void* gate, const 
   const int rc = sf::launch_block_norm(a, d->dtype, d->residual_dtype, static_cast<hipStream_t>(stream));
   if (rc != hipSuccess) return hip_fail(rc, "block_norm launch");
   return SF_OK;
+}
+
+// ---- microscaled 4-bit operators -----------------------------------------------
+
+int sf_mx4_quantize(const void* x, int32_t dtype, int64_t outer, int64_t inner, const int64_t* strides, int64_t dim,
+                    void* codes, void* scales, void* stream) {
+  if (!dtype_ok(dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (outer < 0 || inner < 0 || dim < 1) return fail(SF_ERR_INVALID, "negative rows or no columns");
+  if (outer == 0 || inner == 0) return SF_OK;
+  if (outer > (1ll << 62) / inner / dim) return fail(SF_ERR_UNSUPPORTED, "too many rows");
+  if (x == nullptr || strides == nullptr || codes == nullptr || scales == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  if (!sf::aligned_to(codes, 16)) return fail(SF_ERR_INVALID, "codes are not 16-byte aligned");
+  sf::Mx4Args a{};
+  a.x = x;
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint8_t*>(scales);
+  a.rows = outer * inner;
+  a.inner = inner;
+  a.x_o = strides[0];
+  a.x_i = strides[1];
+  a.dim = dim;
+  a.blocks = (dim + 31) / 32;
+  const int rc = sf::launch_mx4(a, dtype, false, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_mx4_quantize");
+}
+
+int sf_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t dim, void* y, int32_t dtype,
+                      void* stream) {
+  if (!dtype_ok(dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (rows < 0 || dim < 1) return fail(SF_ERR_INVALID, "negative rows or no columns");
+  if (rows == 0) return SF_OK;
+  if (rows > (1ll << 62) / dim) return fail(SF_ERR_UNSUPPORTED, "too many rows");
+  if (codes == nullptr || scales == nullptr || y == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  if (!sf::aligned_to(codes, 16)) return fail(SF_ERR_INVALID, "codes are not 16-byte aligned");
+  sf::Mx4Args a{};
+  a.x = y;
+  a.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
+  a.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  a.rows = rows;
+  a.inner = 1;
+  a.dim = dim;
+  a.blocks = (dim + 31) / 32;
+  const int rc = sf::launch_mx4(a, dtype, true, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_mx4_dequantize");
+}
+
+int sf_mx4_linear(const sf_mx4_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales,
+                  const float* bias, void* y, void* stream) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  const bool four = d->x_dtype == SF_X_MX4;
+  if ((!four && !dtype_ok(d->x_dtype)) || !dtype_ok(d->y_dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (d->m < 0 || d->n < 1 || d->k < 1) return fail(SF_ERR_INVALID, "negative rows or no columns");
+  if (d->m >= 1ll << 40 || d->n >= 1ll << 31 || d->k >= 1ll << 31) return fail(SF_ERR_UNSUPPORTED, "2^31 columns or more");
+  if (d->m == 0) return SF_OK;
+  if (x == nullptr || w == nullptr || w_scales == nullptr || y == nullptr || four != (x_scales != nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  if (!sf::aligned_to(w, 16) || (four && !sf::aligned_to(x, 16))) return fail(SF_ERR_INVALID, "codes are not 16-byte aligned");
+  sf::Mx4LinearArgs a{};
+  a.x = x;
+  a.x_scales = static_cast<const uint8_t*>(x_scales);
+  a.w = static_cast<const uint8_t*>(w);
+  a.w_scales = static_cast<const uint8_t*>(w_scales);
+  a.bias = bias;
+  a.y = y;
+  a.m = d->m;
+  a.n = d->n;
+  a.k = d->k;
+  a.x_stride = d->x_stride;
+  a.y_stride = d->y_stride;
+  a.blocks = (int)((d->k + 31) / 32);
+  a.y_dtype = d->y_dtype;
+  const int rc = sf::launch_mx4_linear(a, d->x_dtype, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_mx4_linear");
+}
+
+namespace {
+
+int check_cache_desc(const sf_mx4_cache_desc* d) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  if (d->batch < 0 || d->tokens < 0 || d->max_len < 0 || d->rows < 0 || d->width < 0 || d->pages < 0)
+    return fail(SF_ERR_INVALID, "negative size");
+  if (d->kv_heads < 1 || d->head_dim < 1 || d->heads < d->kv_heads || d->heads % d->kv_heads != 0)
+    return fail(SF_ERR_INVALID, "kv_heads does not divide heads");
+  if (!dtype_ok(d->dtype)) return fail(SF_ERR_INVALID, "unknown dtype");
+  if (d->head_dim > 256) return fail(SF_ERR_UNSUPPORTED, "head_dim > 256");
+  if (d->page_size < 1 || d->page_size > 4096 || (d->page_size & (d->page_size - 1)) != 0)
+    return fail(SF_ERR_UNSUPPORTED, "page_size is no power of two up to 4096");
+  if (d->width >= 1ll << 31 || d->pages >= 1ll << 31 || d->heads > 65536) return fail(SF_ERR_UNSUPPORTED, "2^31 pages or more");
+  if (d->batch > 0 && d->max_len > (1ll << 40) / d->batch / d->heads) return fail(SF_ERR_UNSUPPORTED, "too many rows");
+  return SF_OK;
+}
+
+int cache_view(const sf_mx4_cache_desc* d, const sf_mx4_cache* c, sf::CacheView& v) {
+  if (c == nullptr || c->tables == nullptr || c->lengths == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  if (d->pages > 0 && (c->k == nullptr || c->k_scales == nullptr || c->v == nullptr || c->v_scales == nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  if (!sf::aligned_to(c->k, 16) || !sf::aligned_to(c->v, 16)) return fail(SF_ERR_INVALID, "codes are not 16-byte aligned");
+  v.k = static_cast<uint8_t*>(c->k);
+  v.k_scales = static_cast<uint8_t*>(c->k_scales);
+  v.v = static_cast<uint8_t*>(c->v);
+  v.v_scales = static_cast<uint8_t*>(c->v_scales);
+  v.tables = c->tables;
+  v.lengths = c->lengths;
+  v.pages = d->pages;
+  v.width = d->width;
+  v.heads = d->kv_heads;
+  v.blocks = (d->head_dim + 31) / 32;
+  v.page_shift = __builtin_ctz((unsigned)d->page_size);
+  return SF_OK;
+}
+
+}  // namespace
+
+int sf_mx4_cache_append(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, const void* k, const void* v,
+                        const int32_t* offsets, const int32_t* slots, void* stream) {
+  int rc = check_cache_desc(d);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0 || d->tokens == 0 || d->max_len == 0 || d->rows == 0) return SF_OK;
+  if (k == nullptr || v == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  sf::Mx4AppendArgs a{};
+  rc = cache_view(d, cache, a.cache);
+  if (rc != SF_OK) return rc;
+  a.seq = {offsets, slots, d->batch, d->tokens, d->rows};
+  a.k = k;
+  a.v = v;
+  for (int i = 0; i < 3; ++i) {
+    a.k_strides[i] = d->k_strides[i];
+    a.v_strides[i] = d->v_strides[i];
+  }
+  if (offsets != nullptr) a.k_strides[0] = a.v_strides[0] = 0;
+  a.max_len = d->max_len < d->tokens ? d->max_len : d->tokens;
+  a.head_dim = d->head_dim;
+  rc = sf::launch_mx4_append(a, d->dtype, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_mx4_cache_append");
+}
+
+namespace {
+
+sf::Mx4AttnPlan attention_plan(const sf_mx4_cache_desc* d) {
+  return sf::mx4_attn_plan(d->batch, d->max_len < d->tokens ? d->max_len : d->tokens, d->heads, d->kv_heads,
+                           (d->head_dim + 31) / 32, d->width * d->page_size);
+}
+
+}  // namespace
+
+size_t sf_mx4_attention_workspace_size(const sf_mx4_cache_desc* d) {
+  return check_cache_desc(d) == SF_OK ? attention_plan(d).bytes : 0;
+}
+
+int sf_mx4_attention(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, const void* q, const int32_t* offsets,
+                     const int32_t* slots, void* y, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_cache_desc(d);
+  if (rc != SF_OK) return rc;
+  if (d->batch == 0 || d->tokens == 0 || d->max_len == 0) return SF_OK;
+  if (q == nullptr || y == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  sf::Mx4AttnArgs a{};
+  if (d->rows > 0) {
+    rc = cache_view(d, cache, a.cache);
+    if (rc != SF_OK) return rc;
+  } else {  // no table has a row: every y is 0
+    a.cache.heads = d->kv_heads;
+    a.cache.blocks = (d->head_dim + 31) / 32;
+  }
+  const sf::Mx4AttnPlan p = attention_plan(d);
+  if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes || !sf::aligned_to(workspace, 16)))
+    return fail(SF_ERR_WORKSPACE, "workspace is too small or not 16-byte aligned");
+  a.seq = {offsets, slots, d->batch, d->tokens, d->rows};
+  a.q = q;
+  a.y = y;
+  a.parts_o = static_cast<float*>(workspace);
+  a.parts_ml = p.bytes > 0 ? a.parts_o + p.parts * (32 * (int64_t)a.cache.blocks) : nullptr;
+  for (int i = 0; i < 3; ++i) {
+    a.q_strides[i] = d->q_strides[i];
+    a.y_strides[i] = d->y_strides[i];
+  }
+  if (offsets != nullptr) a.q_strides[0] = a.y_strides[0] = 0;
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  a.group = d->heads / d->kv_heads;
+  a.head_dim = d->head_dim;
+  a.scale = d->scale;
+  rc = sf::launch_mx4_attn(a, d->dtype, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_mx4_attention");
+}
+
+// ---- pages --------------------------------------------------------------------------
+
+namespace {
+
+int pages_args(const sf_pages_desc* d, sf::PagesArgs& a) {
+  if (d == nullptr) return fail(SF_ERR_INVALID, "desc is NULL");
+  if (d->pages < 0 || d->rows < 0 || d->width < 0 || d->requests < 0) return fail(SF_ERR_INVALID, "negative size");
+  if (d->page_size < 1) return fail(SF_ERR_INVALID, "page_size < 1");
+  if (d->pages >= 1ll << 31 || d->rows >= 1ll << 31 || d->width >= 1ll << 30 || d->requests > 1ll << 24)
+    return fail(SF_ERR_UNSUPPORTED, "too many pages, rows or requests");
+  if (d->pools < 0 || d->pools > SF_MAX_POOLS) return fail(SF_ERR_UNSUPPORTED, "more than 16 pools");
+  for (int i = 0; i < d->pools; ++i) {
+    if (d->page_bytes[i] < 0 || (d->pool[i] == nullptr && d->page_bytes[i] > 0 && d->pages > 0))
+      return fail(SF_ERR_INVALID, "NULL pointer or negative size of a pool");
+    a.pools.at[i] = static_cast<uint8_t*>(d->pool[i]);
+    a.pools.bytes[i] = d->page_bytes[i];
+  }
+  a.pools.count = d->pools;
+  a.pages = d->pages;
+  a.states = d->rows;
+  a.width = d->width;
+  a.requests = d->requests;
+  a.page_size = d->page_size;
+  return SF_OK;
+}
+
+int pages_workspace(sf::PagesArgs& a, void* workspace, size_t bytes) {
+  if (workspace == nullptr || bytes < sf_pages_workspace_size(a.pages, a.requests) || !sf::aligned_to(workspace, 16))
+    return fail(SF_ERR_WORKSPACE, "workspace is too small or not 16-byte aligned");
+  a.counts = static_cast<int32_t*>(workspace);
+  a.need = a.counts + 4;
+  a.first = a.need + a.requests;
+  a.old = a.first + a.requests;
+  a.list = a.old + a.requests;
+  a.to = a.list + a.pages;
+  return SF_OK;
+}
+
+}  // namespace
+
+size_t sf_pages_workspace_size(int64_t pages, int64_t requests) {
+  return pages < 0 || requests < 0 ? 0 : (size_t)(4 + 3 * requests + 2 * pages) * 4;
+}
+
+int sf_pages_resize(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int32_t* lengths, const int32_t* rows,
+                    const int32_t* sizes, int32_t* granted, void* workspace, size_t workspace_bytes, void* stream) {
+  sf::PagesArgs a{};
+  int rc = pages_args(d, a);
+  if (rc != SF_OK) return rc;
+  if (d->requests == 0) return SF_OK;
+  if (rows == nullptr || sizes == nullptr || granted == nullptr || (d->rows > 0 && lengths == nullptr) ||
+      (d->rows > 0 && d->width > 0 && tables == nullptr) || (d->pages > 0 && refs == nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  rc = pages_workspace(a, workspace, workspace_bytes);
+  if (rc != SF_OK) return rc;
+  a.refs = refs;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.rows = rows;
+  a.other = sizes;
+  a.granted = granted;
+  rc = sf::launch_pages_resize(a, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_pages_resize");
+}
+
+int sf_pages_fork(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int32_t* lengths, const int32_t* parents,
+                  const int32_t* children, int32_t* granted, void* workspace, size_t workspace_bytes, void* stream) {
+  sf::PagesArgs a{};
+  int rc = pages_args(d, a);
+  if (rc != SF_OK) return rc;
+  if (d->requests == 0) return SF_OK;
+  if (parents == nullptr || children == nullptr || granted == nullptr || (d->rows > 0 && lengths == nullptr) ||
+      (d->rows > 0 && d->width > 0 && tables == nullptr) || (d->pages > 0 && refs == nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  rc = pages_workspace(a, workspace, workspace_bytes);
+  if (rc != SF_OK) return rc;
+  a.refs = refs;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.rows = children;
+  a.other = parents;
+  a.granted = granted;
+  rc = sf::launch_pages_fork(a, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_pages_fork");
+}
+
+int sf_pages_compact(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int32_t* live, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  sf::PagesArgs a{};
+  int rc = pages_args(d, a);
+  if (rc != SF_OK) return rc;
+  if (live == nullptr || (d->rows > 0 && d->width > 0 && tables == nullptr) || (d->pages > 0 && refs == nullptr))
+    return fail(SF_ERR_INVALID, "NULL pointer");
+  rc = pages_workspace(a, workspace, workspace_bytes);
+  if (rc != SF_OK) return rc;
+  a.refs = refs;
+  a.tables = tables;
+  a.granted = live;
+  rc = sf::launch_pages_compact(a, static_cast<hipStream_t>(stream));
+  return rc == (int)hipSuccess ? SF_OK : hip_fail(rc, "sf_pages_compact");
+}
+
+int sf_pages_copy(const sf_pages_desc* d, const int32_t* sources, const int32_t* targets, void* stream) {
+  sf::PagesArgs a{};
+  const int rc = pages_args(d, a);
+  if (rc != SF_OK) return rc;
+  if (d->requests == 0 || d->pages == 0 || d->pools == 0) return SF_OK;
+  if (sources == nullptr || targets == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
+  a.rows = sources;
+  a.other = targets;
+  const int e = sf::launch_pages_copy(a, static_cast<hipStream_t>(stream));
+  return e == (int)hipSuccess ? SF_OK : hip_fail(e, "sf_pages_copy");
 }
 
 int sf_conv2d_forward(const sf_conv_desc* d, const void* x, const float* wt, const float* bias, float threshold,

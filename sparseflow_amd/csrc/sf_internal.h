@@ -354,6 +354,108 @@ struct NormArgs {
 constexpr int kNormMaxDim = 16384;
 int launch_block_norm(const NormArgs& a, int dtype, int res_dtype, hipStream_t stream);
 
+// Microscaled 4-bit operators (see sparseflow.h for the format).
+constexpr int SF_MX4 = 3;  // an x of the Linear in the format, beside the types of sf_dtype
+
+struct Mx4Args {
+  const void* x;  // the floats (of dequantisation the output)
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t rows, inner;  // row (o, i) = o * inner + i at o * x_o + i * x_i
+  int64_t x_o, x_i, dim;
+  int64_t blocks;  // of a row
+  int64_t block0;
+};
+int launch_mx4(const Mx4Args& a, int dtype, bool back, hipStream_t stream);
+
+struct Mx4LinearArgs {
+  const void* x;
+  const uint8_t* x_scales;  // 4-bit x
+  const uint8_t* w;
+  const uint8_t* w_scales;
+  const float* bias;
+  void* y;
+  int64_t m, n, k;
+  int64_t x_stride, y_stride;  // elements
+  int64_t n_tiles, block0;
+  int blocks, y_dtype;
+};
+int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream);
+
+// The paged cache: rows [pages, heads, page] of 16 * blocks bytes of codes and `blocks`
+// scales; the tables' rows are the states of a SeqAxis.
+struct CacheView {
+  uint8_t* k;
+  uint8_t* k_scales;
+  uint8_t* v;
+  uint8_t* v_scales;
+  const int32_t* tables;   // [states, width]
+  const int32_t* lengths;  // [states]
+  int64_t pages, width;
+  int heads, blocks, page_shift;
+};
+
+struct Mx4AppendArgs {
+  SeqAxis seq;
+  CacheView cache;
+  const void* k;
+  const void* v;
+  int64_t k_strides[3], v_strides[3];  // sequence (packed: 0), token, head
+  int64_t max_len, chunks, block0;
+  int head_dim;
+};
+int launch_mx4_append(const Mx4AppendArgs& a, int dtype, hipStream_t stream);
+
+struct Mx4AttnPlan {
+  int64_t tiles;  // of 16 query rows, of a sequence and shared head
+  int splits;     // parts of a tile's tokens
+  int64_t parts;  // rows of the workspace
+  size_t bytes;   // of it: [parts, 32 blocks] and [parts, 2] floats
+};
+Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int64_t room);
+struct Mx4AttnArgs {
+  SeqAxis seq;
+  CacheView cache;
+  const void* q;
+  void* y;
+  float* parts_o;
+  float* parts_ml;
+  int64_t q_strides[3], y_strides[3];
+  int64_t tiles, block0;
+  int splits, group, head_dim;
+  float scale;
+};
+int launch_mx4_attn(const Mx4AttnArgs& a, int dtype, hipStream_t stream);
+
+// Pages (see sparseflow.h).
+constexpr int kMaxPools = 16;
+struct PagePools {
+  uint8_t* at[kMaxPools];
+  int64_t bytes[kMaxPools];  // of a page
+  int count;
+};
+struct PagesArgs {
+  int32_t* refs;
+  int32_t* tables;
+  int32_t* lengths;
+  const int32_t* rows;   // requests: the row to resize, a fork's child
+  const int32_t* other;  // the sizes, a fork's parents
+  int32_t* granted;      // [requests]; compaction: the live pages [1]
+  int32_t* need;         // workspace: [requests] pages that a request needs, -1: refused
+  int32_t* first;        //            [requests] the first of them in `list`
+  int32_t* old;          //            [requests] the length before (a fork: the parent's)
+  int32_t* list;         //            [pages] free pages in order; compaction: sources
+  int32_t* to;           //            [pages] compaction: targets
+  int32_t* counts;       //            [2] entries of list; compaction: moves
+  int64_t pages, states, width, requests;
+  int page_size;
+  PagePools pools;
+};
+int launch_pages_resize(const PagesArgs& a, hipStream_t stream);
+int launch_pages_fork(const PagesArgs& a, hipStream_t stream);
+int launch_pages_compact(const PagesArgs& a, hipStream_t stream);
+int launch_pages_copy(const PagesArgs& a, hipStream_t stream);
+
 // Raise kernel K's dynamic-LDS ceiling to `bytes` (the default limit is
 // 64 KB) once per device and process.  Thread-safe: two first calls racing
 // set the same attribute twice, which is harmless; a failure is returned and
@@ -377,7 +479,7 @@ void conv_geometry(ConvArgs& a, bool lif);
 // Per-kernel event timing hooks used by the launchers.
 void timing_begin(int kernel_id, hipStream_t stream);
 void timing_end(int kernel_id, hipStream_t stream);
-enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_CONV1D = 20, K_SCAN_SEQ = 21, K_NORM = 22, K_SCAN_CHUNK = 23, K_SCAN_PARTS = 24, K_COUNT = 25 };
+enum KernelId { K_PACK = 0, K_TILES = 1, K_CONV = 2, K_LIF = 3, K_ROWS = 4, K_ROWS_KC = 5, K_FLAT = 6, K_PX3 = 7, K_LIF_PX3 = 8, K_LIF_MS = 9, K_PACK_ROWS = 10, K_LINEAR = 11, K_BMM = 12, K_ATTN = 13, K_LINEAR_MFMA = 14, K_BMM_MFMA = 15, K_LIF_FLAT = 16, K_MFMA_CONV = 17, K_ROWS_FUSED = 18, K_DENSE_MFMA = 19, K_CONV1D = 20, K_SCAN_SEQ = 21, K_NORM = 22, K_SCAN_CHUNK = 23, K_SCAN_PARTS = 24, K_MX4_QUANTIZE = 25, K_MX4_DEQUANTIZE = 26, K_MX4_LINEAR = 27, K_MX4_APPEND = 28, K_MX4_ATTN = 29, K_PAGES = 30, K_COUNT = 31 };
 
 // ---------------------------------------------------------------------------
 // Device helpers.

@@ -1,0 +1,444 @@
+// Attention over a paged cache in the microscaled 4-bit format, and the writing of it:
+//   y_i = sum_t softmax_t(scale q_i . k_t) v_t   over the tokens t <= the query's own
+//
+// A query row is a (token, head) pair; the heads that share keys and values lie side by
+// side, so that a tile of 16 rows is a token's heads, or several tokens'.
+#include "sf_mx4_cache.h"
+
+namespace sf {
+namespace {
+
+// ---- writing -----------------------------------------------------------------
+//
+// Four lanes to a block as in sf_mx4.hip; a workgroup's threads walk the blocks of one
+// sequence's new rows, keys and values in turn.
+constexpr int kAppendThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kAppendThreads) void k_mx4_append(Mx4AppendArgs a) {
+  const CacheView& c = a.cache;
+  const int64_t id = a.block0 + blockIdx.x;
+  const int64_t b = id / a.chunks;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int64_t slot = seq_slot(a.seq, b);
+  const int64_t per = (int64_t)c.heads * c.blocks * 2;  // blocks of a token
+  const int64_t item = (id - b * a.chunks) * (kAppendThreads / 4) + (threadIdx.x >> 2);
+  const int part = threadIdx.x & 3;
+  bool live = slot >= 0 && item < n * per;
+  float v[8];
+  int64_t row = -1;
+  int blk = 0, value = 0;
+  if (live) {
+    const int64_t i = item / per;
+    const int rest = (int)(item - i * per), hb = rest >> 1;
+    value = rest & 1;
+    const int h = hb / c.blocks;
+    blk = hb - h * c.blocks;
+    const int64_t t = (int64_t)c.lengths[slot] - n + i;
+    live = t >= 0 && t < cache_room(c);
+    if (live) {
+      row = cache_row(c, c.tables + slot * c.width, t, h);
+      live = row >= 0;
+    }
+    if (live) {
+      const int64_t* st = value ? a.v_strides : a.k_strides;
+      const T* x = reinterpret_cast<const T*>(value ? a.v : a.k) + b * st[0] + (first + i) * st[1] + (int64_t)h * st[2];
+      load8<T>(x, blk * kMx4Block + part * 8, a.head_dim, v);
+    }
+  }
+  if (!live) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+  uint32_t byte;
+  const uint32_t codes = mx4_encode(v, byte);
+  if (!live) return;
+  const int64_t at = row * c.blocks + blk;
+  reinterpret_cast<uint32_t*>(value ? c.v : c.k)[at * 4 + part] = codes;
+  if (part == 0) (value ? c.v_scales : c.k_scales)[at] = (uint8_t)byte;
+}
+
+// ---- reading: 16 query rows to a workgroup ---------------------------------------
+//
+// One pass with the running maximum and sum of the softmax.  A wavefront takes 32 tokens
+// at a time.  S = K Q^T comes from the matrix cores with a lane's column the query row and
+// its four elements four tokens, which is what the second product wants of its depth when
+// tokens are counted 4 g + i, 16 + 4 g + i; it takes V^T from LDS, where V lies as bf16, by
+// transposing loads.  K's codes go straight from memory into the operand: lane (token, g)
+// holds 8 NB columns of its token from 8 NB g, and Q's fragments are laid out the same.
+constexpr int kAttnWaves = 4;
+constexpr int kAttnTokens = 32;
+
+// log2(e): scores are kept as exponents of 2.
+constexpr float kLog2e = 1.44269504088896340736f;
+
+template <int NB>
+struct AttnLds {
+  static constexpr int stride = 32 * NB + 8;  // of V's rows, bf16 elements: 16 bytes on, another bank
+  union {
+    uint16_t v[kAttnWaves][kAttnTokens * stride];
+    float o[kAttnWaves][16][32 * NB];
+  };
+  float m[kAttnWaves][16], l[kAttnWaves][16];
+};
+
+// The 4 NB bytes of codes of a row from byte 4 NB g.
+template <int NB>
+__device__ __forceinline__ void load_codes(const uint8_t* __restrict__ row, int g, uint32_t (&c)[NB]) {
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + NB * g;
+  if constexpr (NB % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 4; ++i) {
+      const u32x4 u = reinterpret_cast<const u32x4*>(p)[i];
+      c[4 * i] = u.x, c[4 * i + 1] = u.y, c[4 * i + 2] = u.z, c[4 * i + 3] = u.w;
+    }
+  } else if constexpr (NB % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) {
+      const u32x2 u = reinterpret_cast<const u32x2*>(p)[i];
+      c[2 * i] = u.x, c[2 * i + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) c[i] = p[i];
+  }
+}
+
+__device__ __forceinline__ bf16x4v attn_transposed(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) bf16x4v Lds;
+  return __builtin_bit_cast(bf16x4v, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<uint16_t*>(p))));
+}
+
+template <typename T, int NB>
+__global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs a) {
+  constexpr int NP = Parts<T>::n;
+  constexpr int stride = AttnLds<NB>::stride;
+  __shared__ AttnLds<NB> lds;
+  const CacheView& c = a.cache;
+  const int lane = lane_id(), wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
+
+  // Which sequence, shared head, rows and part of the tokens.
+  int64_t id = a.block0 + blockIdx.x;
+  const int split = (int)(id % a.splits);
+  id /= a.splits;
+  const int64_t tile = id % a.tiles;
+  id /= a.tiles;
+  const int kvh = (int)(id % c.heads);
+  const int64_t b = id / c.heads;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int64_t slot = seq_slot(a.seq, b);
+  const int group = a.group;
+  const int64_t row0 = tile * 16, rows = n * group;
+  if (row0 >= rows) return;
+  const int64_t length = slot < 0 ? 0 : c.lengths[slot];
+  const int64_t room = cache_room(c);
+
+  // This lane's query row.
+  const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
+  const int64_t i = row / group;
+  const int head = kvh * group + (int)(row - i * group);
+  const int64_t place = slot < 0 ? -1 : length - n + i;
+  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_strides[0] + (first + i) * a.q_strides[1] + (int64_t)head * a.q_strides[2];
+  bf16x8 qf[NB][NP];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    float v[8];
+    load8<T>(q, 8 * (NB * g + j), a.head_dim, v);
+    split8<NP>(v, qf[j]);
+  }
+
+  // The keys that any of the tile's rows sees, and this part's share of them.
+  const int64_t last_row = row0 + 15 < rows - 1 ? row0 + 15 : rows - 1;
+  int64_t keys = slot < 0 ? 0 : length - n + last_row / group + 1;
+  keys = keys < 0 ? 0 : keys > room ? room : keys;
+  const int64_t chunks = (keys + kAttnTokens - 1) / kAttnTokens;
+  const int64_t begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
+  const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
+
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[2 * NB];
+#pragma unroll
+  for (int d = 0; d < 2 * NB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float c2 = a.scale * kLog2e;
+  uint16_t* vt = lds.v[wave];
+
+  for (int64_t ch = begin + wave; ch < end; ch += kAttnWaves) {
+    const int64_t t0 = ch * kAttnTokens;
+    // Keys: tokens t0 + r and t0 + 16 + r.
+    f32x4 s[2];
+    bool there[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t t = t0 + 16 * u + r;
+      const int64_t at = t < keys ? cache_row(c, table, t, kvh) : -1;
+      there[u] = at >= 0;
+      uint32_t codes[NB];
+      uint64_t scales = 0;
+      if (at >= 0) {
+        load_codes<NB>(c.k + at * (16 * NB), g, codes);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) scales |= (uint64_t)c.k_scales[at * NB + j] << (8 * j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) codes[j] = 0;
+      }
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const bf16x8 kf = mx4_bf16(codes[j], mx4_scale((uint32_t)(scales >> (8 * ((NB * g + j) >> 2))) & 255));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) s[u] = mfma16(kf, qf[j][p], s[u]);
+      }
+    }
+    // Values: block `blk` of token t, as bf16 into LDS.
+    uint32_t worst = 0;
+    wave_lds_sync();
+#pragma unroll
+    for (int u = 0; u < (NB + 1) / 2; ++u) {
+      const int at = lane + kWave * u;
+      if (NB % 2 == 0 || at < kAttnTokens * NB) {
+        const int tok = at / NB, blk = at - tok * NB;
+        const int64_t t = t0 + tok;
+        const int64_t vr = t < keys ? cache_row(c, table, t, kvh) : -1;
+        u32x4 codes = {0, 0, 0, 0};
+        uint32_t byte = 0;
+        if (vr >= 0) {
+          codes = reinterpret_cast<const u32x4*>(c.v)[vr * NB + blk];
+          byte = c.v_scales[vr * NB + blk];
+        }
+        worst = byte > worst ? byte : worst;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<bf16x8*>(vt + tok * stride + blk * 32 + 8 * j) = mx4_bf16(codes[j], mx4_scale(byte));
+      }
+    }
+    wave_lds_sync();
+
+    // Which of this lane's tokens (t0 + 16 u + 4 g + k) its row sees.
+    float top = m;
+    uint32_t seen = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint64_t have = __ballot(there[u]);  // lanes 0-15: tokens t0 + 16 u + lane
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t t = t0 + 16 * u + 4 * g + k;
+        const bool see = t <= place && ((have >> (4 * g + k)) & 1);
+        seen |= (uint32_t)see << (4 * u + k);
+        s[u][k] = see ? s[u][k] * c2 : -INFINITY;
+        top = fmaxf(top, s[u][k]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float back = exp2_hw(m - ref);  // (m = -inf: 0)
+    m = top;
+    float pr[8], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      pr[k] = exp2_hw(s[k >> 2][k & 3] - ref);
+      sum += pr[k];
+    }
+    l = l * back + sum;
+    if (__any(back != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
+    }
+    if (__any(worst >= 253)) {
+      // Values that are no numbers, or beyond a float's range: a row takes only those that it
+      // sees.
+      for (int t = 0; t < kAttnTokens; ++t) {
+        const int from = 16 * ((t & 15) >> 2) + r, k = 4 * (t >> 4) + (t & 3);
+        float p = 0.f;
+        uint32_t see = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == k) {
+            p = __shfl(pr[e], from, kWave);
+            see = __shfl(seen >> e & 1, from, kWave);
+          }
+        if (!see) continue;
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[d][e] += p * __builtin_bit_cast(float, (uint32_t)vt[t * stride + 16 * d + 4 * g + e] << 16);
+      }
+      continue;
+    }
+    bf16x8 pf[NP];
+    if constexpr (NP == 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) pf[0][k] = (__bf16)pr[k];
+    } else {
+      split8<NP>(pr, pf);
+    }
+#pragma unroll
+    for (int d = 0; d < 2 * NB; ++d) {
+      const uint16_t* at = vt + (4 * g + (r >> 2)) * stride + 16 * d + 4 * (r & 3);
+      const bf16x8 vf = __builtin_shufflevector(attn_transposed(at), attn_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+    }
+  }
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+
+  // The wavefronts' parts together.
+  __syncthreads();
+  if (g == 0) lds.m[wave][r] = m, lds.l[wave][r] = l;
+#pragma unroll
+  for (int d = 0; d < 2 * NB; ++d) *reinterpret_cast<f32x4*>(&lds.o[wave][r][16 * d + 4 * g]) = o[d];
+  __syncthreads();
+  // (Thread: row threadIdx.x / 16, columns threadIdx.x % 16 + 16 k.)
+  const int wr = threadIdx.x >> 4, wc = threadIdx.x & 15;
+  const int64_t orow = row0 + wr;
+  if (orow >= rows) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, lds.m[w][wr]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float f[kAttnWaves], total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) {
+    f[w] = exp2_hw(lds.m[w][wr] - ref);
+    total += f[w] * lds.l[w][wr];
+  }
+  if (a.splits > 1) {
+    const int64_t base = (((b * c.heads + kvh) * a.tiles + tile) * a.splits + split) * 16 + wr;
+    if (wc == 0) a.parts_ml[2 * base] = top, a.parts_ml[2 * base + 1] = total;
+#pragma unroll
+    for (int k = 0; k < 2 * NB; ++k) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAttnWaves; ++w) v += f[w] * lds.o[w][wr][16 * k + wc];
+      a.parts_o[base * (32 * NB) + 16 * k + wc] = v;
+    }
+    return;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int64_t oi = orow / group;
+  T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + oi) * a.y_strides[1] +
+         (int64_t)(kvh * group + (int)(orow - oi * group)) * a.y_strides[2];
+#pragma unroll
+  for (int k = 0; k < 2 * NB; ++k) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) v += f[w] * lds.o[w][wr][16 * k + wc];
+    if (16 * k + wc < a.head_dim) y[16 * k + wc] = from_f32<T>(total == 0.f ? 0.f : v * inv);
+  }
+}
+
+// The parts of a row's tokens together: a wavefront to a row, a lane to its columns.
+template <typename T, int NB>
+__global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
+  const CacheView& c = a.cache;
+  const int lane = lane_id();
+  const int64_t id = (a.block0 + blockIdx.x) * 4 + threadIdx.x / kWave;  // (b, kvh, tile, row of it)
+  const int64_t tile_id = id >> 4;
+  const int wr = (int)(id & 15);
+  const int64_t tile = tile_id % a.tiles, bh = tile_id / a.tiles;
+  const int kvh = (int)(bh % c.heads);
+  const int64_t b = bh / c.heads;
+  if (b >= a.seq.batch) return;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int64_t row = tile * 16 + wr;
+  if (row >= n * a.group) return;
+  const int64_t base = tile_id * a.splits * 16 + wr;
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + 16 * s)]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+  const float ref = top == -INFINITY ? 0.f : top;
+  constexpr int C = (32 * NB + kWave - 1) / kWave;
+  float total = 0.f, v[C] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = base + 16 * s;
+    const float f = exp2_hw(a.parts_ml[2 * at] - ref);
+    total += f * a.parts_ml[2 * at + 1];
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+      if (kWave * k + lane < 32 * NB) v[k] += f * a.parts_o[at * (32 * NB) + kWave * k + lane];
+  }
+  const int64_t i = row / a.group;
+  T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + i) * a.y_strides[1] +
+         (int64_t)(kvh * a.group + (int)(row - i * a.group)) * a.y_strides[2];
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+    if (kWave * k + lane < a.head_dim) y[kWave * k + lane] = from_f32<T>(total == 0.f ? 0.f : v[k] / total);
+}
+
+template <typename T, int NB>
+int launch_attn_nb(const Mx4AttnArgs& a, hipStream_t stream) {
+  const int64_t tiles = a.seq.batch * a.cache.heads * a.tiles;
+  int rc = launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.splits, [&](const Mx4AttnArgs& part, unsigned grid) {
+    k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
+  });
+  if (rc != (int)hipSuccess || a.splits == 1) return rc;
+  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * 4, [&](const Mx4AttnArgs& part, unsigned grid) {
+    k_mx4_attn_join<T, NB><<<grid, 256, 0, stream>>>(part);
+  });
+}
+
+template <typename T>
+int launch_attn(const Mx4AttnArgs& a, hipStream_t stream) {
+  switch (a.cache.blocks) {
+    case 1: return launch_attn_nb<T, 1>(a, stream);
+    case 2: return launch_attn_nb<T, 2>(a, stream);
+    case 3: return launch_attn_nb<T, 3>(a, stream);
+    case 4: return launch_attn_nb<T, 4>(a, stream);
+    case 5: return launch_attn_nb<T, 5>(a, stream);
+    case 6: return launch_attn_nb<T, 6>(a, stream);
+    case 7: return launch_attn_nb<T, 7>(a, stream);
+    default: return launch_attn_nb<T, 8>(a, stream);
+  }
+}
+
+template <typename T>
+int launch_append(Mx4AppendArgs a, hipStream_t stream) {
+  const int64_t items = a.max_len * a.cache.heads * a.cache.blocks * 2;
+  a.chunks = (items + kAppendThreads / 4 - 1) / (kAppendThreads / 4);
+  return launch_blocks(a, &Mx4AppendArgs::block0, a.seq.batch * a.chunks, [&](const Mx4AppendArgs& part, unsigned grid) {
+    k_mx4_append<T><<<grid, kAppendThreads, 0, stream>>>(part);
+  });
+}
+
+}  // namespace
+
+Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int64_t room) {
+  Mx4AttnPlan p{};
+  p.tiles = (max_len * (heads / kv_heads) + 15) / 16;
+  const int64_t items = batch * kv_heads * p.tiles;
+  // As many parts of the tokens as give every CU four workgroups, each of 256 tokens or more.
+  int64_t splits = items == 0 ? 1 : (1024 + items - 1) / items;
+  const int64_t most = (room + 255) / 256;
+  splits = splits > most ? most : splits;
+  p.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
+  p.parts = p.splits == 1 ? 0 : items * p.splits * 16;
+  p.bytes = (size_t)p.parts * (size_t)(32 * blocks + 2) * 4;
+  return p;
+}
+
+int launch_mx4_append(const Mx4AppendArgs& a, int dtype, hipStream_t stream) {
+  timing_begin(K_MX4_APPEND, stream);
+  const int rc = dtype == SF_F16    ? launch_append<__half>(a, stream)
+                 : dtype == SF_BF16 ? launch_append<__hip_bfloat16>(a, stream)
+                                    : launch_append<float>(a, stream);
+  timing_end(K_MX4_APPEND, stream);
+  return rc;
+}
+
+int launch_mx4_attn(const Mx4AttnArgs& a, int dtype, hipStream_t stream) {
+  timing_begin(K_MX4_ATTN, stream);
+  const int rc = dtype == SF_F16    ? launch_attn<__half>(a, stream)
+                 : dtype == SF_BF16 ? launch_attn<__hip_bfloat16>(a, stream)
+                                    : launch_attn<float>(a, stream);
+  timing_end(K_MX4_ATTN, stream);
+  return rc;
+}
+
+}  // namespace sf

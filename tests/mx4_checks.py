@@ -1,0 +1,136 @@
+"""Checks of the 4-bit operators against the 64-bit oracle, for a device or the host.
+
+Bounds: a product of x and a 4-bit weight is exact; a float32 sum of n terms in any order is
+off by at most n steps (2^-23 relative, for units that cut instead of rounding) of the sum of
+the terms' magnitudes; a result's rounding by half a step of its type."""
+
+import torch
+
+from oracle import mx4 as ora
+from sparseflow_amd.Kernels.cached_attention import cached_attention_forward, cached_attention_step, mx4_cache, mx4_cache_append
+from sparseflow_amd.Kernels.mx4 import mx4_dequantize, mx4_linear_forward, mx4_quantize
+
+STEP = 2.0 ** -23
+PARTS = {torch.float32: 3, torch.float16: 2, torch.bfloat16: 1}
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(y, ref, bound, what=""):
+    y = y.detach().double().cpu()
+    same = (y == ref) | (torch.isnan(y) & torch.isnan(ref))
+    err = torch.where(same, torch.zeros_like(ref), (y - ref).abs())
+    worst = (err - bound).max() if err.numel() else torch.tensor(0.0)
+    assert bool((err <= bound).all()), f"{what}: off by {float(err.max()):.3g}, {float(worst):.3g} over the bound"
+
+
+def quantize_case(dev, shape, dtype, seed=0, spread=True):
+    """Values over many magnitudes, with ties, zeros and signs."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g)
+    if spread:
+        x = x * torch.exp2(torch.randint(-12, 9, shape[:-1] + (1,), generator=g).float())
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -5.0, 6.0, 7.99, 0.0, -0.0])
+    if shape[-1] > 14 and len(shape) > 1 and shape[0] > 1:
+        x[1::3, ..., :13] = ties
+    return x.to(dtype).to(dev)
+
+
+def check_quantize(x):
+    codes, scales = mx4_quantize(x)
+    c, s = ora.quantize(x.detach().cpu())
+    assert torch.equal(scales.cpu(), s) and torch.equal(ora.unpack(codes.cpu()), c)
+    v = ora.values(codes, scales, x.shape[-1])
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        y = mx4_dequantize(codes, scales, size=x.shape[-1], dtype=dtype)
+        assert torch.equal(torch.nan_to_num(y.cpu(), nan=7.0), torch.nan_to_num(v.to(dtype), nan=7.0))
+        assert torch.equal(torch.isnan(y.cpu()), torch.isnan(v))
+
+
+def check_linear(dev, m, k, n, dtype, bias=False, four=False, out_dtype=None, seed=0, x=None):
+    g = torch.Generator().manual_seed(seed)
+    w = mx4_quantize((torch.randn(n, k, generator=g) * k ** -0.5).to(dev))
+    x = torch.randn(m, k, generator=g).to(dtype).to(dev) if x is None else x
+    b = torch.randn(n, generator=g).to(dev) if bias else None
+    given = mx4_quantize(x) if four else x
+    y = mx4_linear_forward(given, w, bias=b, dtype=out_dtype or (dtype if four else None))
+    xv = ora.values(*given, k) if four else x
+    ref, mag = ora.linear(xv, ora.values(*w, k), b)
+    terms = k * (1 if four else PARTS[dtype]) + 4
+    within(y, ref, terms * STEP * mag + half_step(y.dtype) * ref.abs(), f"{m}x{k}x{n} {dtype}")
+    return y
+
+
+def attention_case(dev, new, old, heads, kv, dim, page, dtype, packed, seed=0, spare=3):
+    """Sequences of `old` tokens before and `new` ones, appended in two calls; -> what
+    the calls need, and every sequence's keys and values as the cache holds them."""
+    g = torch.Generator().manual_seed(seed)
+    batch = len(new)
+    total = [a + b for a, b in zip(new, old)]
+    used = [-(-t // page) for t in total]
+    width = max(1, max(used)) + 1
+    pages = sum(used) + spare
+    order = torch.randperm(pages, generator=g)
+    tables = torch.full((batch, width), -1, dtype=torch.int32)
+    at = 0
+    for b, u in enumerate(used):
+        tables[b, :u] = order[at:at + u].int()
+        at += u
+    cache = mx4_cache(pages, kv, page, dim, device=dev)
+    for t in cache:
+        t.fill_(255)  # stale rows are no numbers
+    tables = tables.to(dev)
+
+    def offsets(n):
+        return torch.tensor([0] + torch.tensor(n).cumsum(0).tolist(), dtype=torch.int32, device=dev)
+
+    def rows(n, h):
+        return torch.randn(sum(n), h, dim, generator=g).to(dtype).to(dev)
+
+    k0, v0, k1, v1, q = rows(old, kv), rows(old, kv), rows(new, kv), rows(new, kv), rows(new, heads)
+    mx4_cache_append(cache, k0, v0, tables, torch.tensor(old, dtype=torch.int32, device=dev), offsets=offsets(old))
+    lengths = torch.tensor(total, dtype=torch.int32, device=dev)
+    if packed:
+        mx4_cache_append(cache, k1, v1, tables, lengths, offsets=offsets(new), max_len=max(new))
+        call = dict(q=q, offsets=offsets(new), max_len=max(new))
+    else:
+        shape = (batch, new[0])
+        mx4_cache_append(cache, k1.unflatten(0, shape), v1.unflatten(0, shape), tables, lengths)
+        call = dict(q=q.unflatten(0, shape))
+    held = []
+    for b in range(batch):
+        parts = []
+        for before, after in ((k0, k1), (v0, v1)):
+            t = torch.cat([before[sum(old[:b]):sum(old[:b + 1])], after[sum(new[:b]):sum(new[:b + 1])]])
+            parts.append(ora.values(*mx4_quantize(t.contiguous()), dim) if t.shape[0] else torch.zeros(0, kv, dim).double())
+        held.append(parts)
+    return dict(call, cache=cache, tables=tables, lengths=lengths), held, q
+
+
+def attention_bound(dtype, dim, tokens, y, mag, big):
+    """Scores are off by (parts dim + 8) steps of sum |q k| scale log2(e); the weights by that, the exponential's and a
+    16-bit weight's rounding; sums over the tokens by their number of steps; then the result's rounding."""
+    parts = PARTS[dtype]
+    score = (parts * dim + 8) * STEP * big * 1.5
+    weight = 2 * score + 8 * STEP + (half_step(torch.bfloat16) if parts == 1 else 2.0 ** -15 if parts == 2 else 0.0)
+    return mag * (weight[..., None] + (parts * tokens + 8) * 2 * STEP) + half_step(dtype) * y.abs()
+
+
+def check_attention(dev, new, old, heads, kv, dim, page, dtype, packed=True, step=False, seed=0):
+    call, held, q = attention_case(dev, new, old, heads, kv, dim, page, dtype, packed or step, seed)
+    if step:
+        y = cached_attention_step(q, call["cache"], call["tables"], call["lengths"])
+    else:
+        y = cached_attention_forward(**call)
+    y = y.reshape(-1, heads, dim)
+    first = 0
+    for b, (n, o) in enumerate(zip(new, old)):
+        see = torch.arange(n + o)[None] <= (torch.arange(n) + o)[:, None]
+        for h in range(heads):
+            k, v = (t[:, h // (heads // kv)] for t in held[b])
+            ref, mag, big = ora.attend(q[first:first + n, h], k, v, see, dim ** -0.5)
+            within(y[first:first + n, h], ref, attention_bound(dtype, dim, n + o, ref, mag, big), f"sequence {b} head {h}")
+        first += n
+    return y
