@@ -453,7 +453,7 @@ def run(s):
             return pages_fork(s["refs"], s["tables"], s["lengths"], parents, children, case["page"], pools=s["pools"])
 
         def compact(s):
-            return pages_compact(s["refs"], s["tables"], pools=s["pools"])
+            return pages_compact(s["refs"], s["tables"], pools=s["pools"])[0]
 
     if op == "fork":
         before, after = s["rows"]
