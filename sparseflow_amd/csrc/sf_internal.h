@@ -381,6 +381,8 @@ struct Mx4LinearArgs {
   int blocks, y_dtype;
 };
 int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream);
+int launch_mx4_gemm(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream);  // many rows
+bool mx4_gemm_takes_four(const Mx4LinearArgs& a);  // x in the format: whole steps of four blocks
 
 // The paged cache: rows [pages, heads, page] of 16 * blocks bytes of codes and `blocks`
 // scales; the tables' rows are the states of a SeqAxis.

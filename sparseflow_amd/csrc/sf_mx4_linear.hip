@@ -3,6 +3,8 @@
 // A weight of the format is a bf16 number, so that bf16 x goes to the matrix cores as it
 // is, f16 in two and float32 in three bf16 parts: every product is exact and the sums are
 // float32.  4-bit x goes to the scaled 4-bit instructions.
+#include <type_traits>
+
 #include "sf_mx4.h"
 
 namespace sf {
@@ -10,107 +12,185 @@ namespace {
 
 // ---- few rows: the weights are read once, straight into the matrix operands -----
 //
-// A wavefront takes 16 weight rows and 16 MT rows of x.  In a step of 128 columns lane
-// (r, g) = (lane % 16, lane / 16) holds the whole block g of weight row r, 16 bytes and one
+// A wavefront takes 16 NT weight rows and 16 MT rows of x.  In a step of 128 columns lane
+// (r, g) = (lane % 16, lane / 16) holds the whole block g of a weight row r, 16 bytes and one
 // scale, and block g of x row r: instruction j takes columns 32 g + 8 j .. + 7 of both (the
-// order of a sum's terms is free).  The wavefronts of a workgroup take steps in turn; their
-// sums meet in LDS.
-constexpr int kRowsWaves = 4;
-
+// order of a sum's terms is free).  The wavefronts of a workgroup take steps in turn, U of them
+// loaded before the first is worked on; their sums meet in LDS.
 struct Four {};  // x in the format
 
-template <typename T, int MT>
-__global__ __launch_bounds__(kRowsWaves* kWave) void k_mx4_linear_rows(Mx4LinearArgs a) {
-  constexpr bool FOUR = sizeof(T) == sizeof(Four);
-  __shared__ float sums[kRowsWaves][MT][kWave][4];
-  const int lane = lane_id(), wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
-  const int64_t tile = a.block0 + blockIdx.x, n0 = (tile % a.n_tiles) * 16, m0 = tile / a.n_tiles * (16 * MT);
-  const int64_t n = n0 + r < a.n ? n0 + r : a.n - 1;
-  const uint8_t* w = a.w + n * a.blocks * 16;
-  const uint8_t* ws = a.w_scales + n * a.blocks;
-  f32x4 acc[MT];
+template <typename T>
+struct XBlock {  // a lane's 32 values, as they lie in memory
+  Vec<T, 8> v[4];
+  // ALL: every block of the step is a whole one.
+  template <bool ALL>
+  __device__ __forceinline__ void load(const Mx4LinearArgs& a, int64_t m, int b) {
+    const T* row = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+    const int64_t k = (int64_t)b * kMx4Block;
+    if (ALL || k + kMx4Block <= a.k) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int64_t m[MT];
+      for (int j = 0; j < 4; ++j) v[j] = load_any<T, 8>(row + k + 8 * j);
+    } else {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) m[t] = m0 + 16 * t + r < a.m ? m0 + 16 * t + r : a.m - 1;
-  const int steps = (a.blocks + 3) / 4;
-  for (int s = wave; s < steps; s += kRowsWaves) {
-    const int b = 4 * s + g;
-    const bool live = b < a.blocks;
-    const u32x4 codes = live ? *reinterpret_cast<const u32x4*>(w + (int64_t)b * 16) : u32x4{0, 0, 0, 0};
-    const uint32_t byte = live ? ws[b] : 0;
-    if constexpr (FOUR) {
-      const i32x8 wa = {(int)codes.x, (int)codes.y, (int)codes.z, (int)codes.w, 0, 0, 0, 0};
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j].e[i] = k + 8 * j + i < a.k ? row[k + 8 * j + i] : from_f32<T>(0.f);
+    }
+  }
+};
+template <>
+struct XBlock<Four> {
+  u32x4 codes;
+  int byte;
+  template <bool ALL>
+  __device__ __forceinline__ void load(const Mx4LinearArgs& a, int64_t m, int b) {
+    const int64_t at = m * a.blocks + b;
+    const bool live = ALL || b < a.blocks;
+    codes = live ? reinterpret_cast<const u32x4*>(a.x)[at] : u32x4{0, 0, 0, 0};
+    byte = live ? a.x_scales[at] : 0;
+  }
+};
+
+template <typename T, int MT, int NT>
+struct RowsStep {
+  u32x4 codes[NT];
+  uint32_t byte[NT];
+  XBlock<T> x[MT];
+
+  template <bool ALL>
+  __device__ __forceinline__ void load(const Mx4LinearArgs& a, const int64_t (&wrow)[NT], const int64_t (&m)[MT], int b) {
+    const bool live = ALL || b < a.blocks;
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      codes[q] = live ? reinterpret_cast<const u32x4*>(a.w)[wrow[q] + b] : u32x4{0, 0, 0, 0};
+      byte[q] = live ? a.w_scales[wrow[q] + b] : 0;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x[t].template load<ALL>(a, m[t], b);
+  }
+
+  __device__ __forceinline__ void add(f32x4 (&acc)[MT][NT]) const {
+    if constexpr (std::is_same<T, Four>::value) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const int64_t at = m[t] * a.blocks + b;
-        const u32x4 xc = live ? reinterpret_cast<const u32x4*>(a.x)[at] : u32x4{0, 0, 0, 0};
-        const int xs = live ? a.x_scales[at] : 0;
+        const u32x4 xc = x[t].codes;
         const i32x8 xb = {(int)xc.x, (int)xc.y, (int)xc.z, (int)xc.w, 0, 0, 0, 0};
-        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[t], 4, 4, 0, (int)byte, 0, xs);
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+          const i32x8 wa = {(int)codes[q].x, (int)codes[q].y, (int)codes[q].z, (int)codes[q].w, 0, 0, 0, 0};
+          acc[t][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[t][q], 4, 4, 0, (int)byte[q], 0, x[t].byte);
+        }
       }
     } else {
       constexpr int NP = Parts<T>::n;
-      const float scale = mx4_scale(byte);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bf16x8 wa = mx4_bf16(codes[j], scale);
+        bf16x8 wa[NT];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) wa[q] = mx4_bf16(codes[q][j], mx4_scale(byte[q]));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          float v[8];
-          load8<T>(reinterpret_cast<const T*>(a.x) + m[t] * a.x_stride, (int64_t)b * kMx4Block + 8 * j, a.k, v);
           bf16x8 p[NP];
-          split8<NP>(v, p);
+          if constexpr (NP == 1) {
+            __builtin_memcpy(&p[0], &x[t].v[j], 16);
+          } else {
+            float v[8];
 #pragma unroll
-          for (int q = 0; q < NP; ++q) acc[t] = mfma16(wa, p[q], acc[t]);
+            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(x[t].v[j].e[i]);
+            split8<NP>(v, p);
+          }
+#pragma unroll
+          for (int k = 0; k < NP; ++k)
+#pragma unroll
+            for (int q = 0; q < NT; ++q) acc[t][q] = mfma16(wa[q], p[k], acc[t][q]);
         }
       }
     }
   }
+};
+
+template <typename T, int MT, int NT, int W, int U>
+__global__ __launch_bounds__(W* kWave) void k_mx4_linear_rows(Mx4LinearArgs a) {
+  __shared__ f32x4 sums[W][MT * NT][kWave];
+  const int lane = lane_id(), wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
+  const int64_t tile = a.block0 + blockIdx.x, n0 = tile % a.n_tiles * (16 * NT), m0 = tile / a.n_tiles * (16 * MT);
+  int64_t wrow[NT], m[MT];
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) wrow[q] = (n0 + 16 * q + r < a.n ? n0 + 16 * q + r : a.n - 1) * a.blocks;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t] = m0 + 16 * t + r < a.m ? m0 + 16 * t + r : a.m - 1;
+#pragma unroll
+    for (int q = 0; q < NT; ++q) acc[t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int steps = (a.blocks + 3) / 4, whole = (int)(a.k / (4 * kMx4Block));
+  int s = __builtin_amdgcn_readfirstlane(wave);
+  for (; s + W * (U - 1) < whole; s += W * U) {
+    RowsStep<T, MT, NT> e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u].template load<true>(a, wrow, m, 4 * (s + W * u) + g);
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u].add(acc);
+  }
+  for (; s < steps; s += W) {
+    RowsStep<T, MT, NT> e;
+    e.template load<false>(a, wrow, m, 4 * s + g);
+    e.add(acc);
+  }
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][t][lane][i] = acc[t][i];
+    for (int q = 0; q < NT; ++q) sums[wave][t * NT + q][lane] = acc[t][q];
   __syncthreads();
-  // Element i of lane (r, g): output n0 + 4 g + i of row m0 + 16 t + r.
-  for (int t = wave; t < MT; t += kRowsWaves) {
-    const int64_t row = m0 + 16 * t + r;
+  // Element i of lane (r, g): output n0 + 16 q + 4 g + i of row m0 + 16 t + r.
+  for (int tq = wave; tq < MT * NT; tq += W) {
+    const int64_t row = m0 + 16 * (tq / NT) + r, c = n0 + 16 * (tq % NT) + 4 * g;
     if (row >= a.m) continue;
+    f32x4 v = sums[0][tq][lane];
+#pragma unroll
+    for (int k = 1; k < W; ++k) v += sums[k][tq][lane];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t c = n0 + 4 * g + i;
-      if (c >= a.n) continue;
-      float v = a.bias == nullptr ? 0.f : a.bias[c];
-#pragma unroll
-      for (int k = 0; k < kRowsWaves; ++k) v += sums[k][t][lane][i];
-      const int64_t at = row * a.y_stride + c;
-      if (a.y_dtype == SF_F16) reinterpret_cast<__half*>(a.y)[at] = from_f32<__half>(v);
-      else if (a.y_dtype == SF_BF16) reinterpret_cast<__hip_bfloat16*>(a.y)[at] = from_f32<__hip_bfloat16>(v);
-      else reinterpret_cast<float*>(a.y)[at] = v;
+      if (c + i >= a.n) continue;
+      const float s = v[i] + (a.bias == nullptr ? 0.f : a.bias[c + i]);
+      const int64_t at = row * a.y_stride + c + i;
+      if (a.y_dtype == SF_F16) reinterpret_cast<__half*>(a.y)[at] = from_f32<__half>(s);
+      else if (a.y_dtype == SF_BF16) reinterpret_cast<__hip_bfloat16*>(a.y)[at] = from_f32<__hip_bfloat16>(s);
+      else reinterpret_cast<float*>(a.y)[at] = s;
     }
   }
 }
 
-template <typename T, int MT>
+template <typename T, int MT, int NT, int W, int U>
 int launch_rows(Mx4LinearArgs a, hipStream_t stream) {
-  a.n_tiles = (a.n + 15) / 16;
+  a.n_tiles = (a.n + 16 * NT - 1) / (16 * NT);
   const int64_t blocks = a.n_tiles * ((a.m + 16 * MT - 1) / (16 * MT));
   return launch_blocks(a, &Mx4LinearArgs::block0, blocks, [&](const Mx4LinearArgs& part, unsigned grid) {
-    k_mx4_linear_rows<T, MT><<<grid, kRowsWaves * kWave, 0, stream>>>(part);
+    k_mx4_linear_rows<T, MT, NT, W, U><<<grid, W * kWave, 0, stream>>>(part);
   });
+}
+
+// Weight rows by how many workgroups they make.
+template <typename T, int MT>
+int launch_rows_n(const Mx4LinearArgs& a, hipStream_t stream) {
+  if (a.n > 64 * 160) return launch_rows<T, MT, MT == 4 ? 2 : 4, 8, 1>(a, stream);
+  if (a.n > 32 * 160) return launch_rows<T, MT, 2, 8, 1>(a, stream);
+  return launch_rows<T, MT, 1, MT == 4 ? 8 : 16, 1>(a, stream);
 }
 
 template <typename T>
 int launch_linear(const Mx4LinearArgs& a, hipStream_t stream) {
-  return a.m <= 16 ? launch_rows<T, 1>(a, stream) : a.m <= 32 ? launch_rows<T, 2>(a, stream) : launch_rows<T, 4>(a, stream);
+  return a.m <= 16 ? launch_rows_n<T, 1>(a, stream) : a.m <= 32 ? launch_rows_n<T, 2>(a, stream) : launch_rows_n<T, 4>(a, stream);
 }
 
 }  // namespace
 
 int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   timing_begin(K_MX4_LINEAR, stream);
-  const int rc = x_dtype == SF_MX4    ? launch_linear<Four>(a, stream)
+  const bool tiles = a.m > 64 && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
+  const int rc = tiles                ? launch_mx4_gemm(a, x_dtype, stream)
+                 : x_dtype == SF_MX4  ? launch_linear<Four>(a, stream)
                  : x_dtype == SF_F16  ? launch_linear<__half>(a, stream)
                  : x_dtype == SF_BF16 ? launch_linear<__hip_bfloat16>(a, stream)
                                       : launch_linear<float>(a, stream);
