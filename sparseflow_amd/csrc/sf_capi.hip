@@ -1115,6 +1115,7 @@ int sf_mx4_attention(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, cons
   }
   if (offsets != nullptr) a.q_strides[0] = a.y_strides[0] = 0;
   a.tiles = p.tiles;
+  a.tile_rows = p.tile_rows;
   a.splits = p.splits;
   a.group = d->heads / d->kv_heads;
   a.head_dim = d->head_dim;

@@ -408,8 +408,12 @@ struct Mx4AppendArgs {
 };
 int launch_mx4_append(const Mx4AppendArgs& a, int dtype, hipStream_t stream);
 
+// Query rows of a workgroup where there are many, and up to how many of a sequence and shared
+// head it takes 16 instead.
+constexpr int kAttnTileRows = 128, kAttnFewRows = 48;
 struct Mx4AttnPlan {
-  int64_t tiles;  // of 16 query rows, of a sequence and shared head
+  int64_t tiles;  // of a sequence's and shared head's query rows
+  int tile_rows;  // 16 or kAttnTileRows
   int splits;     // parts of a tile's tokens
   int64_t parts;  // rows of the workspace
   size_t bytes;   // of it: [parts, 32 blocks] and [parts, 2] floats
@@ -424,9 +428,10 @@ struct Mx4AttnArgs {
   float* parts_ml;
   int64_t q_strides[3], y_strides[3];
   int64_t tiles, block0;
-  int splits, group, head_dim;
+  int tile_rows, splits, group, head_dim;
   float scale;
 };
+int launch_mx4_attn_tiles(const Mx4AttnArgs& a, int dtype, hipStream_t stream);
 int launch_mx4_attn(const Mx4AttnArgs& a, int dtype, hipStream_t stream);
 
 // Pages (see sparseflow.h).

@@ -3,6 +3,8 @@
 //
 // A query row is a (token, head) pair; the heads that share keys and values lie side by
 // side, so that a tile of 16 rows is a token's heads, or several tokens'.
+#include <type_traits>
+
 #include "sf_mx4_cache.h"
 
 namespace sf {
@@ -38,8 +40,9 @@ __global__ __launch_bounds__(kAppendThreads) void k_mx4_append(Mx4AppendArgs a) 
     const int64_t t = (int64_t)c.lengths[slot] - n + i;
     live = t >= 0 && t < cache_room(c);
     if (live) {
-      row = cache_row(c, c.tables + slot * c.width, t, h);
-      live = row >= 0;
+      const int32_t p = cache_page(c, c.tables + slot * c.width, t);
+      row = cache_place(c, p, h, t);
+      live = p >= 0;
     }
     if (live) {
       const int64_t* st = value ? a.v_strides : a.k_strides;
@@ -66,12 +69,10 @@ __global__ __launch_bounds__(kAppendThreads) void k_mx4_append(Mx4AppendArgs a) 
 // its four elements four tokens, which is what the second product wants of its depth when
 // tokens are counted 4 g + i, 16 + 4 g + i; it takes V^T from LDS, where V lies as bf16, by
 // transposing loads.  K's codes go straight from memory into the operand: lane (token, g)
-// holds 8 NB columns of its token from 8 NB g, and Q's fragments are laid out the same.
+// holds 8 NB columns of its token from 8 NB g, and Q's fragments are laid out the same.  The
+// next tokens' codes are loaded before these are worked on, and the pages after those.
 constexpr int kAttnWaves = 4;
 constexpr int kAttnTokens = 32;
-
-// log2(e): scores are kept as exponents of 2.
-constexpr float kLog2e = 1.44269504088896340736f;
 
 template <int NB>
 struct AttnLds {
@@ -105,10 +106,61 @@ __device__ __forceinline__ void load_codes(const uint8_t* __restrict__ row, int 
   }
 }
 
-__device__ __forceinline__ bf16x4v attn_transposed(const uint16_t* p) {
-  typedef __attribute__((address_space(3))) bf16x4v Lds;
-  return __builtin_bit_cast(bf16x4v, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<uint16_t*>(p))));
+// A row's NB scales, at any address.
+template <int NB>
+__device__ __forceinline__ uint64_t load_scales(const uint8_t* __restrict__ p) {
+  if constexpr (NB == 1) {
+    return *p;
+  } else {
+    uint64_t s = 0;
+    __builtin_memcpy(&s, p, NB);
+    return s;
+  }
 }
+
+// 32 tokens as they lie in memory: keys of tokens r and 16 + r, values as 16-byte blocks
+// lane + 64 u, block `% NB` of token `/ NB`.
+template <int NB>
+struct RawTokens {
+  static constexpr int VU = (NB + 1) / 2;
+  uint32_t k[2][NB];
+  uint64_t ks[2];
+  u32x4 v[VU];
+  uint32_t vs[VU];
+  uint32_t have;  // which tokens have a page
+
+  // pages: lane t's is token t0 + t's, or -1 (t < 32).
+  __device__ __forceinline__ void load(const CacheView& c, int64_t t0, int kvh, int32_t pages, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    have = (uint32_t)__ballot(pages >= 0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = 16 * u + r;
+      const int32_t p = __shfl(pages, t, kWave);
+      if (p >= 0) {
+        const int64_t at = cache_place(c, p, kvh, t0 + t);
+        load_codes<NB>(c.k + at * (16 * NB), g, k[u]);
+        ks[u] = load_scales<NB>(c.k_scales + at * NB);
+      } else {
+        ks[u] = 0;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) k[u][j] = 0;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
+      const int32_t p = __shfl(pages, tok & 31, kWave);
+      v[u] = u32x4{0, 0, 0, 0};
+      vs[u] = 0;
+      if (p >= 0 && (NB % 2 == 0 || at < kAttnTokens * NB)) {
+        const int64_t row = cache_place(c, p, kvh, t0 + tok);
+        v[u] = reinterpret_cast<const u32x4*>(c.v)[row * NB + blk];
+        vs[u] = c.v_scales[row * NB + blk];
+      }
+    }
+  }
+};
 
 template <typename T, int NB>
 __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs a) {
@@ -116,7 +168,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   constexpr int stride = AttnLds<NB>::stride;
   __shared__ AttnLds<NB> lds;
   const CacheView& c = a.cache;
-  const int lane = lane_id(), wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane & 15, g = lane >> 4;
 
   // Which sequence, shared head, rows and part of the tokens.
   int64_t id = a.block0 + blockIdx.x;
@@ -140,125 +192,108 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   const int64_t i = row / group;
   const int head = kvh * group + (int)(row - i * group);
   const int64_t place = slot < 0 ? -1 : length - n + i;
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_strides[0] + (first + i) * a.q_strides[1] + (int64_t)head * a.q_strides[2];
   bf16x8 qf[NB][NP];
+  {
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_strides[0] + (first + i) * a.q_strides[1] + (int64_t)head * a.q_strides[2];
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    float v[8];
-    load8<T>(q, 8 * (NB * g + j), a.head_dim, v);
-    split8<NP>(v, qf[j]);
+    for (int j = 0; j < NB; ++j) load_query<T, NP>(q, 8 * (NB * g + j), a.head_dim, a.scale, qf[j]);
   }
 
   // The keys that any of the tile's rows sees, and this part's share of them.
   const int64_t last_row = row0 + 15 < rows - 1 ? row0 + 15 : rows - 1;
   int64_t keys = slot < 0 ? 0 : length - n + last_row / group + 1;
   keys = keys < 0 ? 0 : keys > room ? room : keys;
+  const int64_t place0 = length - n + row0 / group;  // the tile's first row's
   const int64_t chunks = (keys + kAttnTokens - 1) / kAttnTokens;
   const int64_t begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
   const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
+  auto pages_at = [&](int64_t ch) {
+    const int64_t t = ch * kAttnTokens + lane;
+    return lane < kAttnTokens && ch < end && t < keys ? cache_page(c, table, t) : -1;
+  };
 
-  float m = -INFINITY, l = 0.f;
+  float ref = -INFINITY, l = 0.f;  // the running maximum, times scale and log2(e)
   f32x4 o[2 * NB];
 #pragma unroll
   for (int d = 0; d < 2 * NB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float c2 = a.scale * kLog2e;
+  const float c2 = fabsf(a.scale) * kLog2e;
   uint16_t* vt = lds.v[wave];
 
-  for (int64_t ch = begin + wave; ch < end; ch += kAttnWaves) {
+  RawTokens<NB> raw, next;
+  int64_t ch = begin + wave;
+  if (ch < end) raw.load(c, ch * kAttnTokens, kvh, pages_at(ch), lane);
+  int32_t pages = pages_at(ch + kAttnWaves);
+  for (; ch < end; ch += kAttnWaves) {
     const int64_t t0 = ch * kAttnTokens;
-    // Keys: tokens t0 + r and t0 + 16 + r.
+    if (ch + kAttnWaves < end) next.load(c, t0 + kAttnWaves * kAttnTokens, kvh, pages, lane);
+    pages = pages_at(ch + 2 * kAttnWaves);
     f32x4 s[2];
-    bool there[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t t = t0 + 16 * u + r;
-      const int64_t at = t < keys ? cache_row(c, table, t, kvh) : -1;
-      there[u] = at >= 0;
-      uint32_t codes[NB];
-      uint64_t scales = 0;
-      if (at >= 0) {
-        load_codes<NB>(c.k + at * (16 * NB), g, codes);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) scales |= (uint64_t)c.k_scales[at * NB + j] << (8 * j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) codes[j] = 0;
-      }
       s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const bf16x8 kf = mx4_bf16(codes[j], mx4_scale((uint32_t)(scales >> (8 * ((NB * g + j) >> 2))) & 255));
+        const bf16x8 kf = mx4_bf16(raw.k[u][j], mx4_scale((uint32_t)(raw.ks[u] >> (8 * ((NB * g + j) >> 2))) & 255));
 #pragma unroll
         for (int p = 0; p < NP; ++p) s[u] = mfma16(kf, qf[j][p], s[u]);
       }
     }
-    // Values: block `blk` of token t, as bf16 into LDS.
     uint32_t worst = 0;
     wave_lds_sync();
 #pragma unroll
-    for (int u = 0; u < (NB + 1) / 2; ++u) {
+    for (int u = 0; u < RawTokens<NB>::VU; ++u) {
       const int at = lane + kWave * u;
       if (NB % 2 == 0 || at < kAttnTokens * NB) {
         const int tok = at / NB, blk = at - tok * NB;
-        const int64_t t = t0 + tok;
-        const int64_t vr = t < keys ? cache_row(c, table, t, kvh) : -1;
-        u32x4 codes = {0, 0, 0, 0};
-        uint32_t byte = 0;
-        if (vr >= 0) {
-          codes = reinterpret_cast<const u32x4*>(c.v)[vr * NB + blk];
-          byte = c.v_scales[vr * NB + blk];
-        }
-        worst = byte > worst ? byte : worst;
+        worst = raw.vs[u] > worst ? raw.vs[u] : worst;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<bf16x8*>(vt + tok * stride + blk * 32 + 8 * j) = mx4_bf16(codes[j], mx4_scale(byte));
+          *reinterpret_cast<bf16x8*>(vt + tok * stride + blk * 32 + 8 * j) = mx4_bf16(raw.v[u][j], mx4_scale(raw.vs[u]));
       }
     }
     wave_lds_sync();
 
     // Which of this lane's tokens (t0 + 16 u + 4 g + k) its row sees.
-    float top = m;
-    uint32_t seen = 0;
+    uint32_t seen = 255;
+    if (t0 + kAttnTokens - 1 > place0 || raw.have != 0xffffffffu) {
+      const int64_t d = place - t0;
+      const uint32_t to = d < 0 ? 0 : d >= 31 ? 0xffffffffu : (2u << d) - 1, see = (raw.have & to) >> (4 * g);
+      seen = (see & 15) | (see >> 12 & 0xf0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint64_t have = __ballot(there[u]);  // lanes 0-15: tokens t0 + 16 u + lane
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t t = t0 + 16 * u + 4 * g + k;
-        const bool see = t <= place && ((have >> (4 * g + k)) & 1);
-        seen |= (uint32_t)see << (4 * u + k);
-        s[u][k] = see ? s[u][k] * c2 : -INFINITY;
-        top = fmaxf(top, s[u][k]);
-      }
+      for (int k = 0; k < 8; ++k) s[k >> 2][k & 3] = seen >> k & 1 ? s[k >> 2][k & 3] : -INFINITY;
     }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = fmaxf(top, __shfl_xor(top, 16, kWave));
     top = fmaxf(top, __shfl_xor(top, 32, kWave));
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float back = exp2_hw(m - ref);  // (m = -inf: 0)
-    m = top;
+    const float was = ref;
+    ref = top == -INFINITY ? was : fmaxf(was, top * c2);
+    const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
     float pr[8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      pr[k] = exp2_hw(s[k >> 2][k & 3] - ref);
+      pr[k] = exp2_hw(fmaf(s[k >> 2][k & 3], c2, -from));
+      if (seen != 255) pr[k] = seen >> k & 1 ? pr[k] : 0.f;
       sum += pr[k];
     }
-    l = l * back + sum;
-    if (__any(back != 1.f)) {
+    if (__any(ref != was)) {
+      const float back = exp2_hw(was - from);  // (-inf: 0)
+      l *= back;
 #pragma unroll
       for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
     }
+    l += sum;
     if (__any(worst >= 253)) {
       // Values that are no numbers, or beyond a float's range: a row takes only those that it
       // sees.
       for (int t = 0; t < kAttnTokens; ++t) {
-        const int from = 16 * ((t & 15) >> 2) + r, k = 4 * (t >> 4) + (t & 3);
+        const int lane_of = 16 * ((t & 15) >> 2) + r, k = 4 * (t >> 4) + (t & 3);
         float p = 0.f;
         uint32_t see = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (e == k) {
-            p = __shfl(pr[e], from, kWave);
-            see = __shfl(seen >> e & 1, from, kWave);
+            p = __shfl(pr[e], lane_of, kWave);
+            see = __shfl(seen >> e & 1, lane_of, kWave);
           }
         if (!see) continue;
 #pragma unroll
@@ -267,29 +302,25 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
           for (int e = 0; e < 4; ++e)
             o[d][e] += p * __builtin_bit_cast(float, (uint32_t)vt[t * stride + 16 * d + 4 * g + e] << 16);
       }
-      continue;
-    }
-    bf16x8 pf[NP];
-    if constexpr (NP == 1) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) pf[0][k] = (__bf16)pr[k];
     } else {
-      split8<NP>(pr, pf);
-    }
+      bf16x8 pf[NP];
+      weight_parts<NP>(pr, pf);
 #pragma unroll
-    for (int d = 0; d < 2 * NB; ++d) {
-      const uint16_t* at = vt + (4 * g + (r >> 2)) * stride + 16 * d + 4 * (r & 3);
-      const bf16x8 vf = __builtin_shufflevector(attn_transposed(at), attn_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int d = 0; d < 2 * NB; ++d) {
+        const uint16_t* at = vt + (4 * g + (r >> 2)) * stride + 16 * d + 4 * (r & 3);
+        const bf16x8 vf = __builtin_shufflevector(lds_transposed(at), lds_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+        for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+      }
     }
+    raw = next;
   }
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
 
   // The wavefronts' parts together.
   __syncthreads();
-  if (g == 0) lds.m[wave][r] = m, lds.l[wave][r] = l;
+  if (g == 0) lds.m[wave][r] = ref, lds.l[wave][r] = l;
 #pragma unroll
   for (int d = 0; d < 2 * NB; ++d) *reinterpret_cast<f32x4*>(&lds.o[wave][r][16 * d + 4 * g]) = o[d];
   __syncthreads();
@@ -300,11 +331,11 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   float top = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, lds.m[w][wr]);
-  const float ref = top == -INFINITY ? 0.f : top;
+  const float from = top == -INFINITY ? 0.f : top;
   float f[kAttnWaves], total = 0.f;
 #pragma unroll
   for (int w = 0; w < kAttnWaves; ++w) {
-    f[w] = exp2_hw(lds.m[w][wr] - ref);
+    f[w] = exp2_hw(lds.m[w][wr] - from);
     total += f[w] * lds.l[w][wr];
   }
   if (a.splits > 1) {
@@ -338,26 +369,26 @@ __global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
   const CacheView& c = a.cache;
   const int lane = lane_id();
   const int64_t id = (a.block0 + blockIdx.x) * 4 + threadIdx.x / kWave;  // (b, kvh, tile, row of it)
-  const int64_t tile_id = id >> 4;
-  const int wr = (int)(id & 15);
+  const int64_t tile_id = id / a.tile_rows;
+  const int wr = (int)(id - tile_id * a.tile_rows);
   const int64_t tile = tile_id % a.tiles, bh = tile_id / a.tiles;
   const int kvh = (int)(bh % c.heads);
   const int64_t b = bh / c.heads;
   if (b >= a.seq.batch) return;
   int64_t first, n;
   seq_rows(a.seq, b, first, n);
-  const int64_t row = tile * 16 + wr;
+  const int64_t row = tile * a.tile_rows + wr;
   if (row >= n * a.group) return;
-  const int64_t base = tile_id * a.splits * 16 + wr;
+  const int64_t base = tile_id * a.splits * a.tile_rows + wr;
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + 16 * s)]);
+  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + a.tile_rows * s)]);
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
   const float ref = top == -INFINITY ? 0.f : top;
   constexpr int C = (32 * NB + kWave - 1) / kWave;
   float total = 0.f, v[C] = {};
   for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = base + 16 * s;
+    const int64_t at = base + a.tile_rows * s;
     const float f = exp2_hw(a.parts_ml[2 * at] - ref);
     total += f * a.parts_ml[2 * at + 1];
 #pragma unroll
@@ -372,14 +403,20 @@ __global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
     if (kWave * k + lane < a.head_dim) y[kWave * k + lane] = from_f32<T>(total == 0.f ? 0.f : v[k] / total);
 }
 
+template <typename T>
+struct DType {
+  static constexpr int code = sizeof(T) == 4 ? SF_F32 : std::is_same<T, __half>::value ? SF_F16 : SF_BF16;
+};
+
 template <typename T, int NB>
 int launch_attn_nb(const Mx4AttnArgs& a, hipStream_t stream) {
   const int64_t tiles = a.seq.batch * a.cache.heads * a.tiles;
-  int rc = launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.splits, [&](const Mx4AttnArgs& part, unsigned grid) {
-    k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
-  });
+  int rc = a.tile_rows > 16 ? launch_mx4_attn_tiles(a, DType<T>::code, stream)
+                            : launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.splits, [&](const Mx4AttnArgs& part, unsigned grid) {
+                                k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
+                              });
   if (rc != (int)hipSuccess || a.splits == 1) return rc;
-  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * 4, [&](const Mx4AttnArgs& part, unsigned grid) {
+  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.tile_rows / 4, [&](const Mx4AttnArgs& part, unsigned grid) {
     k_mx4_attn_join<T, NB><<<grid, 256, 0, stream>>>(part);
   });
 }
@@ -411,14 +448,17 @@ int launch_append(Mx4AppendArgs a, hipStream_t stream) {
 
 Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int64_t room) {
   Mx4AttnPlan p{};
-  p.tiles = (max_len * (heads / kv_heads) + 15) / 16;
+  const int64_t rows = max_len * (heads / kv_heads);
+  p.tile_rows = rows <= kAttnFewRows ? 16 : kAttnTileRows;
+  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t items = batch * kv_heads * p.tiles;
-  // As many parts of the tokens as give every CU four workgroups, each of 256 tokens or more.
-  int64_t splits = items == 0 ? 1 : (1024 + items - 1) / items;
+  // As many parts of the tokens as fill the CUs, each of 256 tokens or more.
+  const int64_t want = p.tile_rows == 16 ? 1024 : 512;
+  int64_t splits = items == 0 ? 1 : want / items;
   const int64_t most = (room + 255) / 256;
   splits = splits > most ? most : splits;
   p.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
-  p.parts = p.splits == 1 ? 0 : items * p.splits * 16;
+  p.parts = p.splits == 1 ? 0 : items * p.splits * p.tile_rows;
   p.bytes = (size_t)p.parts * (size_t)(32 * blocks + 2) * 4;
   return p;
 }

@@ -1,0 +1,313 @@
+// Attention over the microscaled 4-bit cache for many query rows (see sf_mx4_attn.hip for the
+// mathematics and for few rows).
+//
+// A workgroup takes 128 rows of one sequence and shared head, a wavefront 32; C tokens at a
+// time, whose keys and values the workgroup turns into bf16 rows in LDS once for all of them,
+// while the codes after those are under way.  S = K Q^T has a lane's column the query row and
+// its sixteen elements tokens 8 (e / 4) + 4 h + e % 4 of 32, which is what the second product
+// wants of its depth when its tokens are counted like that; V^T comes by transposing loads.
+// Tiles with the most tokens begin first, and those of one sequence and shared head are a
+// multiple of their number apart: on one XCD where that is a multiple of eight.
+#include "sf_mx4_cache.h"
+
+namespace sf {
+namespace {
+
+constexpr int kTileWaves = kAttnTileRows / 32;
+constexpr int kTileThreads = kTileWaves * kWave;
+
+// Tokens at a time: a 16-byte block of keys and one of values to a thread at most, and half of
+// that where the queries' parts leave no registers for as many scores.
+constexpr int tile_tokens(int nb, int np) { return nb * np <= 4 ? 64 : 32; }
+
+template <int NB, int C>
+struct TileLds {
+  static constexpr int stride = 32 * NB + 8;  // bf16 elements: 16 bytes on, another bank
+  struct Buf {
+    uint16_t k[C][stride], v[C][stride];
+    float hidden[C];                 // -inf: no page
+    uint32_t flags[kTileWaves];      // of what each wavefront brought: 1 values that are no numbers, 2 tokens without a page
+  };
+  union {
+    Buf buf[2];
+    float o[kTileWaves][32][132];    // 128 columns at a time on their way out
+  };
+};
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <typename T, int NB>
+__global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) void k_mx4_attn_tile(Mx4AttnArgs a) {
+  constexpr int NP = Parts<T>::n, C = tile_tokens(NB, NP), U = C / 32;
+  using Lds = TileLds<NB, C>;
+  constexpr int stride = Lds::stride;
+  extern __shared__ __align__(16) char smem[];
+  Lds& lds = *reinterpret_cast<Lds*>(smem);
+  const CacheView& c = a.cache;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane & 31, h = lane >> 5;
+
+  // Which rows, sequence, shared head and part of the tokens.
+  int64_t id = a.block0 + blockIdx.x;
+  const int64_t items = a.seq.batch * c.heads, item = id % items;
+  id /= items;
+  const int split = (int)(id % a.splits);
+  const int64_t tile = a.tiles - 1 - id / a.splits;
+  const int kvh = (int)(item % c.heads);
+  const int64_t b = item / c.heads;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int64_t slot = seq_slot(a.seq, b);
+  const int group = a.group;
+  const int64_t row0 = tile * kAttnTileRows, rows = n * group;
+  if (row0 >= rows) return;
+  const int64_t length = slot < 0 ? 0 : c.lengths[slot];
+  const int64_t room = cache_room(c);
+
+  // This lane's query row.
+  const int64_t wrow0 = row0 + 32 * wave, row = wrow0 + r < rows ? wrow0 + r : rows - 1;
+  const int64_t i = row / group;
+  const int64_t place = slot < 0 ? -1 : length - n + i;
+  bf16x8 qf[2 * NB][NP];
+  {
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_strides[0] + (first + i) * a.q_strides[1] +
+                 (kvh * group + (row - i * group)) * a.q_strides[2];
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j) load_query<T, NP>(q, 16 * j + 8 * h, a.head_dim, a.scale, qf[j]);
+  }
+
+  // The keys that any of the workgroup's rows sees, this part's share of them, and up to where
+  // every row of the wavefront sees all, or one sees any.
+  auto place_of = [&](int64_t at) { return slot < 0 ? -1 : length - n + (at < rows ? at : rows - 1) / group; };
+  int64_t keys = place_of(row0 + kAttnTileRows - 1) + 1;
+  keys = keys < 0 ? 0 : keys > room ? room : keys;
+  const int64_t all = place_of(wrow0) + 1, any = place_of(wrow0 + 31) + 1;
+  const int64_t chunks = (keys + C - 1) / C, begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
+  const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
+
+  // This thread's block of the tokens that are on their way: block `blk` of token `tok`.
+  const int tok = threadIdx.x / NB, blk = threadIdx.x - tok * NB;
+  const bool mine = threadIdx.x < C * NB;
+  auto page_at = [&](int64_t ch) {
+    const int64_t t = ch * C + tok;
+    return mine && ch < end && t < keys ? cache_page(c, table, t) : -1;
+  };
+  u32x4 kc, vc;
+  uint32_t ks, vs;
+  bool there;
+  auto load = [&](int64_t ch, int32_t page) {
+    kc = vc = u32x4{0, 0, 0, 0};
+    ks = vs = 0;
+    there = page >= 0;
+    if (there) {
+      const int64_t at = cache_place(c, page, kvh, ch * C + tok) * NB + blk;
+      kc = reinterpret_cast<const u32x4*>(c.k)[at];
+      vc = reinterpret_cast<const u32x4*>(c.v)[at];
+      ks = c.k_scales[at];
+      vs = c.v_scales[at];
+    }
+  };
+  auto put = [&](int64_t ch, typename Lds::Buf& to) {
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        *reinterpret_cast<bf16x8*>(&to.k[tok][32 * blk + 8 * j]) = mx4_bf16(kc[j], mx4_scale(ks));
+        *reinterpret_cast<bf16x8*>(&to.v[tok][32 * blk + 8 * j]) = mx4_bf16(vc[j], mx4_scale(vs));
+      }
+      if (blk == 0) to.hidden[tok] = there ? 0.f : -INFINITY;
+    }
+    const bool none = mine && !there && ch * C + tok < keys;
+    const uint32_t flags = (__any(vs >= 253) ? 1 : 0) | (__any(none) ? 2 : 0);
+    if (lane == 0) to.flags[wave] = flags;
+  };
+
+  float ref = -INFINITY, l = 0.f;  // the running maximum, times scale and log2(e)
+  f32x16 o[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  const float c2 = fabsf(a.scale) * kLog2e;
+
+  int32_t page = page_at(begin);
+  load(begin, page);
+  page = page_at(begin + 1);
+  put(begin, lds.buf[begin & 1]);
+  load(begin + 1, page);
+  page = page_at(begin + 2);
+  __syncthreads();
+  for (int64_t ch = begin; ch < end; ++ch) {
+    const typename Lds::Buf& t = lds.buf[ch & 1];
+    put(ch + 1, lds.buf[~ch & 1]);
+    load(ch + 2, page);
+    page = page_at(ch + 3);
+    const int64_t t0 = ch * C;
+    if (t0 < any) {
+      f32x16 s[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2 * NB; ++j) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&t.k[32 * u + r][16 * j + 8 * h]);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) s[u] = mfma32(kf, qf[j][p], s[u]);
+        }
+      }
+      uint32_t flags = 0;
+#pragma unroll
+      for (int w = 0; w < kTileWaves; ++w) flags |= t.flags[w];
+      const bool partial = t0 + C > all || (flags & 2) != 0;
+      const int last = (int)(place - t0 < -1 ? -1 : place - t0 > C ? C : place - t0);  // the row's last token of these
+      if (partial) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+            s[u][e] = at <= last && t.hidden[at] == 0.f ? s[u][e] : -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float was = ref;
+      ref = top == -INFINITY ? was : fmaxf(was, top * c2);
+      const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float p = exp2_hw(fmaf(s[u][e], c2, -from));
+          if (partial) p = s[u][e] == -INFINITY ? 0.f : p;
+          s[u][e] = p;
+          sum += p;
+        }
+      if (__any(ref != was)) {
+        const float back = exp2_hw(was - from);  // (-inf: 0)
+        l *= back;
+#pragma unroll
+        for (int d = 0; d < NB; ++d) o[d] *= back;
+      }
+      l += sum;
+      if (flags & 1) {
+        // Values that are no numbers, or beyond a float's range: a row takes only those that it
+        // sees.
+        for (int at = 0; at < C; ++at) {
+          const int lane_of = r + 32 * (at >> 2 & 1), k = 16 * (at >> 5) + 4 * (at >> 3 & 3) + (at & 3);
+          float p = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16 * U; ++e)
+            if (e == k) p = s[e >> 4][e & 15];
+          p = __shfl(p, lane_of, kWave);
+          if (at > last || t.hidden[at] != 0.f) continue;
+#pragma unroll
+          for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[d][e] += p * __builtin_bit_cast(float, (uint32_t)t.v[at][32 * d + 8 * (e >> 2) + 4 * h + (e & 3)] << 16);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < C / 16; ++k) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = s[k >> 1][8 * (k & 1) + e];
+          bf16x8 pf[NP];
+          weight_parts<NP>(w, pf);
+          const uint16_t* at = &t.v[16 * k + 4 * h + (lane >> 2 & 3)][16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+#pragma unroll
+          for (int d = 0; d < NB; ++d) {
+            const bf16x8 vf = __builtin_shufflevector(lds_transposed(at + 32 * d), lds_transposed(at + 32 * d + 8 * stride), 0, 1,
+                                                      2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) o[d] = mfma32(vf, pf[p], o[d]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, kWave);
+
+  // Out by way of LDS, 128 columns at a time, the wavefront's own: two rows of 32 lanes x four
+  // columns an access.
+  const float inv = a.splits > 1 || l == 0.f ? 1.f : 1.f / l;
+  const int64_t base = (((b * c.heads + kvh) * a.tiles + tile) * a.splits + split) * kAttnTileRows + 32 * wave;
+  if (a.splits > 1 && h == 0 && wrow0 + r < rows) a.parts_ml[2 * (base + r)] = ref, a.parts_ml[2 * (base + r) + 1] = l;
+#pragma unroll
+  for (int d0 = 0; d0 < NB; d0 += 4) {
+    wave_lds_sync();
+#pragma unroll
+    for (int d = d0; d < NB && d < d0 + 4; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * q + e] * inv;
+        *reinterpret_cast<f32x4*>(&lds.o[wave][r][32 * (d - d0) + 8 * q + 4 * h]) = v;
+      }
+    wave_lds_sync();
+    const int col = 32 * d0 + 4 * r;
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+      const int wr = 2 * k + h;
+      const int64_t at = wrow0 + wr;
+      if (at >= rows || col >= 32 * NB) continue;
+      float v[4];
+      load_f32<float, 4>(&lds.o[wave][wr][4 * r], v);
+      if (a.splits > 1) {
+        store_f32<float, 4>(a.parts_o + (base + wr) * (32 * NB) + col, v);
+        continue;
+      }
+      const int64_t oi = at / group;
+      T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + oi) * a.y_strides[1] +
+             (kvh * group + (at - oi * group)) * a.y_strides[2] + col;
+      if (col + 4 <= a.head_dim) {
+        store_any_f32<T, 4>(y, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < a.head_dim) y[e] = from_f32<T>(v[e]);
+      }
+    }
+  }
+}
+
+template <typename T, int NB>
+int launch_tile_nb(const Mx4AttnArgs& a, hipStream_t stream) {
+  constexpr int lds = (int)sizeof(TileLds<NB, tile_tokens(NB, Parts<T>::n)>);
+  static_assert(lds <= kMaxLdsBytes, "LDS");
+  const int rc = set_lds_limit_once<k_mx4_attn_tile<T, NB>>(lds);
+  if (rc != (int)hipSuccess) return rc;
+  return launch_blocks(a, &Mx4AttnArgs::block0, a.seq.batch * a.cache.heads * a.tiles * a.splits,
+                       [&](const Mx4AttnArgs& part, unsigned grid) { k_mx4_attn_tile<T, NB><<<grid, kTileThreads, lds, stream>>>(part); });
+}
+
+template <typename T>
+int launch_tile(const Mx4AttnArgs& a, hipStream_t stream) {
+  switch (a.cache.blocks) {
+    case 1: return launch_tile_nb<T, 1>(a, stream);
+    case 2: return launch_tile_nb<T, 2>(a, stream);
+    case 3: return launch_tile_nb<T, 3>(a, stream);
+    case 4: return launch_tile_nb<T, 4>(a, stream);
+    case 5: return launch_tile_nb<T, 5>(a, stream);
+    case 6: return launch_tile_nb<T, 6>(a, stream);
+    case 7: return launch_tile_nb<T, 7>(a, stream);
+    default: return launch_tile_nb<T, 8>(a, stream);
+  }
+}
+
+}  // namespace
+
+int launch_mx4_attn_tiles(const Mx4AttnArgs& a, int dtype, hipStream_t stream) {
+  return dtype == SF_F16 ? launch_tile<__half>(a, stream) : dtype == SF_BF16 ? launch_tile<__hip_bfloat16>(a, stream) : launch_tile<float>(a, stream);
+}
+
+}  // namespace sf

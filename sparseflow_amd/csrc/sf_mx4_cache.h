@@ -6,12 +6,49 @@
 namespace sf {
 namespace {
 
-// Where a row of keys or values lies: token t of a sequence is row t % page of its page
-// table[t / page]; a page holds [heads, page] rows.  -1: no such page.
-__device__ __forceinline__ int64_t cache_row(const CacheView& c, const int32_t* __restrict__ table, int64_t t, int head) {
-  const int64_t p = table[t >> c.page_shift];
-  if (p < 0 || p >= c.pages) return -1;
-  return (((p * c.heads + head) << c.page_shift)) + (t & ((1 << c.page_shift) - 1));
+// log2(e): scores are kept as exponents of 2.
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// The page of token t, or -1.
+__device__ __forceinline__ int32_t cache_page(const CacheView& c, const int32_t* __restrict__ table, int64_t t) {
+  const int32_t p = table[t >> c.page_shift];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+// Where a head's row of keys or values lies: token t is row t % page of its page, and a page
+// holds [heads, page] rows.
+__device__ __forceinline__ int64_t cache_place(const CacheView& c, int32_t page, int head, int64_t t) {
+  return (((int64_t)page * c.heads + head) << c.page_shift) + (t & ((1 << c.page_shift) - 1));
+}
+
+// 16 lanes point at 4 rows' 16 columns of bf16, four to a row, and lane l gets column l of
+// the four rows.
+__device__ __forceinline__ bf16x4v lds_transposed(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) bf16x4v Lds;
+  return __builtin_bit_cast(bf16x4v, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(const_cast<uint16_t*>(p))));
+}
+
+// Columns k .. k + 7 of a query row as bf16 parts.  (Scores are taken with |scale|.)
+template <typename T, int NP>
+__device__ __forceinline__ void load_query(const T* __restrict__ q, int k, int head_dim, float scale, bf16x8 (&p)[NP]) {
+  float v[8];
+  load8<T>(q, k, head_dim, v);
+  if (scale < 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = -v[i];
+  }
+  split8<NP>(v, p);
+}
+
+// Softmax weights for the second product: in one part rounded (half a step, 2^-8 relative, as
+// of the values of a bf16 result), in more parts cut off.
+template <int NP>
+__device__ __forceinline__ void weight_parts(const float (&w)[8], bf16x8 (&p)[NP]) {
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[0][i] = (__bf16)w[i];
+  } else {
+    split8<NP>(w, p);
+  }
 }
 
 // The tokens that a sequence's table has room for.
