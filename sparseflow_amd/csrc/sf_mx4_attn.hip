@@ -76,7 +76,7 @@ constexpr int kAttnTokens = 32;
 
 template <int NB>
 struct AttnLds {
-  static constexpr int stride = 32 * NB + 8;  // of V's rows, bf16 elements: 16 bytes on, another bank
+  static constexpr int stride = value_stride(NB);
   union {
     uint16_t v[kAttnWaves][kAttnTokens * stride];
     float o[kAttnWaves][16][32 * NB];
@@ -128,6 +128,7 @@ struct RawTokens {
   u32x4 v[VU];
   uint32_t vs[VU];
   uint32_t have;  // which tokens have a page
+  bool far;       // some value's scale is kFarScale or more
 
   // pages: lane t's is token t0 + t's, or -1 (t < 32).
   __device__ __forceinline__ void load(const CacheView& c, int64_t t0, int kvh, int32_t pages, int lane) {
@@ -157,6 +158,24 @@ struct RawTokens {
         const int64_t row = cache_place(c, p, kvh, t0 + tok);
         v[u] = reinterpret_cast<const u32x4*>(c.v)[row * NB + blk];
         vs[u] = c.v_scales[row * NB + blk];
+      }
+    }
+  }
+
+  // The values as bf16 into LDS.
+  __device__ __forceinline__ void put(uint16_t* vt, int lane) {
+    far = false;
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
+      const bool off = vs[u] >= kFarScale;
+      far |= off;
+      const float scale = mx4_scale(off ? 0 : vs[u]);
+      if (off) v[u] = u32x4{0, 0, 0, 0};
+      if (NB % 2 == 0 || at < kAttnTokens * NB) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<bf16x8*>(vt + tok * value_stride(NB) + blk * 32 + 8 * value_unit(j, tok)) = mx4_bf16(v[u][j], scale);
       }
     }
   }
@@ -216,7 +235,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   f32x4 o[2 * NB];
 #pragma unroll
   for (int d = 0; d < 2 * NB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float c2 = fabsf(a.scale) * kLog2e;
+  const float c2 = score_factor(a.scale);
   uint16_t* vt = lds.v[wave];
 
   RawTokens<NB> raw, next;
@@ -238,19 +257,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
         for (int p = 0; p < NP; ++p) s[u] = mfma16(kf, qf[j][p], s[u]);
       }
     }
-    uint32_t worst = 0;
     wave_lds_sync();
-#pragma unroll
-    for (int u = 0; u < RawTokens<NB>::VU; ++u) {
-      const int at = lane + kWave * u;
-      if (NB % 2 == 0 || at < kAttnTokens * NB) {
-        const int tok = at / NB, blk = at - tok * NB;
-        worst = raw.vs[u] > worst ? raw.vs[u] : worst;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<bf16x8*>(vt + tok * stride + blk * 32 + 8 * j) = mx4_bf16(raw.v[u][j], mx4_scale(raw.vs[u]));
-      }
-    }
+    raw.put(vt, lane);
     wave_lds_sync();
 
     // Which of this lane's tokens (t0 + 16 u + 4 g + k) its row sees.
@@ -264,53 +272,51 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = fmaxf(top, __shfl_xor(top, 16, kWave));
-    top = fmaxf(top, __shfl_xor(top, 32, kWave));
-    const float was = ref;
-    ref = top == -INFINITY ? was : fmaxf(was, top * c2);
+    top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c2;
+    if (__any(top > ref + kRefSlack)) {
+      const float was = ref;
+      ref = fmaxf(ref, top);
+      const float back = exp2_hw(was - (ref == -INFINITY ? 0.f : ref));  // (was = -inf: 0)
+      l *= back;
+#pragma unroll
+      for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
+    }
     const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
     float pr[8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       pr[k] = exp2_hw(fmaf(s[k >> 2][k & 3], c2, -from));
-      if (seen != 255) pr[k] = seen >> k & 1 ? pr[k] : 0.f;
       sum += pr[k];
     }
-    if (__any(ref != was)) {
-      const float back = exp2_hw(was - from);  // (-inf: 0)
-      l *= back;
-#pragma unroll
-      for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
-    }
     l += sum;
-    if (__any(worst >= 253)) {
-      // Values that are no numbers, or beyond a float's range: a row takes only those that it
-      // sees.
+    bf16x8 pf[NP];
+    weight_parts<NP>(pr, pf);
+#pragma unroll
+    for (int d = 0; d < 2 * NB; ++d) {
+      const int tok = 4 * g + (r >> 2);
+      const uint16_t* at = vt + tok * stride + 32 * (d >> 1) + 8 * value_unit(2 * (d & 1) + (r >> 1 & 1), tok) + 4 * (r & 1);
+      const bf16x8 vf = __builtin_shufflevector(lds_transposed(at), lds_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+    }
+    if (__any(raw.far)) {
       for (int t = 0; t < kAttnTokens; ++t) {
+        if (!(raw.have >> t & 1)) continue;
+        const int64_t at = cache_place(c, cache_page(c, table, t0 + t), kvh, t0 + t) * NB;
         const int lane_of = 16 * ((t & 15) >> 2) + r, k = 4 * (t >> 4) + (t & 3);
         float p = 0.f;
-        uint32_t see = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e == k) {
-            p = __shfl(pr[e], lane_of, kWave);
-            see = __shfl(seen >> e & 1, lane_of, kWave);
-          }
-        if (!see) continue;
+          if (e == k) p = __shfl(pr[e], lane_of, kWave);
+        if (t0 + t > place) continue;
 #pragma unroll
-        for (int d = 0; d < 2 * NB; ++d)
+        for (int d = 0; d < 2 * NB; ++d) {
+          const uint32_t byte = c.v_scales[at + (d >> 1)];
+          if (byte < kFarScale) continue;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            o[d][e] += p * __builtin_bit_cast(float, (uint32_t)vt[t * stride + 16 * d + 4 * g + e] << 16);
-      }
-    } else {
-      bf16x8 pf[NP];
-      weight_parts<NP>(pr, pf);
-#pragma unroll
-      for (int d = 0; d < 2 * NB; ++d) {
-        const uint16_t* at = vt + (4 * g + (r >> 2)) * stride + 16 * d + 4 * (r & 3);
-        const bf16x8 vf = __builtin_shufflevector(lds_transposed(at), lds_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+            o[d][e] += p * far_value(reinterpret_cast<const uint32_t*>(c.v) + (at + (d >> 1)) * 4, byte, 16 * (d & 1) + 4 * g + e);
+        }
       }
     }
     raw = next;
@@ -363,44 +369,63 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   }
 }
 
-// The parts of a row's tokens together: a wavefront to a row, a lane to its columns.
+// The parts of a row's tokens together: a workgroup to a row, a wavefront to every fourth
+// part, a lane to its columns; four parts under way at a time.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
+  constexpr int C = (32 * NB + kWave - 1) / kWave;
+  __shared__ float sums[4][kWave * C + 1];
   const CacheView& c = a.cache;
-  const int lane = lane_id();
-  const int64_t id = (a.block0 + blockIdx.x) * 4 + threadIdx.x / kWave;  // (b, kvh, tile, row of it)
+  const int lane = lane_id(), wave = threadIdx.x / kWave;
+  const int64_t id = a.block0 + blockIdx.x;  // (b, kvh, tile, row of it)
   const int64_t tile_id = id / a.tile_rows;
   const int wr = (int)(id - tile_id * a.tile_rows);
   const int64_t tile = tile_id % a.tiles, bh = tile_id / a.tiles;
   const int kvh = (int)(bh % c.heads);
   const int64_t b = bh / c.heads;
-  if (b >= a.seq.batch) return;
   int64_t first, n;
   seq_rows(a.seq, b, first, n);
   const int64_t row = tile * a.tile_rows + wr;
   if (row >= n * a.group) return;
   const int64_t base = tile_id * a.splits * a.tile_rows + wr;
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + a.tile_rows * s)]);
+  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + (int64_t)a.tile_rows * s)]);
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
-  const float ref = top == -INFINITY ? 0.f : top;
-  constexpr int C = (32 * NB + kWave - 1) / kWave;
+  const float from = top == -INFINITY ? 0.f : top;
   float total = 0.f, v[C] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = base + a.tile_rows * s;
-    const float f = exp2_hw(a.parts_ml[2 * at] - ref);
-    total += f * a.parts_ml[2 * at + 1];
+  for (int s0 = wave; s0 < a.splits; s0 += 16) {
+    float f[4], q[4], p[4][C];
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (kWave * k + lane < 32 * NB) v[k] += f * a.parts_o[at * (32 * NB) + kWave * k + lane];
+    for (int k = 0; k < 4; ++k) {
+      const bool in = s0 + 4 * k < a.splits;
+      const int64_t at = base + (int64_t)a.tile_rows * (in ? s0 + 4 * k : s0);
+      f[k] = in ? a.parts_ml[2 * at] : -INFINITY;
+      q[k] = a.parts_ml[2 * at + 1];
+#pragma unroll
+      for (int e = 0; e < C; ++e) p[k][e] = kWave * e + lane < 32 * NB ? a.parts_o[at * (32 * NB) + kWave * e + lane] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (f[k] == -INFINITY) continue;  // (nothing seen there)
+      const float g = exp2_hw(f[k] - from);
+      total += g * q[k];
+#pragma unroll
+      for (int e = 0; e < C; ++e) v[e] += g * p[k][e];
+    }
   }
+#pragma unroll
+  for (int e = 0; e < C; ++e) sums[wave][kWave * e + lane] = v[e];
+  if (lane == 0) sums[wave][kWave * C] = total;
+  __syncthreads();
   const int64_t i = row / a.group;
   T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + i) * a.y_strides[1] +
          (int64_t)(kvh * a.group + (int)(row - i * a.group)) * a.y_strides[2];
-#pragma unroll
-  for (int k = 0; k < C; ++k)
-    if (kWave * k + lane < a.head_dim) y[kWave * k + lane] = from_f32<T>(total == 0.f ? 0.f : v[k] / total);
+  total = (sums[0][kWave * C] + sums[1][kWave * C]) + (sums[2][kWave * C] + sums[3][kWave * C]);
+  for (int k = threadIdx.x; k < a.head_dim; k += 256) {
+    const float w = (sums[0][k] + sums[1][k]) + (sums[2][k] + sums[3][k]);
+    y[k] = from_f32<T>(total == 0.f ? 0.f : w / total);
+  }
 }
 
 template <typename T>
@@ -416,7 +441,7 @@ int launch_attn_nb(const Mx4AttnArgs& a, hipStream_t stream) {
                                 k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
                               });
   if (rc != (int)hipSuccess || a.splits == 1) return rc;
-  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.tile_rows / 4, [&](const Mx4AttnArgs& part, unsigned grid) {
+  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.tile_rows, [&](const Mx4AttnArgs& part, unsigned grid) {
     k_mx4_attn_join<T, NB><<<grid, 256, 0, stream>>>(part);
   });
 }

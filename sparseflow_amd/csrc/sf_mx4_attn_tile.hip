@@ -22,11 +22,12 @@ constexpr int tile_tokens(int nb, int np) { return nb * np <= 4 ? 64 : 32; }
 
 template <int NB, int C>
 struct TileLds {
-  static constexpr int stride = 32 * NB + 8;  // bf16 elements: 16 bytes on, another bank
+  static constexpr int stride = value_stride(NB);
   struct Buf {
-    uint16_t k[C][stride], v[C][stride];
-    float hidden[C];                 // -inf: no page
-    uint32_t flags[kTileWaves];      // of what each wavefront brought: 1 values that are no numbers, 2 tokens without a page
+    uint16_t k[C][32 * NB + 8];   // bf16 rows: 16 bytes on, another bank
+    uint16_t v[C][stride];
+    uint32_t there[C];            // whether the token has a page
+    uint32_t flags[kTileWaves];   // of what each wavefront brought: 1 values from kFarScale on, 2 tokens without a page
   };
   union {
     Buf buf[2];
@@ -109,16 +110,20 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
     }
   };
   auto put = [&](int64_t ch, typename Lds::Buf& to) {
+    const bool far = vs >= kFarScale;
+    if (far) {
+      vc = u32x4{0, 0, 0, 0};
+      vs = 0;
+    }
     if (mine) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         *reinterpret_cast<bf16x8*>(&to.k[tok][32 * blk + 8 * j]) = mx4_bf16(kc[j], mx4_scale(ks));
-        *reinterpret_cast<bf16x8*>(&to.v[tok][32 * blk + 8 * j]) = mx4_bf16(vc[j], mx4_scale(vs));
+        *reinterpret_cast<bf16x8*>(&to.v[tok][32 * blk + 8 * value_unit(j, tok)]) = mx4_bf16(vc[j], mx4_scale(vs));
       }
-      if (blk == 0) to.hidden[tok] = there ? 0.f : -INFINITY;
+      if (blk == 0) to.there[tok] = there;
     }
-    const bool none = mine && !there && ch * C + tok < keys;
-    const uint32_t flags = (__any(vs >= 253) ? 1 : 0) | (__any(none) ? 2 : 0);
+    const uint32_t flags = (__any(far) ? 1 : 0) | (__any(mine && !there && ch * C + tok < keys) ? 2 : 0);
     if (lane == 0) to.flags[wave] = flags;
   };
 
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
   for (int d = 0; d < NB; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-  const float c2 = fabsf(a.scale) * kLog2e;
+  const float c2 = score_factor(a.scale);
 
   int32_t page = page_at(begin);
   load(begin, page);
@@ -159,75 +164,80 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
       uint32_t flags = 0;
 #pragma unroll
       for (int w = 0; w < kTileWaves; ++w) flags |= t.flags[w];
-      const bool partial = t0 + C > all || (flags & 2) != 0;
+      flags = __builtin_amdgcn_readfirstlane(flags);
       const int last = (int)(place - t0 < -1 ? -1 : place - t0 > C ? C : place - t0);  // the row's last token of these
-      if (partial) {
+      if (t0 + C > all || (flags & 2) != 0) {
+        uint64_t see = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+        if (flags & 2) {
+          for (int at = 0; at < C; ++at)
+            if (!t.there[at]) see &= ~(1ull << at);
+        }
+        see >>= 4 * h;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int at = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-            s[u][e] = at <= last && t.hidden[at] == 0.f ? s[u][e] : -INFINITY;
-          }
+          for (int e = 0; e < 16; ++e)
+            s[u][e] = (uint32_t)(see >> (32 * u)) >> (8 * (e >> 2) + (e & 3)) & 1 ? s[u][e] : -INFINITY;
       }
       float top = s[0][0];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float was = ref;
-      ref = top == -INFINITY ? was : fmaxf(was, top * c2);
-      const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float p = exp2_hw(fmaf(s[u][e], c2, -from));
-          if (partial) p = s[u][e] == -INFINITY ? 0.f : p;
-          s[u][e] = p;
-          sum += p;
-        }
-      if (__any(ref != was)) {
-        const float back = exp2_hw(was - from);  // (-inf: 0)
+      top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c2;
+      if (__any(top > ref + kRefSlack)) {
+        const float was = ref;
+        ref = fmaxf(ref, top);
+        const float back = exp2_hw(was - (ref == -INFINITY ? 0.f : ref));  // (was = -inf: 0)
         l *= back;
 #pragma unroll
         for (int d = 0; d < NB; ++d) o[d] *= back;
       }
-      l += sum;
+      const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[u][e] = exp2_hw(fmaf(s[u][e], c2, -from));
+          sum[e & 3] += s[u][e];
+        }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int k = 0; k < C / 16; ++k) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = s[k >> 1][8 * (k & 1) + e];
+        bf16x8 pf[NP];
+        weight_parts<NP>(w, pf);
+        const int tk = 4 * h + (lane >> 2 & 3), unit = value_unit(2 * (lane >> 4 & 1) + (lane >> 1 & 1), tk);
+        const uint16_t* at = &t.v[16 * k + tk][8 * unit + 4 * (lane & 1)];
+#pragma unroll
+        for (int d = 0; d < NB; ++d) {
+          const bf16x8 vf = __builtin_shufflevector(lds_transposed(at + 32 * d), lds_transposed(at + 32 * d + 8 * stride), 0, 1, 2,
+                                                    3, 4, 5, 6, 7);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) o[d] = mfma32(vf, pf[p], o[d]);
+        }
+      }
       if (flags & 1) {
-        // Values that are no numbers, or beyond a float's range: a row takes only those that it
-        // sees.
-        for (int at = 0; at < C; ++at) {
+        for (int at = 0; at < C && t0 + at < keys; ++at) {
+          if (!t.there[at]) continue;
+          const int64_t place_of_it = cache_place(c, cache_page(c, table, t0 + at), kvh, t0 + at) * NB;
           const int lane_of = r + 32 * (at >> 2 & 1), k = 16 * (at >> 5) + 4 * (at >> 3 & 3) + (at & 3);
           float p = 0.f;
 #pragma unroll
           for (int e = 0; e < 16 * U; ++e)
             if (e == k) p = s[e >> 4][e & 15];
           p = __shfl(p, lane_of, kWave);
-          if (at > last || t.hidden[at] != 0.f) continue;
-#pragma unroll
-          for (int d = 0; d < NB; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              o[d][e] += p * __builtin_bit_cast(float, (uint32_t)t.v[at][32 * d + 8 * (e >> 2) + 4 * h + (e & 3)] << 16);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < C / 16; ++k) {
-          float w[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = s[k >> 1][8 * (k & 1) + e];
-          bf16x8 pf[NP];
-          weight_parts<NP>(w, pf);
-          const uint16_t* at = &t.v[16 * k + 4 * h + (lane >> 2 & 3)][16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+          if (at > last) continue;
 #pragma unroll
           for (int d = 0; d < NB; ++d) {
-            const bf16x8 vf = __builtin_shufflevector(lds_transposed(at + 32 * d), lds_transposed(at + 32 * d + 8 * stride), 0, 1,
-                                                      2, 3, 4, 5, 6, 7);
+            const uint32_t byte = c.v_scales[place_of_it + d];
+            if (byte < kFarScale) continue;
 #pragma unroll
-            for (int p = 0; p < NP; ++p) o[d] = mfma32(vf, pf[p], o[d]);
+            for (int e = 0; e < 16; ++e)
+              o[d][e] += p * far_value(reinterpret_cast<const uint32_t*>(c.v) + (place_of_it + d) * 4, byte, 8 * (e >> 2) + 4 * h + (e & 3));
           }
         }
       }

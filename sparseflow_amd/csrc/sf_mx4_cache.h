@@ -39,16 +39,42 @@ __device__ __forceinline__ void load_query(const T* __restrict__ q, int k, int h
   split8<NP>(v, p);
 }
 
+// V's rows in LDS as bf16: an odd number of 64-byte blocks to a row, and the 16-byte units of a
+// block (32 columns) changed about by the token, so that what the transposing loads and the
+// stores touch at once lies in different banks.
+constexpr int value_stride(int nb) { return 32 * (nb | 1); }  // bf16 elements
+__device__ __forceinline__ int value_unit(int unit, int tok) { return unit ^ (tok & 3) ^ (tok >> 1 & 2); }
+
 // Softmax weights for the second product: in one part rounded (half a step, 2^-8 relative, as
 // of the values of a bf16 result), in more parts cut off.
 template <int NP>
 __device__ __forceinline__ void weight_parts(const float (&w)[8], bf16x8 (&p)[NP]) {
   if constexpr (NP == 1) {
+    u32x4 u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[0][i] = (__bf16)w[i];
+    for (int i = 0; i < 4; ++i)
+      u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{w[2 * i], w[2 * i + 1]}), bf16x2));
+    p[0] = __builtin_bit_cast(bf16x8, u);
   } else {
     split8<NP>(w, p);
   }
+}
+
+// The factor of a score that makes it an exponent of 2.  (Where scale is 0, so little that
+// it is nothing: what is hidden, -infinity, has to stay that.)
+__device__ __forceinline__ float score_factor(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1e-44f); }
+
+// The running maximum of a row's exponents is `ref`; it moves only where it would be passed by
+// more than this, so that the sums are seldom rescaled: weights stay below 2^8.
+constexpr float kRefSlack = 8.f;
+
+// Values from scale 253 on are no numbers or beyond a float's range at times, and 0 times such
+// a one is no 0: they lie in LDS as zeros, and each row adds those that it sees itself.  Column
+// `col` of a block with its codes and scale:
+constexpr uint32_t kFarScale = 253;
+__device__ __forceinline__ float far_value(const uint32_t* codes, uint32_t byte, int col) {
+  const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[col >> 3] >> (4 * (col & 7)) & 15, mx4_scale(byte), 0);
+  return v.x;
 }
 
 // The tokens that a sequence's table has room for.

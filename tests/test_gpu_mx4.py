@@ -9,7 +9,7 @@ from sparseflow_amd.Kernels.cached_attention import MX4Cache, cached_attention_f
 from sparseflow_amd.Kernels.mx4 import mx4_dequantize, mx4_linear_forward, mx4_quantize
 from sparseflow_amd.Kernels.pages import pages_compact, pages_copy, pages_fork, pages_resize
 from tests.gpu_helpers import DEV, announce, native_loaded
-from tests.mx4_checks import attention_case, check_attention, check_linear, check_quantize, half_step, quantize_case, within
+from tests.mx4_checks import attention_bound, attention_case, check_attention, check_linear, check_quantize, half_step, quantize_case, within
 from tests.pages_checks import check_random_calls, start
 
 pytestmark = pytest.mark.gpu
@@ -395,3 +395,15 @@ def test_other_stream_and_two_at_once():
                 got.append(cached_attention_step(q, call["cache"], call["tables"], call["lengths"]))
     torch.cuda.synchronize()
     assert all(torch.equal(y, base) for y in got)
+
+
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 5.0])
+def test_attention_scales(n, scale):
+    """Any scale: 0 weighs every token alike, a negative one turns the order about, a large one picks one token."""
+    call, held, q = attention_case(DEV, [n], [45], 2, 1, 64, 16, torch.float32, False)
+    y = cached_attention_forward(**call, scale=scale)[0]
+    for h in range(2):
+        see = torch.arange(n + 45)[None] <= (torch.arange(n) + 45)[:, None]
+        ref, mag, big = ora.attend(q[:, h], held[0][0][:, 0], held[0][1][:, 0], see, scale)
+        within(y[:, h], ref, attention_bound(torch.float32, 64, n + 45, ref, mag, big), f"scale {scale}")
