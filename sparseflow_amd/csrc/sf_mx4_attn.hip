@@ -84,10 +84,10 @@ struct AttnLds {
   float m[kAttnWaves][16], l[kAttnWaves][16];
 };
 
-// The 4 NB bytes of codes of a row from byte 4 NB g.
+// 4 NB bytes of codes.
 template <int NB>
-__device__ __forceinline__ void load_codes(const uint8_t* __restrict__ row, int g, uint32_t (&c)[NB]) {
-  const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + NB * g;
+__device__ __forceinline__ void load_codes(const uint8_t* __restrict__ from, uint32_t (&c)[NB]) {
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(from);
   if constexpr (NB % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < NB / 4; ++i) {
@@ -138,27 +138,18 @@ struct RawTokens {
     for (int u = 0; u < 2; ++u) {
       const int t = 16 * u + r;
       const int32_t p = __shfl(pages, t, kWave);
-      if (p >= 0) {
-        const int64_t at = cache_place(c, p, kvh, t0 + t);
-        load_codes<NB>(c.k + at * (16 * NB), g, k[u]);
-        ks[u] = load_scales<NB>(c.k_scales + at * NB);
-      } else {
-        ks[u] = 0;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) k[u][j] = 0;
-      }
+      const int64_t at = cache_place(c, p, kvh, t0 + t);
+      load_codes<NB>(token_or_none(p >= 0, c.k + at * (16 * NB) + 4 * NB * g), k[u]);
+      ks[u] = load_scales<NB>(token_or_none(p >= 0, c.k_scales + at * NB));
     }
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
       const int32_t p = __shfl(pages, tok & 31, kWave);
-      v[u] = u32x4{0, 0, 0, 0};
-      vs[u] = 0;
-      if (p >= 0 && (NB % 2 == 0 || at < kAttnTokens * NB)) {
-        const int64_t row = cache_place(c, p, kvh, t0 + tok);
-        v[u] = reinterpret_cast<const u32x4*>(c.v)[row * NB + blk];
-        vs[u] = c.v_scales[row * NB + blk];
-      }
+      const bool there = p >= 0 && (NB % 2 == 0 || at < kAttnTokens * NB);
+      const int64_t row = cache_place(c, p, kvh, t0 + tok) * NB + blk;
+      v[u] = *token_or_none(there, reinterpret_cast<const u32x4*>(c.v) + row);
+      vs[u] = *token_or_none(there, c.v_scales + row);
     }
   }
 
@@ -182,7 +173,7 @@ struct RawTokens {
 };
 
 template <typename T, int NB>
-__global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs a) {
+__global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) void k_mx4_attn_rows(Mx4AttnArgs a) {
   constexpr int NP = Parts<T>::n;
   constexpr int stride = AttnLds<NB>::stride;
   __shared__ AttnLds<NB> lds;
@@ -227,8 +218,9 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   const int64_t begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
   const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
   auto pages_at = [&](int64_t ch) {
-    const int64_t t = ch * kAttnTokens + lane;
-    return lane < kAttnTokens && ch < end && t < keys ? cache_page(c, table, t) : -1;
+    const int64_t t = ch * kAttnTokens + (lane & 31);
+    const int32_t p = cache_page(c, table, t < keys ? t : keys - 1);
+    return ch < end && t < keys ? p : -1;
   };
 
   float ref = -INFINITY, l = 0.f;  // the running maximum, times scale and log2(e)
@@ -238,14 +230,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
   const float c2 = score_factor(a.scale);
   uint16_t* vt = lds.v[wave];
 
-  RawTokens<NB> raw, next;
-  int64_t ch = begin + wave;
-  if (ch < end) raw.load(c, ch * kAttnTokens, kvh, pages_at(ch), lane);
-  int32_t pages = pages_at(ch + kAttnWaves);
-  for (; ch < end; ch += kAttnWaves) {
-    const int64_t t0 = ch * kAttnTokens;
-    if (ch + kAttnWaves < end) next.load(c, t0 + kAttnWaves * kAttnTokens, kvh, pages, lane);
-    pages = pages_at(ch + 2 * kAttnWaves);
+  auto work = [&](int64_t t0, RawTokens<NB>& raw) {
     f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -319,7 +304,26 @@ __global__ __launch_bounds__(kAttnWaves* kWave) void k_mx4_attn_rows(Mx4AttnArgs
         }
       }
     }
-    raw = next;
+  };
+
+  // (The pages first: loads come back in order, and those of the tokens need not be waited for
+  // when the pages are needed.)
+  RawTokens<NB> raw[2];
+  int64_t ch = begin + wave;
+  if (ch < end) {
+    int32_t pages = pages_at(ch), after = pages_at(ch + kAttnWaves);
+    raw[0].load(c, ch * kAttnTokens, kvh, pages, lane);
+    for (; ch < end; ch += 2 * kAttnWaves) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t at = ch + u * kAttnWaves;
+        if (at >= end) break;
+        pages = after;
+        after = pages_at(at + 2 * kAttnWaves);
+        raw[1 - u].load(c, (at + kAttnWaves) * kAttnTokens, kvh, pages, lane);
+        work(at * kAttnTokens, raw[u]);
+      }
+    }
   }
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);

@@ -92,22 +92,19 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
   const bool mine = threadIdx.x < C * NB;
   auto page_at = [&](int64_t ch) {
     const int64_t t = ch * C + tok;
-    return mine && ch < end && t < keys ? cache_page(c, table, t) : -1;
+    const int32_t p = cache_page(c, table, t < keys ? t : keys - 1);
+    return mine && ch < end && t < keys ? p : -1;
   };
   u32x4 kc, vc;
   uint32_t ks, vs;
   bool there;
   auto load = [&](int64_t ch, int32_t page) {
-    kc = vc = u32x4{0, 0, 0, 0};
-    ks = vs = 0;
     there = page >= 0;
-    if (there) {
-      const int64_t at = cache_place(c, page, kvh, ch * C + tok) * NB + blk;
-      kc = reinterpret_cast<const u32x4*>(c.k)[at];
-      vc = reinterpret_cast<const u32x4*>(c.v)[at];
-      ks = c.k_scales[at];
-      vs = c.v_scales[at];
-    }
+    const int64_t at = cache_place(c, page, kvh, ch * C + tok) * NB + blk;
+    kc = *token_or_none(there, reinterpret_cast<const u32x4*>(c.k) + at);
+    vc = *token_or_none(there, reinterpret_cast<const u32x4*>(c.v) + at);
+    ks = *token_or_none(there, c.k_scales + at);
+    vs = *token_or_none(there, c.v_scales + at);
   };
   auto put = [&](int64_t ch, typename Lds::Buf& to) {
     const bool far = vs >= kFarScale;
@@ -135,18 +132,25 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   const float c2 = score_factor(a.scale);
 
-  int32_t page = page_at(begin);
-  load(begin, page);
-  page = page_at(begin + 1);
-  put(begin, lds.buf[begin & 1]);
-  load(begin + 1, page);
-  page = page_at(begin + 2);
+  int32_t page = -1;
+  if (begin < end) {
+    const int32_t now = page_at(begin);
+    page = page_at(begin + 1);
+    load(begin, now);
+    put(begin, lds.buf[begin & 1]);
+    const int32_t after = page_at(begin + 2);
+    load(begin + 1, page);
+    page = after;
+  }
   __syncthreads();
   for (int64_t ch = begin; ch < end; ++ch) {
     const typename Lds::Buf& t = lds.buf[ch & 1];
     put(ch + 1, lds.buf[~ch & 1]);
+    // (The page first: loads come back in order, and the codes need not be waited for when the
+    // page is needed.)
+    const int32_t after = page_at(ch + 3);
     load(ch + 2, page);
-    page = page_at(ch + 3);
+    page = after;
     const int64_t t0 = ch * C;
     if (t0 < any) {
       f32x16 s[U];
