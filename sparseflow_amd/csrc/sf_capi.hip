@@ -1042,7 +1042,7 @@ int cache_view(const sf_mx4_cache_desc* d, const sf_mx4_cache* c, sf::CacheView&
   v.tables = c->tables;
   v.lengths = c->lengths;
   v.pages = d->pages;
-  v.width = d->width;
+  v.width = d->pages > 0 ? d->width : 0;  // (no page: no place)
   v.heads = d->kv_heads;
   v.blocks = (d->head_dim + 31) / 32;
   v.page_shift = __builtin_ctz((unsigned)d->page_size);
@@ -1078,7 +1078,7 @@ namespace {
 
 sf::Mx4AttnPlan attention_plan(const sf_mx4_cache_desc* d) {
   return sf::mx4_attn_plan(d->batch, d->max_len < d->tokens ? d->max_len : d->tokens, d->heads, d->kv_heads,
-                           (d->head_dim + 31) / 32, d->width * d->page_size);
+                           (d->head_dim + 31) / 32, d->dtype, d->width * d->page_size);
 }
 
 }  // namespace
@@ -1107,7 +1107,8 @@ int sf_mx4_attention(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, cons
   a.seq = {offsets, slots, d->batch, d->tokens, d->rows};
   a.q = q;
   a.y = y;
-  a.parts_o = static_cast<float*>(workspace);
+  a.parts_o = p.bytes > 0 ? static_cast<float*>(workspace) : nullptr;
+  a.cuts = p.bytes > p.cuts_at ? reinterpret_cast<sf::AttnCut*>(static_cast<char*>(workspace) + p.cuts_at) : nullptr;
   a.parts_ml = p.bytes > 0 ? a.parts_o + p.parts * (32 * (int64_t)a.cache.blocks) : nullptr;
   for (int i = 0; i < 3; ++i) {
     a.q_strides[i] = d->q_strides[i];
@@ -1115,7 +1116,10 @@ int sf_mx4_attention(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, cons
   }
   if (offsets != nullptr) a.q_strides[0] = a.y_strides[0] = 0;
   a.tiles = p.tiles;
+  a.max_len = d->max_len < d->tokens ? d->max_len : d->tokens;
   a.tile_rows = p.tile_rows;
+  a.unit = p.unit;
+  a.shares = p.shares;
   a.splits = p.splits;
   a.group = d->heads / d->kv_heads;
   a.head_dim = d->head_dim;

@@ -411,24 +411,33 @@ int launch_mx4_append(const Mx4AppendArgs& a, int dtype, hipStream_t stream);
 // Query rows of a workgroup where there are many, and up to how many of a sequence and shared
 // head it takes 16 instead.
 constexpr int kAttnTileRows = 128, kAttnFewRows = 48;
-struct Mx4AttnPlan {
-  int64_t tiles;  // of a sequence's and shared head's query rows
-  int tile_rows;  // 16 or kAttnTileRows
-  int splits;     // parts of a tile's tokens
-  int64_t parts;  // rows of the workspace
-  size_t bytes;   // of it: [parts, 32 blocks] and [parts, 2] floats
+// A tile of 16 query rows that several workgroups have parts of (parts = 0: none).
+struct AttnCut {
+  int64_t b, first, row0, rows;
+  int kvh, parts;
 };
-Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int64_t room);
+struct Mx4AttnPlan {
+  int64_t tiles;   // of a sequence's and shared head's query rows
+  int64_t shares;  // 16 rows: workgroups
+  int64_t parts;   // rows of the workspace
+  size_t bytes;    // of it: [parts, 32 blocks] and [parts, 2] floats, 16 rows: [shares] cuts
+  size_t cuts_at;
+  int tile_rows;   // 16 or kAttnTileRows
+  int unit;        // 16 rows: 128 tokens that are not cut
+  int splits;      // kAttnTileRows: parts of a tile's tokens
+};
+Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int dtype, int64_t room);
 struct Mx4AttnArgs {
   SeqAxis seq;
   CacheView cache;
   const void* q;
   void* y;
-  float* parts_o;
+  float* parts_o;  // NULL: nothing is cut
   float* parts_ml;
+  AttnCut* cuts;
   int64_t q_strides[3], y_strides[3];
-  int64_t tiles, block0;
-  int tile_rows, splits, group, head_dim;
+  int64_t max_len, tiles, shares, block0;
+  int tile_rows, unit, splits, group, head_dim;
   float scale;
 };
 int launch_mx4_attn_tiles(const Mx4AttnArgs& a, int dtype, hipStream_t stream);

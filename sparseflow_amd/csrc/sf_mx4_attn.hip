@@ -71,8 +71,99 @@ __global__ __launch_bounds__(kAppendThreads) void k_mx4_append(Mx4AppendArgs a) 
 // transposing loads.  K's codes go straight from memory into the operand: lane (token, g)
 // holds 8 NB columns of its token from 8 NB g, and Q's fragments are laid out the same.  The
 // next tokens' codes are loaded before these are worked on, and the pages after those.
+//
+// Sequences differ in length, and a workgroup takes some 5 us to begin and to end: so there
+// are as many as the CUs hold, and the units (128 tokens of a tile of rows) of all sequences,
+// one after another, are cut into as many even shares.  A share's ends may lie inside a tile's
+// tokens: those parts go to the workspace, two at most of a workgroup, and k_mx4_attn_join
+// puts them together.  (64 x 8192 tokens in two equal parts a tile 138 us, in four 160, in
+// eight 189.)
 constexpr int kAttnWaves = 4;
 constexpr int kAttnTokens = 32;
+constexpr int kAttnUnit = kAttnWaves;   // chunks of kAttnTokens: one to a wavefront
+constexpr int kAttnShare = 2;           // units that a workgroup takes at least, where they are parts of tiles
+
+// A sequence's part of the work: tiles of 16 query rows of each shared head, of `units` each.
+struct SeqWork {
+  int64_t first, n, slot, length;  // its rows, its row of the tables, its tokens
+  int64_t keys;                    // tokens that its last query sees
+  int64_t tiles, units;
+  __device__ __forceinline__ int64_t all(int heads) const { return tiles * units * heads; }
+};
+__device__ __forceinline__ SeqWork seq_work(const Mx4AttnArgs& a, int64_t b) {
+  SeqWork w;
+  if (a.seq.offsets == nullptr) {
+    w.first = 0;
+    w.n = a.seq.tokens;
+  } else {
+    const int64_t lo = a.seq.offsets[b], hi = a.seq.offsets[b + 1];
+    w.first = lo < 0 ? 0 : lo > a.seq.tokens ? a.seq.tokens : lo;
+    const int64_t end = hi > a.seq.tokens ? a.seq.tokens : hi;
+    w.n = end > w.first ? end - w.first : 0;
+  }
+  w.slot = seq_slot(a.seq, b);
+  w.length = w.slot < 0 ? 0 : a.cache.lengths[w.slot];
+  const int64_t room = cache_room(a.cache);
+  w.keys = w.length < 0 ? 0 : w.length > room ? room : w.length;
+  w.tiles = ((w.n < a.max_len ? w.n : a.max_len) * a.group + 15) / 16;
+  const int64_t chunks = (w.keys + kAttnTokens - 1) / kAttnTokens;
+  w.units = chunks <= kAttnUnit * a.unit ? 1 : (chunks + kAttnUnit * a.unit - 1) / (kAttnUnit * a.unit);
+  return w;
+}
+
+// The sum of the threads' values before this one's, and of all (256 threads).
+__device__ __forceinline__ int64_t work_before(int64_t v, int64_t& total) {
+  __shared__ int64_t part[4];
+  const int lane = lane_id(), wave = threadIdx.x / kWave;
+  int64_t in = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t o = __shfl_up(in, d, kWave);
+    if (lane >= d) in += o;
+  }
+  if (lane == kWave - 1) part[wave] = in;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += w < wave ? part[w] : 0;
+    total += part[w];
+  }
+  return before + in - v;
+}
+
+// Where this thread's sequences begin, and the units of all; the sequences are dealt to the
+// threads in runs.
+__device__ __forceinline__ int64_t run_of_sequences(const Mx4AttnArgs& a) { return (a.seq.batch + 255) / 256; }
+__device__ __forceinline__ int64_t work_of_run(const Mx4AttnArgs& a, int64_t& total) {
+  const int64_t run = run_of_sequences(a), b0 = threadIdx.x * run;
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b0 + run && b < a.seq.batch; ++b) mine += seq_work(a, b).all(a.cache.heads);
+  return work_before(mine, total);
+}
+
+// at[0]: the sequence of a unit, at[1]: where the sequence begins (`before`: where this
+// thread's do).
+__device__ __forceinline__ void find_unit(const Mx4AttnArgs& a, int64_t unit, int64_t before, int64_t (&at)[2]) {
+  const int64_t run = run_of_sequences(a), b0 = threadIdx.x * run;
+  for (int64_t b = b0; b < b0 + run && b < a.seq.batch; ++b) {
+    const int64_t all = seq_work(a, b).all(a.cache.heads);
+    if (unit >= before && unit < before + all) at[0] = b, at[1] = before;
+    before += all;
+  }
+  __syncthreads();
+}
+
+// Shares: workgroup k of `count` takes the units from share_begin(k) to share_begin(k + 1).
+__device__ __forceinline__ int64_t shares(const Mx4AttnArgs& a, int64_t total) {
+  const int64_t most = a.parts_o == nullptr ? total : total / kAttnShare;
+  return most < 1 ? 1 : most < a.shares ? most : a.shares;
+}
+__device__ __forceinline__ int64_t share_begin(int64_t k, int64_t count, int64_t total) { return total * k / count; }
+__device__ __forceinline__ int64_t share_of(int64_t unit, int64_t count, int64_t total) {
+  return ((unit + 1) * count + total - 1) / total - 1;
+}
 
 template <int NB>
 struct AttnLds {
@@ -134,22 +225,23 @@ struct RawTokens {
   __device__ __forceinline__ void load(const CacheView& c, int64_t t0, int kvh, int32_t pages, int lane) {
     const int r = lane & 15, g = lane >> 4;
     have = (uint32_t)__ballot(pages >= 0);
+    int32_t kp[2], vp[VU];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) kp[u] = __shfl(pages, 16 * u + r, kWave);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) vp[u] = __shfl(pages, (lane + kWave * u) / NB & 31, kWave);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int t = 16 * u + r;
-      const int32_t p = __shfl(pages, t, kWave);
-      const int64_t at = cache_place(c, p, kvh, t0 + t);
-      load_codes<NB>(token_or_none(p >= 0, c.k + at * (16 * NB) + 4 * NB * g), k[u]);
-      ks[u] = load_scales<NB>(token_or_none(p >= 0, c.k_scales + at * NB));
+      const int64_t at = cache_place(c, kp[u], kvh, t0 + 16 * u + r);
+      load_codes<NB>(c.k + at * (16 * NB) + 4 * NB * g, k[u]);
+      ks[u] = load_scales<NB>(c.k_scales + at * NB);
     }
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
-      const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
-      const int32_t p = __shfl(pages, tok & 31, kWave);
-      const bool there = p >= 0 && (NB % 2 == 0 || at < kAttnTokens * NB);
-      const int64_t row = cache_place(c, p, kvh, t0 + tok) * NB + blk;
-      v[u] = *token_or_none(there, reinterpret_cast<const u32x4*>(c.v) + row);
-      vs[u] = *token_or_none(there, c.v_scales + row);
+      const int at = lane + kWave * u, tok = at / NB & 31, blk = at % NB;
+      const int64_t row = cache_place(c, vp[u], kvh, t0 + tok) * NB + blk;
+      v[u] = reinterpret_cast<const u32x4*>(c.v)[row];
+      vs[u] = c.v_scales[row];
     }
   }
 
@@ -159,9 +251,10 @@ struct RawTokens {
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
-      const bool off = vs[u] >= kFarScale;
+      // (Of a token without a page scale 0: numbers, which get the weight 0.)
+      const bool there = have >> (tok & 31) & 1, off = there && vs[u] >= kFarScale;
       far |= off;
-      const float scale = mx4_scale(off ? 0 : vs[u]);
+      const float scale = mx4_scale(there && !off ? vs[u] : 0);
       if (off) v[u] = u32x4{0, 0, 0, 0};
       if (NB % 2 == 0 || at < kAttnTokens * NB) {
 #pragma unroll
@@ -172,30 +265,23 @@ struct RawTokens {
   }
 };
 
+// Rows of a tile, and the chunks of their tokens that a workgroup takes.
+struct TileWork {
+  SeqWork seq;
+  int64_t b, row0, begin, end;
+  int64_t part;  // of the workspace, or -1: the tile's tokens are all there
+  int kvh;
+};
+
 template <typename T, int NB>
-__global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) void k_mx4_attn_rows(Mx4AttnArgs a) {
+__device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork& work_of, AttnLds<NB>& lds) {
   constexpr int NP = Parts<T>::n;
   constexpr int stride = AttnLds<NB>::stride;
-  __shared__ AttnLds<NB> lds;
   const CacheView& c = a.cache;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane & 15, g = lane >> 4;
-
-  // Which sequence, shared head, rows and part of the tokens.
-  int64_t id = a.block0 + blockIdx.x;
-  const int split = (int)(id % a.splits);
-  id /= a.splits;
-  const int64_t tile = id % a.tiles;
-  id /= a.tiles;
-  const int kvh = (int)(id % c.heads);
-  const int64_t b = id / c.heads;
-  int64_t first, n;
-  seq_rows(a.seq, b, first, n);
-  const int64_t slot = seq_slot(a.seq, b);
-  const int group = a.group;
-  const int64_t row0 = tile * 16, rows = n * group;
-  if (row0 >= rows) return;
-  const int64_t length = slot < 0 ? 0 : c.lengths[slot];
-  const int64_t room = cache_room(c);
+  const int64_t b = work_of.b, first = work_of.seq.first, n = work_of.seq.n, slot = work_of.seq.slot, length = work_of.seq.length;
+  const int64_t row0 = work_of.row0, rows = n * a.group, begin = work_of.begin, end = work_of.end;
+  const int kvh = work_of.kvh, group = a.group;
 
   // This lane's query row.
   const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
@@ -209,13 +295,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) v
     for (int j = 0; j < NB; ++j) load_query<T, NP>(q, 8 * (NB * g + j), a.head_dim, a.scale, qf[j]);
   }
 
-  // The keys that any of the tile's rows sees, and this part's share of them.
-  const int64_t last_row = row0 + 15 < rows - 1 ? row0 + 15 : rows - 1;
-  int64_t keys = slot < 0 ? 0 : length - n + last_row / group + 1;
-  keys = keys < 0 ? 0 : keys > room ? room : keys;
+  const int64_t keys = work_of.seq.keys;
   const int64_t place0 = length - n + row0 / group;  // the tile's first row's
-  const int64_t chunks = (keys + kAttnTokens - 1) / kAttnTokens;
-  const int64_t begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
   const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
   auto pages_at = [&](int64_t ch) {
     const int64_t t = ch * kAttnTokens + (lane & 31);
@@ -276,13 +357,22 @@ __global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) v
     l += sum;
     bf16x8 pf[NP];
     weight_parts<NP>(pr, pf);
+    constexpr int DG = NB < 4 ? 2 * NB : 8;  // tiles of columns at a time
 #pragma unroll
-    for (int d = 0; d < 2 * NB; ++d) {
-      const int tok = 4 * g + (r >> 2);
-      const uint16_t* at = vt + tok * stride + 32 * (d >> 1) + 8 * value_unit(2 * (d & 1) + (r >> 1 & 1), tok) + 4 * (r & 1);
-      const bf16x8 vf = __builtin_shufflevector(lds_transposed(at), lds_transposed(at + 16 * stride), 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int d0 = 0; d0 < 2 * NB; d0 += DG) {
+      bf16x4v vf[DG][2];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) o[d] = mfma16(vf, pf[p], o[d]);
+      for (int d = d0; d < d0 + DG && d < 2 * NB; ++d) {
+        const int tok = 4 * g + (r >> 2);
+        const uint16_t* at = vt + tok * stride + 32 * (d >> 1) + 8 * value_unit(2 * (d & 1) + (r >> 1 & 1), tok) + 4 * (r & 1);
+        vf[d - d0][0] = lds_transposed(at);
+        vf[d - d0][1] = lds_transposed(at + 16 * stride);
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int d = d0; d < d0 + DG && d < 2 * NB; ++d)
+          o[d] = mfma16(__builtin_shufflevector(vf[d - d0][0], vf[d - d0][1], 0, 1, 2, 3, 4, 5, 6, 7), pf[p], o[d]);
     }
     if (__any(raw.far)) {
       for (int t = 0; t < kAttnTokens; ++t) {
@@ -348,8 +438,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) v
     f[w] = exp2_hw(lds.m[w][wr] - from);
     total += f[w] * lds.l[w][wr];
   }
-  if (a.splits > 1) {
-    const int64_t base = (((b * c.heads + kvh) * a.tiles + tile) * a.splits + split) * 16 + wr;
+  if (work_of.part >= 0) {
+    const int64_t base = work_of.part * 16 + wr;
     if (wc == 0) a.parts_ml[2 * base] = top, a.parts_ml[2 * base + 1] = total;
 #pragma unroll
     for (int k = 0; k < 2 * NB; ++k) {
@@ -373,44 +463,80 @@ __global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) v
   }
 }
 
-// The parts of a row's tokens together: a workgroup to a row, a wavefront to every fourth
-// part, a lane to its columns; four parts under way at a time.
 template <typename T, int NB>
-__global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
-  constexpr int C = (32 * NB + kWave - 1) / kWave;
-  __shared__ float sums[4][kWave * C + 1];
-  const CacheView& c = a.cache;
-  const int lane = lane_id(), wave = threadIdx.x / kWave;
-  const int64_t id = a.block0 + blockIdx.x;  // (b, kvh, tile, row of it)
-  const int64_t tile_id = id / a.tile_rows;
-  const int wr = (int)(id - tile_id * a.tile_rows);
-  const int64_t tile = tile_id % a.tiles, bh = tile_id / a.tiles;
-  const int kvh = (int)(bh % c.heads);
-  const int64_t b = bh / c.heads;
-  int64_t first, n;
-  seq_rows(a.seq, b, first, n);
-  const int64_t row = tile * a.tile_rows + wr;
-  if (row >= n * a.group) return;
-  const int64_t base = tile_id * a.splits * a.tile_rows + wr;
+__global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) void k_mx4_attn_rows(Mx4AttnArgs a) {
+  __shared__ AttnLds<NB> lds;
+  __shared__ int64_t at[2];
+  const int heads = a.cache.heads;
+  int64_t total;
+  const int64_t before = work_of_run(a, total);
+  const int64_t count = shares(a, total), k = a.block0 + blockIdx.x;
+  if (a.cuts != nullptr && threadIdx.x == 0) a.cuts[k].parts = 0;
+  if (total == 0 || k >= count) return;
+  int64_t unit = share_begin(k, count, total);
+  const int64_t stop = share_begin(k + 1, count, total);
+  find_unit(a, unit, before, at);
+  TileWork w;
+  w.b = __builtin_amdgcn_readfirstlane((int)at[0]);
+  int64_t from = at[1];
+  w.seq = seq_work(a, w.b);
+  while (unit < stop) {
+    while (unit >= from + w.seq.all(heads)) {
+      from += w.seq.all(heads);
+      w.seq = seq_work(a, ++w.b);
+    }
+    const int64_t in = unit - from, item = in / w.seq.units, u0 = in - item * w.seq.units;
+    const int64_t left = stop - unit, u1 = u0 + left < w.seq.units ? u0 + left : w.seq.units;
+    w.kvh = (int)(item / w.seq.tiles);
+    w.row0 = (item - w.kvh * w.seq.tiles) * 16;
+    const int64_t chunks = (w.seq.keys + kAttnTokens - 1) / kAttnTokens, per = kAttnUnit * a.unit;
+    w.begin = u0 * per;
+    w.end = u1 * per < chunks ? u1 * per : chunks;
+    w.part = u0 == 0 && u1 == w.seq.units ? -1 : 2 * k + (u0 == 0);
+    // (A tile that the workgroup before is the first to have a part of is this one's to report.)
+    if (u0 > 0 && threadIdx.x == 0 && share_of(unit - u0, count, total) == k - 1) {
+      AttnCut& cut = a.cuts[k];
+      cut.b = w.b;
+      cut.first = w.seq.first;
+      cut.row0 = w.row0;
+      cut.rows = w.seq.n * a.group;
+      cut.kvh = w.kvh;
+      cut.parts = (int)(share_of(unit - u0 + w.seq.units - 1, count, total) - k + 2);
+    }
+    attend_tile<T, NB>(a, w, lds);
+    unit += u1 - u0;
+    __syncthreads();
+  }
+}
+
+// A row's parts together: W wavefronts to a row (of a workgroup's four), a lane to its columns, F
+// parts under way; place(j) is part j's row of the workspace.  W = 1 where there are few parts
+// and many rows (8 x 100 queries of 1100 tokens: 65 us for the call, with W = 4 105), W = 4
+// otherwise (64 parts: 6 us, with W = 1 19).
+template <typename T, int NB, int W, typename Place>
+__device__ __forceinline__ void join_row(const Mx4AttnArgs& a, int64_t parts, Place&& place, T* y) {
+  constexpr int C = (32 * NB + kWave - 1) / kWave, F = C <= 2 ? 16 : 8;
+  __shared__ float sums[W == 1 ? 1 : 4][kWave * C + 1];
+  const int lane = lane_id(), wave = threadIdx.x / kWave % W;
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += kWave) top = fmaxf(top, a.parts_ml[2 * (base + (int64_t)a.tile_rows * s)]);
+  for (int64_t s = lane; s < parts; s += kWave) top = fmaxf(top, a.parts_ml[2 * place(s)]);
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
   const float from = top == -INFINITY ? 0.f : top;
   float total = 0.f, v[C] = {};
-  for (int s0 = wave; s0 < a.splits; s0 += 16) {
-    float f[4], q[4], p[4][C];
+  for (int64_t s0 = wave; s0 < parts; s0 += W * F) {
+    float f[F], q[F], p[F][C];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = s0 + 4 * k < a.splits;
-      const int64_t at = base + (int64_t)a.tile_rows * (in ? s0 + 4 * k : s0);
+    for (int k = 0; k < F; ++k) {
+      const bool in = s0 + W * k < parts;
+      const int64_t at = place(in ? s0 + W * k : s0);
       f[k] = in ? a.parts_ml[2 * at] : -INFINITY;
       q[k] = a.parts_ml[2 * at + 1];
 #pragma unroll
-      for (int e = 0; e < C; ++e) p[k][e] = kWave * e + lane < 32 * NB ? a.parts_o[at * (32 * NB) + kWave * e + lane] : 0.f;
+      for (int e = 0; e < C; ++e) p[k][e] = a.parts_o[at * (32 * NB) + (kWave * e + lane < 32 * NB ? kWave * e + lane : 0)];
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < F; ++k) {
       if (f[k] == -INFINITY) continue;  // (nothing seen there)
       const float g = exp2_hw(f[k] - from);
       total += g * q[k];
@@ -418,18 +544,55 @@ __global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
       for (int e = 0; e < C; ++e) v[e] += g * p[k][e];
     }
   }
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int e = 0; e < C; ++e) sums[wave][kWave * e + lane] = v[e];
-  if (lane == 0) sums[wave][kWave * C] = total;
-  __syncthreads();
-  const int64_t i = row / a.group;
-  T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + i) * a.y_strides[1] +
-         (int64_t)(kvh * a.group + (int)(row - i * a.group)) * a.y_strides[2];
-  total = (sums[0][kWave * C] + sums[1][kWave * C]) + (sums[2][kWave * C] + sums[3][kWave * C]);
-  for (int k = threadIdx.x; k < a.head_dim; k += 256) {
-    const float w = (sums[0][k] + sums[1][k]) + (sums[2][k] + sums[3][k]);
-    y[k] = from_f32<T>(total == 0.f ? 0.f : w / total);
+    for (int e = 0; e < C; ++e) sums[wave][kWave * e + lane] = v[e];
+    if (lane == 0) sums[wave][kWave * C] = total;
+    __syncthreads();
+    if (wave > 0) return;
+    total = (sums[0][kWave * C] + sums[1][kWave * C]) + (sums[2][kWave * C] + sums[3][kWave * C]);
+#pragma unroll
+    for (int e = 0; e < C; ++e)
+      v[e] = (sums[0][kWave * e + lane] + sums[1][kWave * e + lane]) + (sums[2][kWave * e + lane] + sums[3][kWave * e + lane]);
   }
+#pragma unroll
+  for (int e = 0; e < C; ++e)
+    if (kWave * e + lane < a.head_dim) y[kWave * e + lane] = from_f32<T>(total == 0.f ? 0.f : v[e] / total);
+}
+template <typename T>
+__device__ __forceinline__ T* row_of_y(const Mx4AttnArgs& a, int64_t b, int64_t first, int kvh, int64_t row) {
+  const int64_t i = row / a.group;
+  return reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + i) * a.y_strides[1] +
+         (int64_t)(kvh * a.group + (int)(row - i * a.group)) * a.y_strides[2];
+}
+
+// Tiles of 16 rows whose tokens several workgroups had: join_rows rows of each.
+template <typename T, int NB, int W>
+__global__ __launch_bounds__(256) void k_mx4_attn_join_cuts(Mx4AttnArgs a, int join_rows) {
+  const int64_t id = (a.block0 + blockIdx.x) * (4 / W) + threadIdx.x / kWave / W, k = id / join_rows + 1;
+  if (k >= a.shares) return;
+  const AttnCut cut = a.cuts[k];
+  const int wr = (int)(id % join_rows);
+  const int64_t row = cut.row0 + wr;
+  if (cut.parts == 0 || row >= cut.rows) return;
+  // (The first part is a share's second one, the others are the first of theirs.)
+  join_row<T, NB, W>(a, cut.parts, [&](int64_t j) { return (2 * (k - 1 + j) + (j == 0)) * 16 + wr; },
+                     row_of_y<T>(a, cut.b, cut.first, cut.kvh, row));
+}
+
+// Tiles of kAttnTileRows rows.
+template <typename T, int NB, int W>
+__global__ __launch_bounds__(256) void k_mx4_attn_join(Mx4AttnArgs a) {
+  const int64_t id = (a.block0 + blockIdx.x) * (4 / W) + threadIdx.x / kWave / W;  // (b, kvh, tile, row of it)
+  const int64_t tile_id = id / kAttnTileRows;
+  const int wr = (int)(id - tile_id * kAttnTileRows);
+  const int64_t tile = tile_id % a.tiles, bh = tile_id / a.tiles, b = bh / a.cache.heads;
+  int64_t first, n;
+  seq_rows(a.seq, b, first, n);
+  const int64_t row = tile * kAttnTileRows + wr;
+  if (row >= n * a.group) return;
+  join_row<T, NB, W>(a, a.splits, [&](int64_t j) { return (tile_id * a.splits + j) * kAttnTileRows + wr; },
+                     row_of_y<T>(a, b, first, (int)(bh % a.cache.heads), row));
 }
 
 template <typename T>
@@ -440,13 +603,25 @@ struct DType {
 template <typename T, int NB>
 int launch_attn_nb(const Mx4AttnArgs& a, hipStream_t stream) {
   const int64_t tiles = a.seq.batch * a.cache.heads * a.tiles;
-  int rc = a.tile_rows > 16 ? launch_mx4_attn_tiles(a, DType<T>::code, stream)
-                            : launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.splits, [&](const Mx4AttnArgs& part, unsigned grid) {
-                                k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
-                              });
-  if (rc != (int)hipSuccess || a.splits == 1) return rc;
-  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * a.tile_rows, [&](const Mx4AttnArgs& part, unsigned grid) {
-    k_mx4_attn_join<T, NB><<<grid, 256, 0, stream>>>(part);
+  if (a.tile_rows == 16) {
+    const int rc = launch_blocks(a, &Mx4AttnArgs::block0, a.shares, [&](const Mx4AttnArgs& part, unsigned grid) {
+      k_mx4_attn_rows<T, NB><<<grid, kAttnWaves * kWave, 0, stream>>>(part);
+    });
+    if (rc != (int)hipSuccess || a.parts_o == nullptr) return rc;
+    const int join_rows = (int)(a.max_len * a.group < 16 ? a.max_len * a.group : 16);
+    const int64_t rows = (a.shares - 1) * join_rows;
+    const bool few = tiles * 4 >= a.shares;  // parts of a tile
+    return launch_blocks(a, &Mx4AttnArgs::block0, few ? (rows + 3) / 4 : rows, [&](const Mx4AttnArgs& part, unsigned grid) {
+      if (few) k_mx4_attn_join_cuts<T, NB, 1><<<grid, 256, 0, stream>>>(part, join_rows);
+      else k_mx4_attn_join_cuts<T, NB, 4><<<grid, 256, 0, stream>>>(part, join_rows);
+    });
+  }
+  const int rc = launch_mx4_attn_tiles(a, DType<T>::code, stream);
+  if (rc != (int)hipSuccess || a.parts_o == nullptr) return rc;
+  const bool few = a.splits <= 16;
+  return launch_blocks(a, &Mx4AttnArgs::block0, tiles * kAttnTileRows / (few ? 4 : 1), [&](const Mx4AttnArgs& part, unsigned grid) {
+    if (few) k_mx4_attn_join<T, NB, 1><<<grid, 256, 0, stream>>>(part);
+    else k_mx4_attn_join<T, NB, 4><<<grid, 256, 0, stream>>>(part);
   });
 }
 
@@ -475,20 +650,33 @@ int launch_append(Mx4AppendArgs a, hipStream_t stream) {
 
 }  // namespace
 
-Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int64_t room) {
+Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_heads, int blocks, int dtype, int64_t room) {
   Mx4AttnPlan p{};
   const int64_t rows = max_len * (heads / kv_heads);
   p.tile_rows = rows <= kAttnFewRows ? 16 : kAttnTileRows;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.splits = 1;
   const int64_t items = batch * kv_heads * p.tiles;
-  // As many parts of the tokens as fill the CUs, each of 256 tokens or more.
-  const int64_t want = p.tile_rows == 16 ? 1024 : 512;
-  int64_t splits = items == 0 ? 1 : want / items;
-  const int64_t most = (room + 255) / 256;
-  splits = splits > most ? most : splits;
-  p.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
-  p.parts = p.splits == 1 ? 0 : items * p.splits * p.tile_rows;
-  p.bytes = (size_t)p.parts * (size_t)(32 * blocks + 2) * 4;
+  if (p.tile_rows == 16) {
+    // Workgroups: what the CUs hold of them (by registers).  Short tables: a tile is one unit.
+    const int parts = dtype == SF_F32 ? 3 : dtype == SF_F16 ? 2 : 1;
+    p.unit = room <= 512 ? 4 : 1;
+    const int64_t tokens = kAttnTokens * kAttnUnit * p.unit, units = room <= tokens ? 1 : (room + tokens - 1) / tokens;
+    const int64_t hold = blocks * parts <= 2 ? 768 : blocks * parts <= 8 ? 512 : 256;
+    const int64_t most = units > hold || items > hold ? hold : items * units;  // (no product of large numbers)
+    p.shares = units == 1 ? (items < 4 * hold ? items : 4 * hold) : most < hold ? most : hold;
+    p.shares = p.shares < 1 ? 1 : p.shares;
+    p.parts = units == 1 ? 0 : 2 * p.shares * 16;
+  } else {
+    // As many parts of the tokens as fill the CUs, each of 256 tokens or more.
+    int64_t splits = items == 0 ? 1 : 512 / items;
+    const int64_t most = (room + 255) / 256;
+    splits = splits > most ? most : splits;
+    p.splits = (int)(splits < 1 ? 1 : splits);
+    p.parts = p.splits == 1 ? 0 : items * p.splits * p.tile_rows;
+  }
+  p.cuts_at = (size_t)p.parts * (size_t)(32 * blocks + 2) * 4;
+  p.bytes = p.cuts_at + (p.tile_rows == 16 && p.parts > 0 ? (size_t)p.shares * sizeof(AttnCut) : 0);
   return p;
 }
 

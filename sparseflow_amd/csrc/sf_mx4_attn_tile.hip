@@ -100,18 +100,17 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
   bool there;
   auto load = [&](int64_t ch, int32_t page) {
     there = page >= 0;
-    const int64_t at = cache_place(c, page, kvh, ch * C + tok) * NB + blk;
-    kc = *token_or_none(there, reinterpret_cast<const u32x4*>(c.k) + at);
-    vc = *token_or_none(there, reinterpret_cast<const u32x4*>(c.v) + at);
-    ks = *token_or_none(there, c.k_scales + at);
-    vs = *token_or_none(there, c.v_scales + at);
+    const int64_t at = cache_place(c, page, kvh, ch * C + tok) * NB + (mine ? blk : 0);
+    kc = reinterpret_cast<const u32x4*>(c.k)[at];
+    vc = reinterpret_cast<const u32x4*>(c.v)[at];
+    ks = c.k_scales[at];
+    vs = c.v_scales[at];
   };
   auto put = [&](int64_t ch, typename Lds::Buf& to) {
-    const bool far = vs >= kFarScale;
-    if (far) {
-      vc = u32x4{0, 0, 0, 0};
-      vs = 0;
-    }
+    // (Of a token without a page scale 0: numbers, which get the weight 0.)
+    const bool far = there && vs >= kFarScale;
+    if (far) vc = u32x4{0, 0, 0, 0};
+    if (far || !there) vs = 0;
     if (mine) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

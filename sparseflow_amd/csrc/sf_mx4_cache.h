@@ -14,18 +14,13 @@ __device__ __forceinline__ int32_t cache_page(const CacheView& c, const int32_t*
   const int32_t p = table[t >> c.page_shift];
   return p >= 0 && p < c.pages ? p : -1;
 }
-// What the loads of a token without a page read: they are made all the same, since behind loads
-// that only some make the compiler waits for all that are under way.
-__device__ const u32x4 kNoToken[2] = {};
-template <typename T>
-__device__ __forceinline__ const T* token_or_none(bool there, const T* p) {
-  return there ? p : reinterpret_cast<const T*>(kNoToken);
-}
-
 // Where a head's row of keys or values lies: token t is row t % page of its page, and a page
-// holds [heads, page] rows.
+// holds [heads, page] rows.  Without a page: the pool's first
+// row, which is read and left out: behind loads that only some lanes make the compiler waits
+// for all that are under way.
 __device__ __forceinline__ int64_t cache_place(const CacheView& c, int32_t page, int head, int64_t t) {
-  return (((int64_t)page * c.heads + head) << c.page_shift) + (t & ((1 << c.page_shift) - 1));
+  const int64_t at = (((int64_t)page * c.heads + head) << c.page_shift) + (t & ((1 << c.page_shift) - 1));
+  return page >= 0 ? at : 0;
 }
 
 // 16 lanes point at 4 rows' 16 columns of bf16, four to a row, and lane l gets column l of
