@@ -104,6 +104,29 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
+def reaches(*tensors: Optional[torch.Tensor]) -> tuple:
+    """Bytes that each tensor reaches over: what `surely_apart` goes by, kept with a checked call's plan."""
+    return tuple([0 if t is None or t.numel() == 0 else _reach(t) for t in tensors])
+
+
+def surely_apart(written, written_reach, read, read_reach) -> bool:
+    """Whether what a call writes lies in memory of its own, told by where the tensors begin and end.
+    (If not, `check_apart` says whether elements are shared.)"""
+    spans = sorted([(t.data_ptr(), n) for t, n in zip(written, written_reach)])
+    end = 0
+    for at, n in spans:
+        if at < end:
+            return False
+        end = at + n
+    for t, n in zip(read, read_reach):
+        if n:
+            at = t.data_ptr()
+            for w, m in spans:
+                if at < w + m and w < at + n:
+                    return False
+    return True
+
+
 def check_apart(written: torch.Tensor, name: str, others: dict, same: Tuple[str, ...] = ()) -> None:
     """What a call writes shares no memory with what it reads; those of `same` it may be."""
     for other, t in others.items():

@@ -24,7 +24,7 @@ import torch
 
 from .. import _lib
 from ._sequences import Plans, check_apart, check_index, check_input, check_like, check_out, host_slots, host_spans, \
-    last_contiguous, signature
+    last_contiguous, reaches, signature, surely_apart
 from .mx4 import blocks_of, host_dequantize, host_quantize
 
 _appends, _attentions = Plans(), Plans()
@@ -125,10 +125,12 @@ def mx4_cache_append(cache: MX4Cache, k: torch.Tensor, v: torch.Tensor, tables: 
     if max_len is not None:
         max_len = int(max_len)
     key = (signature(*cache, k, v, tables, lengths, slots, offsets), max_len)
-    desc, page, pages = _appends.get(key) or _appends.make(key, _check_append, cache, k, v, tables, lengths, slots, offsets,
-                                                           max_len)
-    for t, name in zip(cache, MX4Cache._fields):
-        check_apart(t, "cache." + name, {"k": k, "v": v, "tables": tables, "lengths": lengths})
+    plan = _appends.get(key) or _appends.make(key, _check_append, cache, k, v, tables, lengths, slots, offsets, max_len)
+    desc, page, pages, written, read = plan
+    if not surely_apart(cache, written, (k, v, tables, lengths, slots, offsets), read):
+        for i, (t, name) in enumerate(zip(cache, MX4Cache._fields)):
+            check_apart(t, "cache." + name, {"k": k, "v": v, "tables": tables, "lengths": lengths, "slots": slots,
+                                             "offsets": offsets, **dict(zip(MX4Cache._fields[i + 1:], cache[i + 1:]))})
     if not k.is_cuda:
         with torch.no_grad():
             ks, vs = host_spans(k, offsets), host_spans(v, offsets)
@@ -146,19 +148,20 @@ def mx4_cache_append(cache: MX4Cache, k: torch.Tensor, v: torch.Tensor, tables: 
 
 
 def _check_append(cache, k, v, tables, lengths, slots, offsets, max_len):
-    """-> (the descriptor of a device call, page_size, pages)."""
+    """-> (the descriptor of a device call, page_size, pages, bytes that the cache and what is read reach over)."""
     batch, tokens = _axes(k, "k", offsets)
     check_like(v, k, "v", tuple(k.shape))
     dim = int(k.shape[-1])
     pages, heads, page, rows, width = _check_cache(cache, k, tables, lengths, slots, batch, dim)
     if heads != k.shape[-2]:
         raise ValueError(f"k has {k.shape[-2]} heads: the cache's {heads} are wanted")
+    spans = reaches(*cache), reaches(k, v, tables, lengths, slots, offsets)
     if not k.is_cuda:
-        return None, page, pages
+        return (None, page, pages) + spans
     longest = tokens if offsets is None or max_len is None else min(max(max_len, 0), tokens)
     zero = (0, 0, 0)
-    return _lib.mx4_cache_desc(batch, tokens, longest, rows, width, pages, zero, _strides(k), _strides(v), zero, heads, heads,
-                               dim, page, k.dtype, 1.0), page, pages
+    return (_lib.mx4_cache_desc(batch, tokens, longest, rows, width, pages, zero, _strides(k), _strides(v), zero, heads, heads,
+                               dim, page, k.dtype, 1.0), page, pages) + spans
 
 
 @torch.no_grad()
@@ -228,7 +231,8 @@ def _attention(q, cache, tables, lengths, slots, offsets, max_len, scale, out):
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
-        check_apart(out, "out", {"q": q, **dict(zip(MX4Cache._fields, cache)), "tables": tables, "lengths": lengths},
+        check_apart(out, "out", {"q": q, **dict(zip(MX4Cache._fields, cache)), "tables": tables, "lengths": lengths,
+                                  "slots": slots, "offsets": offsets},
                     same=("q",))
     if not q.is_cuda:
         spans = host_spans(q, offsets)

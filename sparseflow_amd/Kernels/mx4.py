@@ -26,7 +26,7 @@ Quantized = Tuple[torch.Tensor, torch.Tensor]
 BLOCK = 32
 LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
-_rows_plans, _linear_plans = Plans(), Plans()
+_rows_plans, _back_plans, _linear_plans = Plans(), Plans(), Plans()
 
 
 def blocks_of(size: int) -> int:
@@ -68,19 +68,27 @@ def host_dequantize(codes: torch.Tensor, scales: torch.Tensor, size: int) -> tor
     return (levels[pair.int()].unflatten(-1, (-1, BLOCK)) * factor[..., None]).flatten(-2)[..., :size]
 
 
-def check_quantized(t, name: str, device: torch.device) -> Quantized:
-    if not isinstance(t, (tuple, list)) or len(t) != 2 or not all(isinstance(v, torch.Tensor) for v in t):
+def _pair(t, name: str) -> Quantized:
+    if not isinstance(t, (tuple, list)) or len(t) != 2 or not all([isinstance(v, torch.Tensor) for v in t]):
         raise ValueError(f"{name}: a pair (codes, scales) is wanted")
-    codes, scales = t
+    return tuple(t)
+
+
+def check_quantized(t, name: str, device: torch.device) -> Quantized:
+    codes, scales = _pair(t, name)
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 1 or codes.dim() != scales.dim() \
             or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * scales.shape[-1] or scales.shape[-1] < 1:
         raise ValueError(f"{name} is {tuple(codes.shape)} {codes.dtype} and {tuple(scales.shape)} {scales.dtype}: uint8 "
                          "(..., 16 blocks) and (..., blocks) are wanted")
     if codes.device != device or scales.device != device or not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{name} on {codes.device} and {scales.device}: contiguous tensors on {device} are wanted")
-    if codes.is_cuda and codes.data_ptr() % 16 != 0:
-        raise ValueError(f"{name}: codes that begin at a multiple of 16 bytes are wanted")
     return codes, scales
+
+
+def _check_aligned(codes: torch.Tensor, name: str) -> None:
+    """(At every call: plans know nothing of addresses.)"""
+    if codes.data_ptr() % 16 != 0:
+        raise ValueError(f"{name}: codes that begin at a multiple of 16 bytes are wanted")
 
 
 def _rows(x: torch.Tensor) -> Optional[Tuple[int, int, Tuple[int, int]]]:
@@ -102,23 +110,26 @@ def mx4_quantize(x: torch.Tensor, out: Optional[Quantized] = None) -> Quantized:
     """x [..., dim] -> (codes [..., 16 blocks], scales [..., blocks]); out: such a pair to write."""
     if x.is_cuda and x.dim() > 0:
         x = last_contiguous(x)
+    if out is not None:
+        out = _pair(out, "out")
     key = (signature(x), None if out is None else signature(*out))
     rows, shapes = _rows_plans.get(key) or _rows_plans.make(key, _check_quantize, x, out)
     if out is None:
-        out = tuple([torch.empty(s, dtype=torch.uint8, device=x.device) for s in shapes])
+        out = (torch.empty(shapes[0], dtype=torch.uint8, device=x.device), torch.empty(shapes[1], dtype=torch.uint8, device=x.device))
     else:
-        check_quantized(out, "out", x.device)
+        if x.is_cuda:
+            _check_aligned(out[0], "out")
         check_apart(out[0], "out's codes", {"x": x, "out's scales": out[1]})
         check_apart(out[1], "out's scales", {"x": x})
     if not x.is_cuda:
         for t, v in zip(out, host_quantize(x)):
             t.copy_(v)
-        return tuple(out)
+        return out
     if rows is None:
         x = x.contiguous()
         rows = _rows(x)
     _lib.mx4_quantize(x, *rows, *out)
-    return tuple(out)
+    return out
 
 
 def _check_quantize(x, out):
@@ -138,6 +149,21 @@ def _check_quantize(x, out):
 def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, size: Optional[int] = None,
                    dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(codes, scales) -> [..., size] (default: whole blocks) in `dtype`, or into a contiguous out."""
+    key = (signature(codes, scales, out), size, dtype)
+    shape, dtype, rows = _back_plans.get(key) or _back_plans.make(key, _check_dequantize, codes, scales, size, dtype, out)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=codes.device)
+    else:
+        check_apart(out, "out", {"codes": codes, "scales": scales})
+    if not codes.is_cuda:
+        return out.copy_(host_dequantize(codes, scales, shape[-1]))
+    _check_aligned(codes, "codes, scales")
+    _lib.mx4_dequantize(codes, scales, rows, out)
+    return out
+
+
+def _check_dequantize(codes, scales, size, dtype, out):
+    """-> (the result's shape and type, rows)."""
     check_quantized((codes, scales), "codes, scales", codes.device)
     n = int(scales.shape[-1])
     size = BLOCK * n if size is None else int(size)
@@ -148,15 +174,10 @@ def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, size: Optional[int
         if out.shape != shape or out.dtype not in FLOATS or out.device != codes.device or not out.is_contiguous():
             raise ValueError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}: a contiguous {tuple(shape)} float "
                              f"tensor on {codes.device} is wanted")
-        check_apart(out, "out", {"codes": codes, "scales": scales})
+        dtype = out.dtype
     elif dtype not in FLOATS:
         raise _lib.UnsupportedError(f"dtype is {dtype}: float32, float16 or bfloat16 is wanted")
-    else:
-        out = torch.empty(shape, dtype=dtype, device=codes.device)
-    if not codes.is_cuda:
-        return out.copy_(host_dequantize(codes, scales, size))
-    _lib.mx4_dequantize(codes, scales, codes.numel() // (16 * n), out)
-    return out
+    return shape, dtype, codes.numel() // (16 * n)
 
 
 def mx4_linear_forward(x: Union[torch.Tensor, Quantized], weight: Quantized, bias: Optional[torch.Tensor] = None,
@@ -169,18 +190,17 @@ def mx4_linear_forward(x: Union[torch.Tensor, Quantized], weight: Quantized, bia
     out shares no memory with the inputs.
     """
     four = not isinstance(x, torch.Tensor)
+    x_scales = None
     if four:
-        x, x_scales = check_quantized(x, "x", x[0].device if len(x) and isinstance(x[0], torch.Tensor) else torch.device("cpu"))
-    else:
-        x_scales = None
-    if not isinstance(weight, (tuple, list)) or len(weight) != 2:
-        raise ValueError("weight: a pair (codes, scales) is wanted")
+        x, x_scales = _pair(x, "x")
+    w, w_scales = weight = _pair(weight, "weight")
     key = (signature(x, x_scales, *weight, bias, out), dtype)
     plan = _linear_plans.get(key) or _linear_plans.make(key, _check_linear, x, x_scales, weight, bias, dtype, out)
     shape, dtype, desc, flat = plan
-    w, w_scales = weight
-    if x.is_cuda and w.data_ptr() % 16 != 0:
-        raise ValueError("weight: codes that begin at a multiple of 16 bytes are wanted")
+    if x.is_cuda:
+        _check_aligned(w, "weight")
+        if four:
+            _check_aligned(x, "x")
     if out is None:
         y = torch.empty(shape, dtype=dtype, device=x.device)
     else:
@@ -201,6 +221,8 @@ def mx4_linear_forward(x: Union[torch.Tensor, Quantized], weight: Quantized, bia
 def _check_linear(x, x_scales, weight, bias, dtype, out):
     """-> (y's shape and type, the descriptor of a device call or None where x has to be
     laid out first, (rows, y's row stride))."""
+    if x_scales is not None:
+        check_quantized((x, x_scales), "x", x.device)
     w, w_scales = check_quantized(weight, "weight", x.device)
     if w.dim() != 2 or w.shape[0] < 1:
         raise ValueError(f"weight is {tuple(w.shape)}: (N, 16 blocks) is wanted")

@@ -22,7 +22,7 @@ from typing import Dict, List, Sequence, Tuple
 import torch
 
 from .. import _lib
-from ._sequences import overlap
+from ._sequences import Plans, overlap, reaches, signature, surely_apart
 
 
 def _check_pools(pools: Sequence[torch.Tensor], device: torch.device, pages: int) -> Tuple[torch.Tensor, ...]:
@@ -49,7 +49,24 @@ def _check_apart(written: Dict[str, torch.Tensor], read: Dict[str, torch.Tensor]
                 raise ValueError(f"{name} shares memory with {other}")
 
 
+_plans = Plans()
+
+
 def _check(refs, tables, lengths, page_size, pools, **requests) -> Tuple[int, Tuple[torch.Tensor, ...]]:
+    """-> (page_size, pools) of a call whose arguments fit together and lie apart."""
+    page_size, pools = int(page_size), tuple(pools)
+    written = (refs, tables, *pools) if lengths is None else (refs, tables, lengths, *pools)
+    read = tuple(requests.values())
+    key = (signature(*written), signature(*read), page_size, lengths is None)
+    spans = _plans.get(key) or _plans.make(key, _check_shapes, refs, tables, lengths, page_size, pools, requests)
+    if not surely_apart(written, spans[0], read, spans[1]):
+        named = {"refs": refs, "tables": tables, **({} if lengths is None else {"lengths": lengths})}
+        _check_apart({**named, **{f"pool {i}": t for i, t in enumerate(pools)}}, requests)
+    return page_size, pools
+
+
+def _check_shapes(refs, tables, lengths, page_size, pools, requests) -> tuple:
+    """-> the bytes that what is written, and what is read, reach over."""
     if refs.dim() != 1:
         raise ValueError(f"refs is {tuple(refs.shape)}: (pages,) is wanted")
     _check_ints(refs, "refs", refs.device, tuple(refs.shape))
@@ -58,7 +75,6 @@ def _check(refs, tables, lengths, page_size, pools, **requests) -> Tuple[int, Tu
     _check_ints(tables, "tables", refs.device, tuple(tables.shape))
     if lengths is not None:
         _check_ints(lengths, "lengths", refs.device, (int(tables.shape[0]),))
-    page_size = int(page_size)
     if page_size < 1:
         raise ValueError(f"page_size {page_size}: 1 or more is wanted")
     size = None
@@ -67,12 +83,8 @@ def _check(refs, tables, lengths, page_size, pools, **requests) -> Tuple[int, Tu
             raise ValueError(f"{name} is {tuple(t.shape)}: as many as the other requests are wanted")
         size = t.numel()
         _check_ints(t, name, refs.device, (size,))
-    pools = _check_pools(pools, refs.device, int(refs.shape[0]))
-    written = {"refs": refs, "tables": tables}
-    if lengths is not None:
-        written["lengths"] = lengths
-    _check_apart({**written, **{f"pool {i}": t for i, t in enumerate(pools)}}, requests)
-    return page_size, pools
+    _check_pools(pools, refs.device, int(refs.shape[0]))
+    return reaches(*((refs, tables) if lengths is None else (refs, tables, lengths)), *pools), reaches(*requests.values())
 
 
 def _buffers(refs: torch.Tensor, requests: int, results: int) -> Tuple[torch.Tensor, torch.Tensor]:

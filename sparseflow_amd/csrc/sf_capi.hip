@@ -1144,6 +1144,9 @@ int pages_args(const sf_pages_desc* d, sf::PagesArgs& a) {
       return fail(SF_ERR_INVALID, "NULL pointer or negative size of a pool");
     a.pools.at[i] = static_cast<uint8_t*>(d->pool[i]);
     a.pools.bytes[i] = d->page_bytes[i];
+    const bool whole = d->page_bytes[i] % 16 == 0 && sf::aligned_to(d->pool[i], 16);
+    a.pools.units[i] = (i > 0 ? a.pools.units[i - 1] : 0) + (whole ? d->page_bytes[i] / 16 : 0);
+    if (!whole) a.pools.odd = 1;
   }
   a.pools.count = d->pools;
   a.pages = d->pages;
@@ -1161,7 +1164,8 @@ int pages_workspace(sf::PagesArgs& a, void* workspace, size_t bytes) {
   a.need = a.counts + 4;
   a.first = a.need + a.requests;
   a.old = a.first + a.requests;
-  a.list = a.old + a.requests;
+  a.shared = a.old + a.requests;
+  a.list = a.shared + a.requests;
   a.to = a.list + a.pages;
   return SF_OK;
 }
@@ -1169,7 +1173,7 @@ int pages_workspace(sf::PagesArgs& a, void* workspace, size_t bytes) {
 }  // namespace
 
 size_t sf_pages_workspace_size(int64_t pages, int64_t requests) {
-  return pages < 0 || requests < 0 ? 0 : (size_t)(4 + 3 * requests + 2 * pages) * 4;
+  return pages < 0 || requests < 0 ? 0 : (size_t)(4 + 4 * requests + 2 * pages) * 4;
 }
 
 int sf_pages_resize(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int32_t* lengths, const int32_t* rows,

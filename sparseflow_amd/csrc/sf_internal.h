@@ -447,8 +447,9 @@ int launch_mx4_attn(const Mx4AttnArgs& a, int dtype, hipStream_t stream);
 constexpr int kMaxPools = 16;
 struct PagePools {
   uint8_t* at[kMaxPools];
-  int64_t bytes[kMaxPools];  // of a page
-  int count;
+  int64_t bytes[kMaxPools];    // of a page
+  int64_t units[kMaxPools];    // where a pool's 16-byte units end among all pools' (none: 16 does not divide its pages)
+  int count, odd;              // odd: some pool has none
 };
 struct PagesArgs {
   int32_t* refs;
@@ -460,6 +461,7 @@ struct PagesArgs {
   int32_t* need;         // workspace: [requests] pages that a request needs, -1: refused
   int32_t* first;        //            [requests] the first of them in `list`
   int32_t* old;          //            [requests] the length before (a fork: the parent's)
+  int32_t* shared;       //            [requests] a resize: the page that a copy replaces
   int32_t* list;         //            [pages] free pages in order; compaction: sources
   int32_t* to;           //            [pages] compaction: targets
   int32_t* counts;       //            [2] entries of list; compaction: moves

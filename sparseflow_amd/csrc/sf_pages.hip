@@ -1,10 +1,10 @@
 // The pages of a cache: sequences that grow, shrink, fork and end, and pools that are
 // compacted.  Everything is on the device, so that a serving step can be captured.
 //
-// A call is a few small kernels in turn: one workgroup to a request looks what it needs
-// (and gives back what it frees), one workgroup deals the free pages out, lowest first, to
-// the requests in turn, and workgroups write the tables and copy the pages.  Times are those
-// of the launches, and of the copies.
+// A call is two or three small kernels in turn: one workgroup to a request looks what it needs
+// (and gives back what it frees), one workgroup deals the free pages out, lowest first, to the
+// requests in turn, and workgroups write the tables and copy the pages.  Times are those of the
+// launches, and of the copies.
 #include "sf_seq.h"
 
 namespace sf {
@@ -104,7 +104,10 @@ __global__ __launch_bounds__(kDealThreads) void k_pages_deal(PagesArgs a) {
         const int64_t old = a.old[q], row = a.rows[q], last = old / a.page_size;
         if (a.other[q] > old && old % a.page_size != 0 && last < a.width) {
           const int64_t p = a.tables[row * a.width + last];
-          if (page_ok(a, p) && a.refs[p] > 1) need += 1 << 30;  // (widths are below 2^30)
+          if (page_ok(a, p) && a.refs[p] > 1) {
+            need += 1 << 30;  // (widths are below 2^30)
+            a.shared[q] = (int32_t)p;
+          }
         }
         a.need[q] = (int32_t)need;
         need = (need & ((1 << 30) - 1)) + (need >> 30);
@@ -134,19 +137,35 @@ __global__ __launch_bounds__(kDealThreads) void k_pages_deal(PagesArgs a) {
   if (threadIdx.x == 0) a.counts[0] = (int32_t)found;
 }
 
-// Copies page `from` of every pool to page `to`, the workgroup's share of it.
+// Copies page `from` of every pool to page `to`, the workgroup's share of it: the pools' 16-byte
+// units one pool after another, four of a thread under way at a time.  (A page of 68 KB in four
+// pools by one workgroup, pool by pool: 221 us for a compaction that moves 4100 of them.)
 __device__ __forceinline__ void copy_page(const PagePools& pools, int64_t from, int64_t to, int part, int parts) {
-  for (int i = 0; i < pools.count; ++i) {
-    const int64_t bytes = pools.bytes[i];
-    const uint8_t* s = pools.at[i] + from * bytes;
-    uint8_t* d = pools.at[i] + to * bytes;
-    if (((uintptr_t)pools.at[i] | (uintptr_t)bytes) % 16 == 0) {
-      typedef uint32_t V __attribute__((ext_vector_type(4)));
-      for (int64_t k = part * (int)blockDim.x + threadIdx.x; k < bytes / 16; k += parts * blockDim.x)
-        reinterpret_cast<V*>(d)[k] = reinterpret_cast<const V*>(s)[k];
-    } else {
-      for (int64_t k = part * (int)blockDim.x + threadIdx.x; k < bytes; k += parts * blockDim.x) d[k] = s[k];
+  typedef uint32_t V __attribute__((ext_vector_type(4)));
+  const int64_t all = pools.count > 0 ? pools.units[pools.count - 1] : 0, per = (all + parts - 1) / parts;
+  const int64_t begin = part * per, end = begin + per < all ? begin + per : all;
+  for (int64_t k = begin + threadIdx.x; k < end; k += 4 * kPageThreads) {
+    V v[4];
+    V* d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = k + u * kPageThreads < end ? k + u * kPageThreads : end - 1;
+      int i = 0;
+      while (at >= pools.units[i]) ++i;
+      const int64_t off = 16 * (at - (i > 0 ? pools.units[i - 1] : 0));
+      v[u] = *reinterpret_cast<const V*>(pools.at[i] + from * pools.bytes[i] + off);
+      d[u] = reinterpret_cast<V*>(pools.at[i] + to * pools.bytes[i] + off);
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (k + u * kPageThreads < end) *d[u] = v[u];
+  }
+  if (!pools.odd) return;
+  for (int i = 0; i < pools.count; ++i) {
+    if (pools.units[i] > (i > 0 ? pools.units[i - 1] : 0)) continue;
+    const int64_t bytes = pools.bytes[i];
+    for (int64_t k = part * kPageThreads + threadIdx.x; k < bytes; k += parts * kPageThreads)
+      pools.at[i][to * bytes + k] = pools.at[i][from * bytes + k];
   }
 }
 
@@ -161,31 +180,19 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grown(PagesArgs a, int p
   const bool ok = need >= 0 && (need == 0 || a.first[q] + need <= a.counts[0]);
   if (part == 0 && threadIdx.x == 0) a.granted[q] = ok;
   if (!ok || size <= old) return;
-  int32_t* table = a.tables + row * a.width;
-  const int64_t have = pages_of(old, a.page_size), shared = raw >> 30;
-  if (shared) {
-    const int64_t to = a.list[a.first[q]];
-    // (The page it replaces: its table's entry changes in k_pages_placed.)
-    copy_page(a.pools, table[have - 1], to, part, parts);
-  }
-}
-
-__global__ __launch_bounds__(kPageThreads) void k_pages_placed(PagesArgs a) {
-  const int64_t q = blockIdx.x;
-  const int32_t raw = a.need[q];
-  const int64_t old = a.old[q], size = a.other[q], row = a.rows[q];
-  if (!a.granted[q] || size <= old) return;
-  int32_t* table = a.tables + row * a.width;
-  const int64_t have = pages_of(old, a.page_size), shared = raw >> 30, end = pages_of(size, a.page_size);
-  const int64_t first = a.first[q];
-  if (shared && threadIdx.x == 0) atomicSub(a.refs + table[have - 1], 1);
-  __syncthreads();
-  for (int64_t i = have - shared + threadIdx.x; i < end; i += kPageThreads) {
-    const int32_t p = a.list[first + i - (have - shared)];
-    table[i] = p;
+  const int64_t first = a.first[q], shared = raw >> 30;
+  if (shared) copy_page(a.pools, a.shared[q], a.list[first], part, parts);
+  if (part != 0) return;
+  const int64_t from = pages_of(old, a.page_size) - shared, end = pages_of(size, a.page_size);
+  for (int64_t i = from + threadIdx.x; i < end; i += kPageThreads) {
+    const int32_t p = a.list[first + i - from];
+    a.tables[row * a.width + i] = p;
     a.refs[p] = 1;
   }
-  if (threadIdx.x == 0) a.lengths[row] = (int32_t)size;
+  if (threadIdx.x == 0) {
+    if (shared) atomicSub(a.refs + a.shared[q], 1);
+    a.lengths[row] = (int32_t)size;
+  }
 }
 
 // A fork's child: shares the parent's full pages and has the last, partial one copied.
@@ -257,25 +264,26 @@ __global__ __launch_bounds__(kDealThreads) void k_pages_moves(PagesArgs a) {
   }
 }
 
-// The moves' copies, and their pages' users.
-__global__ __launch_bounds__(kPageThreads) void k_pages_move(PagesArgs a) {
+// The first kMoveBlocks workgroups make the moves' copies and move their pages' users, the others
+// rename the moved pages in the tables: they look for them among the sources, which are in order.
+constexpr int kMoveBlocks = 2048, kRenameBlocks = 512;
+__global__ __launch_bounds__(kPageThreads) void k_pages_move(PagesArgs a, int parts) {
   const int64_t moves = a.counts[0];
-  for (int64_t i = blockIdx.x; i < moves; i += gridDim.x) {
-    const int64_t from = a.list[i], to = a.to[i];
-    copy_page(a.pools, from, to, 0, 1);
-    if (threadIdx.x == 0) {
-      a.refs[to] = a.refs[from];
-      a.refs[from] = 0;
+  if (blockIdx.x < kMoveBlocks) {
+    for (int64_t w = blockIdx.x; w < moves * parts; w += kMoveBlocks) {
+      const int64_t i = w / parts;
+      const int32_t from = a.list[i], to = a.to[i];
+      copy_page(a.pools, from, to, (int)(w - i * parts), parts);
+      if (w == i * parts && threadIdx.x == 0) {
+        a.refs[to] = a.refs[from];
+        a.refs[from] = 0;
+      }
     }
+    return;
   }
-}
-
-// Table entries of moved pages: found among the sources, which are in order.
-__global__ __launch_bounds__(kPageThreads) void k_pages_rename(PagesArgs a) {
-  const int64_t moves = a.counts[0];
   if (moves == 0) return;
   const int64_t low = a.list[0], n = a.states * a.width;
-  for (int64_t i = (int64_t)blockIdx.x * kPageThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kPageThreads) {
+  for (int64_t i = (int64_t)(blockIdx.x - kMoveBlocks) * kPageThreads + threadIdx.x; i < n; i += kRenameBlocks * kPageThreads) {
     const int32_t p = a.tables[i];
     if (p < low || p >= a.pages) continue;
     int64_t lo = 0, hi = moves;
@@ -315,7 +323,6 @@ int launch_pages_resize(const PagesArgs& a, hipStream_t stream) {
   k_pages_release<<<n, kPageThreads, 0, stream>>>(a);
   k_pages_deal<true><<<1, kDealThreads, 0, stream>>>(a);
   k_pages_grown<<<n * parts, kPageThreads, 0, stream>>>(a, parts);
-  k_pages_placed<<<n, kPageThreads, 0, stream>>>(a);
   timing_end(K_PAGES, stream);
   return last_error();
 }
@@ -334,8 +341,7 @@ int launch_pages_fork(const PagesArgs& a, hipStream_t stream) {
 int launch_pages_compact(const PagesArgs& a, hipStream_t stream) {
   timing_begin(K_PAGES, stream);
   k_pages_moves<<<1, kDealThreads, 0, stream>>>(a);
-  k_pages_move<<<2048, kPageThreads, 0, stream>>>(a);
-  k_pages_rename<<<512, kPageThreads, 0, stream>>>(a);
+  k_pages_move<<<kMoveBlocks + kRenameBlocks, kPageThreads, 0, stream>>>(a, page_parts(a));
   timing_end(K_PAGES, stream);
   return last_error();
 }
