@@ -669,7 +669,7 @@ Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_head
     p.parts = units == 1 ? 0 : 2 * p.shares * 16;
   } else {
     // As many parts of the tokens as fill the CUs, each of 256 tokens or more.
-    int64_t splits = items == 0 ? 1 : 512 / items;
+    int64_t splits = items == 0 ? 1 : (3072 + items - 1) / items;
     const int64_t most = (room + 255) / 256;
     splits = splits > most ? most : splits;
     p.splits = (int)(splits < 1 ? 1 : splits);
