@@ -16,6 +16,7 @@ namespace {
 
 // The fewest tiles of a size that it is taken for: what is left of a round of the CUs.
 constexpr int64_t kGemmTiles = 192;
+constexpr int64_t kCus = 256;
 
 // What a load of columns that are not there reads.
 __device__ const u32x4 kNothing = {0, 0, 0, 0};
@@ -106,7 +107,6 @@ __device__ __forceinline__ void gemm_store(const Mx4LinearArgs& a, const f32x16 
 template <int MT, int NT>
 __device__ __forceinline__ void gemm_store(const Mx4LinearArgs& a, const f32x16 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane,
                                            int wave, char* smem) {
-  __syncthreads();  // (the stages are done with)
   char* lds = smem + wave * 32 * kEpilogueRow;
   if (a.y_dtype == SF_BF16) gemm_store<__hip_bfloat16>(a, acc, m0, n0, lane, lds);
   else if (a.y_dtype == SF_F16) gemm_store<__half>(a, acc, m0, n0, lane, lds);
@@ -126,13 +126,13 @@ struct Shape {
 
 // The sums begin with the bias of their columns from n0.
 template <int MT, int NT>
-__device__ __forceinline__ void gemm_begin(const Mx4LinearArgs& a, int64_t n0, int h, f32x16 (&acc)[MT][NT]) {
+__device__ __forceinline__ void gemm_begin(const Mx4LinearArgs& a, int64_t n0, int h, f32x16 (&acc)[MT][NT], bool bias = true) {
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int64_t c = n0 + 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
-      const float b = a.bias == nullptr ? 0.f : a.bias[c < a.n ? c : a.n - 1];
+      const float b = a.bias == nullptr || !bias ? 0.f : a.bias[c < a.n ? c : a.n - 1];
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i][j][e] = b;
     }
@@ -244,6 +244,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_bf16(Mx4LinearArgs a
       }
     }
   }
+  __syncthreads();  // (the stages are done with)
   gemm_store(a, acc, m0 + wm, n0 + wc, lane, wave, smem);
 }
 
@@ -353,6 +354,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_four(Mx4LinearArgs a
       }
     }
   }
+  __syncthreads();  // (the stages are done with)
   gemm_store(a, acc, m0 + wm, n0 + wc, lane, wave, smem);
 }
 
@@ -361,6 +363,11 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_four(Mx4LinearArgs a
 // Two stages in LDS, and the two after them on their way in registers: loaded as they lie,
 // taken apart and written to LDS while the stage before is worked on.  A barrier does not wait
 // for loads.  (With x loaded one stage ahead only, bf16 of 8192 x 4100 x 16380: 1990 us.)
+//
+// KG groups of wavefronts take stages in turn, each with LDS of its own, and add up what they
+// have at the end: where y has no more tiles than there are CUs, the time is a tile's stages one
+// after another, half a us each (128 x 4096 x 4096: bf16 32.6 -> 20.4 us, f32 63.6 -> 40.2;
+// 128 x 8192 x 1024: 61 -> 33, 123 -> 77).
 template <typename P, int NP>
 struct alignas(16) AnyStage {
   uint16_t x[NP][P::BM][64];
@@ -370,13 +377,14 @@ struct alignas(16) AnyStage {
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <typename T, typename P>
-__global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_any(Mx4LinearArgs a) {
+template <typename T, typename P, int KG>
+__global__ __launch_bounds__(P::threads* KG, KG == 4 ? 4 : 2) void k_mx4_gemm_any(Mx4LinearArgs a) {
   constexpr int NP = Parts<T>::n, XL = P::BM * 8 / P::threads, RL = P::threads / 8, WL = P::BN * 2 < P::threads ? 1 : P::BN * 2 / P::threads;
   static_assert(P::BM * 8 % P::threads == 0 && (P::BN * 2 % P::threads == 0 || P::threads % (P::BN * 2) == 0), "whole loads to a thread");
   extern __shared__ __align__(16) char smem[];
-  auto* stage = reinterpret_cast<AnyStage<P, NP>*>(smem);
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane & 31, h = lane >> 5;
+  const int lane = lane_id(), wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane & 31, h = lane >> 5;
+  const int group = wave_all / P::waves, wave = wave_all % P::waves, tid = threadIdx.x % P::threads;
+  auto* stage = reinterpret_cast<AnyStage<P, NP>*>(smem) + 2 * group;
   int64_t mi, ni;
   gemm_tile(a.block0 + blockIdx.x, (a.m + P::BM - 1) / P::BM, a.n_tiles, mi, ni);
   const int64_t m0 = mi * P::BM, n0 = ni * P::BN;
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_any(Mx4LinearArgs a)
 
   // Unit tid % 8 of x's rows tid / 8 + RL i; block tid % 2 of the weights' rows tid / 2 + threads / 2 i
   // (more threads than blocks: some load the same).
-  const int xr = threadIdx.x >> 3, xu = threadIdx.x & 7, wt = threadIdx.x % (2 * P::BN), wr = wt >> 1, wu = wt & 1;
+  const int xr = tid >> 3, xu = tid & 7, wt = tid % (2 * P::BN), wr = wt >> 1, wu = wt & 1;
   const T* xp[XL];
   const uint8_t *wp[WL], *sp[WL];
 #pragma unroll
@@ -439,7 +447,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_any(Mx4LinearArgs a)
 
   const int wm = wave % P::WM * (32 * P::MT), wc = wave / P::WM * (32 * P::NT);
   f32x16 acc[P::MT][P::NT];
-  gemm_begin(a, n0 + wc, h, acc);
+  gemm_begin(a, n0 + wc, h, acc, group == 0);
   auto work = [&](const AnyStage<P, NP>& t) {
     u32x4 codes[P::NT];
     float scale[P::NT];
@@ -469,25 +477,26 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_any(Mx4LinearArgs a)
   if (whole > 0) {
     // (Behind the last whole stage it is loaded again: loads that only some iterations make would
     // be waited for at once.)
-    auto up_to = [&](int s) { return s < whole ? s : whole - 1; };
+    auto stage_of = [&](int i) { return group + KG * i < whole ? group + KG * i : whole - 1; };
+    const int turns = (whole + KG - 1) / KG;
     Raw raw[2];
-    load(0, raw[0]);
-    load(up_to(1), raw[1]);
+    load(stage_of(0), raw[0]);
+    load(stage_of(1), raw[1]);
     put(raw[0], stage[0]);
-    load(up_to(2), raw[0]);
+    load(stage_of(2), raw[0]);
     lds_barrier();
-    for (int s = 0; s < whole; s += 2) {
+    for (int i = 0; i < turns; i += 2) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (s + u >= whole) break;
-        work(stage[u]);
+        if (i + u >= turns) break;
+        if (KG == 1 || group + KG * (i + u) < whole) work(stage[u]);
         put(raw[1 - u], stage[1 - u]);
-        load(up_to(s + u + 3), raw[1 - u]);
+        load(stage_of(i + u + 3), raw[1 - u]);
         lds_barrier();
       }
     }
   }
-  if (a.k % 64 != 0) {
+  if (a.k % 64 != 0 && group == 0) {
     Raw end;
 #pragma unroll
     for (int i = 0; i < XL; ++i)
@@ -503,21 +512,54 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_any(Mx4LinearArgs a)
       end.s[i] = there ? sp[i][2 * (int64_t)whole] : 0;
     }
     put(end, stage[0]);
+  }
+  if (a.k % 64 != 0) {
     lds_barrier();
-    work(stage[0]);
+    if (group == 0) work(stage[0]);
+  }
+  if constexpr (KG > 1) {
+    // A wavefront's sums of the groups behind the first, [tile, element, lane].
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);
+    constexpr int per = P::MT * P::NT * 16 * kWave;
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < P::NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            sums[((group - 1) * P::waves + wave) * per + ((i * P::NT + j) * 16 + e) * kWave + lane] = acc[i][j][e];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+        for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+          for (int j = 0; j < P::NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[(g * P::waves + wave) * per + ((i * P::NT + j) * 16 + e) * kWave + lane];
+    }
+    if (group > 0) return;
+  } else {
+    __syncthreads();  // (the stages are done with)
   }
   gemm_store(a, acc, m0 + wm, n0 + wc, lane, wave, smem);
 }
 
-template <auto K, typename P, typename Stage>
+template <auto K, typename P, typename Stage, int KG = 1>
 int launch_gemm(Mx4LinearArgs a, hipStream_t stream) {
-  constexpr int stages = P::S * (int)sizeof(Stage), rows = P::waves * 32 * kEpilogueRow, lds = stages > rows ? stages : rows;
+  constexpr int stages = KG * P::S * (int)sizeof(Stage), rows = P::waves * 32 * kEpilogueRow;
+  constexpr int sums = (KG - 1) * P::waves * P::MT * P::NT * 16 * kWave * 4;
+  constexpr int most = rows > sums ? rows : sums, lds = stages > most ? stages : most;
   static_assert(lds <= kMaxLdsBytes, "LDS");
   const int rc = set_lds_limit_once<K>(lds);
   if (rc != (int)hipSuccess) return rc;
   a.n_tiles = (a.n + P::BN - 1) / P::BN;
   return launch_blocks(a, &Mx4LinearArgs::block0, a.n_tiles * ((a.m + P::BM - 1) / P::BM),
-                       [&](const Mx4LinearArgs& part, unsigned grid) { K<<<grid, P::threads, lds, stream>>>(part); });
+                       [&](const Mx4LinearArgs& part, unsigned grid) { K<<<grid, P::threads * KG, lds, stream>>>(part); });
 }
 
 template <typename P>
@@ -528,9 +570,9 @@ template <typename P>
 int launch_four(const Mx4LinearArgs& a, hipStream_t stream) {
   return launch_gemm<k_mx4_gemm_four<P>, P, FourStage<P>>(a, stream);
 }
-template <typename T, typename P>
+template <typename T, typename P, int KG>
 int launch_any(const Mx4LinearArgs& a, hipStream_t stream) {
-  return launch_gemm<k_mx4_gemm_any<T, P>, P, AnyStage<P, Parts<T>::n>>(a, stream);
+  return launch_gemm<k_mx4_gemm_any<T, P, KG>, P, AnyStage<P, Parts<T>::n>, KG>(a, stream);
 }
 
 // How many tiles of bm x bn y has.
@@ -539,10 +581,13 @@ int64_t tiles_of(const Mx4LinearArgs& a, int bm, int bn) { return (a.m + bm - 1)
 template <typename T>
 int launch_any(const Mx4LinearArgs& a, hipStream_t stream) {
   if constexpr (Parts<T>::n == 1) {
-    if (tiles_of(a, 256, 256) >= kGemmTiles) return launch_any<T, Shape<4, 2, 2, 4, 2>>(a, stream);
+    if (tiles_of(a, 256, 256) >= kGemmTiles) return launch_any<T, Shape<4, 2, 2, 4, 2>, 1>(a, stream);
   }
-  if (tiles_of(a, 128, 256) >= kGemmTiles) return launch_any<T, Shape<2, 4, 2, 2, 2>>(a, stream);
-  return launch_any<T, Shape<2, 2, 1, 1, 2>>(a, stream);
+  if (tiles_of(a, 128, 256) >= kGemmTiles) return launch_any<T, Shape<2, 4, 2, 2, 2>, 1>(a, stream);
+  // (2050 x 6000, bf16 / f32 in us: 64 rows of 94 tiles take 13.4 / 25.1 in groups and 15.6 / 38.3
+  // without, 256 rows of 376 tiles 26.7 / 50.4 and 21.4 / 49.7.)
+  if (tiles_of(a, 64, 64) <= kCus) return launch_any<T, Shape<2, 2, 1, 1, 2>, Parts<T>::n == 1 ? 4 : 2>(a, stream);
+  return launch_any<T, Shape<2, 2, 1, 1, 2>, 1>(a, stream);
 }
 
 }  // namespace
@@ -563,8 +608,11 @@ int launch_mx4_gemm(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   const bool direct = aligned_to(a.x, 16) && a.x_stride % 8 == 0 && a.k % 8 == 0 && a.blocks % 4 == 0 &&
                       aligned_to(a.w_scales, 4) && a.x_stride >= 0 && a.x_stride < 1 << 22 && a.blocks < 1 << 19;
   if (!direct) return launch_any<__hip_bfloat16>(a, stream);
+  // (The smallest tiles, one to a CU: 100 x 4096 x 4096 20.6 us in groups of stages, 32.5 here.)
+  const bool few = tiles_of(a, 64, 64) <= kCus;
   return large    ? launch_bf16<Shape<4, 2, 2, 4, 3>>(a, stream)
          : middle ? launch_bf16<Shape<2, 2, 2, 2, 3>>(a, stream)
+         : few    ? launch_any<__hip_bfloat16>(a, stream)
                   : launch_bf16<Shape<2, 2, 1, 1, 6>>(a, stream);
 }
 

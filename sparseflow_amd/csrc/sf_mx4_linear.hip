@@ -188,7 +188,13 @@ int launch_linear(const Mx4LinearArgs& a, hipStream_t stream) {
 
 int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   timing_begin(K_MX4_LINEAR, stream);
-  const bool tiles = a.m > 64 && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
+  // Where tiles of 64 rows fill the CUs by themselves they are better from 33 rows on; with less
+  // of them, a wavefront to few columns reads W sooner (x K x N in us, this kernel / tiles; 64 x
+  // 4096 x 12288: bf16 41 / 22, f32 102 / 45, four 25 / 16; 33 x 4096 x 4096: bf16 13 / 20, f32
+  // 45 / 39, four 9 / 14; 48 x 8192 x 1024: bf16 29 / 34, f32 69 / 74, four 18 / 27; 17 to 32
+  // rows: never worse by more than a us).
+  const int64_t filling = x_dtype == SF_F32 ? 2048 : 10240;
+  const bool tiles = a.m > (a.n > filling ? 32 : 64) && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
   const int rc = tiles                ? launch_mx4_gemm(a, x_dtype, stream)
                  : x_dtype == SF_MX4  ? launch_linear<Four>(a, stream)
                  : x_dtype == SF_F16  ? launch_linear<__half>(a, stream)
