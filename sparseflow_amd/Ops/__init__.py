@@ -1,4 +1,6 @@
 """nn.Module wrappers of the sparse kernels (Ops/ of the reference)."""
+from .cached_attention import CachedAttention  # noqa: F401
+from .mx4_linear import MX4Linear, quantize_linears_  # noqa: F401
 from .sparse_attention import SparseAttention  # noqa: F401
 from .sparse_attention_block import SparseAttentionBlock  # noqa: F401
 from .sparse_bmm import SparseBMM, SparseMatmul  # noqa: F401

@@ -186,6 +186,16 @@ class DispatchAudit:
             self.mismatch += 1
 
 
+def host_parents(parents: torch.Tensor, batch: int) -> torch.Tensor:
+    """The sequences of a batch that go on in each other's places, checked: int64 on the host."""
+    if tuple(parents.shape) != (batch,) or parents.is_floating_point() or parents.dtype == torch.bool:
+        raise ValueError(f"parents is {tuple(parents.shape)} {parents.dtype}: ({batch},) integers are wanted")
+    parents = parents.detach().cpu().long()
+    if batch and not 0 <= int(parents.min()) <= int(parents.max()) < batch:
+        raise ValueError(f"parents from {int(parents.min())} to {int(parents.max())}: sequences 0 to {batch - 1} are wanted")
+    return parents
+
+
 def bias_rows(bias: Optional[torch.Tensor], lead, channels: int, trailing, dtype, device) -> torch.Tensor:
     """A fresh tensor of shape (*lead, channels, *trailing) holding bias[c]
     at every position (zeros without a bias): the exact output of a conv or

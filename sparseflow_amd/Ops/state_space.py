@@ -18,7 +18,7 @@ import torch.nn as nn
 from ..Kernels.block_norm import block_norm_forward
 from ..Kernels.causal_conv1d import causal_conv1d_forward, causal_conv1d_step
 from ..Kernels.selective_scan import selective_scan_forward, selective_scan_step
-from ._runtime import WeightLayout
+from ._runtime import WeightLayout, host_parents
 
 
 def _cast(param: torch.Tensor) -> torch.Tensor:
@@ -46,6 +46,11 @@ class _Stateful(nn.Module):
 
     def reset(self):
         self.state = None
+
+    def select(self, parents: torch.Tensor) -> None:
+        """Sequence i becomes what sequence parents[i] was (integers [batch])."""
+        if self.state is not None:
+            self.state = self.state.index_select(0, host_parents(parents, self.state.shape[0]).to(self.state.device))
 
     def _state_for(self, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device) -> Optional[torch.Tensor]:
         """The kept state, if it is one for such a batch (as the neurons decide)."""

@@ -347,11 +347,11 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
 #pragma unroll
       for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
     }
-    const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
+    const float from = ref_from<NP>(ref);
     float pr[8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      pr[k] = exp2_hw(fmaf(s[k >> 2][k & 3], c2, -from));
+      pr[k] = weight_of<NP>(s[k >> 2][k & 3], c2, from);
       sum += pr[k];
     }
     l += sum;

@@ -196,13 +196,13 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
 #pragma unroll
         for (int d = 0; d < NB; ++d) o[d] *= back;
       }
-      const float from = ref == -INFINITY ? 0.f : ref;  // (a row that has seen nothing yet)
+      const float from = ref_from<NP>(ref);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[u][e] = exp2_hw(fmaf(s[u][e], c2, -from));
+          s[u][e] = weight_of<NP>(s[u][e], c2, from);
           sum[e & 3] += s[u][e];
         }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);

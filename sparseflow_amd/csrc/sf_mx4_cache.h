@@ -68,8 +68,22 @@ __device__ __forceinline__ void weight_parts(const float (&w)[8], bf16x8 (&p)[NP
 __device__ __forceinline__ float score_factor(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1e-44f); }
 
 // The running maximum of a row's exponents is `ref`; it moves only where it would be passed by
-// more than this, so that the sums are seldom rescaled: weights stay below 2^8.
-constexpr float kRefSlack = 8.f;
+// more than this, so that the sums are seldom rescaled.  Weights are 2^(exponent - ref - 30),
+// below 2^-22: up to 2^22 of them times values at the end of float32 stay in its range.  (What
+// goes missing at the other end, products below 2^-126, is less than 2^-96 a token.)
+constexpr float kRefSlack = 8.f, kRefRoom = 30.f;
+
+// A weight: with 16-bit weights in one rounding of its exponent (2^-19 of it at 38); where they
+// are held in parts the exponent stays small, and the room is a factor.
+template <int NP>
+__device__ __forceinline__ float ref_from(float ref) {
+  return ref == -INFINITY ? 0.f : NP == 1 ? ref + kRefRoom : ref;  // (a row that has seen nothing yet)
+}
+template <int NP>
+__device__ __forceinline__ float weight_of(float score, float c2, float from) {
+  const float w = exp2_hw(fmaf(score, c2, -from));
+  return NP == 1 ? w : w * 0x1p-30f;
+}
 
 // Values from scale 253 on are no numbers or beyond a float's range at times, and 0 times such
 // a one is no 0: they lie in LDS as zeros, and each row adds those that it sees itself.  Column

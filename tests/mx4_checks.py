@@ -111,11 +111,13 @@ def attention_case(dev, new, old, heads, kv, dim, page, dtype, packed, seed=0, s
 
 def attention_bound(dtype, dim, tokens, y, mag, big):
     """Scores are off by (parts dim + 8) steps of sum |q k| scale log2(e); the weights by that, the exponential's and a
-    16-bit weight's rounding; sums over the tokens by their number of steps; then the result's rounding."""
+    16-bit weight's rounding; sums over the tokens by their number of steps; then the result's rounding.  Weights are held
+    as 2^-30 of themselves and the largest is 1 at least, so that a part of a weight, or of a product, below float32's
+    normal numbers (2^-126) is 2^-96 of the result's scale: for values below 8, (8 + 1) 2^-96 for each part and token."""
     parts = PARTS[dtype]
     score = (parts * dim + 8) * STEP * big * 1.5
     weight = 2 * score + 8 * STEP + (half_step(torch.bfloat16) if parts == 1 else 2.0 ** -15 if parts == 2 else 0.0)
-    return mag * (weight[..., None] + (parts * tokens + 8) * 2 * STEP) + half_step(dtype) * y.abs()
+    return mag * (weight[..., None] + (parts * tokens + 8) * 2 * STEP) + half_step(dtype) * y.abs() + parts * tokens * 9 * 2.0 ** -96
 
 
 def check_attention(dev, new, old, heads, kv, dim, page, dtype, packed=True, step=False, seed=0):
