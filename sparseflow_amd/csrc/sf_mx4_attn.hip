@@ -657,9 +657,9 @@ Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_head
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.splits = 1;
   const int64_t items = batch * kv_heads * p.tiles;
+  const int parts = dtype == SF_F32 ? 3 : dtype == SF_F16 ? 2 : 1;
   if (p.tile_rows == 16) {
     // Workgroups: what the CUs hold of them (by registers).  Short tables: a tile is one unit.
-    const int parts = dtype == SF_F32 ? 3 : dtype == SF_F16 ? 2 : 1;
     p.unit = room <= 512 ? 4 : 1;
     const int64_t tokens = kAttnTokens * kAttnUnit * p.unit, units = room <= tokens ? 1 : (room + tokens - 1) / tokens;
     const int64_t hold = blocks * parts <= 2 ? 768 : blocks * parts <= 8 ? 512 : 256;
@@ -668,9 +668,13 @@ Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_head
     p.shares = p.shares < 1 ? 1 : p.shares;
     p.parts = units == 1 ? 0 : 2 * p.shares * 16;
   } else {
-    // As many parts of the tokens as fill the CUs, each of 256 tokens or more.
-    int64_t splits = items == 0 ? 1 : (3072 + items - 1) / items;
-    const int64_t most = (room + 255) / 256;
+    // Parts of the tokens only while all of them are on the CUs at once (of what they hold, by
+    // registers), and where a part is long enough to be worth its rows' way through memory (bf16,
+    // 32 / 8 heads of 128, 1024 tokens: 38 us whole, 63 in two parts; 188 tiles of 8000 tokens: 205
+    // and 155; with parts up to six times what the CUs hold, 256 tiles of 2048: 66 whole, 117).
+    const int64_t hold = blocks <= 4 && blocks * parts <= 8 ? 512 : 256;
+    int64_t splits = items == 0 || room < 2048 ? 1 : hold / items;
+    const int64_t most = room / 256;
     splits = splits > most ? most : splits;
     p.splits = (int)(splits < 1 ? 1 : splits);
     p.parts = p.splits == 1 ? 0 : items * p.splits * p.tile_rows;
