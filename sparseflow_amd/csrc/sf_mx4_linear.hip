@@ -15,8 +15,9 @@ namespace {
 // A wavefront takes 16 NT weight rows and 16 MT rows of x.  In a step of 128 columns lane
 // (r, g) = (lane % 16, lane / 16) holds the whole block g of a weight row r, 16 bytes and one
 // scale, and block g of x row r: instruction j takes columns 32 g + 8 j .. + 7 of both (the
-// order of a sum's terms is free).  The wavefronts of a workgroup take steps in turn, U of them
-// loaded before the first is worked on; their sums meet in LDS.
+// order of a sum's terms is free).  The wavefronts of a workgroup take steps in turn, or U steps
+// of which a lane has U blocks next to each other, loaded before the first is worked on; their
+// sums meet in LDS.
 struct Four {};  // x in the format
 
 template <typename T>
@@ -124,16 +125,17 @@ __global__ __launch_bounds__(W* kWave) void k_mx4_linear_rows(Mx4LinearArgs a) {
 #pragma unroll
     for (int q = 0; q < NT; ++q) acc[t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int steps = (a.blocks + 3) / 4, whole = (int)(a.k / (4 * kMx4Block));
-  int s = __builtin_amdgcn_readfirstlane(wave);
-  for (; s + W * (U - 1) < whole; s += W * U) {
+  const int steps = (a.blocks + 3) / 4, whole = (int)(a.k / (4 * U * kMx4Block));
+  const int first = __builtin_amdgcn_readfirstlane(wave);
+  for (int s = first; s < whole; s += W) {
     RowsStep<T, MT, NT> e[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) e[u].template load<true>(a, wrow, m, 4 * (s + W * u) + g);
+    for (int u = 0; u < U; ++u) e[u].template load<true>(a, wrow, m, U * (4 * s + g) + u);
 #pragma unroll
     for (int u = 0; u < U; ++u) e[u].add(acc);
   }
-  for (; s < steps; s += W) {
+  // (The rest begins with the wavefront whose turn it is.)
+  for (int s = U * whole + ((first - whole) & (W - 1)); s < steps; s += W) {
     RowsStep<T, MT, NT> e;
     e.template load<false>(a, wrow, m, 4 * s + g);
     e.add(acc);
@@ -171,12 +173,31 @@ int launch_rows(Mx4LinearArgs a, hipStream_t stream) {
   });
 }
 
+template <typename T>
+constexpr bool four_bits = std::is_same<T, Four>::value;
+
 // Weight rows by how many workgroups they make.
 template <typename T, int MT>
 int launch_rows_n(const Mx4LinearArgs& a, hipStream_t stream) {
-  if (a.n > 64 * 160) return launch_rows<T, MT, MT == 4 ? 2 : 4, 8, 1>(a, stream);
-  if (a.n > 32 * 160) return launch_rows<T, MT, 2, 8, 1>(a, stream);
-  return launch_rows<T, MT, 1, MT == 4 ? 8 : 16, 1>(a, stream);
+  if constexpr (MT == 1) {
+    // As long as x is little beside W, few weight rows a workgroup and four blocks of each at a
+    // time (128 bytes of a weight row in one place; x K x N in us: 1 x 4096 x 12288 bf16 12.5 ->
+    // 10.4, four 11.7 -> 8.5, 1 x 12288 x 4096 bf16 13.4 -> 11.4, 16 x 12288 x 4096 f32 41 -> 34;
+    // but 16 x 12288 x 4096 bf16 20 -> 22, 4 x 8192 x 8192 bf16 15 -> 17 and f32 24 -> 27, f32 of
+    // 1000 columns, which are the first wavefronts' alone, 4.7 -> 6.0, 1 x 12288 x 4096 f16 16 -> 19).
+    const bool narrow = a.n <= 32 * 160;
+    if constexpr (four_bits<T>) return launch_rows<T, 1, 1, 8, 4>(a, stream);
+    else if constexpr (Parts<T>::n == 1) {
+      if (a.m <= 2 || (narrow && a.m <= 8)) return launch_rows<T, 1, 1, 8, 4>(a, stream);
+    } else if constexpr (Parts<T>::n == 3) {
+      if (narrow && a.k >= 4096) return launch_rows<T, 1, 1, 8, 4>(a, stream);
+    }
+  }
+  if constexpr (MT > 1 || !four_bits<T>) {
+    if (a.n > 64 * 160) return launch_rows<T, MT, MT == 4 ? 2 : 4, 8, 1>(a, stream);
+    if (a.n > 32 * 160) return launch_rows<T, MT, 2, 8, 1>(a, stream);
+    return launch_rows<T, MT, 1, MT == 4 ? 8 : 16, 1>(a, stream);
+  }
 }
 
 template <typename T>
