@@ -2,7 +2,8 @@
 //
 // Four lanes to a block, eight values each: a lane's load is 16 bytes of 16-bit rows,
 // the block's largest magnitude is two exchanges away, and a lane writes its four bytes
-// of codes.  Both directions are bound by memory.
+// of codes.  Both directions are bound by memory: 32768 x 8192 of bf16 take 136 us there (4.9
+// TB/s) and 116 back (5.8), where a large copy moves 5.15 TB/s.
 #include "sf_mx4.h"
 
 namespace sf {

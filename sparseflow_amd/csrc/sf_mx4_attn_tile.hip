@@ -8,6 +8,11 @@
 // wants of its depth when its tokens are counted like that; V^T comes by transposing loads.
 // Tiles with the most tokens begin first, and those of one sequence and shared head are a
 // multiple of their number apart: on one XCD where that is a multiple of eight.
+//
+// Bound by its instructions: of 64 tokens a wavefront has 32 products (32 cycles each) and some
+// 330 vector instructions (4 cycles), of which the softmax is 130 and the widening of the codes
+// 80.  2 x 8192 tokens, 32 / 8 heads of 128: bf16 1250 us (880 TFLOP/s), f16 2030, float32 4000;
+// 4 x 4096, 16 heads of 64: 238 us (573).
 #include "sf_mx4_cache.h"
 
 namespace sf {
