@@ -13,7 +13,7 @@ other entry points of token sequences.  heads / kv_heads query heads in a row sh
 and values.  `Kernels/pages.py` deals pages out.
 
 Device tensors run sf_mx4_cache_append / sf_mx4_attention; host tensors the torch forms
-below (the checker too).  Softmax statistics and sums are float32.  Inference only:
+below.  Softmax statistics and sums are float32.  Inference only:
 nothing is recorded for a backward pass."""
 
 from __future__ import annotations

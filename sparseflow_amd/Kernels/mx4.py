@@ -9,7 +9,7 @@ value, halfway to the even code, past 6 to 6; a block with an infinity or NaN be
 Spikes (0 and 1) are exact.
 
 Device tensors run sf_mx4_quantize / sf_mx4_dequantize / sf_mx4_linear; host tensors the
-torch forms below (the checker too).  Inference only: nothing is recorded for a backward
+torch forms below.  Inference only: nothing is recorded for a backward
 pass."""
 
 from __future__ import annotations

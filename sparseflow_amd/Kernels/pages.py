@@ -13,7 +13,7 @@ Refused too: a row outside tables, a size that is negative or wider than the tab
 that an earlier request of the call names.  `pools` are the tensors whose pages have to be
 copied along.
 
-Device tensors run sf_pages_*; host tensors the torch forms below (the checker too)."""
+Device tensors run sf_pages_*; host tensors the torch forms below."""
 
 from __future__ import annotations
 

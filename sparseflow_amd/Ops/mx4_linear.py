@@ -17,6 +17,10 @@ from ..Kernels.mx4 import blocks_of, mx4_dequantize, mx4_linear_forward, mx4_qua
 from ._runtime import WeightLayout
 
 
+def _float32(bias: torch.Tensor) -> torch.Tensor:
+    return bias.detach().float().contiguous()
+
+
 class MX4Linear(nn.Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, quantize_input: bool = False,
                  device=None):
@@ -26,7 +30,7 @@ class MX4Linear(nn.Module):
         self.register_buffer("codes", torch.zeros(self.out_features, 16 * n, dtype=torch.uint8, device=device))
         self.register_buffer("scales", torch.zeros(self.out_features, n, dtype=torch.uint8, device=device))
         self.register_buffer("bias", torch.zeros(self.out_features, device=device) if bias else None)
-        self._bias = WeightLayout(lambda b: b.detach().float().contiguous())
+        self._bias = WeightLayout(_float32)
 
     @classmethod
     def from_dense(cls, linear: nn.Linear, quantize_input: bool = False) -> "MX4Linear":

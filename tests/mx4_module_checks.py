@@ -1,6 +1,7 @@
 """Checks of the modules over the 4-bit operators, for a device or the host."""
 
 import copy
+import io
 
 import torch
 import torch.nn as nn
@@ -117,3 +118,51 @@ def dequantized(model):
             if isinstance(mod, nn.Linear):
                 mod.weight.copy_(ora.values(*mx4_quantize(mod.weight), mod.weight.shape[1]).float())
     return m
+
+
+def check_select_of_nothing(dev):
+    """Sequences without tokens, and a batch without sequences, go on like others."""
+    q, k, v = _sequences(dev, 2, 3, 4, 2, 32, torch.float32)
+    mod = CachedAttention(page_size=4)
+    assert mod(q[:, :0], k[:, :0], v[:, :0]).shape == (2, 0, 4, 32)
+    mod.select(torch.tensor([1, 1]))
+    mod.compact()
+    y = mod(q, k, v)
+    assert torch.equal(y, CachedAttention(page_size=4)(q, k, v))
+    mod = CachedAttention(page_size=4)
+    assert mod(q[:0], k[:0], v[:0]).shape == (0, 3, 4, 32)
+    mod.select(torch.zeros(0, dtype=torch.long))
+    mod.compact()
+
+
+def check_hybrid_in_16_bits(dev, dtype):
+    """A prompt, its next token, and the sequences in other places, in a model of 16 bits."""
+    m = hybrid(1).to(dev).to(dtype)
+    with torch.no_grad():
+        y = m(ids(2, 7).to(dev))
+        m.select(torch.tensor([1, 1]))
+        z = m(ids(1, 1).expand(2, 1).to(dev))
+    assert y.dtype == dtype and y.shape == (2, 7, 32) and torch.isfinite(y).all()
+    assert torch.equal(z[0], z[1]) and torch.isfinite(z).all()
+    q = hybrid(1).quantize_().to(dev).to(dtype)
+    with torch.no_grad():
+        assert torch.isfinite(q(ids(2, 7).to(dev))).all()
+
+
+def check_saved(dev):
+    """A model in the middle of its sequences goes on after it was written and read, or copied."""
+    m = hybrid(4).quantize_().to(dev)
+    with torch.no_grad():
+        m(ids(2, 5).to(dev))
+        m.select(torch.tensor([1, 0]))
+        file = io.BytesIO()
+        torch.save(m, file)
+        file.seek(0)
+        others = [torch.load(file, weights_only=False), copy.deepcopy(m)]
+        token = ids(2, 1, seed=8).to(dev)
+        want = m(token)
+        for other in others:
+            assert torch.equal(other(token), want)
+            other.select(torch.tensor([0, 0]))
+            y = other(token[:1].expand(2, 1))  # (the same sequence twice, and the same next token)
+            assert torch.equal(y[0], y[1])

@@ -8,7 +8,8 @@ import torch
 from sparseflow_amd import _lib
 from sparseflow_amd.Ops import CachedAttention
 from tests.gpu_helpers import DEV, announce, native_loaded
-from tests.mx4_module_checks import check_cached_attention, check_linear_module, check_select, hybrid, ids, search
+from tests.mx4_module_checks import check_cached_attention, check_hybrid_in_16_bits, check_linear_module, \
+    check_saved, check_select, check_select_of_nothing, hybrid, ids, search
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -75,3 +76,16 @@ def test_hybrid_search_matches_the_host(quantized):
     assert {"mx4_append", "mx4_attention", "pages"} <= launched, launched
     assert not quantized or {"mx4_quantize", "mx4_linear"} <= launched, launched
     _logits_agree(got, want)
+
+
+def test_select_of_nothing():
+    check_select_of_nothing(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_hybrid_in_16_bits(dtype):
+    check_hybrid_in_16_bits(DEV, dtype)
+
+
+def test_saved_in_the_middle():
+    check_saved(DEV)

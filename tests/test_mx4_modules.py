@@ -11,7 +11,8 @@ from sparseflow_amd import _lib
 from sparseflow_amd.Models import spiking_ssm_tiny
 from sparseflow_amd.neuron import reset_net
 from sparseflow_amd.Ops import CachedAttention, MX4Linear, quantize_linears_
-from tests.mx4_module_checks import check_cached_attention, check_linear_module, check_select, dequantized, hybrid, ids, search
+from tests.mx4_module_checks import check_cached_attention, check_hybrid_in_16_bits, check_linear_module, \
+    check_saved, check_select, check_select_of_nothing, dequantized, hybrid, ids, search
 
 CPU = torch.device("cpu")
 
@@ -118,3 +119,16 @@ def test_models_without_attention_are_what_they_were():
         a.select(torch.tensor([1, 1]))
         y = a(ids(2, 1, 8)[:1].expand(2, 1))
     assert torch.equal(y[0], y[1])
+
+
+def test_select_of_nothing():
+    check_select_of_nothing(CPU)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_hybrid_in_16_bits(dtype):
+    check_hybrid_in_16_bits(CPU, dtype)
+
+
+def test_saved_in_the_middle():
+    check_saved(CPU)
