@@ -371,7 +371,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_four(Mx4LinearArgs a
 // KG groups of wavefronts take stages in turn, each with LDS of its own, and add up what they
 // have at the end: where y has no more tiles than there are CUs, the time is a tile's stages one
 // after another, half a us each (128 x 4096 x 4096: bf16 32.6 -> 20.4 us, f32 63.6 -> 40.2;
-// 128 x 8192 x 1024: 61 -> 33, 123 -> 77).
+// 256 x 8192 x 1024: 70 -> 36, 123 -> 78).
 template <typename P, int NP>
 struct alignas(16) AnyStage {
   uint16_t x[NP][P::BM][64];
@@ -588,7 +588,7 @@ int launch_any(const Mx4LinearArgs& a, hipStream_t stream) {
     if (tiles_of(a, 256, 256) >= kGemmTiles) return launch_any<T, Shape<4, 2, 2, 4, 2>, 1>(a, stream);
   }
   if (tiles_of(a, 128, 256) >= kGemmTiles) return launch_any<T, Shape<2, 4, 2, 2, 2>, 1>(a, stream);
-  // (2050 x 6000, bf16 / f32 in us: 64 rows of 94 tiles take 13.4 / 25.1 in groups and 15.6 / 38.3
+  // (2050 x 6000, bf16 / f32 in us: 65 rows of 188 tiles take 13.7 / 26.4 in groups and 15.2 / 37.6
   // without, 256 rows of 376 tiles 26.7 / 50.4 and 21.4 / 49.7.)
   if (tiles_of(a, 64, 64) <= kCus) return launch_any<T, Shape<2, 2, 1, 1, 2>, Parts<T>::n == 1 ? 4 : 2>(a, stream);
   return launch_any<T, Shape<2, 2, 1, 1, 2>, 1>(a, stream);

@@ -205,26 +205,32 @@ int launch_rows_n(const Mx4LinearArgs& a, hipStream_t stream) {
 }
 
 template <typename T>
-int launch_linear(const Mx4LinearArgs& a, hipStream_t stream) {
-  return a.m <= 16 ? launch_rows_n<T, 1>(a, stream) : a.m <= 32 ? launch_rows_n<T, 2>(a, stream) : launch_rows_n<T, 4>(a, stream);
+int launch_linear(const Mx4LinearArgs& a, bool few, hipStream_t stream) {
+  return few || a.m <= 16 ? launch_rows_n<T, 1>(a, stream) : a.m <= 32 ? launch_rows_n<T, 2>(a, stream) : launch_rows_n<T, 4>(a, stream);
 }
 
 }  // namespace
 
 int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   timing_begin(K_MX4_LINEAR, stream);
+  // Where y is so few pieces of 16 x 16 that the CUs hold a workgroup for each, the wavefronts
+  // that share its K are worth more than what they read twice (x K x N in us, as wider pieces or
+  // tiles / so; 37 x 1000 x 1037: f32 10.3 / 6.1, bf16 8.0 / 4.9; 64 x 8192 x 1024: bf16 35 / 14,
+  // f32 77 / 21, four 21 / 8; 128 x 8192 x 1024: bf16 36 / 24; but 200 x 4096 x 1024 bf16 21 / 23,
+  // 20 x 4096 x 4096 bf16 10.6 / 12.2).
+  const int64_t pieces = (a.m + 15) / 16 * ((a.n + 15) / 16);
+  const bool few = pieces <= (a.m <= 32 ? 320 : 512) || (x_dtype == SF_MX4 && a.k >= 4096 && pieces <= 1024);
   // Where tiles of 64 rows fill the CUs by themselves they are better from 33 rows on; with less
-  // of them, a wavefront to few columns reads W sooner (x K x N in us, this kernel / tiles; 64 x
-  // 4096 x 12288: bf16 41 / 22, f32 102 / 45, four 25 / 16; 33 x 4096 x 4096: bf16 13 / 20, f32
-  // 45 / 39, four 9 / 14; 48 x 8192 x 1024: bf16 29 / 34, f32 69 / 74, four 18 / 27; 17 to 32
-  // rows: never worse by more than a us).
+  // of them, a wavefront to few columns reads W sooner (this kernel / tiles; 64 x 4096 x 12288:
+  // bf16 41 / 22, f32 102 / 45, four 25 / 16; 33 x 4096 x 4096: bf16 13 / 20, f32 45 / 39, four
+  // 9 / 14; 17 to 32 rows: never worse by more than a us).
   const int64_t filling = x_dtype == SF_F32 ? 2048 : 10240;
-  const bool tiles = a.m > (a.n > filling ? 32 : 64) && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
+  const bool tiles = !few && a.m > (a.n > filling ? 32 : 64) && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
   const int rc = tiles                ? launch_mx4_gemm(a, x_dtype, stream)
-                 : x_dtype == SF_MX4  ? launch_linear<Four>(a, stream)
-                 : x_dtype == SF_F16  ? launch_linear<__half>(a, stream)
-                 : x_dtype == SF_BF16 ? launch_linear<__hip_bfloat16>(a, stream)
-                                      : launch_linear<float>(a, stream);
+                 : x_dtype == SF_MX4  ? launch_linear<Four>(a, few, stream)
+                 : x_dtype == SF_F16  ? launch_linear<__half>(a, few, stream)
+                 : x_dtype == SF_BF16 ? launch_linear<__hip_bfloat16>(a, few, stream)
+                                      : launch_linear<float>(a, few, stream);
   timing_end(K_MX4_LINEAR, stream);
   return rc;
 }
