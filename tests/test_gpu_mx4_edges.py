@@ -211,3 +211,22 @@ def test_steps_of_sequences_that_share_a_slot():
     y = cached_attention_step(q[[1, 0, 1, 0]].contiguous(), call["cache"], call["tables"], call["lengths"], slots=slots)
     base = cached_attention_step(q, call["cache"], call["tables"], call["lengths"])
     assert torch.equal(y[0], base[1]) and torch.equal(y[1], base[0]) and torch.equal(y[2], base[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("four", [False, True], ids=["floats", "4-bit"])
+@pytest.mark.parametrize("shape", [(300, 512, 2100), (1100, 256, 1290), (1000, 100, 2561), (3500, 192, 3601), (3333, 70, 4100), (3585, 384, 3600)], ids=str)
+def test_linear_tiles_of_every_size(shape, dtype, four):
+    """Rows and columns that end inside a tile, in tiles of 64, 128 and 256, few stages and many."""
+    announce(f"tiles {shape} {dtype} {four}")
+    m, k, n = shape
+    check_linear(DEV, m, k, n, dtype, bias=n % 2 == 1, four=four)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(5, 4100, 30), (16, 8200, 40), (64, 4096, 300), (260, 600, 250), (2000, 4224, 50)], ids=str)
+def test_linear_pieces(shape, dtype):
+    """Few pieces of y, K over many wavefronts: ends of K and of the pieces."""
+    m, k, n = shape
+    for four in (False, True):
+        check_linear(DEV, m, k, n, dtype, bias=True, four=four)
