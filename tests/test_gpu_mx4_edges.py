@@ -230,3 +230,11 @@ def test_linear_pieces(shape, dtype):
     m, k, n = shape
     for four in (False, True):
         check_linear(DEV, m, k, n, dtype, bias=True, four=four)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 200])
+def test_prompts_in_parts_of_their_tokens(dim, dtype):
+    """Few tiles after long contexts: parts joined, among them parts that see nothing, and a sequence without rows."""
+    announce(f"prompt parts {dim} {dtype}")
+    check_attention(DEV, [60, 0, 130, 1], [2500, 10, 300, 0], 4, 2, dim, 64, dtype)
