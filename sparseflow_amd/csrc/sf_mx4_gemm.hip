@@ -546,6 +546,7 @@ __global__ __launch_bounds__(P::threads* KG, KG == 4 ? 4 : 2) void k_mx4_gemm_an
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[(g * P::waves + wave) * per + ((i * P::NT + j) * 16 + e) * kWave + lane];
     }
+    __syncthreads();  // (a wavefront's rows on their way out lie over sums that others read)
     if (group > 0) return;
   } else {
     __syncthreads();  // (the stages are done with)
