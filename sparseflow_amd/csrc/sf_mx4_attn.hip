@@ -530,14 +530,15 @@ __device__ __forceinline__ void join_row(const Mx4AttnArgs& a, int64_t parts, Pl
     for (int k = 0; k < F; ++k) {
       const bool in = s0 + W * k < parts;
       const int64_t at = place(in ? s0 + W * k : s0);
-      f[k] = in ? a.parts_ml[2 * at] : -INFINITY;
+      f[k] = a.parts_ml[2 * at];
       q[k] = a.parts_ml[2 * at + 1];
 #pragma unroll
       for (int e = 0; e < C; ++e) p[k][e] = a.parts_o[at * (32 * NB) + (kWave * e + lane < 32 * NB ? kWave * e + lane : 0)];
     }
 #pragma unroll
     for (int k = 0; k < F; ++k) {
-      if (f[k] == -INFINITY) continue;  // (nothing seen there)
+      // (A part where nothing is seen has 0 times its zeros; NaN has -infinity for a maximum too, and stays.)
+      if (s0 + W * k >= parts) continue;
       const float g = exp2_hw(f[k] - from);
       total += g * q[k];
 #pragma unroll
