@@ -69,12 +69,13 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
   const int64_t row0 = tile * kAttnTileRows, rows = n * group;
   if (row0 >= rows) return;
   const int64_t length = slot < 0 ? 0 : c.lengths[slot];
-  const int64_t room = cache_room(c);
 
   // This lane's query row.
   const int64_t wrow0 = row0 + 32 * wave, row = wrow0 + r < rows ? wrow0 + r : rows - 1;
   const int64_t i = row / group;
-  const int64_t place = slot < 0 ? -1 : length - n + i;
+  const int64_t last_place = slot < 0 ? -1 : cache_room(c) - 1;  // (tokens past the table are seen by nobody)
+  auto place_in = [&](int64_t at) { return length - n + at < last_place ? length - n + at : last_place; };
+  const int64_t place = place_in(i);
   bf16x8 qf[2 * NB][NP];
   {
     const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_strides[0] + (first + i) * a.q_strides[1] +
@@ -85,9 +86,9 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
 
   // The keys that any of the workgroup's rows sees, this part's share of them, and up to where
   // every row of the wavefront sees all, or one sees any.
-  auto place_of = [&](int64_t at) { return slot < 0 ? -1 : length - n + (at < rows ? at : rows - 1) / group; };
+  auto place_of = [&](int64_t at) { return place_in((at < rows ? at : rows - 1) / group); };
   int64_t keys = place_of(row0 + kAttnTileRows - 1) + 1;
-  keys = keys < 0 ? 0 : keys > room ? room : keys;
+  keys = keys < 0 ? 0 : keys;
   const int64_t all = place_of(wrow0) + 1, any = place_of(wrow0 + 31) + 1;
   const int64_t chunks = (keys + C - 1) / C, begin = chunks * split / a.splits, end = chunks * (split + 1) / a.splits;
   const int32_t* table = slot < 0 ? nullptr : c.tables + slot * c.width;
