@@ -188,7 +188,7 @@ def _host_attend(q, cache, length: int, table: torch.Tensor, scale: float) -> to
         if bad.any():  # 0 times such a value is no 0: each row takes those that it sees
             for j in range(n):
                 out[j] = w[j, see[j]] @ v[see[j]]
-        y[:, h] = torch.where(total == 0, torch.zeros(()), out / total)
+        y[:, h] = torch.where(see.any(-1, keepdim=True), out / total, torch.zeros(()))
     return y
 
 

@@ -417,6 +417,7 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
   }
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
+  ref = ref_of_seen(c, table, begin * kAttnTokens, end * kAttnTokens < keys ? end * kAttnTokens : keys, place, ref, l);
 
   // The wavefronts' parts together.
   __syncthreads();
@@ -450,7 +451,8 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
     }
     return;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const bool none = nothing_seen(top, total);
+  const float inv = 1.f / total;
   const int64_t oi = orow / group;
   T* y = reinterpret_cast<T*>(a.y) + b * a.y_strides[0] + (first + oi) * a.y_strides[1] +
          (int64_t)(kvh * group + (int)(orow - oi * group)) * a.y_strides[2];
@@ -459,7 +461,7 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kAttnWaves; ++w) v += f[w] * lds.o[w][wr][16 * k + wc];
-    if (16 * k + wc < a.head_dim) y[16 * k + wc] = from_f32<T>(total == 0.f ? 0.f : v * inv);
+    if (16 * k + wc < a.head_dim) y[16 * k + wc] = from_f32<T>(none ? 0.f : v * inv);
   }
 }
 
@@ -558,7 +560,7 @@ __device__ __forceinline__ void join_row(const Mx4AttnArgs& a, int64_t parts, Pl
   }
 #pragma unroll
   for (int e = 0; e < C; ++e)
-    if (kWave * e + lane < a.head_dim) y[kWave * e + lane] = from_f32<T>(total == 0.f ? 0.f : v[e] / total);
+    if (kWave * e + lane < a.head_dim) y[kWave * e + lane] = from_f32<T>(nothing_seen(top, total) ? 0.f : v[e] / total);
 }
 template <typename T>
 __device__ __forceinline__ T* row_of_y(const Mx4AttnArgs& a, int64_t b, int64_t first, int kvh, int64_t row) {

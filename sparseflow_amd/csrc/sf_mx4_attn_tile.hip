@@ -254,10 +254,11 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
     __syncthreads();
   }
   l += __shfl_xor(l, 32, kWave);
+  ref = ref_of_seen(c, table, begin * C, end * C < keys ? end * C : keys, place, ref, l);
 
   // Out by way of LDS, 128 columns at a time, the wavefront's own: two rows of 32 lanes x four
   // columns an access.
-  const float inv = a.splits > 1 || l == 0.f ? 1.f : 1.f / l;
+  const float inv = a.splits > 1 || nothing_seen(ref, l) ? 1.f : 1.f / l;
   const int64_t base = (((b * c.heads + kvh) * a.tiles + tile) * a.splits + split) * kAttnTileRows + 32 * wave;
   if (a.splits > 1 && h == 0 && wrow0 + r < rows) a.parts_ml[2 * (base + r)] = ref, a.parts_ml[2 * (base + r) + 1] = l;
 #pragma unroll

@@ -94,6 +94,23 @@ __device__ __forceinline__ float far_value(const uint32_t* codes, uint32_t byte,
   return v.x;
 }
 
+// A row that sees no token is zeros; one that sees tokens whose scores are all -infinity has a
+// softmax of 0 / 0.  Both have no sum and -infinity for a maximum after the tokens from `begin` to
+// `end` - 1: the maximum of the latter, which any other score passes, becomes the lowest number.
+__device__ __forceinline__ bool nothing_seen(float ref, float sum) { return ref == -INFINITY && sum == 0.f; }
+__device__ __forceinline__ float ref_of_seen(const CacheView& c, const int32_t* __restrict__ table, int64_t begin, int64_t end,
+                                             int64_t place, float ref, float sum) {
+  if (!__any(nothing_seen(ref, sum) && place >= begin)) return ref;
+  for (int64_t p0 = begin >> c.page_shift; p0 << c.page_shift < end; p0 += kWave) {
+    const int64_t at = (p0 + lane_id()) << c.page_shift, t = at > begin ? at : begin;
+    const uint64_t there = __ballot(t < end && cache_page(c, table, t < end ? t : end - 1) >= 0);
+    if (there == 0) continue;
+    const int64_t first = (p0 + __builtin_ctzll(there)) << c.page_shift;  // (the first page there is)
+    return nothing_seen(ref, sum) && place >= begin && place >= first ? -__FLT_MAX__ : ref;
+  }
+  return ref;
+}
+
 // The tokens that a sequence's table has room for.
 __device__ __forceinline__ int64_t cache_room(const CacheView& c) { return (int64_t)c.width << c.page_shift; }
 
