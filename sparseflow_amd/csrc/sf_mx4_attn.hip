@@ -355,8 +355,9 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
       sum += pr[k];
     }
     l += sum;
-    bf16x8 pf[NP];
-    weight_parts<NP>(pr, pf);
+    constexpr int WP = kWeightParts<T>;
+    bf16x8 pf[WP];
+    weight_parts<WP>(pr, pf);
     constexpr int DG = NB < 4 ? 2 * NB : 8;  // tiles of columns at a time
 #pragma unroll
     for (int d0 = 0; d0 < 2 * NB; d0 += DG) {
@@ -369,7 +370,7 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
         vf[d - d0][1] = lds_transposed(at + 16 * stride);
       }
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+      for (int p = 0; p < WP; ++p)
 #pragma unroll
         for (int d = d0; d < d0 + DG && d < 2 * NB; ++d)
           o[d] = mfma16(__builtin_shufflevector(vf[d - d0][0], vf[d - d0][1], 0, 1, 2, 3, 4, 5, 6, 7), pf[p], o[d]);
@@ -466,7 +467,7 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
 }
 
 template <typename T, int NB>
-__global__ __launch_bounds__(kAttnWaves* kWave, NB * Parts<T>::n <= 8 ? 2 : 1) void k_mx4_attn_rows(Mx4AttnArgs a) {
+__global__ __launch_bounds__(kAttnWaves* kWave, NB * kWeightParts<T> <= 8 ? 2 : 1) void k_mx4_attn_rows(Mx4AttnArgs a) {
   __shared__ AttnLds<NB> lds;
   __shared__ int64_t at[2];
   const int heads = a.cache.heads;
@@ -665,7 +666,7 @@ Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_head
     // Workgroups: what the CUs hold of them (by registers).  Short tables: a tile is one unit.
     p.unit = room <= 512 ? 4 : 1;
     const int64_t tokens = kAttnTokens * kAttnUnit * p.unit, units = room <= tokens ? 1 : (room + tokens - 1) / tokens;
-    const int64_t hold = blocks * parts <= 2 ? 768 : blocks * parts <= 8 ? 512 : 256;
+    const int64_t hold = blocks * parts <= 2 ? 768 : blocks * (parts == 1 ? 2 : parts) <= 8 ? 512 : 256;
     const int64_t most = units > hold || items > hold ? hold : items * units;  // (no product of large numbers)
     p.shares = units == 1 ? (items < 4 * hold ? items : 4 * hold) : most < hold ? most : hold;
     p.shares = p.shares < 1 ? 1 : p.shares;

@@ -9,10 +9,11 @@
 // Tiles with the most tokens begin first, and those of one sequence and shared head are a
 // multiple of their number apart: on one XCD where that is a multiple of eight.
 //
-// Bound by its instructions: of 64 tokens a wavefront has 32 products (32 cycles each) and some
-// 330 vector instructions (4 cycles), of which the softmax is 130 and the widening of the codes
-// 80.  2 x 8192 tokens, 32 / 8 heads of 128: bf16 1250 us (880 TFLOP/s), f16 2030, float32 4000;
-// 4 x 4096, 16 heads of 64: 238 us (573).
+// Bound by its instructions: of 64 tokens a wavefront has 48 products of bf16 (32 cycles each; 32 of
+// them take the weights' two parts) and some 400 vector instructions (4 cycles), of which the softmax
+// is 200 and the widening of the codes 80.  2 x 8192 tokens, 32 / 8 heads of 128: bf16 1490 us (740
+// TFLOP/s; with weights of one part 1200), f16 1915, float32 3950; 4 x 4096, 16 heads of 64: 274 us
+// (500).
 #include "sf_mx4_cache.h"
 
 namespace sf {
@@ -217,8 +218,9 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = s[k >> 1][8 * (k & 1) + e];
-        bf16x8 pf[NP];
-        weight_parts<NP>(w, pf);
+        constexpr int WP = kWeightParts<T>;
+        bf16x8 pf[WP];
+        weight_parts<WP>(w, pf);
         const int tk = 4 * h + (lane >> 2 & 3), unit = value_unit(2 * (lane >> 4 & 1) + (lane >> 1 & 1), tk);
         const uint16_t* at = &t.v[16 * k + tk][8 * unit + 4 * (lane & 1)];
 #pragma unroll
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
           const bf16x8 vf = __builtin_shufflevector(lds_transposed(at + 32 * d), lds_transposed(at + 32 * d + 8 * stride), 0, 1, 2,
                                                     3, 4, 5, 6, 7);
 #pragma unroll
-          for (int p = 0; p < NP; ++p) o[d] = mfma32(vf, pf[p], o[d]);
+          for (int p = 0; p < WP; ++p) o[d] = mfma32(vf, pf[p], o[d]);
         }
       }
       if (flags & 1) {

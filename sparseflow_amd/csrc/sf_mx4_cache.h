@@ -48,16 +48,26 @@ __device__ __forceinline__ void load_query(const T* __restrict__ q, int k, int h
 constexpr int value_stride(int nb) { return 32 * (nb | 1); }  // bf16 elements
 __device__ __forceinline__ int value_unit(int unit, int tok) { return unit ^ (tok & 3) ^ (tok >> 1 & 2); }
 
-// Softmax weights for the second product: in one part rounded (half a step, 2^-8 relative, as
-// of the values of a bf16 result), in more parts cut off.
+// Softmax weights for the second product, in bf16 parts: three for float32, which lose nothing, and
+// two for f16 and bf16, the second rounded: off by 2^-16 of a weight.  (One part, rounded, is off by
+// 2^-9: as much as a bf16 result's own rounding, and a third more error against 64 bits.)
+template <typename T>
+constexpr int kWeightParts = Parts<T>::n == 3 ? 3 : 2;
 template <int NP>
 __device__ __forceinline__ void weight_parts(const float (&w)[8], bf16x8 (&p)[NP]) {
-  if constexpr (NP == 1) {
-    u32x4 u;
+  if constexpr (NP == 2) {
+    u32x4 high, low;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{w[2 * i], w[2 * i + 1]}), bf16x2));
-    p[0] = __builtin_bit_cast(bf16x8, u);
+    for (int i = 0; i < 4; ++i) {
+      float rest[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        rest[k] = w[2 * i + k] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, w[2 * i + k]) & 0xffff0000u);
+      high[i] = pack_high(w[2 * i], w[2 * i + 1]);
+      low[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{rest[0], rest[1]}), bf16x2));
+    }
+    p[0] = __builtin_bit_cast(bf16x8, high);
+    p[1] = __builtin_bit_cast(bf16x8, low);
   } else {
     split8<NP>(w, p);
   }
