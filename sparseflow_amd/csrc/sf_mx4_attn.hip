@@ -219,7 +219,7 @@ struct RawTokens {
   u32x4 v[VU];
   uint32_t vs[VU];
   uint32_t have;  // which tokens have a page
-  bool far;       // some value's scale is kFarScale or more
+  bool large, far;  // some value's scale is kLargeScale, kFarScale or more
 
   // pages: lane t's is token t0 + t's, or -1 (t < 32).
   __device__ __forceinline__ void load(const CacheView& c, int64_t t0, int kvh, int32_t pages, int lane) {
@@ -247,12 +247,13 @@ struct RawTokens {
 
   // The values as bf16 into LDS.
   __device__ __forceinline__ void put(uint16_t* vt, int lane) {
-    far = false;
+    large = far = false;
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       const int at = lane + kWave * u, tok = at / NB, blk = at - tok * NB;
       // (Of a token without a page scale 0: numbers, which get the weight 0.)
       const bool there = have >> (tok & 31) & 1, off = there && vs[u] >= kFarScale;
+      large |= there && vs[u] >= kLargeScale;
       far |= off;
       const float scale = mx4_scale(there && !off ? vs[u] : 0);
       if (off) v[u] = u32x4{0, 0, 0, 0};
@@ -304,7 +305,8 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
     return ch < end && t < keys ? p : -1;
   };
 
-  float ref = -INFINITY, l = 0.f;  // the running maximum, times scale and log2(e)
+  float ref = -INFINITY, l = 0.f;
+  bool roomy = false;
   f32x4 o[2 * NB];
 #pragma unroll
   for (int d = 0; d < 2 * NB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -339,19 +341,21 @@ __device__ __forceinline__ void attend_tile(const Mx4AttnArgs& a, const TileWork
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = fmaxf(top, __shfl_xor(top, 16, kWave));
     top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c2;
-    if (__any(top > ref + kRefSlack)) {
+    const bool more = !roomy && __any(raw.large);
+    if (more || ref_passed(top, ref, roomy)) {
       const float was = ref;
-      ref = fmaxf(ref, top);
+      roomy |= more;
+      ref = ref_moved(ref, top, roomy, more);
       const float back = exp2_hw(was - (ref == -INFINITY ? 0.f : ref));  // (was = -inf: 0)
       l *= back;
 #pragma unroll
       for (int d = 0; d < 2 * NB; ++d) o[d] *= back;
     }
-    const float from = ref_from<NP>(ref);
+    const float from = ref_from<NP>(ref, roomy);
     float pr[8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      pr[k] = weight_of<NP>(s[k >> 2][k & 3], c2, from);
+      pr[k] = weight_of<NP>(s[k >> 2][k & 3], c2, from, roomy);
       sum += pr[k];
     }
     l += sum;

@@ -33,7 +33,8 @@ struct TileLds {
     uint16_t k[C][32 * NB + 8];   // bf16 rows: 16 bytes on, another bank
     uint16_t v[C][stride];
     uint32_t there[C];            // whether the token has a page
-    uint32_t flags[kTileWaves];   // of what each wavefront brought: 1 values from kFarScale on, 2 tokens without a page
+    // Of what each wavefront brought: 1 values from kFarScale on, 2 tokens without a page, 4 values from kLargeScale on.
+    uint32_t flags[kTileWaves];
   };
   union {
     Buf buf[2];
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
   };
   auto put = [&](int64_t ch, typename Lds::Buf& to) {
     // (Of a token without a page scale 0: numbers, which get the weight 0.)
-    const bool far = there && vs >= kFarScale;
+    const bool far = there && vs >= kFarScale, large = there && vs >= kLargeScale;
     if (far) vc = u32x4{0, 0, 0, 0};
     if (far || !there) vs = 0;
     if (mine) {
@@ -126,11 +127,12 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
       }
       if (blk == 0) to.there[tok] = there;
     }
-    const uint32_t flags = (__any(far) ? 1 : 0) | (__any(mine && !there && ch * C + tok < keys) ? 2 : 0);
+    const uint32_t flags = (__any(far) ? 1 : 0) | (__any(mine && !there && ch * C + tok < keys) ? 2 : 0) | (__any(large) ? 4 : 0);
     if (lane == 0) to.flags[wave] = flags;
   };
 
-  float ref = -INFINITY, l = 0.f;  // the running maximum, times scale and log2(e)
+  float ref = -INFINITY, l = 0.f;
+  bool roomy = false;
   f32x16 o[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d)
@@ -195,21 +197,23 @@ __global__ __launch_bounds__(kTileThreads, NB <= 4 && Parts<T>::n < 3 ? 2 : 1) v
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
       top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c2;
-      if (__any(top > ref + kRefSlack)) {
+      const bool more = !roomy && (flags & 4) != 0;
+      if (more || ref_passed(top, ref, roomy)) {
         const float was = ref;
-        ref = fmaxf(ref, top);
+        roomy |= more;
+        ref = ref_moved(ref, top, roomy, more);
         const float back = exp2_hw(was - (ref == -INFINITY ? 0.f : ref));  // (was = -inf: 0)
         l *= back;
 #pragma unroll
         for (int d = 0; d < NB; ++d) o[d] *= back;
       }
-      const float from = ref_from<NP>(ref);
+      const float from = ref_from<NP>(ref, roomy);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[u][e] = weight_of<NP>(s[u][e], c2, from);
+          s[u][e] = weight_of<NP>(s[u][e], c2, from, roomy);
           sum[e & 3] += s[u][e];
         }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);

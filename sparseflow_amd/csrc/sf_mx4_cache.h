@@ -77,25 +77,36 @@ __device__ __forceinline__ void weight_parts(const float (&w)[8], bf16x8 (&p)[NP
 // it is nothing: what is hidden, -infinity, has to stay that.)
 __device__ __forceinline__ float score_factor(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1e-44f); }
 
-// The running maximum of a row's exponents is `ref`; it moves only where it would be passed by
-// more than this, so that the sums are seldom rescaled.  Weights are 2^(exponent - ref - 30),
-// below 2^-22: up to 2^22 of them times values at the end of float32 stay in its range.  (What
-// goes missing at the other end, products below 2^-126, is less than 2^-96 a token.)
+// Exponents are taken against a row's `ref`, a whole number at its running maximum or above; it moves
+// only where the maximum would pass it by more than kRefSlack, so that the sums are seldom rescaled.
+// Weights are at most 2^8 then, and up to 2^22 of them times values of scales below kLargeScale (less
+// than 2^97) stay in float32's range.  From the first chunk on that holds a larger value the
+// wavefront's refs have kRefRoom more room, and weights are 2^-22 at most: values at the end of float32
+// stay in range too.  (Beside those, float32's smallest product, 2^-149, is one of 2^-119 and a weight
+// of 1; with the room from the start values of 2^-118 had one bit left.)
 constexpr float kRefSlack = 8.f, kRefRoom = 30.f;
+constexpr uint32_t kLargeScale = 222;
+__device__ __forceinline__ bool ref_passed(float top, float ref, bool roomy) {
+  return __any(top > ref + (roomy ? kRefSlack - kRefRoom : kRefSlack));
+}
+// Of a chunk with the maximum `top`; `more`: with the room from here on.
+__device__ __forceinline__ float ref_moved(float ref, float top, bool roomy, bool more) {
+  return fmaxf(ref + (more ? kRefRoom : 0.f), ceilf(top) + (roomy ? kRefRoom : 0.f));
+}
 
-// A weight: with 16-bit weights in one rounding of its exponent (2^-19 of it at 38); where they
-// are held in parts the exponent stays small, and the room is a factor.
+// A weight: with the queries in one part in one rounding of its exponent (2^-19 of it at 38); where
+// they are held in more the exponent stays small, and the room is a factor.
 template <int NP>
-__device__ __forceinline__ float ref_from(float ref) {
-  return ref == -INFINITY ? 0.f : NP == 1 ? ref + kRefRoom : ref;  // (a row that has seen nothing yet)
+__device__ __forceinline__ float ref_from(float ref, bool roomy) {
+  return ref == -INFINITY ? 0.f : NP > 1 && roomy ? ref - kRefRoom : ref;  // (a row that has seen nothing yet)
 }
 template <int NP>
-__device__ __forceinline__ float weight_of(float score, float c2, float from) {
+__device__ __forceinline__ float weight_of(float score, float c2, float from, bool roomy) {
   const float w = exp2_hw(fmaf(score, c2, -from));
-  return NP == 1 ? w : w * 0x1p-30f;
+  return NP == 1 ? w : w * (roomy ? 0x1p-30f : 1.f);
 }
 
-// Values from scale 253 on are no numbers or beyond a float's range at times, and 0 times such
+// Values from scale kFarScale on are no numbers or beyond a float's range at times, and 0 times such
 // a one is no 0: they lie in LDS as zeros, and each row adds those that it sees itself.  Column
 // `col` of a block with its codes and scale:
 constexpr uint32_t kFarScale = 253;
