@@ -149,6 +149,8 @@ def _check_quantize(x, out):
 def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, size: Optional[int] = None,
                    dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(codes, scales) -> [..., size] (default: whole blocks) in `dtype`, or into a contiguous out."""
+    if size is not None:
+        size = int(size)
     key = (signature(codes, scales, out), size, dtype)
     shape, dtype, rows = _back_plans.get(key) or _back_plans.make(key, _check_dequantize, codes, scales, size, dtype, out)
     if out is None:
@@ -166,7 +168,7 @@ def _check_dequantize(codes, scales, size, dtype, out):
     """-> (the result's shape and type, rows)."""
     check_quantized((codes, scales), "codes, scales", codes.device)
     n = int(scales.shape[-1])
-    size = BLOCK * n if size is None else int(size)
+    size = BLOCK * n if size is None else size
     if blocks_of(size) != n:
         raise ValueError(f"size {size}: rows of {n} blocks have {BLOCK * (n - 1) + 1} to {BLOCK * n} values")
     shape = codes.shape[:-1] + (size,)
