@@ -610,8 +610,11 @@ int sf_mx4_attention(const sf_mx4_cache_desc* desc, const sf_mx4_cache* cache,
  * requests in turn, until one cannot have what it needs; it and those behind that
  * need pages are refused.  granted int32 [requests]: 1, or 0 for a refused request,
  * which changes nothing; refused too: a row outside tables, a size that is negative
- * or wider than the table, a row that an earlier request names. */
+ * or wider than the table, a row that an earlier request names.  A resize or fork
+ * has at most 2^20 requests (each looks through those before it for its row), a
+ * copy 2^24 pairs. */
 #define SF_MAX_POOLS 16
+#define SF_MAX_REQUESTS (1 << 20)
 typedef struct sf_pages_desc {
   int64_t pages, rows, width, requests;
   int32_t page_size, pools;

@@ -10,8 +10,9 @@ A call's requests are dealt with as one: what is freed comes first, then the fre
 go, lowest first, to the requests in turn, until one cannot have what it needs; that one
 and those behind it that need pages are refused, and a refused request changes nothing.
 Refused too: a row outside tables, a size that is negative or wider than the table, a row
-that an earlier request of the call names.  `pools` are the tensors whose pages have to be
-copied along.
+that an earlier request of the call names.  A call on the device takes 2^20 requests at most,
+each of which looks through those before it, and a copy 2^24 pairs.  `pools` are the tensors
+whose pages have to be copied along.
 
 Device tensors run sf_pages_*; host tensors the torch forms below."""
 

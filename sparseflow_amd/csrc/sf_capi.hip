@@ -1182,6 +1182,7 @@ int sf_pages_resize(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int3
   int rc = pages_args(d, a);
   if (rc != SF_OK) return rc;
   if (d->requests == 0) return SF_OK;
+  if (d->requests > SF_MAX_REQUESTS) return fail(SF_ERR_UNSUPPORTED, "more than 2^20 requests");
   if (rows == nullptr || sizes == nullptr || granted == nullptr || (d->rows > 0 && lengths == nullptr) ||
       (d->rows > 0 && d->width > 0 && tables == nullptr) || (d->pages > 0 && refs == nullptr))
     return fail(SF_ERR_INVALID, "NULL pointer");
@@ -1203,6 +1204,7 @@ int sf_pages_fork(const sf_pages_desc* d, int32_t* refs, int32_t* tables, int32_
   int rc = pages_args(d, a);
   if (rc != SF_OK) return rc;
   if (d->requests == 0) return SF_OK;
+  if (d->requests > SF_MAX_REQUESTS) return fail(SF_ERR_UNSUPPORTED, "more than 2^20 requests");
   if (parents == nullptr || children == nullptr || granted == nullptr || (d->rows > 0 && lengths == nullptr) ||
       (d->rows > 0 && d->width > 0 && tables == nullptr) || (d->pages > 0 && refs == nullptr))
     return fail(SF_ERR_INVALID, "NULL pointer");

@@ -466,6 +466,7 @@ struct PagesArgs {
   int32_t* to;           //            [pages] compaction: targets
   int32_t* counts;       //            [2] entries of list; compaction: moves
   int64_t pages, states, width, requests;
+  int64_t block0;
   int page_size;
   PagePools pools;
 };

@@ -170,11 +170,11 @@ __device__ __forceinline__ void copy_page(const PagePools& pools, int64_t from, 
   }
 }
 
-// Request blockIdx.x / parts after the deal: the table, the users' counts and the copy of a
+// Request `id / parts` after the deal: the table, the users' counts and the copy of a
 // page that is no longer shared.
 __global__ __launch_bounds__(kPageThreads) void k_pages_grown(PagesArgs a, int parts) {
-  const int64_t q = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
+  const int64_t id = a.block0 + blockIdx.x, q = id / parts;
+  const int part = (int)(id - q * parts);
   const int32_t raw = a.need[q];
   const int64_t old = a.old[q], size = a.other[q], row = a.rows[q];
   const int64_t need = raw < 0 ? -1 : (raw & ((1 << 30) - 1)) + (raw >> 30);
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grown(PagesArgs a, int p
 
 // A fork's child: shares the parent's full pages and has the last, partial one copied.
 __global__ __launch_bounds__(kPageThreads) void k_pages_forked(PagesArgs a, int parts) {
-  const int64_t q = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
+  const int64_t id = a.block0 + blockIdx.x, q = id / parts;
+  const int part = (int)(id - q * parts);
   const int64_t need = a.need[q], n = a.old[q], child = a.rows[q], parent = a.other[q];
   const bool ok = need >= 0 && (need == 0 || a.first[q] + need <= a.counts[0]);
   if (part == 0 && threadIdx.x == 0) a.granted[q] = ok;
@@ -299,10 +299,10 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_move(PagesArgs a, int pa
 
 // Pages rows[i] of the pools to pages other[i].
 __global__ __launch_bounds__(kPageThreads) void k_pages_copy(PagesArgs a, int parts) {
-  const int64_t q = blockIdx.x / parts;
+  const int64_t id = a.block0 + blockIdx.x, q = id / parts;
   const int64_t from = a.rows[q], to = a.other[q];
   if (!page_ok(a, from) || !page_ok(a, to) || from == to) return;
-  copy_page(a.pools, from, to, (int)(blockIdx.x % parts), parts);
+  copy_page(a.pools, from, to, (int)(id - q * parts), parts);
 }
 
 // Workgroups to a page: 16 KB each.
@@ -315,28 +315,36 @@ int page_parts(const PagesArgs& a) {
 
 int last_error() { return (int)hipGetLastError(); }
 
+// Calls kernel(args, parts) with `parts` workgroups to a request, in as many launches as that takes.
+template <typename Kernel>
+int launch_parts(const PagesArgs& a, Kernel kernel, hipStream_t stream) {
+  const int parts = page_parts(a);
+  return launch_blocks(a, &PagesArgs::block0, a.requests * parts, [&](const PagesArgs& part, unsigned grid) {
+    kernel<<<grid, kPageThreads, 0, stream>>>(part, parts);
+  });
+}
+
 }  // namespace
 
+// (requests: at most 2^20, see sparseflow.h)
 int launch_pages_resize(const PagesArgs& a, hipStream_t stream) {
   timing_begin(K_PAGES, stream);
-  const unsigned n = (unsigned)a.requests;
-  const int parts = page_parts(a);
-  k_pages_release<<<n, kPageThreads, 0, stream>>>(a);
+  k_pages_release<<<(unsigned)a.requests, kPageThreads, 0, stream>>>(a);
   k_pages_deal<true><<<1, kDealThreads, 0, stream>>>(a);
-  k_pages_grown<<<n * parts, kPageThreads, 0, stream>>>(a, parts);
+  int rc = last_error();
+  if (rc == (int)hipSuccess) rc = launch_parts(a, k_pages_grown, stream);
   timing_end(K_PAGES, stream);
-  return last_error();
+  return rc;
 }
 
 int launch_pages_fork(const PagesArgs& a, hipStream_t stream) {
   timing_begin(K_PAGES, stream);
-  const unsigned n = (unsigned)a.requests;
-  const int parts = page_parts(a);
-  k_pages_fork_need<<<n, kPageThreads, 0, stream>>>(a);
+  k_pages_fork_need<<<(unsigned)a.requests, kPageThreads, 0, stream>>>(a);
   k_pages_deal<false><<<1, kDealThreads, 0, stream>>>(a);
-  k_pages_forked<<<n * parts, kPageThreads, 0, stream>>>(a, parts);
+  int rc = last_error();
+  if (rc == (int)hipSuccess) rc = launch_parts(a, k_pages_forked, stream);
   timing_end(K_PAGES, stream);
-  return last_error();
+  return rc;
 }
 
 int launch_pages_compact(const PagesArgs& a, hipStream_t stream) {
@@ -349,10 +357,9 @@ int launch_pages_compact(const PagesArgs& a, hipStream_t stream) {
 
 int launch_pages_copy(const PagesArgs& a, hipStream_t stream) {
   timing_begin(K_PAGES, stream);
-  const int parts = page_parts(a);
-  k_pages_copy<<<(unsigned)(a.requests * parts), kPageThreads, 0, stream>>>(a, parts);
+  const int rc = launch_parts(a, k_pages_copy, stream);
   timing_end(K_PAGES, stream);
-  return last_error();
+  return rc;
 }
 
 }  // namespace sf
