@@ -759,7 +759,8 @@ def _pair(a: int, b: int):
 
 def mx4_quantize(x: torch.Tensor, outer: int, inner: int, strides: tuple, codes: torch.Tensor,
                  scales: torch.Tensor) -> None:
-    _launch("sf_mx4_quantize", x.device, x.data_ptr(), _DTYPE_CODE[x.dtype], outer, inner, _pair(*strides)[1], x.shape[-1],
+    pair = _pair(*strides)  # (held until the call is back: the cache may let go of it)
+    _launch("sf_mx4_quantize", x.device, x.data_ptr(), _DTYPE_CODE[x.dtype], outer, inner, pair[1], x.shape[-1],
             codes.data_ptr(), scales.data_ptr())
 
 
