@@ -62,11 +62,13 @@ class MX4Linear(nn.Module):
 def quantize_linears_(net: nn.Module, quantize_input: bool = False,
                       only: Optional[Callable[[str, nn.Module], bool]] = None) -> int:
     """Replaces the nn.Linear and SparseLinear modules of `net` (those that only(name,
-    module) picks) by MX4Linear -> how many."""
+    module) picks) by MX4Linear -> how many.  Subclasses stay: their forward may be another,
+    or their owner read the weight by itself (nn.MultiheadAttention).  Hooks are the old
+    module's, as everywhere that modules are replaced."""
     from .sparse_linear import SparseLinear
 
     found = [(name, m) for name, m in net.named_modules(remove_duplicate=False)
-             if name and isinstance(m, (nn.Linear, SparseLinear)) and (only is None or only(name, m))]
+             if name and type(m) in (nn.Linear, SparseLinear) and (only is None or only(name, m))]
     made = {}  # (a module that stands in two places is one afterwards too)
     for name, m in found:
         if m not in made:
