@@ -70,9 +70,10 @@ def quantize_linears_(net: nn.Module, quantize_input: bool = False,
     found = [(name, m) for name, m in net.named_modules(remove_duplicate=False)
              if name and type(m) in (nn.Linear, SparseLinear) and (only is None or only(name, m))]
     made = {}  # (a module that stands in two places is one afterwards too)
-    for name, m in found:
+    for _, m in found:
         if m not in made:
             made[m] = MX4Linear.from_dense(m, quantize_input)
+    for name, m in found:
         parent, _, leaf = name.rpartition(".")
         setattr(net.get_submodule(parent), leaf, made[m])
     return len(found)

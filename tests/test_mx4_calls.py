@@ -28,7 +28,7 @@ def test_strides_live_as_long_as_the_call(monkeypatch):
     def launch(name, device, *args):
         _lib._pair.cache_clear()
         at = args[4]
-        held.append([list(o) for o in gc.get_objects() if isinstance(o, ctypes.c_int64 * 2) and ctypes.addressof(o) == at])
+        held.append([list(o) for o in gc.get_objects() if type(o) is ctypes.c_int64 * 2 and ctypes.addressof(o) == at])
 
     monkeypatch.setattr(_lib, "_launch", launch)
     x = torch.randn(3, 40)

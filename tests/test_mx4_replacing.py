@@ -23,3 +23,10 @@ def test_subclasses_with_a_forward_or_an_owner_of_their_own():
         assert quantize_linears_(net) == 2
         assert isinstance(net["c"], MX4Linear) and isinstance(net["d"], MX4Linear)
         assert torch.equal(net["a"](x), want[0]) and torch.equal(net["b"](x, x, x)[0], want[1])
+
+
+def test_a_net_that_is_refused_is_left_as_it_was():
+    net = nn.Sequential(nn.Linear(32, 32), nn.Linear(32, 8).double())
+    with pytest.raises(_lib.UnsupportedError):
+        quantize_linears_(net)
+    assert [type(m) for m in net] == [nn.Linear, nn.Linear]
