@@ -595,7 +595,8 @@ int sf_mx4_cache_append(const sf_mx4_cache_desc* desc, const sf_mx4_cache* cache
                         const int32_t* slots, void* stream);
 /* y = softmax(scale q k) v per query row of q [tokens, heads, head_dim], over the
  * cached tokens up to its own (heads / kv_heads in a row share keys and values).  A
- * query that sees no token: 0.  The workspace is 16-byte aligned. */
+ * query that sees no token: 0; scores that are all -infinity, or that hold a NaN or
+ * +infinity: NaN.  |scale| < 2^127.  The workspace is 16-byte aligned. */
 size_t sf_mx4_attention_workspace_size(const sf_mx4_cache_desc* desc);
 int sf_mx4_attention(const sf_mx4_cache_desc* desc, const sf_mx4_cache* cache,
                      const void* q, const int32_t* offsets, const int32_t* slots,

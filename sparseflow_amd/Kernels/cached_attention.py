@@ -192,6 +192,13 @@ def _host_attend(q, cache, length: int, table: torch.Tensor, scale: float) -> to
     return y
 
 
+def check_scale(scale: float) -> float:
+    """(NaN is below nothing; times log2(e) it has to be a float32.)"""
+    if not abs(scale) < 2.0 ** 127:
+        raise ValueError(f"scale is {scale}: a number below 2^127 is wanted")
+    return scale
+
+
 def cached_attention_forward(q: torch.Tensor, cache: MX4Cache, tables: torch.Tensor, lengths: torch.Tensor,
                              slots: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
                              max_len: Optional[int] = None, scale: Optional[float] = None,
@@ -201,7 +208,8 @@ def cached_attention_forward(q: torch.Tensor, cache: MX4Cache, tables: torch.Ten
     The queries are each sequence's last tokens, whose keys and values the cache holds
     (mx4_cache_append): query i of n has place lengths[slot] - n + i and sees the tokens up
     to it.  One that sees none (an empty sequence, a place before the first, a slot
-    outside tables, no page): zeros.  scale: head_dim ** -0.5 by default.  out may be q;
+    outside tables, no page): zeros.  scale: head_dim ** -0.5 by default, a number below 2^127;
+    scores that are all -infinity, or that hold a NaN or +infinity, give NaN.  out may be q;
     apart from that it shares no memory with what is read.  Rows of a packed q that are no
     sequence's are left as they are in out.
     """
@@ -225,6 +233,7 @@ def _attention(q, cache, tables, lengths, slots, offsets, max_len, scale, out):
     if max_len is not None:
         max_len = int(max_len)
     scale = float(q.shape[-1]) ** -0.5 if scale is None and q.dim() > 0 and q.shape[-1] > 0 else float(scale or 0.0)
+    check_scale(scale)
     key = (signature(q, *cache, tables, lengths, slots, offsets, out), max_len, scale)
     desc, = _attentions.get(key) or _attentions.make(key, _check_attention, q, cache, tables, lengths, slots, offsets,
                                                      max_len, scale, out)

@@ -17,7 +17,8 @@ import torch.nn as nn
 
 from .. import _lib
 from ..Kernels._sequences import check_input, check_like
-from ..Kernels.cached_attention import MAX_HEAD_DIM, MAX_PAGE, MX4Cache, cached_attention_forward, mx4_cache, mx4_cache_append
+from ..Kernels.cached_attention import MAX_HEAD_DIM, MAX_PAGE, MX4Cache, cached_attention_forward, check_scale, mx4_cache, \
+    mx4_cache_append
 from ..Kernels.mx4 import blocks_of
 from ..Kernels.pages import pages_compact, pages_fork, pages_resize
 from ._runtime import host_parents
@@ -85,6 +86,8 @@ class CachedAttention(nn.Module):
         self.page_size, self.scale = int(page_size), scale
         if not 1 <= self.page_size <= MAX_PAGE or self.page_size & (self.page_size - 1):
             raise ValueError(f"page_size={page_size}: a power of two up to {MAX_PAGE} is wanted")
+        if scale is not None:
+            check_scale(float(scale))
         self.state: Optional[_Sequences] = None
 
     def reset(self):

@@ -1091,6 +1091,7 @@ int sf_mx4_attention(const sf_mx4_cache_desc* d, const sf_mx4_cache* cache, cons
                      const int32_t* slots, void* y, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_cache_desc(d);
   if (rc != SF_OK) return rc;
+  if (!(d->scale < 0x1p127f && d->scale > -0x1p127f)) return fail(SF_ERR_INVALID, "scale is no number below 2^127");
   if (d->batch == 0 || d->tokens == 0 || d->max_len == 0) return SF_OK;
   if (q == nullptr || y == nullptr) return fail(SF_ERR_INVALID, "NULL pointer");
   sf::Mx4AttnArgs a{};
