@@ -186,8 +186,9 @@ def mx4_linear_forward(x: Union[torch.Tensor, Quantized], weight: Quantized, bia
                        dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] W^T + bias -> [..., N], W a quantised [N, K], bias float32 [N].
 
-    x as floats is taken as it is (every product is exact, sums are float32); as a
-    pair (codes, scales) of rows of as many blocks it goes to the 4-bit matrix
+    x as floats is taken as it is (every product is exact, sums are float32; of float32 x
+    the bits from 2^-133 on count, and weights past float32, of scales 253 and 254, are
+    infinite or NaN); as a pair (codes, scales) of rows of as many blocks it goes to the 4-bit matrix
     instructions.  The result has `dtype` (default x's, for a pair float32) or out's;
     out shares no memory with the inputs.
     """

@@ -1,7 +1,7 @@
 // The microscaled 4-bit format on the device: blocks of 32 values, a byte 127 + e
 // (255: not a number) and 32 codes of 4 bits, +-{0, .5, 1, 1.5, 2, 3, 4, 6} 2^e.
 // gfx950 only: its conversions take the block's scale along and round to nearest
-// even, for every scale byte; a value of the format is a bf16 one exactly.
+// even, for every scale byte; a value of the format below 2^128 is a bf16 one exactly.
 #pragma once
 
 #include "sf_seq.h"
@@ -83,7 +83,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int6
   }
 }
 
-// A float as a sum of bf16 parts of 8 bits each: exact in three (float32) and two (f16).
+// A float as a sum of bf16 parts of 8 bits each: exact in three (float32 from 2^-109 on; bf16 numbers
+// are multiples of 2^-133) and two (f16).
 // Cut off, not rounded: nothing overflows.  An infinity is the first part alone.
 template <typename T>
 struct Parts {
