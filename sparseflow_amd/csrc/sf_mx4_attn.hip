@@ -76,8 +76,8 @@ __global__ __launch_bounds__(kAppendThreads) void k_mx4_append(Mx4AppendArgs a) 
 // are as many as the CUs hold, and the units (128 tokens of a tile of rows) of all sequences,
 // one after another, are cut into as many even shares.  A share's ends may lie inside a tile's
 // tokens: those parts go to the workspace, two at most of a workgroup, and k_mx4_attn_join
-// puts them together.  (64 x 8192 tokens in two equal parts a tile 138 us, in four 160, in
-// eight 189.)
+// puts them together.  (64 x 8192 tokens, with bf16 weights in one part: 119 us; in two equal parts
+// a tile 138, in four 160, in eight 189.)
 constexpr int kAttnWaves = 4;
 constexpr int kAttnTokens = 32;
 constexpr int kAttnUnit = kAttnWaves;   // chunks of kAttnTokens: one to a wavefront
@@ -518,8 +518,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, NB * kWeightParts<T> <= 8 ? 2 : 
 
 // A row's parts together: W wavefronts to a row (of a workgroup's four), a lane to its columns, F
 // parts under way; place(j) is part j's row of the workspace.  W = 1 where there are few parts
-// and many rows (8 x 100 queries of 1100 tokens: 65 us for the call, with W = 4 105), W = 4
-// otherwise (64 parts: 6 us, with W = 1 19).
+// and many rows (32 / 8 heads of 128, the call in us: 4 x 100 queries after 6000 tokens 115, with
+// W = 4 152; 32 x 4 after 3000 45 and 61), W = 4 otherwise (one after 100,000: 48, with W = 1 60).
 template <typename T, int NB, int W, typename Place>
 __device__ __forceinline__ void join_row(const Mx4AttnArgs& a, int64_t parts, Place&& place, T* y) {
   constexpr int C = (32 * NB + kWave - 1) / kWave, F = C <= 2 ? 16 : 8;
@@ -678,8 +678,9 @@ Mx4AttnPlan mx4_attn_plan(int64_t batch, int64_t max_len, int heads, int kv_head
   } else {
     // Parts of the tokens only while all of them are on the CUs at once (of what they hold, by
     // registers), and where a part is long enough to be worth its rows' way through memory (bf16,
-    // 32 / 8 heads of 128, 1024 tokens: 38 us whole, 63 in two parts; 188 tiles of 8000 tokens: 205
-    // and 155; with parts up to six times what the CUs hold, 256 tiles of 2048: 66 whole, 117).
+    // 32 / 8 heads of 128 in us: 1024 tokens 44 whole, 70 in two parts; 128 tiles of 4096 130 whole,
+    // 97 in two, 84 in the four that fit, 92 in eight; 192 of 8000 261, 236 in the two that fit; but
+    // 256 of 4000 146 and 153, of 2078 79 and 102).
     const int64_t hold = blocks <= 4 && blocks * parts <= 8 ? 512 : 256;
     int64_t splits = items == 0 || room < 2048 ? 1 : hold / items;
     const int64_t most = room / 256;

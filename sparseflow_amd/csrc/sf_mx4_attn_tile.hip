@@ -10,10 +10,10 @@
 // multiple of their number apart: on one XCD where that is a multiple of eight.
 //
 // Bound by its instructions: of 64 tokens a wavefront has 48 products of bf16 (32 cycles each; 32 of
-// them take the weights' two parts) and some 400 vector instructions (4 cycles), of which the softmax
-// is 200 and the widening of the codes 80.  2 x 8192 tokens, 32 / 8 heads of 128: bf16 1490 us (740
-// TFLOP/s; with weights of one part 1200), f16 1915, float32 3950; 4 x 4096, 16 heads of 64: 274 us
-// (500).
+// them take the weights' two parts) and some 420 vector instructions (4 cycles), of which the softmax
+// is 220 and the widening of the codes 80.  2 x 8192 tokens, 32 / 8 heads of 128: bf16 1500 us (730
+// TFLOP/s; with weights of one part 1200), f16 1950, float32 4000; 4 x 4096, 16 heads of 64: 282 us
+// (490).
 #include "sf_mx4_cache.h"
 
 namespace sf {

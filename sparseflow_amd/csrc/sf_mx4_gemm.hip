@@ -370,7 +370,7 @@ __global__ __launch_bounds__(P::threads, 2) void k_mx4_gemm_four(Mx4LinearArgs a
 //
 // KG groups of wavefronts take stages in turn, each with LDS of its own, and add up what they
 // have at the end: where y has no more tiles than there are CUs, the time is a tile's stages one
-// after another, half a us each (128 x 4096 x 4096: bf16 32.6 -> 20.4 us, f32 63.6 -> 40.2;
+// after another, half a us each (128 x 4096 x 4096: bf16 32.6 -> 21.4 us, f32 63.6 -> 43;
 // 256 x 8192 x 1024: 70 -> 36, 123 -> 78).
 template <typename P, int NP>
 struct alignas(16) AnyStage {
@@ -589,8 +589,8 @@ int launch_any(const Mx4LinearArgs& a, hipStream_t stream) {
     if (tiles_of(a, 256, 256) >= kGemmTiles) return launch_any<T, Shape<4, 2, 2, 4, 2>, 1>(a, stream);
   }
   if (tiles_of(a, 128, 256) >= kGemmTiles) return launch_any<T, Shape<2, 4, 2, 2, 2>, 1>(a, stream);
-  // (2050 x 6000, bf16 / f32 in us: 65 rows of 188 tiles take 13.7 / 26.4 in groups and 15.2 / 37.6
-  // without, 256 rows of 376 tiles 26.7 / 50.4 and 21.4 / 49.7.)
+  // (2050 x 6000, bf16 / f32 in us: 65 rows of 188 tiles take 13.3 / 24.9 in groups and 15.2 / 37.6
+  // without, 256 rows of 376 tiles 26.7 / 50.4 and 19.5 / 45.7.)
   if (tiles_of(a, 64, 64) <= kCus) return launch_any<T, Shape<2, 2, 1, 1, 2>, Parts<T>::n == 1 ? 4 : 2>(a, stream);
   return launch_any<T, Shape<2, 2, 1, 1, 2>, 1>(a, stream);
 }
@@ -613,7 +613,7 @@ int launch_mx4_gemm(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   const bool direct = aligned_to(a.x, 16) && a.x_stride % 8 == 0 && a.k % 8 == 0 && a.blocks % 4 == 0 &&
                       aligned_to(a.w_scales, 4) && a.x_stride >= 0 && a.x_stride < 1 << 22 && a.blocks < 1 << 19;
   if (!direct) return launch_any<__hip_bfloat16>(a, stream);
-  // (The smallest tiles, one to a CU: 100 x 4096 x 4096 20.6 us in groups of stages, 32.5 here.)
+  // (The smallest tiles, one to a CU: 100 x 4096 x 4096 20.8 us in groups of stages, 32.5 here.)
   const bool few = tiles_of(a, 64, 64) <= kCus;
   return large    ? launch_bf16<Shape<4, 2, 2, 4, 3>>(a, stream)
          : middle ? launch_bf16<Shape<2, 2, 2, 2, 3>>(a, stream)

@@ -224,6 +224,9 @@ int launch_mx4_linear(const Mx4LinearArgs& a, int x_dtype, hipStream_t stream) {
   // of them, a wavefront to few columns reads W sooner (this kernel / tiles; 64 x 4096 x 12288:
   // bf16 41 / 22, f32 102 / 45, four 25 / 16; 33 x 4096 x 4096: bf16 13 / 20, f32 45 / 39, four
   // 9 / 14; 17 to 32 rows: never worse by more than a us).
+  // (4-bit x whose blocks are no multiple of four, or whose scales or W's are not 4-byte aligned, has
+  // no tiles and stays here at any number of rows, where floats would be sooner; four / bf16: 8192 x
+  // 4100 x 16380 1860 / 1050, 8192 x 1056 x 4096 201 / 91, 4096 x 192 x 904 13.5 / 8.6.)
   const int64_t filling = x_dtype == SF_F32 ? 2048 : 10240;
   const bool tiles = !few && a.m > (a.n > filling ? 32 : 64) && (x_dtype != SF_MX4 || mx4_gemm_takes_four(a));
   const int rc = tiles                ? launch_mx4_gemm(a, x_dtype, stream)
